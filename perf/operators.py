@@ -390,7 +390,9 @@ def _run_own(s):
         call = pc.rotary_grad if case["grad"] else pc.rotary
         q, k = call(s["q"], s["k"], s["positions"], s["inv_freq"], s["sections"])
         return {"q": q, "k": k}
-    cache = pc.PagedCache(s["k_pages"], s["v_pages"], s.get("weight"), s.get("pos"))
+    if "cache" not in s:                                   # a program keeps its cache
+        s["cache"] = pc.PagedCache(s["k_pages"], s["v_pages"], s.get("weight"), s.get("pos"))
+    cache = s["cache"]
     if case["op"] == "append":
         lens = pc.cache_append(cache, s["k"], s["v"], s["table"], s["lens"], s["starts"])
         return {"k": cache.k, "v": cache.v, "lens": lens}
