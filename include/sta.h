@@ -536,6 +536,134 @@ int sta_decode_attend(const sta_decode_args* args, void* stream);
  * Q queries at once. */
 int sta_decode_attention(const sta_decode_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * The paged key-value cache and the operators around it.  No counterpart in the reference, whose
+ * decode keeps one contiguous cache of one sequence.
+ *
+ * A cache is `pages` pages of `page_size` slots.  Key j of sequence b, kv head h, is row
+ * (table[b][j / page_size], h, j % page_size) of k and v; the heads of a sequence share its length
+ * lens[b] but not its keys (sta_cache_evict drops other keys in each head).  Keys are attended as
+ * they are stored: rotate them before they are written (sta_rotary).  Per key and kv head the
+ * cache may hold the attention weight that the key has drawn (weight) and its token's number in
+ * the sequence (pos).
+ *
+ * A length below 0 counts as 0 and one past the table as the table's end (table_width *
+ * page_size, or max_len where an entry point takes one).  A key whose table entry is not in
+ * [0, pages) does not exist: it is not attended, not written, and the first to be evicted.
+ * Sequences may share pages that are only read.  A page that a call writes (the new keys' page,
+ * any page under accumulate, any page of an eviction) must appear once in that call's tables.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct sta_cache {
+  void* k;                 /* rows of D elements, 16-byte aligned; element strides */
+  void* v;
+  int64_t k_page_stride, k_head_stride, k_slot_stride;
+  int64_t v_page_stride, v_head_stride, v_slot_stride;
+  float* weight;           /* (pages, Hkv, page_size), slot stride 1; NULL: none */
+  int64_t weight_page_stride, weight_head_stride;
+  int32_t* pos;            /* (pages, Hkv, page_size), slot stride 1; NULL: none */
+  int64_t pos_page_stride, pos_head_stride;
+  int32_t dtype;           /* STA_DTYPE_* of k and v */
+  int32_t pages, page_size; /* page_size: a power of two up to 65536 */
+  int32_t Hkv, D;          /* D in {64, 128} */
+  const int32_t* table;    /* (B, table_width), rows table_stride apart */
+  int64_t table_stride;
+  int32_t table_width, B;
+  const int32_t* lens;     /* (B,) */
+} sta_cache;
+
+#define STA_POS_I32 0
+#define STA_POS_I64 1
+#define STA_POS_F32 2
+#define STA_ROTARY_MAX_AXES 4
+
+/* Rotary positions with 1 to 4 axes over the rows of T tokens.  Pair (i, R/2 + i) of a row turns by
+ * the angle pos[axis(i)][t] * pos_scale * inv_freq[i] (in 64 bits) and is scaled by rope_scale;
+ * R = 2 * (section[0] + ... + section[axes - 1]), axis a owning section[a] frequencies in order;
+ * the elements behind R are copied.  inverse != 0 turns the other way: the gradient of the rotation
+ * with respect to its input.  Outputs may be the inputs. */
+typedef struct sta_rotary_args {
+  const void* q;           /* (T, H, D); NULL with H = 0 */
+  const void* k;           /* (T, Hkv, D); NULL with Hkv = 0 */
+  void* q_out;
+  void* k_out;
+  int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride;
+  int64_t q_out_tok_stride, q_out_head_stride, k_out_tok_stride, k_out_head_stride;
+  int32_t dtype, T, H, Hkv, D; /* D: a multiple of 8 up to 512 */
+  int32_t axes;
+  int32_t section[STA_ROTARY_MAX_AXES]; /* R / 2 = their sum, a multiple of 8 */
+  const void* positions;   /* (axes, T) of pos_type */
+  int64_t pos_axis_stride, pos_tok_stride;
+  int32_t pos_type;        /* STA_POS_* */
+  const float* inv_freq;   /* (R / 2,) */
+  float pos_scale, rope_scale;
+  int32_t inverse;
+} sta_rotary_args;
+
+int sta_rotary(const sta_rotary_args* args, void* stream);
+
+/* Write T new keys and values behind the sequences' keys: rows starts[b] .. starts[b + 1] - 1 of k
+ * and v go to the slots lens[b] .. of sequence b (starts NULL: one row a sequence, T = B; rows
+ * outside [starts[0], starts[B]) are not read).  A cache with weight gets 0 there, one with pos
+ * seen[b] + i (seen NULL: the slot).  Keys past the table's end are dropped.  new_lens[b], not the
+ * lens array itself, receives the new length. */
+typedef struct sta_append_args {
+  sta_cache cache;
+  const void* k;           /* (T, Hkv, D) in the cache's dtype, 16-byte rows */
+  const void* v;
+  int64_t k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+  int32_t T;
+  const int32_t* starts;   /* (B + 1,) ascending, or NULL */
+  const int32_t* seen;     /* (B,) or NULL */
+  int32_t* new_lens;       /* (B,) */
+} sta_append_args;
+
+int sta_cache_append(const sta_append_args* args, void* stream);
+
+/* Attention of Q new tokens of every sequence over its cached keys, theirs the last Q of them:
+ * query i of sequence b sees the keys j < lens[b] - (Q - 1 - i), out = sum_j p_j v_j with p the
+ * softmax of sm_scale * q . k_j over them.  A query that sees no key gets zeros and lse -inf.
+ * accumulate != 0 adds each key's p, summed over the Q queries and the heads of its kv head, to
+ * cache.weight. */
+typedef struct sta_paged_args {
+  sta_cache cache;
+  const void* q;           /* (B, H, Q, D), element strides, 16-byte rows */
+  int64_t q_batch_stride, q_head_stride, q_tok_stride;
+  int32_t H, Q;
+  float sm_scale;          /* finite */
+  int32_t max_len;         /* lengths are at most this; sizes the workspace and the grid */
+  int32_t accumulate;
+  void* out;               /* (B, H, Q, D) contiguous */
+  float* lse;              /* (B, H, Q): log sum exp of the scaled scores; NULL to skip */
+  void* workspace;
+  size_t workspace_bytes;
+} sta_paged_args;
+
+size_t sta_paged_workspace_size(const sta_paged_args* args);
+int sta_paged_attention(const sta_paged_args* args, void* stream);
+
+/* Keep the min(lens[b], budget) keys of each kv head that come first in this order: those with
+ * pos < n_global or pos > (the head's largest pos) - n_local, then the others by weight, the
+ * largest first (NaN before all), equal ones by slot, the lower first.
+ * dst_table NULL: the kept keys in slots >= budget move, with weight and pos, into the dropped ones'
+ * slots < budget, both in ascending order; the others stay.  Nothing moves where lens[b] <= budget.
+ * dst_table: the kept keys are copied in ascending order of their slots to the slots 0, 1, ... of
+ * the pages of dst_table, none of which the tables of this call may hold otherwise; the source stays.
+ * new_lens[b], not the lens array itself, receives min(lens[b], budget). */
+typedef struct sta_evict_args {
+  sta_cache cache;         /* weight and pos required */
+  int32_t budget, n_global, n_local; /* budget >= 1 */
+  int32_t max_len;         /* lengths are at most this */
+  const int32_t* dst_table; /* (B, dst_width), dst_width * page_size >= min(budget, max_len) */
+  int64_t dst_stride;
+  int32_t dst_width;
+  int32_t* new_lens;       /* (B,) */
+  void* workspace;
+  size_t workspace_bytes;
+} sta_evict_args;
+
+size_t sta_evict_workspace_size(const sta_evict_args* args);
+int sta_cache_evict(const sta_evict_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

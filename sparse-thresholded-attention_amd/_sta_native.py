@@ -24,7 +24,9 @@ EXPORTS = ["sta_abi_version", "sta_last_error", "sta_shared_workspace_size", "st
            "sta_pqstream_workspace_size", "sta_pqstream_attention",
            "sta_dca_workspace_size", "sta_dca_attention", "sta_dca_rotate_keys", "sta_dca_decode_workspace_size",
            "sta_dca_decode", "sta_decode_workspace_size", "sta_decode_scores",
-           "sta_decode_build_sets", "sta_decode_build_sets_chunk", "sta_decode_attend", "sta_decode_attention"]
+           "sta_decode_build_sets", "sta_decode_build_sets_chunk", "sta_decode_attend", "sta_decode_attention",
+           "sta_rotary", "sta_cache_append", "sta_paged_workspace_size", "sta_paged_attention",
+           "sta_evict_workspace_size", "sta_cache_evict"]
 SCORES = {"freq": 0, "margin": 1, "expmass": 2}
 
 
@@ -184,6 +186,68 @@ class DecodeArgsC(ctypes.Structure):
     ]
 
 
+class CacheC(ctypes.Structure):
+    """Mirror of sta_cache (include/sta.h)."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_page_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64), ("k_slot_stride", ctypes.c_int64),
+        ("v_page_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64), ("v_slot_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p), ("weight_page_stride", ctypes.c_int64), ("weight_head_stride", ctypes.c_int64),
+        ("pos", ctypes.c_void_p), ("pos_page_stride", ctypes.c_int64), ("pos_head_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32),
+        ("B", ctypes.c_int32), ("lens", ctypes.c_void_p),
+    ]
+
+
+class RotaryArgsC(ctypes.Structure):
+    """Mirror of sta_rotary_args (include/sta.h)."""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+        ("q_tok_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("k_tok_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("q_out_tok_stride", ctypes.c_int64), ("q_out_head_stride", ctypes.c_int64),
+        ("k_out_tok_stride", ctypes.c_int64), ("k_out_head_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("T", ctypes.c_int32), ("H", ctypes.c_int32), ("Hkv", ctypes.c_int32),
+        ("D", ctypes.c_int32), ("axes", ctypes.c_int32), ("section", ctypes.c_int32 * 4),
+        ("positions", ctypes.c_void_p), ("pos_axis_stride", ctypes.c_int64), ("pos_tok_stride", ctypes.c_int64),
+        ("pos_type", ctypes.c_int32), ("inv_freq", ctypes.c_void_p), ("pos_scale", ctypes.c_float),
+        ("rope_scale", ctypes.c_float), ("inverse", ctypes.c_int32),
+    ]
+
+
+class AppendArgsC(ctypes.Structure):
+    """Mirror of sta_append_args (include/sta.h)."""
+    _fields_ = [
+        ("cache", CacheC), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_tok_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("v_tok_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+        ("T", ctypes.c_int32), ("starts", ctypes.c_void_p), ("seen", ctypes.c_void_p), ("new_lens", ctypes.c_void_p),
+    ]
+
+
+class PagedArgsC(ctypes.Structure):
+    """Mirror of sta_paged_args (include/sta.h)."""
+    _fields_ = [
+        ("cache", CacheC), ("q", ctypes.c_void_p),
+        ("q_batch_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64), ("q_tok_stride", ctypes.c_int64),
+        ("H", ctypes.c_int32), ("Q", ctypes.c_int32), ("sm_scale", ctypes.c_float), ("max_len", ctypes.c_int32),
+        ("accumulate", ctypes.c_int32), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class EvictArgsC(ctypes.Structure):
+    """Mirror of sta_evict_args (include/sta.h)."""
+    _fields_ = [
+        ("cache", CacheC), ("budget", ctypes.c_int32), ("n_global", ctypes.c_int32), ("n_local", ctypes.c_int32),
+        ("max_len", ctypes.c_int32), ("dst_table", ctypes.c_void_p), ("dst_stride", ctypes.c_int64),
+        ("dst_width", ctypes.c_int32), ("new_lens", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 RULES = {"shared": 0, "pq": 1, "stream": 2}    # STA_RULE_SHARED / STA_RULE_PQ / STA_RULE_STREAM
 
 
@@ -251,6 +315,15 @@ def lib():
         L.sta_dca_decode_workspace_size.argtypes = [ctypes.POINTER(DcaDecodeArgsC)]
         L.sta_dca_decode.restype = ctypes.c_int
         L.sta_dca_decode.argtypes = [ctypes.POINTER(DcaDecodeArgsC), ctypes.c_void_p]
+        for name, args in (("sta_rotary", RotaryArgsC), ("sta_cache_append", AppendArgsC),
+                           ("sta_paged_attention", PagedArgsC), ("sta_cache_evict", EvictArgsC)):
+            fn = getattr(L, name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        for name, args in (("sta_paged_workspace_size", PagedArgsC), ("sta_evict_workspace_size", EvictArgsC)):
+            fn = getattr(L, name)
+            fn.restype = ctypes.c_size_t
+            fn.argtypes = [ctypes.POINTER(args)]
         if L.sta_abi_version() != 5:
             raise ImportError("libsta_hip.so ABI version mismatch")
         _LIB = L
@@ -1357,3 +1430,234 @@ def perquery_prefill_attention(q, k, v, tau, inv_freq_a, inv_freq_c, pos_scale_a
     ic = inv_freq_c.to(device=q.device, dtype=torch.float32).contiguous()
     return PerQueryPrefillPlan(q, k, v, tau, ia, ic, pos_scale_a, rope_scale_a, sm_scale, n_global, n_local,
                                k_max, heads_per_group, query_chunk=query_chunk).run()
+
+
+# ---------------------------------------------------------------------------------------------
+# the paged key-value cache and the operators around it (paged_cache.py)
+# ---------------------------------------------------------------------------------------------
+POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}   # STA_POS_*
+
+
+def _launch(fn, args, dev, what):
+    """fn on dev's current stream, with dev current while it launches."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        _check(fn(ctypes.byref(args), _stream(dev)), what)
+    else:
+        with torch.cuda.device(dev):
+            _check(fn(ctypes.byref(args), _stream(dev)), what)
+
+
+def _require(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _device_input(x, name):
+    if not x.is_cuda:
+        raise RuntimeError(f"sparse-thresholded attention runs on a HIP device only; {name} is a CPU tensor")
+    if x.dtype not in DTYPES:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+
+
+def _rows(x):
+    """x with unit stride in its last dim, and 16-byte rows at strides that are not negative."""
+    esz = x.element_size()
+    if (x.stride(-1) != 1 and x.shape[-1] != 1) or x.data_ptr() % 16 or any(s * esz % 16 for s in x.stride()[:-1]):
+        x = x.contiguous()
+    return x
+
+
+def _ints(x, dev):
+    """A device int32 tensor with unit stride in its last dim."""
+    if x.dtype != torch.int32 or x.device != dev:
+        x = x.to(device=dev, dtype=torch.int32)
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
+class PagedCache:
+    """The pages of one layer's key-value cache: k, v (pages, Hkv, page_size, D), and, for each key and kv head,
+    the attention weight it has drawn (weight, fp32) and its token's number in the sequence (pos,
+    int32), both (pages, Hkv, page_size) or None.  The tensors are used as they are, whatever their
+    strides over pages, heads and slots."""
+
+    def __init__(self, k, v, weight=None, pos=None):
+        for name, x in (("k", k), ("v", v)):
+            _device_input(x, f"cache {name}")
+            _require(x.dim() == 4, f"cache {name} must be (pages, kv heads, page_size, D), not {tuple(x.shape)}")
+            _require(x.stride(3) == 1, f"cache {name} needs unit stride in its last dim")
+        if v.dtype != k.dtype:
+            raise TypeError("cache k and v must share one dtype")
+        _require(v.shape == k.shape and v.device == k.device, "cache k and v must share shape and device")
+        for name, x, dtype in (("weight", weight, torch.float32), ("pos", pos, torch.int32)):
+            if x is None:
+                continue
+            if x.dtype != dtype:
+                raise TypeError(f"cache {name} must be {dtype}, not {x.dtype}")
+            _require(x.shape == k.shape[:3] and x.device == k.device,
+                     f"cache {name} must be {tuple(k.shape[:3])} on the device of k")
+            _require(x.stride(2) == 1 or x.shape[2] == 1, f"cache {name} needs unit stride in its last dim")
+        self.k, self.v, self.weight, self.pos, self.device = k, v, weight, pos, k.device
+        self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        self._c = c = CacheC()
+        c.k, c.v = k.data_ptr(), v.data_ptr()
+        c.k_page_stride, c.k_head_stride, c.k_slot_stride = k.stride()[:3]
+        c.v_page_stride, c.v_head_stride, c.v_slot_stride = v.stride()[:3]
+        if weight is not None:
+            c.weight, c.weight_page_stride, c.weight_head_stride = weight.data_ptr(), weight.stride(0), weight.stride(1)
+        if pos is not None:
+            c.pos, c.pos_page_stride, c.pos_head_stride = pos.data_ptr(), pos.stride(0), pos.stride(1)
+        c.dtype, c.pages, c.page_size = DTYPES[k.dtype], self.pages, self.page_size
+        c.Hkv, c.D = self.kv_heads, self.head_dim
+
+    @classmethod
+    def empty(cls, pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda", evictable=True):
+        """A cache of uninitialised pages; evictable: with weight and pos."""
+        shape = (pages, kv_heads, page_size, head_dim)
+        k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+        if not evictable:
+            return cls(k, v)
+        return cls(k, v, torch.zeros(shape[:3], dtype=torch.float32, device=device),
+                   torch.zeros(shape[:3], dtype=torch.int32, device=device))
+
+    def _fill(self, a, table, lens):
+        """a.cache for sequences with these page tables and lengths; the tensors it points to."""
+        table, lens = _ints(table, self.device), _ints(lens, self.device)
+        _require(table.dim() == 2 and lens.dim() == 1 and lens.shape[0] == table.shape[0],
+                 "table must be (B, pages of a sequence) and lens (B,)")
+        a.cache = self._c
+        c = a.cache
+        c.table, c.table_stride, (c.B, c.table_width) = table.data_ptr(), table.stride(0), table.shape
+        c.lens = lens.data_ptr()
+        return table, lens
+
+    def _max_len(self, table, max_len):
+        most = table.shape[1] * self.page_size
+        return most if max_len is None else min(int(max_len), most)
+
+
+def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1.0, inverse=False):
+    """sta_rotary of q (T, H, D) and k (T, Hkv, D) or None -> their rotations."""
+    _device_input(q, "q")
+    dev = q.device
+    _require(q.dim() == 3, f"q must be (T, heads, D), not {tuple(q.shape)}")
+    q = _rows(q)
+    T, H, D = q.shape
+    a = RotaryArgsC()
+    q_out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+    a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+    a.q_tok_stride, a.q_head_stride, _ = q.stride()
+    a.q_out_tok_stride, a.q_out_head_stride = H * D, D
+    k_out = None
+    if k is not None:
+        if k.dtype != q.dtype:
+            raise TypeError("q and k must share one dtype")
+        _require(k.dim() == 3 and k.shape[0] == T and k.shape[2] == D, f"k must be ({T}, kv heads, {D})")
+        k = _rows(k.to(dev))
+        a.Hkv = k.shape[1]
+        k_out = torch.empty((T, a.Hkv, D), dtype=q.dtype, device=dev)
+        a.k, a.k_out = k.data_ptr(), k_out.data_ptr()
+        a.k_tok_stride, a.k_head_stride, _ = k.stride()
+        a.k_out_tok_stride, a.k_out_head_stride = a.Hkv * D, D
+    if positions.dtype not in POS_TYPES:
+        raise TypeError(f"positions must be int32, int64 or float32, not {positions.dtype}")
+    positions = positions.to(dev)
+    if positions.dim() == 1:
+        positions = positions[None]
+    if inv_freq.dtype != torch.float32 or inv_freq.device != dev or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.to(device=dev, dtype=torch.float32).contiguous()
+    sections = (inv_freq.numel(),) if sections is None else tuple(int(s) for s in sections)
+    _require(len(sections) <= 4, "at most 4 axes")
+    _require(tuple(positions.shape) == (len(sections), T), f"positions must be ({len(sections)}, {T})")
+    _require(sum(sections) == inv_freq.numel(), f"sections {sections} do not share out {inv_freq.numel()} frequencies")
+    a.dtype, a.T, a.H, a.D, a.axes = DTYPES[q.dtype], T, H, D, len(sections)
+    a.section[:len(sections)] = sections
+    a.positions, a.pos_type = positions.data_ptr(), POS_TYPES[positions.dtype]
+    a.pos_axis_stride, a.pos_tok_stride = positions.stride()
+    a.inv_freq, a.pos_scale, a.rope_scale = inv_freq.data_ptr(), float(pos_scale), float(rope_scale)
+    a.inverse = int(inverse)
+    _launch(lib().sta_rotary, a, dev, "sta_rotary")
+    return q_out, k_out
+
+
+def cache_append(cache, k, v, table, lens, starts=None, seen=None):
+    """sta_cache_append of k, v (T, Hkv, D) -> the new lengths (B,) int32."""
+    _device_input(k, "k")
+    dev = cache.device
+    if k.dtype != cache.k.dtype or v.dtype != cache.k.dtype:
+        raise TypeError("k, v and the cache must share one dtype")
+    _require(k.dim() == 3 and k.shape[1:] == (cache.kv_heads, cache.head_dim) and v.shape == k.shape,
+             f"k and v must be (T, {cache.kv_heads}, {cache.head_dim})")
+    k, v = _rows(k.to(dev)), _rows(v.to(dev))
+    a = AppendArgsC()
+    keep = cache._fill(a, table, lens)
+    B = a.cache.B
+    a.k, a.v, a.T = k.data_ptr(), v.data_ptr(), k.shape[0]
+    a.k_tok_stride, a.k_head_stride, _ = k.stride()
+    a.v_tok_stride, a.v_head_stride, _ = v.stride()
+    if starts is not None:
+        starts = _ints(starts, dev)
+        _require(tuple(starts.shape) == (B + 1,), f"starts must be ({B + 1},)")
+        a.starts = starts.data_ptr()
+    if seen is not None:
+        seen = _ints(seen, dev)
+        _require(tuple(seen.shape) == (B,), f"seen must be ({B},)")
+        a.seen = seen.data_ptr()
+    new_lens = torch.empty(B, dtype=torch.int32, device=dev)
+    a.new_lens = new_lens.data_ptr()
+    _launch(lib().sta_cache_append, a, dev, "sta_cache_append")
+    del keep
+    return new_lens
+
+
+def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want_lse=False, max_len=None):
+    """sta_paged_attention of q (B, H, D) or (B, H, Q, D) -> out like q, and with want_lse the
+    log-sum-exp (B, H) or (B, H, Q) fp32."""
+    _device_input(q, "q")
+    dev = cache.device
+    if q.dtype != cache.k.dtype:
+        raise TypeError("q and the cache must share one dtype")
+    _require(q.dim() in (3, 4) and q.shape[-1] == cache.head_dim,
+             f"q must be (B, heads, {cache.head_dim}) or (B, heads, queries, {cache.head_dim})")
+    shape = q.shape
+    q = _rows((q if q.dim() == 4 else q.unsqueeze(2)).to(dev))
+    a = PagedArgsC()
+    table, lens = cache._fill(a, table, lens)
+    _require(shape[0] == a.cache.B, f"q holds {shape[0]} sequences, table {a.cache.B}")
+    a.q, a.H, a.Q = q.data_ptr(), q.shape[1], q.shape[2]
+    a.q_batch_stride, a.q_head_stride, a.q_tok_stride, _ = q.stride()
+    a.sm_scale = 1.0 / math.sqrt(cache.head_dim) if sm_scale is None else float(sm_scale)
+    a.max_len, a.accumulate = cache._max_len(table, max_len), int(bool(accumulate))
+    out = torch.empty(shape, dtype=q.dtype, device=dev)
+    a.out = out.data_ptr()
+    lse = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if want_lse else None
+    a.lse = _ptr(lse)
+    n = lib().sta_paged_workspace_size(ctypes.byref(a))
+    if n == 0:
+        _check(-1, "sta_paged_workspace_size")
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    _launch(lib().sta_paged_attention, a, dev, "sta_paged_attention")
+    return (out, lse) if want_lse else out
+
+
+def cache_evict(cache, table, lens, budget, n_global=32, n_local=32, dst_table=None, max_len=None):
+    """sta_cache_evict -> the new lengths (B,) int32."""
+    dev = cache.device
+    a = EvictArgsC()
+    table, lens = cache._fill(a, table, lens)
+    a.budget, a.n_global, a.n_local = int(budget), int(n_global), int(n_local)
+    a.max_len = cache._max_len(table, max_len)
+    if dst_table is not None:
+        dst_table = _ints(dst_table, dev)
+        _require(dst_table.dim() == 2 and dst_table.shape[0] == a.cache.B, "dst_table must have a row a sequence")
+        a.dst_table, a.dst_width = dst_table.data_ptr(), dst_table.shape[1]
+        a.dst_stride = dst_table.stride(0)
+    new_lens = torch.empty(a.cache.B, dtype=torch.int32, device=dev)
+    a.new_lens = new_lens.data_ptr()
+    n = lib().sta_evict_workspace_size(ctypes.byref(a))
+    if n == 0:
+        _check(-1, "sta_evict_workspace_size")
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    _launch(lib().sta_cache_evict, a, dev, "sta_cache_evict")
+    return new_lens

@@ -1,0 +1,123 @@
+// sta_rotary.hip -- rotary positions with one or several axes over the rows of a batch of tokens.
+//
+// Pair (x, y) = (row[i], row[R/2 + i]) becomes scale * (x cos t - y sin t, y cos t + x sin t) with
+// t = pos[axis(i)] * pos_scale * inv_freq[i]; the gradient with respect to the row is the same with
+// -sin.  The angle is formed and reduced to a fraction of a turn in 64 bits, since a position of
+// 10^5 leaves fp32 an absolute error near 10^-2 of a radian; the fraction's sine and cosine and the
+// rotation are fp32, rounded once into the row's type.
+//
+// Bound by memory: each element is read and written once.  The (cos, sin) pairs of a token serve
+// all of its heads, so a workgroup computes them once into LDS and then streams the token's rows,
+// 16 bytes of both rotation halves a thread.
+#include "sta_cache.h"
+#include "sta_device.h"
+
+namespace sta {
+
+namespace {
+
+template <int DT>
+constexpr int ROT_V = DT == DT_F32 ? 4 : 8;       // elements in 16 bytes
+
+template <int DT>
+__device__ __forceinline__ void unpack16(const u32x4& w, float* o) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (DT == DT_F32) {
+      o[e] = __uint_as_float(w[e]);
+    } else if constexpr (DT == DT_BF16) {
+      o[2 * e] = __uint_as_float(w[e] << 16);
+      o[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    } else {
+      o[2 * e] = f16_bits_to_f32(w[e] & 0xffffu);
+      o[2 * e + 1] = f16_bits_to_f32(w[e] >> 16);
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ u32x4 pack16(const float* o) {
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (DT == DT_F32) w[e] = __float_as_uint(o[e]);
+    else w[e] = pack2_dt<DT>(o[2 * e], o[2 * e + 1]);
+  }
+  return w;
+}
+
+__device__ __forceinline__ double position(const sta_rotary_args& a, int axis, int64_t t) {
+  const int64_t i = axis * a.pos_axis_stride + t * a.pos_tok_stride;
+  if (a.pos_type == STA_POS_I64) return (double)((const int64_t*)a.positions)[i];
+  if (a.pos_type == STA_POS_F32) return (double)((const float*)a.positions)[i];
+  return (double)((const int32_t*)a.positions)[i];
+}
+
+// TPB tokens a workgroup
+template <int DT, int TPB>
+__global__ __launch_bounds__(256) void rotary_kernel(sta_rotary_args a, int half) {
+  constexpr int V = ROT_V<DT>;
+  extern __shared__ float2 trig[];                 // [TPB][half]
+  const int64_t t0 = (int64_t)blockIdx.x * TPB;
+  const int nt = (int)min((int64_t)TPB, a.T - t0);
+  for (int i = threadIdx.x; i < nt * half; i += 256) {
+    const int t = i / half, f = i - t * half;
+    int axis = 0, first = 0;
+    while (axis + 1 < a.axes && f >= first + a.section[axis]) first += a.section[axis++];
+    double turns = position(a, axis, t0 + t) * (double)a.pos_scale * (double)a.inv_freq[f];
+    turns *= 0.15915494309189533577;
+    turns -= rint(turns);
+    float s, c;
+    sincospif((float)(2.0 * turns), &s, &c);
+    trig[i] = make_float2(c * a.rope_scale, (a.inverse ? -s : s) * a.rope_scale);
+  }
+  __syncthreads();
+  const int rot = half / V, chunks = rot + (a.D - 2 * half) / V;     // of a row
+  const int rows = a.H + a.Hkv;
+  for (int i = threadIdx.x; i < nt * rows * chunks; i += 256) {
+    const int c = i % chunks, r = i / chunks;
+    const int t = r / rows, h = r - t * rows;
+    const bool is_q = h < a.H;
+    const int64_t ts = is_q ? a.q_tok_stride : a.k_tok_stride, hs = is_q ? a.q_head_stride : a.k_head_stride;
+    const int64_t ots = is_q ? a.q_out_tok_stride : a.k_out_tok_stride;
+    const int64_t ohs = is_q ? a.q_out_head_stride : a.k_out_head_stride;
+    const int hh = is_q ? h : h - a.H;
+    constexpr int E = DT == DT_F32 ? 4 : 2;
+    const char* x = (const char*)(is_q ? a.q : a.k) + ((t0 + t) * ts + hh * hs) * E;
+    char* o = (char*)(is_q ? a.q_out : a.k_out) + ((t0 + t) * ots + hh * ohs) * E;
+    if (c >= rot) {                                // behind the rotated part
+      const int at = (2 * half + (c - rot) * V) * E;
+      *(u32x4*)(o + at) = *(const u32x4*)(x + at);
+      continue;
+    }
+    float p[V], q[V], u[V], w[V];
+    unpack16<DT>(*(const u32x4*)(x + c * 16), p);
+    unpack16<DT>(*(const u32x4*)(x + half * E + c * 16), q);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float2 cs = trig[t * half + c * V + e];
+      u[e] = p[e] * cs.x - q[e] * cs.y;
+      w[e] = q[e] * cs.x + p[e] * cs.y;
+    }
+    *(u32x4*)(o + c * 16) = pack16<DT>(u);
+    *(u32x4*)(o + half * E + c * 16) = pack16<DT>(w);
+  }
+}
+
+template <int DT>
+hipError_t launch_dt(const sta_rotary_args& a, hipStream_t st) {
+  int half = 0;
+  for (int i = 0; i < a.axes; ++i) half += a.section[i];
+  rotary_kernel<DT, 1><<<a.T, 256, (size_t)half * sizeof(float2), st>>>(a, half);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_rotary(const sta_rotary_args& a, hipStream_t st) {
+  if (a.dtype == STA_DTYPE_F32) return launch_dt<DT_F32>(a, st);
+  if (a.dtype == STA_DTYPE_BF16) return launch_dt<DT_BF16>(a, st);
+  return launch_dt<DT_F16>(a, st);
+}
+
+}  // namespace sta
