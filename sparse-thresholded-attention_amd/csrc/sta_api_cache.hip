@@ -103,8 +103,8 @@ int paged_check(const sta_paged_args* a) {
   if (rc != STA_OK) return rc;
   if (a->H < 1 || a->H % a->cache.Hkv != 0)
     return fail(STA_ERR_INVALID_ARG, "H=%d must be a positive multiple of Hkv=%d", a->H, a->cache.Hkv);
-  if (a->Q < 1 || (int64_t)a->H * a->Q > (1 << 20))
-    return fail(STA_ERR_INVALID_ARG, "Q=%d must be >= 1 and H * Q <= 2^20", a->Q);
+  if (a->Q < 1 || (int64_t)a->H * a->Q > (1 << 20) || (int64_t)a->H * a->Q * a->cache.B > (1 << 26))
+    return fail(STA_ERR_INVALID_ARG, "Q=%d must be >= 1, H * Q <= 2^20 and B * H * Q <= 2^26", a->Q);
   if (a->max_len < 1 || a->max_len >= (1 << 28))
     return fail(STA_ERR_INVALID_ARG, "max_len=%d outside [1, 2^28)", a->max_len);
   if (!isfinite(a->sm_scale)) return fail(STA_ERR_INVALID_ARG, "sm_scale must be finite");
@@ -112,19 +112,31 @@ int paged_check(const sta_paged_args* a) {
 }
 
 struct PagedLayout {
-  size_t scores_off, lse_off, total;
+  PagedCut cut;
+  size_t part_off, ml_off, lse_off, scores_off, total;
   int64_t score_stride;
 };
+
+int paged_cap(const sta_paged_args* a) {
+  const int64_t cap = (int64_t)a->cache.table_width * a->cache.page_size;
+  return (int)(cap < a->max_len ? cap : a->max_len);
+}
 
 PagedLayout paged_layout(const sta_paged_args* a) {
   PagedLayout L{};
   const size_t rows = (size_t)a->cache.B * a->H * a->Q;
-  L.score_stride = ((int64_t)a->max_len + 63) / 64 * 64;
+  L.cut = paged_cut(a->cache.dtype, a->H, a->cache.Hkv, a->Q, a->cache.B, paged_cap(a));
+  L.score_stride = ((int64_t)paged_cap(a) + 63) / 64 * 64;
+  const size_t part_rows = L.cut.single ? 0 : (size_t)L.cut.grid * L.cut.rows;
   size_t off = 0;
-  L.scores_off = off;
-  off = align256(off + rows * L.score_stride * 4);
-  L.lse_off = off;
+  L.part_off = off;                                   // the pieces' outputs, fp32
+  off = align256(off + part_rows * a->cache.D * 4);
+  L.ml_off = off;                                     // their maxima and sums
+  off = align256(off + part_rows * 8);
+  L.lse_off = off;                                    // (B, H, Q) when not an output
   off = align256(off + rows * 4);
+  L.scores_off = off;                                 // (B, H, Q, score_stride)
+  if (a->accumulate) off = align256(off + rows * L.score_stride * 4);
   L.total = off;
   return L;
 }
@@ -273,6 +285,9 @@ int sta_paged_attention(const sta_paged_args* a, void* stream) {
   d.lse = a->lse ? a->lse : (float*)(ws + L.lse_off);
   d.scores = (float*)(ws + L.scores_off);
   d.score_stride = L.score_stride;
+  d.part_o = (float*)(ws + L.part_off);
+  d.part_ml = (float2*)(ws + L.ml_off);
+  d.grid = L.cut.grid;
   hipError_t e = launch_paged(a->cache.dtype, a->cache.D, d, (hipStream_t)stream);
   return e == hipSuccess ? STA_OK : hip_fail(e, "paged attention");
 }

@@ -53,7 +53,17 @@ struct PagedArgs {
   float* lse;                       // (B, H, Q), the caller's or in the workspace
   float* scores;                    // (B, H, Q, score_stride), accumulate only
   int64_t score_stride;
+  float* part_o;                    // (grid, rows, D) unnormalised outputs of the pieces, rows x D permuted
+  float2* part_ml;                  // (grid, rows) their maxima and sums
+  int grid;
 };
+
+// how a call of the attention is cut (host): a workgroup takes `rows` query rows of one kv head over
+// one piece of a sequence's keys, counted in units of `unit` keys
+struct PagedCut {
+  int rows, tiles, unit, grid, single;   // tiles: row tiles a kv head; single: no sequence has two pieces
+};
+PagedCut paged_cut(int dtype, int H, int Hkv, int Q, int B, int cap);
 
 struct EvictArgs {
   CacheView c;
