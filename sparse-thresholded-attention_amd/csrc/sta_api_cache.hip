@@ -125,11 +125,11 @@ int paged_cap(const sta_paged_args* a) {
 PagedLayout paged_layout(const sta_paged_args* a) {
   PagedLayout L{};
   const size_t rows = (size_t)a->cache.B * a->H * a->Q;
-  L.cut = paged_cut(a->cache.dtype, a->H, a->cache.Hkv, a->Q, a->cache.B, paged_cap(a));
-  L.score_stride = ((int64_t)paged_cap(a) + 63) / 64 * 64;
-  const size_t part_rows = L.cut.single ? 0 : (size_t)L.cut.grid * L.cut.rows;
+  L.cut = paged_cut(a->cache.dtype, a->cache.D, a->H, a->cache.Hkv, a->Q, a->cache.B, paged_cap(a));
+  L.score_stride = ((int64_t)paged_cap(a) + 255) / 256 * 256;   // whole units, and 256 keys of the weights
+  const size_t part_rows = (size_t)L.cut.records * L.cut.rows;
   size_t off = 0;
-  L.part_off = off;                                   // the pieces' outputs, fp32
+  L.part_off = off;                                   // unfinished row tiles, fp32
   off = align256(off + part_rows * a->cache.D * 4);
   L.ml_off = off;                                     // their maxima and sums
   off = align256(off + part_rows * 8);

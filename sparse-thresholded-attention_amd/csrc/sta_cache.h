@@ -53,17 +53,19 @@ struct PagedArgs {
   float* lse;                       // (B, H, Q), the caller's or in the workspace
   float* scores;                    // (B, H, Q, score_stride), accumulate only
   int64_t score_stride;
-  float* part_o;                    // (grid, rows, D) unnormalised outputs of the pieces, rows x D permuted
-  float2* part_ml;                  // (grid, rows) their maxima and sums
+  float* part_o;                    // (records, rows, D) unnormalised outputs of unfinished row tiles, permuted
+  float2* part_ml;                  // (records, rows) their maxima and sums
   int grid;
 };
 
-// how a call of the attention is cut (host): a workgroup takes `rows` query rows of one kv head over
-// one piece of a sequence's keys, counted in units of `unit` keys
+// how a call of the attention is cut (host): `grid` workgroups; a row tile is `rows` query rows of
+// one kv head, `tiles` of them a kv head
 struct PagedCut {
-  int rows, tiles, unit, grid, single;   // tiles: row tiles a kv head; single: no sequence has two pieces
+  int rows, tiles, grid;
+  bool single;                      // no sequence has two units and one query each: nothing to join
+  int64_t records;                  // of unfinished row tiles, in the workspace
 };
-PagedCut paged_cut(int dtype, int H, int Hkv, int Q, int B, int cap);
+PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap);
 
 struct EvictArgs {
   CacheView c;

@@ -72,17 +72,13 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 // widened.  The fp32 instruction runs at 1/16 of the 16-bit rate and still needs a quarter of the time
 // that a CU's share of the memory bandwidth takes for K and V with one tile of rows.
 //
-// Pieces.  The sequences' lengths are known to the device alone.  Every wave sums their units (of 4 KT
-// keys) and cuts each sequence into pieces of at most `per` units, the smallest number with which the
-// whole call has at most about W pieces; a prefix sum over the sequences says whose piece a workgroup
-// has.  Pieces of one sequence have consecutive numbers, which are also their places in the
-// workspace, and the join kernel repeats the prefix sum to find them.
-constexpr int PIECES = 1024;
+// Work.  The sequences' lengths are known to the device alone, and differ.  Every wave sums their units (of
+// 4 KT keys; an empty sequence counts one, which writes its zeros) over all row tiles, and the call's
+// workgroups, as many as the chip holds at once, take equal runs of units in the order (sequence, row
+// tile, unit).  A run covers the end of one row tile, some whole ones and the beginning of another; whole
+// ones are written out, the two others leave a record in the workspace for the join kernel, which
+// finds the workgroups of a row tile by the same division.
 constexpr float LOG2E = 1.44269504088896340736f;
-
-struct Piece {
-  int b, base, n, per;          // sequence, number of its first piece, pieces of a row tile, units of a piece
-};
 
 __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
 #pragma unroll
@@ -90,37 +86,58 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
   return x;
 }
 
-// the piece with number blk (want_b < 0), or the pieces of sequence want_b; false: there is none.  Every
-// lane of the wave takes part; the answer is uniform.
-__device__ __forceinline__ bool find_piece(const CacheView& c, int unit, int segs, int blk, int want_b, Piece& p) {
-  const int lane = threadIdx.x & 63;
+// whole part of x / y, 0 <= x < 2^40, 1 <= y < 2^40 (the quotient's distance from a whole number above it is
+// at least 1 / y, beyond the rounding of the division)
+__device__ __forceinline__ int div40(int64_t x, int64_t y) { return (int)((double)x / (double)y); }
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
+
+__device__ __forceinline__ int units_of(int keys, int unit) { return max(1, (keys + unit - 1) / unit); }
+
+// keys that every query of sequence b sees
+__device__ __forceinline__ int common(const PagedArgs& a, int b) { return max(a.c.len(b) - (a.Q - 1), 0); }
+
+// units that a workgroup takes (at least one); every lane of the wave takes part
+__device__ __forceinline__ int64_t units_each(const PagedArgs& a, int unit, int segs) {
   int64_t sum = 0;
-  for (int b = lane; b < c.B; b += 64) sum += (c.len(b) + unit - 1) / unit;
-  sum = wave_sum64(sum) * segs;
-  const int per = (int)max((int64_t)1, (sum + PIECES - 1) / PIECES);
-  int run = 0;
+  for (int b = threadIdx.x & 63; b < a.c.B; b += 64) sum += units_of(common(a, b), unit);
+  const int64_t all = uniform(wave_sum64(sum)) * segs;
+  return all <= a.grid ? 1 : uniform(div40(all + a.grid - 1, a.grid));
+}
+
+// The sequence that holds unit `at` (or, at < 0, sequence b) and the number of its first unit; -1: behind
+// the last.  Uniform; every lane takes part.
+__device__ __forceinline__ int find_seq(const PagedArgs& a, int unit, int segs, int64_t at, int b, int64_t& base) {
+  const CacheView& c = a.c;
+  const int lane = threadIdx.x & 63;
+  int64_t run = 0;
   for (int b0 = 0; b0 < c.B; b0 += 64) {
-    const int b = b0 + lane;
-    int n = 0;
-    if (b < c.B) n = max(1, ((c.len(b) + unit - 1) / unit + per - 1) / per);
-    const int incl = wave_incl_sum(n * segs);
-    const int total = __builtin_amdgcn_readlane(incl, 63);
-    const unsigned long long hit = want_b < 0 ? __ballot(run + incl > blk) : __ballot(b == want_b);
+    const int mine = b0 + lane;
+    // up to 64 * 2^22 units of a row tile
+    const int n = mine < c.B ? units_of(common(a, mine), unit) : 0;
+    const int incl = wave_incl_sum(n);
+    const unsigned long long hit = at < 0 ? __ballot(mine == b) : __ballot(run + (int64_t)incl * segs > at);
     if (hit) {
       const int first = __builtin_amdgcn_readfirstlane(__ffsll(hit) - 1);
-      p.n = __builtin_amdgcn_readlane(n, first);
-      p.base = run + __builtin_amdgcn_readlane(incl, first) - p.n * segs;
-      p.b = b0 + first;
-      p.per = per;
-      return true;
+      base = run + (int64_t)(__builtin_amdgcn_readlane(incl, first) - __builtin_amdgcn_readlane(n, first)) * segs;
+      return b0 + first;
     }
-    run += total;
+    run += (int64_t)__builtin_amdgcn_readlane(incl, 63) * segs;
   }
-  return false;
+  return -1;
+}
+
+// the record of a row tile that one workgroup finished, MULTI calls only: behind the two of each workgroup
+__device__ __forceinline__ int64_t whole_record(const PagedArgs& a, int segs, int b, int seg) {
+  return 2 * (int64_t)a.grid + (int64_t)b * segs + seg;
 }
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 __device__ __forceinline__ float at_least(float m) { return m == -INFINITY ? 0.f : m; }   // what p is relative to
+
+__device__ const u32x4 zero_row[32] = {};              // 512 bytes: a row of 128 fp32 elements
 
 template <int DT, int D, int NT_>
 struct Tile {
@@ -132,6 +149,10 @@ struct Tile {
   static constexpr int VE = D / 16;                    // V elements of a lane
   static constexpr int VW = VE * E / 4;                // their words
   static constexpr int NT = NT_, ROWS = 16 * NT;
+  // Waves of a SIMD, and so workgroups of a CU (256 a grid and wave): what the registers hold without spills.
+  // Three at D = 64 (bf16, 32q / 8kv heads: 37 us, with two 41), two at D = 128 (the other way round: 146 us
+  // for 190 MB of keys and as much of values, with three 166, most of the loss from spilled accumulators).
+  static constexpr int WAVES = D == 64 && NT == 1 ? 3 : 2;
 };
 
 template <int DT>
@@ -156,15 +177,18 @@ __device__ __forceinline__ float v_elem(const uint32_t* w, int e) {
   else return f16_bits_to_f32(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu);
 }
 
+// loads at an address in global memory (one that went through a lane exchange is no pointer to the compiler)
+typedef const __attribute__((address_space(1))) u32x4* global4;
+typedef const __attribute__((address_space(1))) u32x2* global2;
 template <int W>
-__device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
+__device__ __forceinline__ void load_words(int64_t p, uint32_t* w) {
   if constexpr (W == 2) {
-    const u32x2 x = *(const u32x2*)p;
+    const u32x2 x = *(global2)p;
     w[0] = x[0], w[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < W; i += 4) {
-      const u32x4 x = *(const u32x4*)(p + 4 * i);
+      const u32x4 x = *(global4)(p + 4 * i);
       w[i] = x[0], w[i + 1] = x[1], w[i + 2] = x[2], w[i + 3] = x[3];
     }
   }
@@ -190,8 +214,12 @@ __device__ __forceinline__ void store_out(char* out, const float* y, int n) {   
   }
 }
 
-template <int DT, int D, int NT, bool ACC>
-__global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_attend_kernel(PagedArgs a, int tiles) {
+// MULTI: a.Q may exceed 1.  Then len stands for the keys that all queries see and every row tile is joined:
+// paged_join_kernel adds the last Q - 1 keys, of which each query sees others, row by row, so that the rows
+// of an instruction always see the same keys (0 times a NaN or an infinity would reach rows that do not
+// see its key).
+template <int DT, int D, int NT, bool ACC, bool MULTI>
+__global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_kernel(PagedArgs a, int tiles) {
   using T = Tile<DT, D, NT>;
   constexpr int KS = T::KS, VE = T::VE, VW = T::VW, SUB = T::SUB, KT = T::KT;
   __shared__ floatx4 merge[4][VE * 4 * 16];
@@ -199,22 +227,36 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_attend_kernel(Page
   const CacheView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g4 = lane >> 4;
-  Piece pc;
-  if (!find_piece(c, T::UNIT, c.Hkv * tiles, blockIdx.x, -1, pc)) return;
-  const int b = pc.b, x = blockIdx.x - pc.base;
-  const int seg = x / pc.n, piece = x - seg * pc.n;
-  const int hk = seg / tiles, row0 = (seg - hk * tiles) * T::ROWS;
-  const int G = a.H / c.Hkv, R = G * a.Q;
-  const int len = c.len(b);
-  const int u0 = piece * pc.per, u1 = min(u0 + pc.per, (len + T::UNIT - 1) / T::UNIT);
+  const int segs = c.Hkv * tiles, G = a.H / c.Hkv, R = G * a.Q;
+  const int64_t each = units_each(a, T::UNIT, segs);
+  const int64_t run0 = blockIdx.x * each, run1 = run0 + each;
+  int64_t base = 0;
+  int b = find_seq(a, T::UNIT, segs, run0, -1, base);
+  if (b < 0) return;
+  int len = uniform(common(a, b)), units = units_of(len, T::UNIT);
+  int seg = uniform(div40(run0 - base, units));
+  for (int64_t at = run0; at < run1;) {
+    if (seg == segs) {
+      if (++b == c.B) return;
+      base = at;
+      seg = 0;
+      len = uniform(common(a, b));
+      units = units_of(len, T::UNIT);
+    }
+    const int64_t first = base + (int64_t)seg * units;
+    const int u0 = (int)(at - first), u1 = (int)min((int64_t)units, run1 - first);
+    const bool whole_tile = u1 - u0 == units, done = !MULTI && whole_tile;
+    const int64_t record = whole_tile ? whole_record(a, segs, b, seg) : 2 * (int64_t)blockIdx.x + (at != run0);
+    at = first + u1;
+    const int hk = tiles == 1 ? seg : seg / tiles, row0 = (seg - hk * tiles) * T::ROWS;
+    ++seg;
 
   u32x4 q[NT][KS];
   int64_t srow[NT];
-  int end[NT];                                         // keys that the lane's rows see
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int row = row0 + t * 16 + r;
-    const int i = row % a.Q, h = hk * G + row / a.Q;
+    const int g = MULTI ? row / a.Q : row, i = MULTI ? row - g * a.Q : 0, h = hk * G + g;
     const bool real = row < R;
     const char* qp = (const char*)a.q + (b * a.q_bs + (real ? h : 0) * a.q_hs + (real ? i : 0) * a.q_ts) * T::E + g4 * 16;
 #pragma unroll
@@ -222,10 +264,8 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_attend_kernel(Page
       q[t][s] = *(const u32x4*)(qp + s * 64);
       if (!real) q[t][s] = u32x4{0, 0, 0, 0};
     }
-    end[t] = real ? len - (a.Q - 1 - i) : len;
-    if (ACC) srow[t] = real ? (((int64_t)b * a.H + h) * a.Q + i) * a.score_stride : -1;
+    if (ACC) srow[t] = real ? (((int64_t)b * a.H + h) * a.Q + i) * a.score_stride + g4 * 4 : -1;
   }
-  const int all_see = len - (a.Q - 1);                 // keys that every row sees
 
   floatx4 acc[NT][VE];
   float m[NT], l[NT];
@@ -238,42 +278,40 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_attend_kernel(Page
   }
 
   const int32_t* table = c.table + (int64_t)b * c.t_stride;
-  const char* kbase = c.k + hk * c.k_hs + g4 * 16;
-  const char* vbase = c.v + hk * c.v_hs + r * (VW * 4);
-  // lane's key of a turn: lane % KT; -1 behind the sequence
-  auto page_at = [&](int u) {
-    const int j = (u * 4 + wave) * KT + (lane & (KT - 1));
-    return u < u1 && j < len ? c.page_of(table, j) : -1;
+  // The table entry of the lane's key of a turn, lane % KT, and whether that key exists.  The entry is
+  // loaded two turns ahead and judged one turn later, so that no turn waits for it.
+  const int last = max(len - 1, 0) >> c.shift;
+  auto entry_at = [&](int u) { return table[min(((u * 4 + wave) * KT + (lane & (KT - 1))) >> c.shift, last)]; };
+  auto page_at = [&](int u, int entry) {
+    return (u * 4 + wave) * KT + (lane & (KT - 1)) < len && (unsigned)entry < (unsigned)c.pages ? entry : -1;
   };
   u32x4 k[SUB][KS];
-  int64_t koff = 0, voff = 0;
-  auto offsets = [&](int u, int page) {
+  int64_t krow, vrow;                                  // addresses of the lane's key; a key that does not exist is a row of zeros
+  auto rows_of = [&](int u, int page) {
     const int slot = c.slot_of((u * 4 + wave) * KT + (lane & (KT - 1)));
-    koff = page < 0 ? 0 : page * c.k_ps + slot * c.k_ss;   // a key that does not exist reads page 0's first
-    voff = page < 0 ? 0 : page * c.v_ps + slot * c.v_ss;
+    krow = (int64_t)(page < 0 ? (const char*)zero_row : c.k + hk * c.k_hs + page * c.k_ps + slot * c.k_ss);
+    vrow = (int64_t)(page < 0 ? (const char*)zero_row : c.v + hk * c.v_hs + page * c.v_ps + slot * c.v_ss);
   };
   auto load_k = [&]() {
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-      const char* p = kbase + __shfl(koff, s * 16 + r, 64);
+      const int64_t p = __shfl(krow, s * 16 + r, 64) + g4 * 16;
 #pragma unroll
-      for (int i = 0; i < KS; ++i) k[s][i] = *(const u32x4*)(p + i * 64);
+      for (int i = 0; i < KS; ++i) k[s][i] = *(global4)(p + i * 64);
     }
   };
-  int page = page_at(u0), next_page = page_at(u0 + 1);
-  if (u0 < u1) {
-    offsets(u0, page);
-    load_k();
-  }
+  int page = page_at(u0, entry_at(u0)), next_entry = entry_at(u0 + 1);
+  rows_of(u0, page);
+  load_k();
   for (int u = u0; u < u1; ++u) {
     const int key0 = (u * 4 + wave) * KT;
-    const unsigned long long there = __ballot(page >= 0);
+    const uint32_t there = (uint32_t)__ballot(page >= 0);  // lanes beyond KT repeat the first ones
     uint32_t v[SUB][4][VW];
 #pragma unroll
     for (int s = 0; s < SUB; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) load_words<VW>(vbase + __shfl(voff, s * 16 + g4 * 4 + i, 64), v[s][i]);
-    const int after = page_at(u + 2);
+      for (int i = 0; i < 4; ++i) 
+        load_words<VW>(__shfl(vrow, s * 16 + g4 * 4 + i, 64) + r * (VW * 4), v[s][i]);
 
     floatx4 sc[NT][SUB];
 #pragma unroll
@@ -285,44 +323,27 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_attend_kernel(Page
         for (int i = 0; i < KS; ++i) x = mfma_qk<DT>(k[s][i], q[t][i], x);
         sc[t][s] = x * a.sm_scale;
       }
-    page = next_page;
-    next_page = after;
     if (u + 1 < u1) {
-      offsets(u + 1, page);
+      page = page_at(u + 1, next_entry);
+      next_entry = entry_at(u + 2);
+      rows_of(u + 1, page);
       load_k();
     }
 
-    const bool whole = there == ~0ull, mixed = key0 + KT > all_see;
-    if (!whole) {
-      // keys that do not exist: no score, and zeros for whatever lies where they would
+    if (there != ~0u) {
 #pragma unroll
       for (int s = 0; s < SUB; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool is = there >> (s * 16 + g4 * 4 + i) & 1;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int t = 0; t < NT; ++t) sc[t][s][i] = is ? sc[t][s][i] : -INFINITY;
-#pragma unroll
-          for (int w = 0; w < VW; ++w) v[s][i][w] = is ? v[s][i][w] : 0u;
-        }
-    }
-    if (mixed) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int s = 0; s < SUB; ++s)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (key0 + s * 16 + g4 * 4 + i >= end[t]) sc[t][s][i] = -INFINITY;
+          for (int t = 0; t < NT; ++t)
+            if (!(there >> (g4 * 4) & 1u << (s * 16 + i))) sc[t][s][i] = -INFINITY;
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (ACC && srow[t] >= 0) {
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-          const int j = key0 + s * 16 + g4 * 4;
-          if (j < len) *(floatx4*)(a.scores + srow[t] + j) = sc[t][s];
-        }
+        for (int s = 0; s < SUB; ++s) *(floatx4*)(a.scores + srow[t] + key0 + s * 16) = sc[t][s];
       }
       float top = fmaxf(fmaxf(sc[t][0][0], sc[t][0][1]), fmaxf(sc[t][0][2], sc[t][0][3]));
       if (SUB == 2) top = fmaxf(top, fmaxf(fmaxf(sc[t][SUB - 1][0], sc[t][SUB - 1][1]), fmaxf(sc[t][SUB - 1][2], sc[t][SUB - 1][3])));
@@ -345,38 +366,18 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_attend_kernel(Page
           l[t] += p;
         }
     }
-    if (!(mixed && a.Q > 1)) {
 #pragma unroll
-      for (int s = 0; s < SUB; ++s)
+    for (int s = 0; s < SUB; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i) {
+    #pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float ve = v_elem<DT>(v[s][i], e);
 #pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const float ve = v_elem<DT>(v[s][i], e);
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-              acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(ve, sc[t][s][i], acc[t][e], 0, 0, 0);
-          }
-    } else {
-      // rows of one instruction see different keys: one key at a time, kept by the rows that see it, so
-      // that a value of 0 * infinity or NaN reaches no other row
-#pragma unroll
-      for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          for (int j = 0; j < 4; ++j) {
-            const int key = key0 + s * 16 + j * 4 + i;
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-              const float ve = g4 == j ? v_elem<DT>(v[s][i], e) : 0.f;
-#pragma unroll
-              for (int t = 0; t < NT; ++t) {
-                const floatx4 y = __builtin_amdgcn_mfma_f32_16x16x4f32(ve, g4 == j ? sc[t][s][i] : 0.f, acc[t][e], 0, 0, 0);
-                acc[t][e] = key < end[t] ? y : acc[t][e];
-              }
-            }
-          }
-    }
+          for (int t = 0; t < NT; ++t)
+            acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(ve, sc[t][s][i], acc[t][e], 0, 0, 0);
+        }
+      }
   }
 
   // the four waves' states into one
@@ -400,16 +401,16 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_attend_kernel(Page
     for (int w = 0; w < 4; ++w) ll += merge_l[w][row] * exp_of(merge_m[w][row] - m0);
 #pragma unroll
     for (int e = 0; e < VE; ++e) merge[wave][(e * 4 + g4) * 16 + r] = acc[t][e] * f;
-    if (pc.n > 1) {
-      if (wave == 0 && g4 == 0) a.part_ml[(int64_t)blockIdx.x * T::ROWS + row] = make_float2(mm, ll);
+    if (!done) {
+      if (wave == 0 && g4 == 0) a.part_ml[record * T::ROWS + row] = make_float2(mm, ll);
     } else if (wave == 0 && g4 == 0 && row0 + row < R) {
       const int rr = row0 + row;
       a.lse[((int64_t)b * a.H + hk * G + rr / a.Q) * a.Q + rr % a.Q] = ll == 0.f ? -INFINITY : m0 + logf(ll);
     }
     if (wave == 0 && g4 == 0) merge_sum[row] = ll;
     __syncthreads();
-    if (pc.n > 1) {
-      floatx4* part = (floatx4*)(a.part_o + ((int64_t)blockIdx.x * T::ROWS + t * 16) * D);
+    if (!done) {
+      floatx4* part = (floatx4*)(a.part_o + (record * T::ROWS + t * 16) * D);
       for (int i = tid; i < VE * 64; i += 256) part[i] = (merge[0][i] + merge[1][i]) + (merge[2][i] + merge[3][i]);
     } else {
       // thread: one 16th of a row
@@ -430,46 +431,107 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_attend_kernel(Page
     }
     __syncthreads();
   }
+  }
 }
 
-// one workgroup per query row: the pieces of its sequence, a wave each in turn
-template <int DT, int D, int NT>
+// One workgroup per query row: the records of its row tile, a wave each in turn, and (MULTI) the keys behind
+// the common ones.
+template <int DT, int D, int NT, bool MULTI>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles) {
   using T = Tile<DT, D, NT>;
-  __shared__ float o[4][D];
+  constexpr int TAIL = 256, W = D / 64;               // a lane's dims
+  __shared__ float o[4][D], tail[MULTI ? TAIL : 1];
+  __shared__ int tail_page[MULTI ? TAIL : 1];
   const CacheView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int hi = blockIdx.x, b = blockIdx.y, G = a.H / c.Hkv;
-  Piece pc;
-  if (!find_piece(c, T::UNIT, c.Hkv * tiles, 0, b, pc) || pc.n == 1) return;
-  const int h = hi / a.Q, i = hi % a.Q, hk = h / G, row = (h - hk * G) * a.Q + i;
-  const int first = pc.base + (hk * tiles + row / T::ROWS) * pc.n, rr = row % T::ROWS;
-  const float2* ml = a.part_ml + (int64_t)first * T::ROWS + rr;
+  const int hi = blockIdx.x, b = blockIdx.y, G = a.H / c.Hkv, segs = c.Hkv * tiles;
+  const int h = MULTI ? hi / a.Q : hi, i = hi - h * a.Q, hk = h / G, row = (h - hk * G) * a.Q + i, rr = row % T::ROWS;
+  const int64_t each = units_each(a, T::UNIT, segs);
+  int64_t base = 0;
+  find_seq(a, T::UNIT, segs, -1, b, base);
+  const int n0 = common(a, b), units = units_of(n0, T::UNIT), seg = hk * tiles + row / T::ROWS;
+  const int64_t first = base + (int64_t)seg * units;
+  const int64_t w0 = div40(first, each);
+  const int n = (int)(div40(first + units - 1, each) - w0) + 1;
+  if (!MULTI && n == 1) return;
+  // the first workgroup's record is its second one unless the row tile begins its run
+  const int64_t rec0 = n == 1 ? whole_record(a, segs, b, seg) : 2 * w0 + (first != w0 * each);
+  auto record = [&](int p) { return (p ? 2 * (w0 + p) : rec0) * T::ROWS; };
+  const float2* ml = a.part_ml + rr;
   float m = -INFINITY;
-  for (int p = lane; p < pc.n; p += 64) m = fmaxf(m, ml[(int64_t)p * T::ROWS].x);
+  for (int p = lane; p < n; p += 64) m = fmaxf(m, ml[record(p)].x);
   m = wave_max_f32(m);
-  const float m0 = at_least(m);
-  float l = 0.f;
-  for (int p = lane; p < pc.n; p += 64) {
-    const float2 x = ml[(int64_t)p * T::ROWS];
+  float m0 = at_least(m), l = 0.f;
+  for (int p = lane; p < n; p += 64) {
+    const float2 x = ml[record(p)];
     l += x.y * exp_of(x.x - m0);
   }
 #pragma unroll
   for (int s = 32; s; s >>= 1) l += __shfl_xor(l, s, 64);
-  float y[D / 64];
+  float y[W];
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) y[e] = 0.f;
-  const float* part = a.part_o + ((int64_t)first * T::ROWS + rr / 16 * 16) * D;
-  for (int p = wave; p < pc.n; p += 4) {
-    const float f = exp_of(ml[(int64_t)p * T::ROWS].x - m0);
+  for (int e = 0; e < W; ++e) y[e] = 0.f;
+  const float* part = a.part_o + rr / 16 * 16 * D;
+  for (int p = wave; p < n; p += 4) {
+    const int64_t rec = record(p);
+    const float f = exp_of(ml[rec].x - m0);
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e)
-      y[e] += f * part[(int64_t)p * T::ROWS * D + part_index<T::VE>(rr % 16, lane * (D / 64) + e)];
+    for (int e = 0; e < W; ++e) y[e] += f * part[rec * D + part_index<T::VE>(rr % 16, lane * W + e)];
+  }
+  const int64_t row_out = ((int64_t)b * a.H + h) * a.Q + i;
+  if constexpr (MULTI) {
+    const int end = c.len(b) - (a.Q - 1 - i), l16 = lane & 15;
+    const int32_t* table = c.table + (int64_t)b * c.t_stride;
+    uint32_t q[T::VW];
+    load_words<T::VW>((int64_t)((const char*)a.q + (b * a.q_bs + h * a.q_hs + i * a.q_ts) * T::E + l16 * (T::VW * 4)), q);
+    for (int j0 = n0; j0 < end; j0 += TAIL) {
+      const int keys = min(end - j0, TAIL);
+      for (int t = tid / 16; t < keys; t += 16) {      // 16 lanes a key
+        const int page = c.page_of(table, j0 + t);
+        float dot = 0.f;
+        if (page >= 0) {
+          uint32_t k[T::VW];
+          load_words<T::VW>((int64_t)(c.k + page * c.k_ps + hk * c.k_hs + c.slot_of(j0 + t) * c.k_ss + l16 * (T::VW * 4)), k);
+#pragma unroll
+          for (int e = 0; e < T::VE; ++e) dot = fmaf(v_elem<DT>(q, e), v_elem<DT>(k, e), dot);
+        }
+#pragma unroll
+        for (int s = 8; s; s >>= 1) dot += __shfl_xor(dot, s, 64);
+        if (l16 == 0) {
+          const float s = page >= 0 ? dot * a.sm_scale : -INFINITY;
+          tail[t] = s;
+          tail_page[t] = page;
+          if (a.accumulate) a.scores[row_out * a.score_stride + j0 + t] = s;
+        }
+      }
+      __syncthreads();
+      float top = -INFINITY;
+      for (int t = lane; t < keys; t += 64) top = fmaxf(top, tail[t]);
+      top = fmaxf(wave_max_f32(top), m);
+      m0 = at_least(top);
+      const float f = exp_of(m - m0);
+      m = top;
+      float sum = 0.f;
+      for (int t = lane; t < keys; t += 64) sum += exp_of(tail[t] - m0);
+#pragma unroll
+      for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s, 64);
+      l = l * f + sum;
+#pragma unroll
+      for (int e = 0; e < W; ++e) y[e] *= f;
+      for (int t = wave; t < keys; t += 4) {
+        const int page = tail_page[t];
+        if (page < 0) continue;
+        const float p = exp_of(tail[t] - m0);
+        const char* v = c.v + page * c.v_ps + hk * c.v_hs + c.slot_of(j0 + t) * c.v_ss;
+#pragma unroll
+        for (int e = 0; e < W; ++e) y[e] = fmaf(p, load_scalar<DT>(v, lane * W + e), y[e]);
+      }
+      __syncthreads();
+    }
   }
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) o[wave][lane * (D / 64) + e] = y[e];
+  for (int e = 0; e < W; ++e) o[wave][lane * W + e] = y[e];
   __syncthreads();
-  const int64_t row_out = ((int64_t)b * a.H + h) * a.Q + i;
   if (tid < D) {
     const float z = l == 0.f ? 0.f : ((o[0][tid] + o[1][tid]) + (o[2][tid] + o[3][tid])) / l;
     char* out = (char*)a.out + (row_out * D + tid) * T::E;
@@ -479,31 +541,64 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
   if (tid == 0) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l);
 }
 
-// one thread per key and kv head: the p of its head's rows in order
+// The weights that a step's rows give the keys of a kv head: a workgroup takes 256 keys, its waves the rows in
+// turn, four keys a lane; the waves' sums are added in order.  Reads each score once.
 __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
+  constexpr int ROWS = 256;
+  __shared__ float lse[ROWS];
+  __shared__ floatx4 sums[4][64];
   const CacheView& c = a.c;
-  const int b = blockIdx.z, hk = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
+  const int b = blockIdx.z, hk = blockIdx.y, j0 = blockIdx.x * 256, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int len = c.len(b);
-  if (j >= len) return;
-  const int p = c.page_of(c.table + (int64_t)b * c.t_stride, j);
-  if (p < 0) return;
+  if (j0 >= len) return;
   const int rows = a.H / c.Hkv * a.Q;
   const int64_t row0 = ((int64_t)b * c.Hkv + hk) * rows;
-  float sum = 0.f;
-  for (int r = 0; r < rows; ++r) {
-    const float lse = a.lse[row0 + r];
-    if (j < len - (a.Q - 1 - r % a.Q) && lse != -INFINITY) sum += expf(a.scores[(row0 + r) * a.score_stride + j] - lse);
+  const int j = j0 + lane * 4;
+  const bool all = j0 + 256 <= common(a, b);           // every row sees every key
+  floatx4 sum = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int r0 = 0; r0 < rows; r0 += ROWS) {
+    const int n = min(rows - r0, ROWS);
+    __syncthreads();
+    // a row that saw nothing has lse -inf: 0 for every key
+    if (tid < n) lse[tid] = a.lse[row0 + r0 + tid];
+    __syncthreads();
+    const float* s = a.scores + (row0 + r0) * a.score_stride + j;
+    if (all) {
+#pragma unroll 4
+      for (int r = wave; r < n; r += 4) {
+        const floatx4 x = *(const floatx4*)(s + r * a.score_stride);
+        const float z = lse[r];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += z == -INFINITY ? 0.f : exp_of(x[e] - z);
+      }
+    } else {
+      for (int r = wave; r < n; r += 4) {
+        const int end = len - (a.Q - 1 - (r0 + r) % a.Q);
+        if (j >= end) continue;                        // beyond: not written
+        const floatx4 x = *(const floatx4*)(s + r * a.score_stride);
+        const float z = lse[r];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += j + e >= end || z == -INFINITY ? 0.f : exp_of(x[e] - z);
+      }
+    }
   }
-  c.weight[p * c.w_ps + hk * c.w_hs + c.slot_of(j)] += sum;
+  sums[wave][lane] = sum;
+  __syncthreads();
+  const int mine = j0 + tid;
+  if (mine >= len) return;
+  const int p = c.page_of(c.table + (int64_t)b * c.t_stride, mine);
+  if (p < 0) return;
+  const float* w = (const float*)sums;
+  c.weight[p * c.w_ps + hk * c.w_hs + c.slot_of(mine)] += (w[tid] + w[256 + tid]) + (w[512 + tid] + w[768 + tid]);
 }
 
-template <int DT, int D, int NT>
+template <int DT, int D, int NT, bool MULTI>
 hipError_t launch_attend(const PagedArgs& a, const PagedCut& cut, hipStream_t st) {
-  if (a.accumulate) paged_attend_kernel<DT, D, NT, true><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
-  else paged_attend_kernel<DT, D, NT, false><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
+  if (a.accumulate) paged_attend_kernel<DT, D, NT, true, MULTI><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
+  else paged_attend_kernel<DT, D, NT, false, MULTI><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && !cut.single) {
-    paged_join_kernel<DT, D, NT><<<dim3(a.H * a.Q, a.c.B), 256, 0, st>>>(a, cut.tiles);
+    paged_join_kernel<DT, D, NT, MULTI><<<dim3(a.H * a.Q, a.c.B), 256, 0, st>>>(a, cut.tiles);
     e = hipGetLastError();
   }
   if (e != hipSuccess || !a.accumulate) return e;
@@ -513,7 +608,8 @@ hipError_t launch_attend(const PagedArgs& a, const PagedCut& cut, hipStream_t st
 
 template <int DT, int D>
 hipError_t launch_rows(const PagedArgs& a, const PagedCut& cut, hipStream_t st) {
-  return cut.rows == 16 ? launch_attend<DT, D, 1>(a, cut, st) : launch_attend<DT, D, 2>(a, cut, st);
+  if (cut.rows == 32) return a.Q == 1 ? launch_attend<DT, D, 2, false>(a, cut, st) : launch_attend<DT, D, 2, true>(a, cut, st);
+  return a.Q == 1 ? launch_attend<DT, D, 1, false>(a, cut, st) : launch_attend<DT, D, 1, true>(a, cut, st);
 }
 
 }  // namespace
@@ -525,21 +621,23 @@ hipError_t launch_append(const AppendArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-PagedCut paged_cut(int dtype, int H, int Hkv, int Q, int B, int cap) {
+PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap) {
   PagedCut cut;
   const int R = H / Hkv * Q;
   cut.rows = R > 16 ? 32 : 16;
   cut.tiles = (R + cut.rows - 1) / cut.rows;
-  cut.unit = dtype == STA_DTYPE_F32 ? Tile<DT_F32, 64, 1>::UNIT : Tile<DT_BF16, 64, 1>::UNIT;
-  const int64_t segs = (int64_t)Hkv * cut.tiles * B, most = (cap + cut.unit - 1) / cut.unit;
-  cut.single = most <= 1;
-  const int64_t all = segs * most, some = segs + PIECES;
-  cut.grid = (int)(all < some ? all : some);
+  const int unit = dtype == STA_DTYPE_F32 ? Tile<DT_F32, 64, 1>::UNIT : Tile<DT_BF16, 64, 1>::UNIT;
+  const int waves = cut.rows == 32 ? 2 : (D == 64 ? Tile<DT_BF16, 64, 1>::WAVES : Tile<DT_BF16, 128, 1>::WAVES);
+  const int64_t most = cap <= unit ? 1 : (cap + unit - 1) / unit;
+  const int64_t all = (int64_t)Hkv * cut.tiles * B * most;
+  cut.grid = (int)(all < 256 * waves ? all : 256 * waves);
+  cut.single = most == 1 && Q == 1;
+  cut.records = cut.single ? 0 : 2 * (int64_t)cut.grid + (Q > 1 ? (int64_t)Hkv * cut.tiles * B : 0);
   return cut;
 }
 
 hipError_t launch_paged(int dtype, int D, const PagedArgs& a, hipStream_t st) {
-  const PagedCut cut = paged_cut(dtype, a.H, a.c.Hkv, a.Q, a.c.B, a.c.cap);
+  const PagedCut cut = paged_cut(dtype, D, a.H, a.c.Hkv, a.Q, a.c.B, a.c.cap);
   if (dtype == STA_DTYPE_F32) return D == 64 ? launch_rows<DT_F32, 64>(a, cut, st) : launch_rows<DT_F32, 128>(a, cut, st);
   if (dtype == STA_DTYPE_BF16) return D == 64 ? launch_rows<DT_BF16, 64>(a, cut, st) : launch_rows<DT_BF16, 128>(a, cut, st);
   return D == 64 ? launch_rows<DT_F16, 64>(a, cut, st) : launch_rows<DT_F16, 128>(a, cut, st);
