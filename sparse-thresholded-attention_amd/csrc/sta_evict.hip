@@ -3,7 +3,7 @@
 // Every kv head of a sequence keeps m = min(len, budget) keys.  A key's rank is one 32-bit word,
 // larger first: all ones for a forced key (pos < n_global or pos > largest pos - n_local), else
 // its weight's bits in an order-preserving form (NaN above +inf, -0 as +0), 0 for a key without a
-// page.  The m-th largest word T comes from four counting passes over its bytes; a key stays if
+// page.  The m-th largest word T comes from three counting passes over 11, 11 and 10 bits; a key stays if
 // its word is above T, or equal to T and among the first of those by slot.
 //
 // The kept keys need no order in a cache that stores rotated keys, so in place only the kept keys
@@ -17,6 +17,10 @@ namespace sta {
 namespace {
 
 constexpr int SEL_T = 1024;
+constexpr int BINS = 2048;             // of a counting pass
+constexpr int PER = 8;                 // consecutive keys of a thread
+constexpr int LDS_KEYS = 32768;        // 128 KB of words
+constexpr int INLINE_MOVES = 64;       // rows a head that the selecting workgroup moves itself
 constexpr uint32_t FORCED = 0xffffffffu;
 
 __device__ __forceinline__ uint32_t weight_word(float w) {
@@ -25,115 +29,32 @@ __device__ __forceinline__ uint32_t weight_word(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// exclusive prefix and total of two flags over the workgroup; lds: 2 * 16 words
-struct Ranks { int a, b, total_a, total_b; };
-__device__ __forceinline__ Ranks rank_flags(bool fa, bool fb, int (*lds)[SEL_T / 64]) {
-  const int wave = threadIdx.x >> 6;
-  const unsigned long long ma = __ballot(fa), mb = __ballot(fb);
-  const unsigned long long below = (1ull << (threadIdx.x & 63)) - 1;
+// exclusive prefix sum over the workgroup and its total; lds: SEL_T / 64 words, free on return
+__device__ __forceinline__ int block_prefix(int x, int* lds, int& total) {
+  const int wave = threadIdx.x >> 6, incl = wave_incl_sum(x);
+  if ((threadIdx.x & 63) == 63) lds[wave] = incl;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    lds[0][wave] = __popcll(ma);
-    lds[1][wave] = __popcll(mb);
-  }
-  __syncthreads();
-  Ranks r{(int)__popcll(ma & below), (int)__popcll(mb & below), 0, 0};
-  for (int w = 0; w < SEL_T / 64; ++w) {
-    if (w < wave) r.a += lds[0][w], r.b += lds[1][w];
-    r.total_a += lds[0][w];
-    r.total_b += lds[1][w];
-  }
-  return r;
-}
-
-__global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
-  __shared__ int hist[256], scan[2][SEL_T / 64], pick[2];
-  __shared__ int wave_max[SEL_T / 64];
-  const CacheView& c = a.c;
-  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int len = c.len(b), m = min(len, a.budget);
-  const int seg = b * c.Hkv + hk;
-  if (hk == 0 && tid == 0) a.new_lens[b] = m;
-  const bool in_place = a.dst_table == nullptr;
-  if (m == 0 || (in_place && len <= a.budget)) {
-    if (tid == 0) a.counts[seg] = 0;
-    return;
-  }
-  const int32_t* table = c.table + (int64_t)b * c.t_stride;
-  int last = INT32_MIN;
-  for (int j = tid; j < len; j += SEL_T) {
-    const int p = c.page_of(table, j);
-    if (p >= 0) last = max(last, c.pos[p * c.p_ps + hk * c.p_hs + c.slot_of(j)]);
-  }
+  int before = 0;
+  total = 0;
 #pragma unroll
-  for (int x = 32; x; x >>= 1) last = max(last, __shfl_xor(last, x, 64));
-  if ((tid & 63) == 0) wave_max[tid >> 6] = last;
+  for (int w = 0; w < SEL_T / 64; ++w) {
+    const int t = lds[w];
+    if (w < wave) before += t;
+    total += t;
+  }
   __syncthreads();
-  for (int w = 0; w < SEL_T / 64; ++w) last = max(last, wave_max[w]);
-  const int64_t local = (int64_t)last - a.n_local;
-
-  auto word = [&](int j) -> uint32_t {
-    const int p = c.page_of(table, j);
-    if (p < 0) return 0u;
-    const int s = c.slot_of(j);
-    const int pos = c.pos[p * c.p_ps + hk * c.p_hs + s];
-    if (pos < a.n_global || pos > local) return FORCED;
-    return weight_word(c.weight[p * c.w_ps + hk * c.w_hs + s]);
-  };
-
-  // the m-th largest word, byte by byte; `left` of the words that share its bytes so far stay
-  uint32_t T = 0;
-  int left = m;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += SEL_T) hist[i] = 0;
-    __syncthreads();
-    for (int j = tid; j < len; j += SEL_T) {
-      const uint32_t w = word(j);
-      if (shift == 24 || (w >> (shift + 8)) == (T >> (shift + 8))) atomicAdd(&hist[(w >> shift) & 255], 1);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int above = 0, d = 255;
-      while (d > 0 && above + hist[d] < left) above += hist[d--];
-      pick[0] = d;
-      pick[1] = left - above;
-    }
-    __syncthreads();
-    T |= (uint32_t)pick[0] << shift;
-    left = pick[1];
-    __syncthreads();
-  }
-
-  int ties = 0, n_from = 0, n_to = 0;
-  int32_t* from = a.from + (int64_t)seg * a.moves;
-  int32_t* to = a.to + (int64_t)seg * a.moves;
-  for (int j0 = 0; j0 < len; j0 += SEL_T) {
-    const int j = j0 + tid;
-    const uint32_t w = j < len ? word(j) : 0u;
-    const bool tie = j < len && w == T;
-    const Ranks rt = rank_flags(tie, false, scan);
-    const bool keep = j < len && (w > T || (tie && ties + rt.a < left));
-    ties += rt.total_a;
-    const bool src = keep && (!in_place || j >= m), dst = in_place && !keep && j < m;
-    const Ranks r = rank_flags(src, dst, scan);
-    if (src && n_from + r.a < a.moves) from[n_from + r.a] = j;
-    if (dst && n_to + r.b < a.moves) to[n_to + r.b] = j;
-    n_from += r.total_a;
-    n_to += r.total_b;
-  }
-  if (tid == 0) a.counts[seg] = min(n_from, a.moves);
+  return before + incl - x;
 }
 
-// one group of row_bytes / 16 lanes moves a row's key and value
-__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
+// A row's worth of lanes moves a key's row and its value's, r-th of n, with weight and pos.
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int hk, int b, int n, int r0, int step, int tid) {
   const CacheView& c = a.c;
-  const int hk = blockIdx.y, b = blockIdx.z, chunks = a.row_bytes / 16;
-  const int seg = b * c.Hkv + hk, n = a.counts[seg];
-  const int per = 256 / chunks, at = threadIdx.x % chunks * 16;
+  const int chunks = a.row_bytes / 16, at = tid % chunks * 16;
+  const int64_t list = (int64_t)(b * c.Hkv + hk) * a.moves;
   const int32_t* table = c.table + (int64_t)b * c.t_stride;
   const int32_t* out_table = a.dst_table ? a.dst_table + (int64_t)b * a.dst_stride : table;
-  for (int r = blockIdx.x * per + threadIdx.x / chunks; r < n; r += gridDim.x * per) {
-    const int j = a.from[(int64_t)seg * a.moves + r], i = a.dst_table ? r : a.to[(int64_t)seg * a.moves + r];
+  for (int r = r0 + tid / chunks; r < n; r += step) {
+    const int j = a.from[list + r], i = a.dst_table ? r : a.to[list + r];
     if (a.dst_table && i >= a.dst_cap) break;
     const int p = c.page_of(table, j), g = c.page_of(out_table, i);
     if (p < 0 || g < 0) continue;
@@ -149,12 +70,158 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
   }
 }
 
+// One workgroup per sequence and kv head.  IN_LDS: the words stay in LDS (calls of at most LDS_KEYS keys); else each
+// pass reads weight and pos again.  INLINE: the few rows that can move are moved here.
+template <bool IN_LDS, bool INLINE>
+__global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
+  extern __shared__ uint32_t words[];
+  __shared__ int hist[BINS], scan[SEL_T / 64], pick[2];
+  const CacheView& c = a.c;
+  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int len = c.len(b), m = min(len, a.budget);
+  const int seg = b * c.Hkv + hk;
+  if (hk == 0 && tid == 0) a.new_lens[b] = m;
+  const bool in_place = a.dst_table == nullptr;
+  if (m == 0 || (in_place && len <= a.budget)) {
+    if (tid == 0) a.counts[seg] = 0;
+    return;
+  }
+  const int32_t* table = c.table + (int64_t)b * c.t_stride;
+  const float* weight = c.weight + hk * c.w_hs;
+  const int32_t* posp = c.pos + hk * c.p_hs;
+  for (int i = tid; i < BINS; i += SEL_T) hist[i] = 0;
+  int last = INT32_MIN;
+#pragma unroll 4
+  for (int j = tid; j < len; j += SEL_T) {
+    const int p = c.page_of(table, j);
+    if (p >= 0) last = max(last, posp[p * c.p_ps + c.slot_of(j)]);
+  }
+#pragma unroll
+  for (int x = 32; x; x >>= 1) last = max(last, __shfl_xor(last, x, 64));
+  if ((tid & 63) == 0) scan[tid >> 6] = last;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < SEL_T / 64; ++w) last = max(last, scan[w]);
+  const int64_t local = (int64_t)last - a.n_local;
+
+  auto fresh = [&](int j) -> uint32_t {
+    const int p = c.page_of(table, j);
+    if (p < 0) return 0u;
+    const int s = c.slot_of(j);
+    const int pos = posp[p * c.p_ps + s];
+    const float w = weight[p * c.w_ps + s];
+    return pos < a.n_global || pos > local ? FORCED : weight_word(w);
+  };
+  auto word = [&](int j) { return IN_LDS ? words[j] : fresh(j); };
+
+  // the m-th largest word, 11 bits and then twice their rest; `left` of the words equal to it stay
+  uint32_t T = 0;
+  int left = m;
+  for (int shift = 21, bits = 11; shift >= 0; bits = shift == 10 ? 10 : 11, shift -= bits) {
+#pragma unroll 4
+    for (int j = tid; j < len; j += SEL_T) {
+      uint32_t w;
+      if (shift == 21) {
+        w = fresh(j);
+        if (IN_LDS) words[j] = w;
+      } else {
+        w = word(j);
+        if (w >> (shift + bits) != T >> (shift + bits)) continue;
+      }
+      atomicAdd(&hist[(w >> shift) & ((1u << bits) - 1)], 1);
+    }
+    __syncthreads();
+    // the bins from the top, BINS / SEL_T a thread: the one in which the left-th word lies
+    int mine[BINS / SEL_T], sum = 0, total;
+#pragma unroll
+    for (int i = 0; i < BINS / SEL_T; ++i) {
+      mine[i] = hist[BINS - 1 - (tid * (BINS / SEL_T) + i)];
+      sum += mine[i];
+    }
+    int above = block_prefix(sum, scan, total);
+#pragma unroll
+    for (int i = 0; i < BINS / SEL_T; ++i) {
+      const int d = BINS - 1 - (tid * (BINS / SEL_T) + i);
+      if (above < left && above + mine[i] >= left) {
+        pick[0] = d;
+        pick[1] = left - above;
+      }
+      above += mine[i];
+      hist[d] = 0;
+    }
+    __syncthreads();
+    T |= (uint32_t)pick[0] << shift;
+    left = pick[1];
+    __syncthreads();
+  }
+
+  // who stays, in the order of the slots, PER consecutive ones a thread
+  int ties = 0, n_from = 0, n_to = 0;
+  int32_t* from = a.from + (int64_t)seg * a.moves;
+  int32_t* to = a.to + (int64_t)seg * a.moves;
+  for (int j0 = 0; j0 < len; j0 += SEL_T * PER) {
+    const int j = j0 + tid * PER;
+    uint32_t above = 0, equal = 0;                     // a bit a key
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const uint32_t w = j + i < len ? word(j + i) : 0u;
+      above |= (uint32_t)(j + i < len && w > T) << i;
+      equal |= (uint32_t)(j + i < len && w == T) << i;
+    }
+    int total;
+    int rank = ties + block_prefix(__popc(equal), scan, total);
+    ties += total;
+    uint32_t keep = above;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (equal >> i & 1) keep |= (uint32_t)(rank++ < left) << i;
+    // slots of this thread's keys in front of m
+    const int front = min(max(m - j, 0), PER);
+    const uint32_t before = (1u << front) - 1;
+    const uint32_t src = in_place ? keep & ~before : keep, dst = in_place ? ~keep & before : 0u;
+    int at = n_from + block_prefix(__popc(src), scan, total);
+    n_from += total;
+    for (uint32_t x = src; x; x &= x - 1, ++at)
+      if (at < a.moves) from[at] = j + __ffs(x) - 1;
+    if (in_place) {
+      at = n_to + block_prefix(__popc(dst), scan, total);
+      n_to += total;
+      for (uint32_t x = dst; x; x &= x - 1, ++at)
+        if (at < a.moves) to[at] = j + __ffs(x) - 1;
+    }
+  }
+  n_from = min(n_from, a.moves);
+  if (INLINE) {
+    __threadfence_block();
+    __syncthreads();
+    move_rows(a, hk, b, n_from, 0, SEL_T / (a.row_bytes / 16), tid);
+  } else if (tid == 0) {
+    a.counts[seg] = n_from;
+  }
+}
+
+__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
+  const int hk = blockIdx.y, b = blockIdx.z, per = 256 / (a.row_bytes / 16);
+  move_rows(a, hk, b, a.counts[b * a.c.Hkv + hk], blockIdx.x * per, gridDim.x * per, threadIdx.x);
+}
+
+template <bool IN_LDS, bool INLINE>
+hipError_t launch_select(const EvictArgs& a, size_t lds, hipStream_t st) {
+  hipError_t e = hipFuncSetAttribute((const void*)evict_select_kernel<IN_LDS, INLINE>,
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (e != hipSuccess) return e;
+  evict_select_kernel<IN_LDS, INLINE><<<dim3(a.c.Hkv, a.c.B), SEL_T, lds, st>>>(a);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_evict(const EvictArgs& a, hipStream_t st) {
-  evict_select_kernel<<<dim3(a.c.Hkv, a.c.B), SEL_T, 0, st>>>(a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.moves == 0) return e;
+  const bool in_lds = a.c.cap <= LDS_KEYS, few = a.moves <= INLINE_MOVES;
+  const size_t lds = in_lds ? (size_t)a.c.cap * 4 : 0;
+  hipError_t e = in_lds ? (few ? launch_select<true, true>(a, lds, st) : launch_select<true, false>(a, lds, st))
+                        : (few ? launch_select<false, true>(a, lds, st) : launch_select<false, false>(a, lds, st));
+  if (e != hipSuccess || few) return e;
   const int per = 256 / (a.row_bytes / 16);
   const int blocks = (a.moves + per - 1) / per;
   evict_move_kernel<<<dim3(blocks < 64 ? blocks : 64, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
