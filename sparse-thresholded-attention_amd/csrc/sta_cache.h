@@ -62,7 +62,7 @@ struct PagedArgs {
 // one kv head, `tiles` of them a kv head
 struct PagedCut {
   int rows, tiles, grid;
-  bool single;                      // no sequence has two units and one query each: nothing to join
+  bool small;                       // short sequences, one query each: one launch, nothing to join
   int64_t records;                  // of unfinished row tiles, in the workspace
 };
 PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap);

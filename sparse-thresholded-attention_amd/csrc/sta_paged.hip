@@ -64,13 +64,12 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 //
 //   S^T = K Q^T     K rows as operand A (lane: key l % 16, 16 bytes of its row), Q rows as B; the
 //                   result holds row l % 16, keys 4 (l / 16) + i in slot i
-//   O^T += V^T P^T  with the fp32 instruction of depth 4: slot i of P is, as it stands, operand B for
-//                   the keys 4 (l / 16) + i, and lane l loads 1/16 of the V row of that key, whose
-//                   elements e are operand A of the dims (l % 16) * VE + e
+//   O^T += V^T P^T  slots 4 (l / 16) + i of both subtiles are, as they stand, the eight contraction elements of
+//                   operand B, and lane l loads 1/16 of the V rows of those keys, whose elements e are operand
+//                   A of the dims (l % 16) * VE + e
 //
-// so neither P nor V moves between lanes, P is never rounded, and V's 16-bit elements are only
-// widened.  The fp32 instruction runs at 1/16 of the 16-bit rate and still needs a quarter of the time
-// that a CU's share of the memory bandwidth takes for K and V with one tile of rows.
+// so neither P nor V moves between lanes.  P goes in two 16-bit parts, P = hi + lo within 2^-17 of itself, two
+// instructions for each; fp32 caches use the fp32 instruction of depth 4, whose operands P and V are as well.
 //
 // Work.  The sequences' lengths are known to the device alone, and differ.  Every wave sums their units (of
 // 4 KT keys; an empty sequence counts one, which writes its zeros) over all row tiles, and the call's
@@ -137,6 +136,13 @@ __device__ __forceinline__ int64_t whole_record(const PagedArgs& a, int segs, in
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 __device__ __forceinline__ float at_least(float m) { return m == -INFINITY ? 0.f : m; }   // what p is relative to
 
+// waves of a workgroup in a call of short sequences: four a SIMD where a wave gets by with 128 registers
+template <int D, int NT>
+constexpr int SMALL_WAVES = D == 64 && NT == 1 ? 16 : 8;
+// Up to this bound on the lengths (32q / 8kv heads x 128, bf16, one sequence / 32 of them): at 1000 keys 16.0 / 16.2 us in
+// one launch, 18.5 / 19.7 split and joined; at 2000 keys 22.2 / 23.7 and 18.1 / 25.2, at 4000 40.2 / 41.9 and 18.4 / 31.5.
+constexpr int SMALL_KEYS = 1024;
+
 __device__ const u32x4 zero_row[32] = {};              // 512 bytes: a row of 128 fp32 elements
 
 template <int DT, int D, int NT_>
@@ -149,9 +155,11 @@ struct Tile {
   static constexpr int VE = D / 16;                    // V elements of a lane
   static constexpr int VW = VE * E / 4;                // their words
   static constexpr int NT = NT_, ROWS = 16 * NT;
+  // P is below 1: times 2^14 its fp16 halves stay clear of the subnormal range down to 2^-28
+  static constexpr float P_SCALE = DT == DT_F16 ? 16384.f : 1.f;
   // Waves of a SIMD, and so workgroups of a CU (256 a grid and wave): what the registers hold without spills.
-  // Three at D = 64 (bf16, 32q / 8kv heads: 37 us, with two 41), two at D = 128 (the other way round: 146 us
-  // for 190 MB of keys and as much of values, with three 166, most of the loss from spilled accumulators).
+  // Three at D = 64 (bf16, 32q / 8kv heads, up to 8192 keys: 37 us, with two 41), two at D = 128 (two sequences of up
+  // to 131072 keys: 146 us, with three 166: spilled accumulators).
   static constexpr int WAVES = D == 64 && NT == 1 ? 3 : 2;
 };
 
@@ -169,12 +177,17 @@ __device__ __forceinline__ floatx4 mfma_qk(u32x4 k, u32x4 q, floatx4 s) {
   }
 }
 
+// the low or high 16-bit element of a word, in fp32
+template <int DT>
+__device__ __forceinline__ float half_of(uint32_t w, int high) {
+  if constexpr (DT == DT_BF16) return __uint_as_float(high ? w & 0xffff0000u : w << 16);
+  else return f16_bits_to_f32(high ? w >> 16 : w & 0xffffu);
+}
 // element e of a lane's share of a V row, in fp32
 template <int DT>
 __device__ __forceinline__ float v_elem(const uint32_t* w, int e) {
   if constexpr (DT == DT_F32) return __uint_as_float(w[e]);
-  else if constexpr (DT == DT_BF16) return e & 1 ? __uint_as_float(w[e / 2] & 0xffff0000u) : __uint_as_float(w[e / 2] << 16);
-  else return f16_bits_to_f32(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu);
+  else return half_of<DT>(w[e / 2], e & 1);
 }
 
 // loads at an address in global memory (one that went through a lane exchange is no pointer to the compiler)
@@ -202,54 +215,39 @@ __device__ __forceinline__ int part_index(int row, int dim) {
   return ((e * 4 + m / 4) * 16 + row) * 4 + m % 4;
 }
 
-template <int DT>
-__device__ __forceinline__ void store_out(char* out, const float* y, int n) {   // n = 4 or 8
+template <int DT, int N>
+__device__ __forceinline__ void store_out(char* out, const float* y) {   // N = 4 or 8
   if constexpr (DT == DT_F32) {
-    for (int e = 0; e < n; e += 4) *(float4*)(out + 4 * e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+#pragma unroll
+    for (int e = 0; e < N; e += 4) *(float4*)(out + 4 * e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+  } else if constexpr (N == 8) {
+    *(u32x4*)out = u32x4{pack2_dt<DT>(y[0], y[1]), pack2_dt<DT>(y[2], y[3]), pack2_dt<DT>(y[4], y[5]), pack2_dt<DT>(y[6], y[7])};
   } else {
-    u32x4 w;
-    for (int e = 0; e < n; e += 2) w[e / 2] = pack2_dt<DT>(y[e], y[e + 1]);
-    if (n == 8) *(u32x4*)out = w;
-    else *(u32x2*)out = u32x2{w[0], w[1]};
+    *(u32x2*)out = u32x2{pack2_dt<DT>(y[0], y[1]), pack2_dt<DT>(y[2], y[3])};
   }
 }
 
+template <int D, int NT, int VE>
+struct MergeLds {
+  floatx4 acc[4][VE * 4 * 16];
+  float m[16][16 * NT], l[16][16 * NT], sum[16 * NT], lse[16 * NT];
+};
+
+// A workgroup of NW waves takes the units u0 .. u1 - 1 of a row tile: out and lse where that is all of it
+// (done), else a record.
 // MULTI: a.Q may exceed 1.  Then len stands for the keys that all queries see and every row tile is joined:
 // paged_join_kernel adds the last Q - 1 keys, of which each query sees others, row by row, so that the rows
 // of an instruction always see the same keys (0 times a NaN or an infinity would reach rows that do not
 // see its key).
-template <int DT, int D, int NT, bool ACC, bool MULTI>
-__global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_kernel(PagedArgs a, int tiles) {
+template <int DT, int D, int NT, bool ACC, bool MULTI, int NW>
+__device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, D / 16>& lds, int b, int len, int hk,
+                                            int row0, int u0, int u1, bool done, int64_t record) {
   using T = Tile<DT, D, NT>;
   constexpr int KS = T::KS, VE = T::VE, VW = T::VW, SUB = T::SUB, KT = T::KT;
-  __shared__ floatx4 merge[4][VE * 4 * 16];
-  __shared__ float merge_m[4][T::ROWS], merge_l[4][T::ROWS], merge_sum[T::ROWS];
   const CacheView& c = a.c;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int r = lane & 15, g4 = lane >> 4;
-  const int segs = c.Hkv * tiles, G = a.H / c.Hkv, R = G * a.Q;
-  const int64_t each = units_each(a, T::UNIT, segs);
-  const int64_t run0 = blockIdx.x * each, run1 = run0 + each;
-  int64_t base = 0;
-  int b = find_seq(a, T::UNIT, segs, run0, -1, base);
-  if (b < 0) return;
-  int len = uniform(common(a, b)), units = units_of(len, T::UNIT);
-  int seg = uniform(div40(run0 - base, units));
-  for (int64_t at = run0; at < run1;) {
-    if (seg == segs) {
-      if (++b == c.B) return;
-      base = at;
-      seg = 0;
-      len = uniform(common(a, b));
-      units = units_of(len, T::UNIT);
-    }
-    const int64_t first = base + (int64_t)seg * units;
-    const int u0 = (int)(at - first), u1 = (int)min((int64_t)units, run1 - first);
-    const bool whole_tile = u1 - u0 == units, done = !MULTI && whole_tile;
-    const int64_t record = whole_tile ? whole_record(a, segs, b, seg) : 2 * (int64_t)blockIdx.x + (at != run0);
-    at = first + u1;
-    const int hk = tiles == 1 ? seg : seg / tiles, row0 = (seg - hk * tiles) * T::ROWS;
-    ++seg;
+  const int G = a.H / c.Hkv, R = G * a.Q;
 
   u32x4 q[NT][KS];
   int64_t srow[NT];
@@ -269,29 +267,21 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
 
   floatx4 acc[NT][VE];
   float m[NT], l[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    m[t] = -INFINITY;
-    l[t] = 0.f;
-#pragma unroll
-    for (int e = 0; e < VE; ++e) acc[t][e] = floatx4{0.f, 0.f, 0.f, 0.f};
-  }
-
   const int32_t* table = c.table + (int64_t)b * c.t_stride;
-  // The table entry of the lane's key of a turn, lane % KT, and whether that key exists.  The entry is
-  // loaded two turns ahead and judged one turn later, so that no turn waits for it.
+  // A turn's rows: lane l knows those of key l % KT, and the others ask it.  The table entry is loaded two turns
+  // ahead, K one turn, V at its turn's beginning.  The last turn, which loads nothing for a next one, is a copy of
+  // its own: past a branch that may skip loads the compiler would wait for all loads in flight.
   const int last = max(len - 1, 0) >> c.shift;
-  auto entry_at = [&](int u) { return table[min(((u * 4 + wave) * KT + (lane & (KT - 1))) >> c.shift, last)]; };
-  auto page_at = [&](int u, int entry) {
-    return (u * 4 + wave) * KT + (lane & (KT - 1)) < len && (unsigned)entry < (unsigned)c.pages ? entry : -1;
+  auto entry_at = [&](int u) { return table[min(((u * NW + wave) * KT + (lane & (KT - 1))) >> c.shift, last)]; };
+  int64_t krow, vrow;                                  // a key that does not exist is a row of zeros
+  auto rows_of = [&](int u, int entry) {               // and which keys exist; lanes beyond KT repeat the first ones
+    const int j = (u * NW + wave) * KT + (lane & (KT - 1)), slot = c.slot_of(j);
+    const bool is = j < len && (unsigned)entry < (unsigned)c.pages;
+    krow = (int64_t)(is ? c.k + hk * c.k_hs + entry * c.k_ps + slot * c.k_ss : (const char*)zero_row);
+    vrow = (int64_t)(is ? c.v + hk * c.v_hs + entry * c.v_ps + slot * c.v_ss : (const char*)zero_row);
+    return (uint32_t)__ballot(is);
   };
   u32x4 k[SUB][KS];
-  int64_t krow, vrow;                                  // addresses of the lane's key; a key that does not exist is a row of zeros
-  auto rows_of = [&](int u, int page) {
-    const int slot = c.slot_of((u * 4 + wave) * KT + (lane & (KT - 1)));
-    krow = (int64_t)(page < 0 ? (const char*)zero_row : c.k + hk * c.k_hs + page * c.k_ps + slot * c.k_ss);
-    vrow = (int64_t)(page < 0 ? (const char*)zero_row : c.v + hk * c.v_hs + page * c.v_ps + slot * c.v_ss);
-  };
   auto load_k = [&]() {
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
@@ -300,19 +290,17 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
       for (int i = 0; i < KS; ++i) k[s][i] = *(global4)(p + i * 64);
     }
   };
-  int page = page_at(u0, entry_at(u0)), next_entry = entry_at(u0 + 1);
-  rows_of(u0, page);
-  load_k();
-  for (int u = u0; u < u1; ++u) {
-    const int key0 = (u * 4 + wave) * KT;
-    const uint32_t there = (uint32_t)__ballot(page >= 0);  // lanes beyond KT repeat the first ones
+  int next_entry;
+  uint32_t there;
+  // EXACT: P.V in fp32 throughout
+  auto turn = [&](int u, auto last_turn, auto exact) {
+    constexpr bool LAST = decltype(last_turn)::value, EXACT = decltype(exact)::value;
     uint32_t v[SUB][4][VW];
 #pragma unroll
     for (int s = 0; s < SUB; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) 
+      for (int i = 0; i < 4; ++i)
         load_words<VW>(__shfl(vrow, s * 16 + g4 * 4 + i, 64) + r * (VW * 4), v[s][i]);
-
     floatx4 sc[NT][SUB];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -321,15 +309,9 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
         floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < KS; ++i) x = mfma_qk<DT>(k[s][i], q[t][i], x);
-        sc[t][s] = x * a.sm_scale;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[t][s][i] = x[i] * a.sm_scale;
       }
-    if (u + 1 < u1) {
-      page = page_at(u + 1, next_entry);
-      next_entry = entry_at(u + 2);
-      rows_of(u + 1, page);
-      load_k();
-    }
-
     if (there != ~0u) {
 #pragma unroll
       for (int s = 0; s < SUB; ++s)
@@ -339,12 +321,22 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
           for (int t = 0; t < NT; ++t)
             if (!(there >> (g4 * 4) & 1u << (s * 16 + i))) sc[t][s][i] = -INFINITY;
     }
+    if (ACC && (u * NW + wave) * KT < len) {           // a turn that begins in the sequence ends in its score rows
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        if (srow[t] >= 0) {
+#pragma unroll
+          for (int s = 0; s < SUB; ++s)
+            *(floatx4*)(a.scores + srow[t] + (u * NW + wave) * KT + s * 16) = sc[t][s];
+        }
+    }
+    if (!LAST) {
+      there = rows_of(u + 1, next_entry);
+      load_k();
+      next_entry = entry_at(u + 2);
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      if (ACC && srow[t] >= 0) {
-#pragma unroll
-        for (int s = 0; s < SUB; ++s) *(floatx4*)(a.scores + srow[t] + key0 + s * 16) = sc[t][s];
-      }
       float top = fmaxf(fmaxf(sc[t][0][0], sc[t][0][1]), fmaxf(sc[t][0][2], sc[t][0][3]));
       if (SUB == 2) top = fmaxf(top, fmaxf(fmaxf(sc[t][SUB - 1][0], sc[t][SUB - 1][1]), fmaxf(sc[t][SUB - 1][2], sc[t][SUB - 1][3])));
       top = fmaxf(top, __shfl_xor(top, 16, 64));
@@ -361,76 +353,198 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
       for (int s = 0; s < SUB; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = exp_of(sc[t][s][i] - m0);
+          const float p = T::P_SCALE * exp_of(sc[t][s][i] - m0);
           sc[t][s][i] = p;
           l[t] += p;
         }
     }
+    if constexpr (EXACT) {
 #pragma unroll
-    for (int s = 0; s < SUB; ++s)
+      for (int s = 0; s < SUB; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-    #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const float ve = v_elem<DT>(v[s][i], e);
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
-            acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(ve, sc[t][s][i], acc[t][e], 0, 0, 0);
+          for (int e = 0; e < VE; ++e) {
+            const float ve = v_elem<DT>(v[s][i], e);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(ve, sc[t][s][i], acc[t][e], 0, 0, 0);
+          }
+    } else {
+      u32x4 hi[NT], lo[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float p0 = sc[t][x / 2][x % 2 * 2], p1 = sc[t][x / 2][x % 2 * 2 + 1];
+          hi[t][x] = pack2_dt<DT>(p0, p1);
+          lo[t][x] = pack2_dt<DT>(p0 - half_of<DT>(hi[t][x], 0), p1 - half_of<DT>(hi[t][x], 1));
+        }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        u32x4 ve;                                      // element e of the lane's eight keys
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          ve[x] = __builtin_amdgcn_perm(v[x / 2][x % 2 * 2 + 1][e / 2], v[x / 2][x % 2 * 2][e / 2],
+                                        e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          acc[t][e] = mfma_qk<DT>(ve, hi[t], acc[t][e]);
+          acc[t][e] = mfma_qk<DT>(ve, lo[t], acc[t][e]);
         }
       }
+    }
+  };
+  auto sweep = [&](auto exact) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t] = -INFINITY;
+      l[t] = 0.f;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[t][e] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    there = rows_of(u0, entry_at(u0));
+    next_entry = entry_at(u0 + 1);
+    load_k();
+    int u = u0;
+    while (u + 1 < u1) turn(u++, std::integral_constant<bool, false>(), exact);
+    turn(u, std::integral_constant<bool, true>(), exact);
+  };
+  if constexpr (DT == DT_F32) {
+    sweep(std::integral_constant<bool, true>());
+  } else {
+    sweep(std::integral_constant<bool, false>());
+    // an infinite value times a part of P that is 0 or below 0 is NaN where the formula says infinity: then once
+    // more with P whole
+    bool nan = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) nan |= acc[t][e][i] != acc[t][e][i];
+    if (__any(nan)) sweep(std::integral_constant<bool, true>());
   }
 
-  // the four waves' states into one
+  // the waves' states into one
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     l[t] += __shfl_xor(l[t], 16, 64);
     l[t] += __shfl_xor(l[t], 32, 64);
     if (g4 == 0) {
-      merge_m[wave][t * 16 + r] = m[t];
-      merge_l[wave][t * 16 + r] = l[t];
+      lds.m[wave][t * 16 + r] = m[t];
+      lds.l[wave][t * 16 + r] = l[t];
     }
   }
   __syncthreads();
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int row = t * 16 + r;
-    const float mm = fmaxf(fmaxf(merge_m[0][row], merge_m[1][row]), fmaxf(merge_m[2][row], merge_m[3][row]));
+    const int row = t * 16 + r, rr = row0 + row;
+    float mm = lds.m[0][row];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mm = fmaxf(mm, lds.m[w][row]);
     const float m0 = at_least(mm), f = exp_of(m[t] - m0);
     float ll = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) ll += merge_l[w][row] * exp_of(merge_m[w][row] - m0);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) merge[wave][(e * 4 + g4) * 16 + r] = acc[t][e] * f;
-    if (!done) {
-      if (wave == 0 && g4 == 0) a.part_ml[record * T::ROWS + row] = make_float2(mm, ll);
-    } else if (wave == 0 && g4 == 0 && row0 + row < R) {
-      const int rr = row0 + row;
-      a.lse[((int64_t)b * a.H + hk * G + rr / a.Q) * a.Q + rr % a.Q] = ll == 0.f ? -INFINITY : m0 + logf(ll);
+    for (int w = 0; w < NW; ++w) ll += lds.l[w][row] * exp_of(lds.m[w][row] - m0);
+    if (wave == 0 && g4 == 0) {
+      const float lse = ll == 0.f ? -INFINITY : m0 + logf(ll * (1.f / T::P_SCALE));
+      lds.sum[row] = ll;
+      lds.lse[row] = lse;
+      if (!done) a.part_ml[record * T::ROWS + row] = make_float2(mm, ll);
+      else if (rr < R) a.lse[(int64_t)b * a.H + hk * G + rr] = lse;          // done: one query
     }
-    if (wave == 0 && g4 == 0) merge_sum[row] = ll;
-    __syncthreads();
+    for (int w = 0; w < NW; w += 4) {                  // four waves' sums at a time
+      if (wave / 4 == w / 4) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          floatx4& at = lds.acc[wave % 4][(e * 4 + g4) * 16 + r];
+          at = w == 0 ? acc[t][e] * f : at + acc[t][e] * f;
+        }
+      }
+      __syncthreads();
+    }
     if (!done) {
       floatx4* part = (floatx4*)(a.part_o + (record * T::ROWS + t * 16) * D);
-      for (int i = tid; i < VE * 64; i += 256) part[i] = (merge[0][i] + merge[1][i]) + (merge[2][i] + merge[3][i]);
-    } else {
+      for (int i = tid; i < VE * 64; i += 64 * NW)
+        part[i] = (lds.acc[0][i] + lds.acc[1][i]) + (lds.acc[2][i] + lds.acc[3][i]);
+    } else if (tid < 256) {
       // thread: one 16th of a row
       const int orow = tid / 16, m16 = tid % 16, rr = row0 + t * 16 + orow;
-      const float sum = merge_sum[t * 16 + orow], inv = sum == 0.f ? 0.f : 1.f / sum;
+      const float sum = lds.sum[t * 16 + orow], inv = sum == 0.f ? 0.f : 1.f / sum;
       if (rr < R) {
         float y[VE];
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           const int at = part_index<VE>(orow, m16 * VE + e);
-          const float* p0 = (const float*)merge[0];
+          const float* p0 = (const float*)lds.acc[0];
           constexpr int W = VE * 64 * 4;
           y[e] = sum == 0.f ? 0.f : ((p0[at] + p0[W + at]) + (p0[2 * W + at] + p0[3 * W + at])) * inv;
         }
-        const int64_t row_out = ((int64_t)b * a.H + hk * G + rr / a.Q) * a.Q + rr % a.Q;
-        store_out<DT>((char*)a.out + (row_out * D + m16 * VE) * T::E, y, VE);
+        store_out<DT, VE>((char*)a.out + (((int64_t)b * a.H + hk * G + rr) * D + m16 * VE) * T::E, y);
       }
     }
     __syncthreads();
   }
+}
+
+template <int DT, int D, int NT, bool ACC, bool MULTI>
+__global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_kernel(PagedArgs a, int tiles) {
+  using T = Tile<DT, D, NT>;
+  __shared__ MergeLds<D, NT, T::VE> lds;
+  const CacheView& c = a.c;
+  const int segs = c.Hkv * tiles;
+  const int64_t each = units_each(a, T::UNIT, segs);
+  const int64_t run0 = blockIdx.x * each, run1 = run0 + each;
+  int64_t base = 0;
+  int b = find_seq(a, T::UNIT, segs, run0, -1, base);
+  if (b < 0) return;
+  int len = uniform(common(a, b)), units = units_of(len, T::UNIT);
+  int seg = uniform(div40(run0 - base, units));
+  for (int64_t at = run0; at < run1;) {
+    if (seg == segs) {
+      if (++b == c.B) return;
+      base = at;
+      seg = 0;
+      len = uniform(common(a, b));
+      units = units_of(len, T::UNIT);
+    }
+    const int64_t first = base + (int64_t)seg * units;
+    const int u0 = (int)(at - first), u1 = (int)min((int64_t)units, run1 - first);
+    const bool whole = u1 - u0 == units;               // the row tile is this workgroup's alone
+    const int64_t record = whole ? whole_record(a, segs, b, seg) : 2 * (int64_t)blockIdx.x + (at != run0);
+    const int hk = tiles == 1 ? seg : seg / tiles, row0 = (seg - hk * tiles) * T::ROWS;
+    attend_tile<DT, D, NT, ACC, MULTI, 4>(a, lds, b, len, hk, row0, u0, u1, !MULTI && whole, record);
+    at = first + u1;
+    ++seg;
+  }
+}
+
+// Calls whose sequences are all short: one launch.  A workgroup of 8 waves (16 where the registers allow) takes a kv
+// head's whole row tile, and adds the weights it gives itself.
+template <int DT, int D, int NT, bool ACC>
+__global__ __launch_bounds__((64 * SMALL_WAVES<D, NT>), (SMALL_WAVES<D, NT> / 4)) void paged_small_kernel(PagedArgs a) {
+  using T = Tile<DT, D, NT>;
+  constexpr int NW = SMALL_WAVES<D, NT>;
+  __shared__ MergeLds<D, NT, T::VE> lds;
+  const CacheView& c = a.c;
+  const int hk = blockIdx.x, b = blockIdx.y;
+  const int len = uniform(c.len(b)), R = a.H / c.Hkv;
+  attend_tile<DT, D, NT, ACC, false, NW>(a, lds, b, len, hk, 0, 0, units_of(len, NW * T::KT), true, 0);
+  if constexpr (ACC) {
+    // the scores are this workgroup's own: its barriers order them, and its L1 has never held them before
+    __threadfence_block();
+    __syncthreads();
+    const float* s = a.scores + ((int64_t)b * a.H + hk * R) * a.score_stride;
+    for (int j = threadIdx.x; j < len; j += 64 * NW) {
+      float sum = 0.f;
+      for (int r = 0; r < R; ++r) {
+        const float z = lds.lse[r];
+        sum += z == -INFINITY ? 0.f : exp_of(s[r * a.score_stride + j] - z);
+      }
+      const int p = c.page_of(c.table + (int64_t)b * c.t_stride, j);
+      if (p >= 0) c.weight[p * c.w_ps + hk * c.w_hs + c.slot_of(j)] += sum;
+    }
   }
 }
 
@@ -512,7 +626,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
       const float f = exp_of(m - m0);
       m = top;
       float sum = 0.f;
-      for (int t = lane; t < keys; t += 64) sum += exp_of(tail[t] - m0);
+      for (int t = lane; t < keys; t += 64) sum += T::P_SCALE * exp_of(tail[t] - m0);
 #pragma unroll
       for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s, 64);
       l = l * f + sum;
@@ -521,7 +635,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
       for (int t = wave; t < keys; t += 4) {
         const int page = tail_page[t];
         if (page < 0) continue;
-        const float p = exp_of(tail[t] - m0);
+        const float p = T::P_SCALE * exp_of(tail[t] - m0);
         const char* v = c.v + page * c.v_ps + hk * c.v_hs + c.slot_of(j0 + t) * c.v_ss;
 #pragma unroll
         for (int e = 0; e < W; ++e) y[e] = fmaf(p, load_scalar<DT>(v, lane * W + e), y[e]);
@@ -538,7 +652,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
     if constexpr (DT == DT_F32) *(float*)out = z;
     else *(uint16_t*)out = (uint16_t)(DT == DT_F16 ? f32_to_f16_bits(z) : f32_to_bf16_bits(z));
   }
-  if (tid == 0) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l);
+  if (tid == 0) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l * (1.f / T::P_SCALE));
 }
 
 // The weights that a step's rows give the keys of a kv head: a workgroup takes 256 keys, its waves the rows in
@@ -594,10 +708,18 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
 
 template <int DT, int D, int NT, bool MULTI>
 hipError_t launch_attend(const PagedArgs& a, const PagedCut& cut, hipStream_t st) {
+  if constexpr (!MULTI) {
+    if (cut.small) {
+      constexpr int threads = 64 * SMALL_WAVES<D, NT>;
+      if (a.accumulate) paged_small_kernel<DT, D, NT, true><<<dim3(a.c.Hkv, a.c.B), threads, 0, st>>>(a);
+      else paged_small_kernel<DT, D, NT, false><<<dim3(a.c.Hkv, a.c.B), threads, 0, st>>>(a);
+      return hipGetLastError();
+    }
+  }
   if (a.accumulate) paged_attend_kernel<DT, D, NT, true, MULTI><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
   else paged_attend_kernel<DT, D, NT, false, MULTI><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && !cut.single) {
+  if (e == hipSuccess) {
     paged_join_kernel<DT, D, NT, MULTI><<<dim3(a.H * a.Q, a.c.B), 256, 0, st>>>(a, cut.tiles);
     e = hipGetLastError();
   }
@@ -631,8 +753,8 @@ PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap) {
   const int64_t most = cap <= unit ? 1 : (cap + unit - 1) / unit;
   const int64_t all = (int64_t)Hkv * cut.tiles * B * most;
   cut.grid = (int)(all < 256 * waves ? all : 256 * waves);
-  cut.single = most == 1 && Q == 1;
-  cut.records = cut.single ? 0 : 2 * (int64_t)cut.grid + (Q > 1 ? (int64_t)Hkv * cut.tiles * B : 0);
+  cut.small = Q == 1 && cut.tiles == 1 && cap <= SMALL_KEYS;
+  cut.records = cut.small ? 0 : 2 * (int64_t)cut.grid + (Q > 1 ? (int64_t)Hkv * cut.tiles * B : 0);
   return cut;
 }
 

@@ -308,6 +308,35 @@ def test_attention_of_extreme_scores():
     assert torch.isnan(got[0]).all() and torch.isfinite(got[1:]).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("Q", [1, 3])
+def test_attention_of_infinite_values(dtype, Q):
+    """A value of infinity makes its dim infinite for every query that sees its key, with either sign NaN, and
+    leaves the other dims alone."""
+    import paged_cache as pc
+    inf = float("inf")
+    for lens in ([600, 50], [3000, 50]):                      # one launch, and split
+        made = Made(350, lens, 2, 64, 16, dtype)
+        q = _randn(351, (2, 8, Q, 64), dtype)
+        clean = pc.paged_attention(q, made.cache, made.table, made.lens)
+        p, v = made.rows[0][2], made.cache.v
+        v[p, 0, 5, 7], v[p, 0, 6, 9], v[p, 0, 7, 9], v[p, 0, 8, 11] = inf, inf, -inf, -inf
+        v[made.rows[1][0], 1, 0, 0] = inf
+        got = pc.paged_attention(q, made.cache, made.table, made.lens).float()
+        assert torch.all(got[0, :4, :, 7] == inf) and torch.isnan(got[0, :4, :, 9]).all()
+        assert torch.all(got[0, :4, :, 11] == -inf) and torch.all(got[1, 4:, :, 0] == inf)
+        want = clean.float()
+        for x in (got, want):
+            x[0, :4, :, [7, 9, 11]] = 0.0
+            x[1, 4:, :, 0] = 0.0
+        # P whole or in two parts: both within the bound of the definition, so within twice that of each other
+        made.cache.v.nan_to_num_(0.0, 0.0, 0.0)
+        out, _, _, reach, score = made.attend_ref(q, 0.125)
+        rel = 2 * 72 * U * score + (max(lens) + 64) * U
+        tol = 2 * (rel[..., None] * reach + _half_step(dtype) * out.abs()) * 1.01 + torch.finfo(dtype).smallest_normal
+        assert torch.all((got - want).abs().cpu().double() <= tol)
+
+
 def test_attention_past_4_gib_of_cache():
     """Pages whose rows lie beyond 32-bit byte offsets."""
     import paged_cache as pc
