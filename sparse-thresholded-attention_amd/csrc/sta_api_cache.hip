@@ -136,7 +136,7 @@ PagedLayout paged_layout(const sta_paged_args* a) {
   L.lse_off = off;                                    // (B, H, Q) when not an output
   off = align256(off + rows * 4);
   L.scores_off = off;                                 // (B, H, Q, score_stride)
-  if (a->accumulate) off = align256(off + rows * L.score_stride * 4);
+  if (a->accumulate && !L.cut.reform) off = align256(off + rows * L.score_stride * 4);
   L.total = off;
   return L;
 }
@@ -283,11 +283,11 @@ int sta_paged_attention(const sta_paged_args* a, void* stream) {
   d.accumulate = a->accumulate != 0;
   d.out = a->out;
   d.lse = a->lse ? a->lse : (float*)(ws + L.lse_off);
-  d.scores = (float*)(ws + L.scores_off);
+  d.scores = a->accumulate && !L.cut.reform ? (float*)(ws + L.scores_off) : nullptr;
   d.score_stride = L.score_stride;
   d.part_o = (float*)(ws + L.part_off);
   d.part_ml = (float2*)(ws + L.ml_off);
-  d.grid = L.cut.grid;
+  d.runs = L.cut.runs;
   hipError_t e = launch_paged(a->cache.dtype, a->cache.D, d, (hipStream_t)stream);
   return e == hipSuccess ? STA_OK : hip_fail(e, "paged attention");
 }

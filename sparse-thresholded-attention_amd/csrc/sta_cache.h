@@ -51,17 +51,18 @@ struct PagedArgs {
   int accumulate;
   void* out;
   float* lse;                       // (B, H, Q), the caller's or in the workspace
-  float* scores;                    // (B, H, Q, score_stride), accumulate only
+  float* scores;                    // (B, H, Q, score_stride); NULL: not stored
   int64_t score_stride;
   float* part_o;                    // (records, rows, D) unnormalised outputs of unfinished row tiles, permuted
   float2* part_ml;                  // (records, rows) their maxima and sums
-  int grid;
+  int runs;
 };
 
-// how a call of the attention is cut (host): `grid` workgroups; a row tile is `rows` query rows of
-// one kv head, `tiles` of them a kv head
+// how a call of the attention is cut (host): a row tile is `rows` query rows of one kv head, `tiles` of them a
+// kv head; `runs` runs of units of keys; `grid` workgroups, one a run and row tile
 struct PagedCut {
-  int rows, tiles, grid;
+  int rows, tiles, runs, grid;
+  bool reform;                      // weights from scores formed again, not from stored ones
   bool small;                       // short sequences, one query each: one launch, nothing to join
   int64_t records;                  // of unfinished row tiles, in the workspace
 };

@@ -72,11 +72,11 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 // instructions for each; fp32 caches use the fp32 instruction of depth 4, whose operands P and V are as well.
 //
 // Work.  The sequences' lengths are known to the device alone, and differ.  Every wave sums their units (of
-// 4 KT keys; an empty sequence counts one, which writes its zeros) over all row tiles, and the call's
-// workgroups, as many as the chip holds at once, take equal runs of units in the order (sequence, row
-// tile, unit).  A run covers the end of one row tile, some whole ones and the beginning of another; whole
-// ones are written out, the two others leave a record in the workspace for the join kernel, which
-// finds the workgroups of a row tile by the same division.
+// 4 KT keys; an empty sequence counts one, which writes its zeros) over the kv heads, and the call's runs, as many
+// as the chip holds workgroups (times the row tiles) at once, take equal numbers of units in the order (sequence, kv
+// head, unit).  A run covers the end of one kv head's keys, some whole ones and the beginning of another; whole ones
+// are written out, the two others leave a record in the workspace for the join kernel, which finds the runs of a kv
+// head by the same division.
 constexpr float LOG2E = 1.44269504088896340736f;
 
 __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
@@ -98,17 +98,17 @@ __device__ __forceinline__ int units_of(int keys, int unit) { return max(1, (key
 // keys that every query of sequence b sees
 __device__ __forceinline__ int common(const PagedArgs& a, int b) { return max(a.c.len(b) - (a.Q - 1), 0); }
 
-// units that a workgroup takes (at least one); every lane of the wave takes part
-__device__ __forceinline__ int64_t units_each(const PagedArgs& a, int unit, int segs) {
+// units of a run (at least one); every lane of the wave takes part
+__device__ __forceinline__ int64_t units_each(const PagedArgs& a, int unit) {
   int64_t sum = 0;
   for (int b = threadIdx.x & 63; b < a.c.B; b += 64) sum += units_of(common(a, b), unit);
-  const int64_t all = uniform(wave_sum64(sum)) * segs;
-  return all <= a.grid ? 1 : uniform(div40(all + a.grid - 1, a.grid));
+  const int64_t all = uniform(wave_sum64(sum)) * a.c.Hkv;
+  return all <= a.runs ? 1 : uniform(div40(all + a.runs - 1, a.runs));
 }
 
 // The sequence that holds unit `at` (or, at < 0, sequence b) and the number of its first unit; -1: behind
 // the last.  Uniform; every lane takes part.
-__device__ __forceinline__ int find_seq(const PagedArgs& a, int unit, int segs, int64_t at, int b, int64_t& base) {
+__device__ __forceinline__ int find_seq(const PagedArgs& a, int unit, int64_t at, int b, int64_t& base) {
   const CacheView& c = a.c;
   const int lane = threadIdx.x & 63;
   int64_t run = 0;
@@ -117,20 +117,21 @@ __device__ __forceinline__ int find_seq(const PagedArgs& a, int unit, int segs, 
     // up to 64 * 2^22 units of a row tile
     const int n = mine < c.B ? units_of(common(a, mine), unit) : 0;
     const int incl = wave_incl_sum(n);
-    const unsigned long long hit = at < 0 ? __ballot(mine == b) : __ballot(run + (int64_t)incl * segs > at);
+    const unsigned long long hit = at < 0 ? __ballot(mine == b) : __ballot(run + (int64_t)incl * c.Hkv > at);
     if (hit) {
       const int first = __builtin_amdgcn_readfirstlane(__ffsll(hit) - 1);
-      base = run + (int64_t)(__builtin_amdgcn_readlane(incl, first) - __builtin_amdgcn_readlane(n, first)) * segs;
+      base = run + (int64_t)(__builtin_amdgcn_readlane(incl, first) - __builtin_amdgcn_readlane(n, first)) * c.Hkv;
       return b0 + first;
     }
-    run += (int64_t)__builtin_amdgcn_readlane(incl, 63) * segs;
+    run += (int64_t)__builtin_amdgcn_readlane(incl, 63) * c.Hkv;
   }
   return -1;
 }
 
-// the record of a row tile that one workgroup finished, MULTI calls only: behind the two of each workgroup
-__device__ __forceinline__ int64_t whole_record(const PagedArgs& a, int segs, int b, int seg) {
-  return 2 * (int64_t)a.grid + (int64_t)b * segs + seg;
+// records: two of every run, for its first and its last kv head where those are unfinished, and (calls of several
+// queries) one of every kv head, for those that one run finishes; `tiles` of each
+__device__ __forceinline__ int64_t whole_record(const PagedArgs& a, int b, int hk) {
+  return 2 * (int64_t)a.runs + (int64_t)b * a.c.Hkv + hk;
 }
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
@@ -193,6 +194,8 @@ __device__ __forceinline__ float v_elem(const uint32_t* w, int e) {
 // loads at an address in global memory (one that went through a lane exchange is no pointer to the compiler)
 typedef const __attribute__((address_space(1))) u32x4* global4;
 typedef const __attribute__((address_space(1))) u32x2* global2;
+typedef const __attribute__((address_space(1))) uint32_t* global1;
+typedef const __attribute__((address_space(1))) uint16_t* global_half;
 template <int W>
 __device__ __forceinline__ void load_words(int64_t p, uint32_t* w) {
   if constexpr (W == 2) {
@@ -493,30 +496,32 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
   using T = Tile<DT, D, NT>;
   __shared__ MergeLds<D, NT, T::VE> lds;
   const CacheView& c = a.c;
-  const int segs = c.Hkv * tiles;
-  const int64_t each = units_each(a, T::UNIT, segs);
-  const int64_t run0 = blockIdx.x * each, run1 = run0 + each;
+  // workgroups go to the XCDs in turn: the row tiles of a run are 8 apart, on one XCD, and find each other's keys in
+  // its L2 (32 queries of 32 heads over 8 kv heads, 4 sequences up to 12288 keys: 69 -> 52 us)
+  const int x = blockIdx.x / 8, tile = tiles == 1 ? 0 : x % tiles;
+  const int run = tiles == 1 ? blockIdx.x : x / tiles * 8 + blockIdx.x % 8;
+  const int64_t each = units_each(a, T::UNIT);
+  const int64_t run0 = run * each, run1 = run0 + each;
   int64_t base = 0;
-  int b = find_seq(a, T::UNIT, segs, run0, -1, base);
+  int b = find_seq(a, T::UNIT, run0, -1, base);
   if (b < 0) return;
   int len = uniform(common(a, b)), units = units_of(len, T::UNIT);
-  int seg = uniform(div40(run0 - base, units));
+  int hk = uniform(div40(run0 - base, units));
   for (int64_t at = run0; at < run1;) {
-    if (seg == segs) {
+    if (hk == c.Hkv) {
       if (++b == c.B) return;
       base = at;
-      seg = 0;
+      hk = 0;
       len = uniform(common(a, b));
       units = units_of(len, T::UNIT);
     }
-    const int64_t first = base + (int64_t)seg * units;
+    const int64_t first = base + (int64_t)hk * units;
     const int u0 = (int)(at - first), u1 = (int)min((int64_t)units, run1 - first);
-    const bool whole = u1 - u0 == units;               // the row tile is this workgroup's alone
-    const int64_t record = whole ? whole_record(a, segs, b, seg) : 2 * (int64_t)blockIdx.x + (at != run0);
-    const int hk = tiles == 1 ? seg : seg / tiles, row0 = (seg - hk * tiles) * T::ROWS;
-    attend_tile<DT, D, NT, ACC, MULTI, 4>(a, lds, b, len, hk, row0, u0, u1, !MULTI && whole, record);
+    const bool whole = u1 - u0 == units;               // the kv head's keys are this run's alone
+    const int64_t record = (whole ? whole_record(a, b, hk) : 2 * (int64_t)run + (at != run0)) * tiles + tile;
+    attend_tile<DT, D, NT, ACC, MULTI, 4>(a, lds, b, len, hk, tile * T::ROWS, u0, u1, !MULTI && whole, record);
     at = first + u1;
-    ++seg;
+    ++hk;
   }
 }
 
@@ -548,35 +553,68 @@ __global__ __launch_bounds__((64 * SMALL_WAVES<D, NT>), (SMALL_WAVES<D, NT> / 4)
   }
 }
 
-// One workgroup per query row: the records of its row tile, a wave each in turn, and (MULTI) the keys behind
-// the common ones.
-template <int DT, int D, int NT, bool MULTI>
+// the records of a kv head's keys
+struct Records {
+  int n;
+  int64_t w0, first;
+  __device__ __forceinline__ int64_t at(int p) const { return p ? 2 * (w0 + p) : first; }
+};
+__device__ __forceinline__ Records records_of(const PagedArgs& a, int unit, int b, int hk) {
+  const int64_t each = units_each(a, unit);
+  int64_t base = 0;
+  find_seq(a, unit, -1, b, base);
+  const int units = units_of(common(a, b), unit);
+  const int64_t first = base + (int64_t)hk * units;
+  Records r;
+  r.w0 = div40(first, each);
+  r.n = (int)(div40(first + units - 1, each) - r.w0) + 1;
+  // the first run's record is its second one unless the kv head begins it
+  r.first = r.n == 1 ? whole_record(a, b, hk) : 2 * r.w0 + (first != r.w0 * each);
+  return r;
+}
+
+// lane n of each row of 16 lanes, to all of its row; n is a constant
+__device__ __forceinline__ uint32_t row_lane(int n, uint32_t x) {
+  switch (n) {
+#define STA_ROW_LANE(i) case i: return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x150 + i, 0xf, 0xf, false)
+    STA_ROW_LANE(0); STA_ROW_LANE(1); STA_ROW_LANE(2); STA_ROW_LANE(3); STA_ROW_LANE(4); STA_ROW_LANE(5);
+    STA_ROW_LANE(6); STA_ROW_LANE(7); STA_ROW_LANE(8); STA_ROW_LANE(9); STA_ROW_LANE(10); STA_ROW_LANE(11);
+    STA_ROW_LANE(12); STA_ROW_LANE(13); STA_ROW_LANE(14); STA_ROW_LANE(15);
+#undef STA_ROW_LANE
+  }
+  return x;
+}
+// the sum over each row of 16 lanes, in every lane
+__device__ __forceinline__ float row_sum(float x) {
+  x = group8_sum(x);
+  return x + __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), 0x140, 0xf, 0xf, false));
+}
+
+template <int DT>
+__device__ __forceinline__ void store_elem(void* out, int64_t at, float x) {
+  if constexpr (DT == DT_F32) ((float*)out)[at] = x;
+  else ((uint16_t*)out)[at] = (uint16_t)(DT == DT_F16 ? f32_to_f16_bits(x) : f32_to_bf16_bits(x));
+}
+
+// One query: a workgroup per row takes its records, a wave each in turn.
+template <int DT, int D, int NT>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles) {
   using T = Tile<DT, D, NT>;
-  constexpr int TAIL = 256, W = D / 64;               // a lane's dims
-  __shared__ float o[4][D], tail[MULTI ? TAIL : 1];
-  __shared__ int tail_page[MULTI ? TAIL : 1];
-  const CacheView& c = a.c;
+  constexpr int W = D / 64;                            // a lane's dims
+  __shared__ float o[4][D];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int hi = blockIdx.x, b = blockIdx.y, G = a.H / c.Hkv, segs = c.Hkv * tiles;
-  const int h = MULTI ? hi / a.Q : hi, i = hi - h * a.Q, hk = h / G, row = (h - hk * G) * a.Q + i, rr = row % T::ROWS;
-  const int64_t each = units_each(a, T::UNIT, segs);
-  int64_t base = 0;
-  find_seq(a, T::UNIT, segs, -1, b, base);
-  const int n0 = common(a, b), units = units_of(n0, T::UNIT), seg = hk * tiles + row / T::ROWS;
-  const int64_t first = base + (int64_t)seg * units;
-  const int64_t w0 = div40(first, each);
-  const int n = (int)(div40(first + units - 1, each) - w0) + 1;
-  if (!MULTI && n == 1) return;
-  // the first workgroup's record is its second one unless the row tile begins its run
-  const int64_t rec0 = n == 1 ? whole_record(a, segs, b, seg) : 2 * w0 + (first != w0 * each);
-  auto record = [&](int p) { return (p ? 2 * (w0 + p) : rec0) * T::ROWS; };
+  const int h = blockIdx.x, b = blockIdx.y, G = a.H / a.c.Hkv, hk = h / G, row = h - hk * G;
+  const int tile = row / T::ROWS, rr = row - tile * T::ROWS;
+  const Records rec = records_of(a, T::UNIT, b, hk);
+  if (rec.n == 1) return;                              // written by its workgroup
+  auto record = [&](int p) { return (rec.at(p) * tiles + tile) * T::ROWS; };
   const float2* ml = a.part_ml + rr;
   float m = -INFINITY;
-  for (int p = lane; p < n; p += 64) m = fmaxf(m, ml[record(p)].x);
+  for (int p = lane; p < rec.n; p += 64) m = fmaxf(m, ml[record(p)].x);
   m = wave_max_f32(m);
-  float m0 = at_least(m), l = 0.f;
-  for (int p = lane; p < n; p += 64) {
+  const float m0 = at_least(m);
+  float l = 0.f;
+  for (int p = lane; p < rec.n; p += 64) {
     const float2 x = ml[record(p)];
     l += x.y * exp_of(x.x - m0);
   }
@@ -586,73 +624,125 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
 #pragma unroll
   for (int e = 0; e < W; ++e) y[e] = 0.f;
   const float* part = a.part_o + rr / 16 * 16 * D;
-  for (int p = wave; p < n; p += 4) {
-    const int64_t rec = record(p);
-    const float f = exp_of(ml[rec].x - m0);
+#pragma unroll 4
+  for (int p = wave; p < rec.n; p += 4) {
+    const int64_t at = record(p);
+    const float f = exp_of(ml[at].x - m0);
 #pragma unroll
-    for (int e = 0; e < W; ++e) y[e] += f * part[rec * D + part_index<T::VE>(rr % 16, lane * W + e)];
-  }
-  const int64_t row_out = ((int64_t)b * a.H + h) * a.Q + i;
-  if constexpr (MULTI) {
-    const int end = c.len(b) - (a.Q - 1 - i), l16 = lane & 15;
-    const int32_t* table = c.table + (int64_t)b * c.t_stride;
-    uint32_t q[T::VW];
-    load_words<T::VW>((int64_t)((const char*)a.q + (b * a.q_bs + h * a.q_hs + i * a.q_ts) * T::E + l16 * (T::VW * 4)), q);
-    for (int j0 = n0; j0 < end; j0 += TAIL) {
-      const int keys = min(end - j0, TAIL);
-      for (int t = tid / 16; t < keys; t += 16) {      // 16 lanes a key
-        const int page = c.page_of(table, j0 + t);
-        float dot = 0.f;
-        if (page >= 0) {
-          uint32_t k[T::VW];
-          load_words<T::VW>((int64_t)(c.k + page * c.k_ps + hk * c.k_hs + c.slot_of(j0 + t) * c.k_ss + l16 * (T::VW * 4)), k);
-#pragma unroll
-          for (int e = 0; e < T::VE; ++e) dot = fmaf(v_elem<DT>(q, e), v_elem<DT>(k, e), dot);
-        }
-#pragma unroll
-        for (int s = 8; s; s >>= 1) dot += __shfl_xor(dot, s, 64);
-        if (l16 == 0) {
-          const float s = page >= 0 ? dot * a.sm_scale : -INFINITY;
-          tail[t] = s;
-          tail_page[t] = page;
-          if (a.accumulate) a.scores[row_out * a.score_stride + j0 + t] = s;
-        }
-      }
-      __syncthreads();
-      float top = -INFINITY;
-      for (int t = lane; t < keys; t += 64) top = fmaxf(top, tail[t]);
-      top = fmaxf(wave_max_f32(top), m);
-      m0 = at_least(top);
-      const float f = exp_of(m - m0);
-      m = top;
-      float sum = 0.f;
-      for (int t = lane; t < keys; t += 64) sum += T::P_SCALE * exp_of(tail[t] - m0);
-#pragma unroll
-      for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s, 64);
-      l = l * f + sum;
-#pragma unroll
-      for (int e = 0; e < W; ++e) y[e] *= f;
-      for (int t = wave; t < keys; t += 4) {
-        const int page = tail_page[t];
-        if (page < 0) continue;
-        const float p = T::P_SCALE * exp_of(tail[t] - m0);
-        const char* v = c.v + page * c.v_ps + hk * c.v_hs + c.slot_of(j0 + t) * c.v_ss;
-#pragma unroll
-        for (int e = 0; e < W; ++e) y[e] = fmaf(p, load_scalar<DT>(v, lane * W + e), y[e]);
-      }
-      __syncthreads();
-    }
+    for (int e = 0; e < W; ++e) y[e] += f * part[at * D + part_index<T::VE>(rr % 16, lane * W + e)];
   }
 #pragma unroll
   for (int e = 0; e < W; ++e) o[wave][lane * W + e] = y[e];
   __syncthreads();
-  if (tid < D) {
-    const float z = l == 0.f ? 0.f : ((o[0][tid] + o[1][tid]) + (o[2][tid] + o[3][tid])) / l;
-    char* out = (char*)a.out + (row_out * D + tid) * T::E;
-    if constexpr (DT == DT_F32) *(float*)out = z;
-    else *(uint16_t*)out = (uint16_t)(DT == DT_F16 ? f32_to_f16_bits(z) : f32_to_bf16_bits(z));
-  }
+  const int64_t row_out = (int64_t)b * a.H + h;
+  if (tid < D)
+    store_elem<DT>(a.out, row_out * D + tid, l == 0.f ? 0.f : ((o[0][tid] + o[1][tid]) + (o[2][tid] + o[3][tid])) / l);
   if (tid == 0) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l * (1.f / T::P_SCALE));
+}
+
+// Several queries: a wave per row takes its records and then the keys behind the common ones.  The waves of a workgroup
+// are rows of one query and kv head where there are four, so that those keys are fetched once.
+template <int DT, int D, int NT>
+__global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int tiles) {
+  using T = Tile<DT, D, NT>;
+  constexpr int W = D / 64, VW = T::VW;
+  const CacheView& c = a.c;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, G = a.H / c.Hkv;
+  const int x = blockIdx.x * 4 + uniform((int)threadIdx.x >> 6), b = blockIdx.y;
+  if (x >= a.H * a.Q) return;
+  const int g = x % G, i = x / G % a.Q, hk = x / (G * a.Q), h = hk * G + g, row = g * a.Q + i;
+  const int tile = row / T::ROWS, rr = row - tile * T::ROWS;
+  const Records rec = records_of(a, T::UNIT, b, hk);
+  auto record = [&](int p) { return (rec.at(p) * tiles + tile) * T::ROWS; };
+  const float2* ml = a.part_ml + rr;
+  float m = -INFINITY;
+  for (int p = lane; p < rec.n; p += 64) m = fmaxf(m, ml[record(p)].x);
+  m = wave_max_f32(m);
+  float m0 = at_least(m), l = 0.f;
+  for (int p = lane; p < rec.n; p += 64) {
+    const float2 s = ml[record(p)];
+    l += s.y * exp_of(s.x - m0);
+  }
+  float y[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) y[e] = 0.f;
+  const float* part = a.part_o + rr / 16 * 16 * D;
+#pragma unroll 4
+  for (int p = 0; p < rec.n; ++p) {
+    const int64_t at = record(p);
+    const float f = exp_of(ml[at].x - m0);
+#pragma unroll
+    for (int e = 0; e < W; ++e) y[e] += f * part[at * D + part_index<T::VE>(rr % 16, lane * W + e)];
+  }
+  const int64_t row_out = ((int64_t)b * a.H + h) * a.Q + i;
+  const int n0 = common(a, b), end = c.len(b) - (a.Q - 1 - i);
+  const int32_t* table = c.table + (int64_t)b * c.t_stride;
+  uint32_t q[VW];
+  load_words<VW>((int64_t)((const char*)a.q + (b * a.q_bs + h * a.q_hs + i * a.q_ts) * T::E + l16 * (VW * 4)), q);
+  for (int j0 = n0; j0 < end; j0 += 64) {
+    const int keys = min(end - j0, 64);
+    // lane 16 i + j has key 4 j + i: its rows and, at last, its score; lanes behind the keys have rows of zeros
+    const int key = l16 * 4 + (lane >> 4);
+    const int page = key < keys ? c.page_of(table, j0 + key) : -1, slot = c.slot_of(j0 + key);
+    const int64_t krow = (int64_t)(page < 0 ? (const char*)zero_row : c.k + hk * c.k_hs + page * c.k_ps + slot * c.k_ss);
+    const int64_t vrow = (int64_t)(page < 0 ? (const char*)zero_row : c.v + hk * c.v_hs + page * c.v_ps + slot * c.v_ss);
+    float mine = -INFINITY;
+    // 16 lanes a key, four keys an instruction
+    auto four = [&](auto step) {
+      constexpr int S = decltype(step)::value;
+      uint32_t k[4][VW];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t lo = row_lane(S + x, (uint32_t)krow), hi = row_lane(S + x, (uint32_t)(krow >> 32));
+        load_words<VW>((int64_t)((uint64_t)hi << 32 | lo) + l16 * (VW * 4), k[x]);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float dot = 0.f;
+#pragma unroll
+        for (int e = 0; e < T::VE; ++e) dot = fmaf(v_elem<DT>(q, e), v_elem<DT>(k[x], e), dot);
+        dot = row_sum(dot) * a.sm_scale;
+        if (l16 == S + x && page >= 0) mine = dot;
+      }
+    };
+    four(std::integral_constant<int, 0>());
+    if (keys > 16) four(std::integral_constant<int, 4>());
+    if (keys > 32) four(std::integral_constant<int, 8>());
+    if (keys > 48) four(std::integral_constant<int, 12>());
+    if (a.scores && key < keys) a.scores[row_out * a.score_stride + j0 + key] = mine;
+    const float m1 = fmaxf(wave_max_f32(mine), m);
+    m0 = at_least(m1);
+    const float f = exp_of(m - m0), p = T::P_SCALE * exp_of(mine - m0);
+    m = m1;
+    l = l * f + p;
+#pragma unroll
+    for (int e = 0; e < W; ++e) y[e] *= f;
+    // a key that does not exist has p = 0 and a row of zeros
+    for (int t0 = 0; t0 < keys; t0 += 8) {
+      uint32_t w[8][2];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int from = ((t0 + x) & 3) * 16 + ((t0 + x) >> 2);
+        const uint32_t lo = __builtin_amdgcn_readlane((int)vrow, from), hi = __builtin_amdgcn_readlane((int)(vrow >> 32), from);
+        const int64_t v = (int64_t)((uint64_t)hi << 32 | lo) + lane * (W * T::E);
+        if constexpr (W * T::E == 8) load_words<2>(v, w[x]);
+        else if constexpr (W * T::E == 4) w[x][0] = *(global1)v;
+        else w[x][0] = *(global_half)v;
+      }
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int from = ((t0 + x) & 3) * 16 + ((t0 + x) >> 2);
+        const float pt = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), from));
+#pragma unroll
+        for (int e = 0; e < W; ++e) y[e] = fmaf(pt, v_elem<DT>(w[x], e), y[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 32; s; s >>= 1) l += __shfl_xor(l, s, 64);
+#pragma unroll
+  for (int e = 0; e < W; ++e) store_elem<DT>(a.out, row_out * D + lane * W + e, l == 0.f ? 0.f : y[e] / l);
+  if (lane == 0) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l * (1.f / T::P_SCALE));
 }
 
 // The weights that a step's rows give the keys of a kv head: a workgroup takes 256 keys, its waves the rows in
@@ -706,6 +796,93 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
   c.weight[p * c.w_ps + hk * c.w_hs + c.slot_of(mine)] += (w[tid] + w[256 + tid]) + (w[512 + tid] + w[768 + tid]);
 }
 
+// The same from the scores formed again, where a kv head has many rows (PagedCut::reform): a wave holds 64 keys
+// in registers, the rows come 64 at a time through LDS, and each lane adds up its row's p of four keys a subtile over
+// the row tiles; the 16 lanes of those keys meet at the end.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void paged_reform_kernel(PagedArgs a) {
+  using T = Tile<DT, D, 1>;
+  constexpr int KS = T::KS, SUBS = 4, ROWS = 64, STRIDE = T::RB / 16 + 1;   // 16-byte words, padded
+  __shared__ u32x4 rows[ROWS * STRIDE];
+  __shared__ float minus[ROWS];
+  __shared__ int ends[ROWS];
+  const CacheView& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, g4 = lane >> 4;
+  const int b = blockIdx.z, hk = blockIdx.y, block0 = blockIdx.x * (64 * SUBS), key0 = block0 + wave * (16 * SUBS);
+  const int len = uniform(c.len(b)), R = a.H / c.Hkv * a.Q;
+  if (block0 >= len) return;
+  const int32_t* table = c.table + (int64_t)b * c.t_stride;
+  // the lane's key of the wave's, and all of them in their lanes
+  const int mine = key0 + (lane & (16 * SUBS - 1));
+  const int page = mine < len ? c.page_of(table, mine) : -1;
+  const int64_t krow =
+      (int64_t)(page < 0 ? (const char*)zero_row : c.k + hk * c.k_hs + page * c.k_ps + c.slot_of(mine) * c.k_ss);
+  u32x4 k[SUBS][KS];
+#pragma unroll
+  for (int s = 0; s < SUBS; ++s) {
+    const int64_t p = __shfl(krow, s * 16 + r, 64) + g4 * 16;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) k[s][i] = *(global4)(p + i * 64);
+  }
+  const bool all = key0 + 16 * SUBS <= common(a, b);   // every row sees every key of the wave
+  floatx4 w[SUBS];
+#pragma unroll
+  for (int s = 0; s < SUBS; ++s) w[s] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int r0 = 0; r0 < R; r0 += ROWS) {
+    const int n = min(R - r0, ROWS);
+    __syncthreads();
+    for (int x = tid; x < ROWS * (T::RB / 16); x += 256) {
+      const int row = x / (T::RB / 16), at = x - row * (T::RB / 16), rr = r0 + row;
+      const int h = hk * (a.H / c.Hkv) + rr / a.Q, i = rr % a.Q;
+      if (row < n)
+        rows[row * STRIDE + at] = *(global4)((int64_t)((const char*)a.q + (b * a.q_bs + h * a.q_hs + i * a.q_ts) * T::E + at * 16));
+      else
+        rows[row * STRIDE + at] = u32x4{0, 0, 0, 0};
+    }
+    if (tid < ROWS) {
+      const int rr = r0 + tid, i = rr % a.Q;
+      // a row that saw nothing, or is none, gives nothing: exp(s - inf)
+      const float z = tid < n ? a.lse[((int64_t)b * a.H + hk * (a.H / c.Hkv) + rr / a.Q) * a.Q + i] : INFINITY;
+      minus[tid] = z == -INFINITY ? INFINITY : z;
+      ends[tid] = len - (a.Q - 1 - i);
+    }
+    __syncthreads();
+    for (int t = 0; t < n; t += 16) {
+      u32x4 q[KS];
+#pragma unroll
+      for (int i = 0; i < KS; ++i) q[i] = rows[(t + r) * STRIDE + i * 4 + g4];
+      const float z = minus[t + r];
+      const int end = ends[t + r];
+      const bool live = z != INFINITY;
+#pragma unroll
+      for (int s = 0; s < SUBS; ++s) {
+        floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < KS; ++i) x = mfma_qk<DT>(k[s][i], q[i], x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = exp_of(x[i] * a.sm_scale - z);
+          w[s][i] += live && (all || key0 + s * 16 + g4 * 4 + i < end) ? p : 0.f;
+        }
+      }
+    }
+  }
+  // lane 4 s + i of a row of lanes keeps key 16 s + 4 (lane / 16) + i
+  float out = 0.f;
+#pragma unroll
+  for (int s = 0; s < SUBS; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = row_sum(w[s][i]);
+      if (r == s * 4 + i) out = x;
+    }
+  const int j = key0 + r / 4 * 16 + g4 * 4 + r % 4;
+  if (r < SUBS * 4 && j < len) {
+    const int p = c.page_of(table, j);
+    if (p >= 0) c.weight[p * c.w_ps + hk * c.w_hs + c.slot_of(j)] += out;
+  }
+}
+
 template <int DT, int D, int NT, bool MULTI>
 hipError_t launch_attend(const PagedArgs& a, const PagedCut& cut, hipStream_t st) {
   if constexpr (!MULTI) {
@@ -716,14 +893,21 @@ hipError_t launch_attend(const PagedArgs& a, const PagedCut& cut, hipStream_t st
       return hipGetLastError();
     }
   }
-  if (a.accumulate) paged_attend_kernel<DT, D, NT, true, MULTI><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
+  if (a.scores) paged_attend_kernel<DT, D, NT, true, MULTI><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
   else paged_attend_kernel<DT, D, NT, false, MULTI><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess) {
-    paged_join_kernel<DT, D, NT, MULTI><<<dim3(a.H * a.Q, a.c.B), 256, 0, st>>>(a, cut.tiles);
+    if constexpr (MULTI) paged_join_rows_kernel<DT, D, NT><<<dim3((a.H * a.Q + 3) / 4, a.c.B), 256, 0, st>>>(a, cut.tiles);
+    else paged_join_kernel<DT, D, NT><<<dim3(a.H, a.c.B), 256, 0, st>>>(a, cut.tiles);
     e = hipGetLastError();
   }
   if (e != hipSuccess || !a.accumulate) return e;
+  if constexpr (DT != DT_F32) {
+    if (cut.reform) {
+      paged_reform_kernel<DT, D><<<dim3((a.c.cap + 255) / 256, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
+      return hipGetLastError();
+    }
+  }
   paged_weight_kernel<<<dim3((a.c.cap + 255) / 256, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
   return hipGetLastError();
 }
@@ -751,10 +935,17 @@ PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap) {
   const int unit = dtype == STA_DTYPE_F32 ? Tile<DT_F32, 64, 1>::UNIT : Tile<DT_BF16, 64, 1>::UNIT;
   const int waves = cut.rows == 32 ? 2 : (D == 64 ? Tile<DT_BF16, 64, 1>::WAVES : Tile<DT_BF16, 128, 1>::WAVES);
   const int64_t most = cap <= unit ? 1 : (cap + unit - 1) / unit;
-  const int64_t all = (int64_t)Hkv * cut.tiles * B * most;
-  cut.grid = (int)(all < 256 * waves ? all : 256 * waves);
+  const int64_t all = (int64_t)Hkv * B * most;
+  int runs = 256 * waves;
+  if (cut.tiles > 1) runs = runs / cut.tiles < 8 ? 8 : runs / cut.tiles / 8 * 8;
+  cut.runs = (int)(all < runs ? all : runs);
+  cut.grid = cut.tiles == 1 ? cut.runs : (cut.runs + 7) / 8 * 8 * cut.tiles;
+  // stored scores cost 8 bytes a row and key, reformed ones the keys once more and their products: 32q / 8kv heads
+  // x 128, bf16, 8 sequences up to 8192 keys, R = 32 / 64 rows: 56 / 87 us stored, 66 / 86 reformed, and 117 / 97 at
+  // R = 128 (4 up to 12288); fp32 97 / 147 and 118 / 184
   cut.small = Q == 1 && cut.tiles == 1 && cap <= SMALL_KEYS;
-  cut.records = cut.small ? 0 : 2 * (int64_t)cut.grid + (Q > 1 ? (int64_t)Hkv * cut.tiles * B : 0);
+  cut.reform = !cut.small && R > 64 && dtype != STA_DTYPE_F32;
+  cut.records = cut.small ? 0 : cut.tiles * (2 * (int64_t)cut.runs + (Q > 1 ? (int64_t)Hkv * B : 0));
   return cut;
 }
 
