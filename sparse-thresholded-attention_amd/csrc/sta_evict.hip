@@ -19,7 +19,9 @@ namespace {
 constexpr int SEL_T = 1024;
 constexpr int BINS = 2048;             // of a counting pass
 constexpr int PER = 8;                 // consecutive keys of a thread
-constexpr int LDS_KEYS = 32768;        // 128 KB of words
+constexpr int COPIES = 4;              // of the counting table, one int4 a bin
+constexpr int LDS_KEYS = 28672;        // 112 KB of words
+constexpr int FOURS = LDS_KEYS / 4 / SEL_T;
 constexpr int INLINE_MOVES = 64;       // rows a head that the selecting workgroup moves itself
 constexpr uint32_t FORCED = 0xffffffffu;
 
@@ -70,12 +72,14 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int hk, int b, int
   }
 }
 
-// One workgroup per sequence and kv head.  IN_LDS: the words stay in LDS (calls of at most LDS_KEYS keys); else each
-// pass reads weight and pos again.  INLINE: the few rows that can move are moved here.
-template <bool IN_LDS, bool INLINE>
+// One workgroup per sequence and kv head.
+// KEPT: the words stay in LDS, and weight and pos are read once, four keys a load, into registers (calls of at most
+// LDS_KEYS keys whose pages hold four keys in 16 aligned bytes); else each pass reads them again.
+// INLINE: the few rows that can move are moved here.
+template <bool KEPT, bool INLINE>
 __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
   extern __shared__ uint32_t words[];
-  __shared__ int hist[BINS], scan[SEL_T / 64], pick[2];
+  __shared__ int hist[BINS * COPIES], scan[SEL_T / 64], pick[2];
   const CacheView& c = a.c;
   const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int len = c.len(b), m = min(len, a.budget);
@@ -89,12 +93,42 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
   const int32_t* table = c.table + (int64_t)b * c.t_stride;
   const float* weight = c.weight + hk * c.w_hs;
   const int32_t* posp = c.pos + hk * c.p_hs;
-  for (int i = tid; i < BINS; i += SEL_T) hist[i] = 0;
+  for (int i = tid; i < BINS * COPIES; i += SEL_T) hist[i] = 0;
   int last = INT32_MIN;
+  int4 kp[KEPT ? FOURS : 1];
+  float4 kw[KEPT ? FOURS : 1];
+  bool there[KEPT ? FOURS : 1];
+  if constexpr (KEPT) {
+#pragma unroll
+    for (int i = 0; i < FOURS; ++i) {
+      const int j = (i * SEL_T + tid) * 4;
+      there[i] = false;
+      if (i * SEL_T * 4 < len) {
+        const int p = c.page_of(table, min(j, len - 1));
+        there[i] = p >= 0 && j < len;
+        const int s = c.slot_of(j);
+        if (there[i]) {
+          kp[i] = *(const int4*)(posp + p * c.p_ps + s);
+          kw[i] = *(const float4*)(weight + p * c.w_ps + s);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < FOURS; ++i) {
+      const int j = (i * SEL_T + tid) * 4;
+      if (there[i]) {
+        last = max(last, kp[i].x);
+        if (j + 1 < len) last = max(last, kp[i].y);
+        if (j + 2 < len) last = max(last, kp[i].z);
+        if (j + 3 < len) last = max(last, kp[i].w);
+      }
+    }
+  } else {
 #pragma unroll 4
-  for (int j = tid; j < len; j += SEL_T) {
-    const int p = c.page_of(table, j);
-    if (p >= 0) last = max(last, posp[p * c.p_ps + c.slot_of(j)]);
+    for (int j = tid; j < len; j += SEL_T) {
+      const int p = c.page_of(table, j);
+      if (p >= 0) last = max(last, posp[p * c.p_ps + c.slot_of(j)]);
+    }
   }
 #pragma unroll
   for (int x = 32; x; x >>= 1) last = max(last, __shfl_xor(last, x, 64));
@@ -104,50 +138,61 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
   for (int w = 0; w < SEL_T / 64; ++w) last = max(last, scan[w]);
   const int64_t local = (int64_t)last - a.n_local;
 
+  auto rank = [&](int pos, float w) { return pos < a.n_global || pos > local ? FORCED : weight_word(w); };
   auto fresh = [&](int j) -> uint32_t {
     const int p = c.page_of(table, j);
     if (p < 0) return 0u;
     const int s = c.slot_of(j);
-    const int pos = posp[p * c.p_ps + s];
-    const float w = weight[p * c.w_ps + s];
-    return pos < a.n_global || pos > local ? FORCED : weight_word(w);
+    return rank(posp[p * c.p_ps + s], weight[p * c.w_ps + s]);
   };
-  auto word = [&](int j) { return IN_LDS ? words[j] : fresh(j); };
+  auto word = [&](int j) { return KEPT ? words[j] : fresh(j); };
+  // weights crowd into few bins: lanes count in COPIES tables side by side
+  auto count = [&](uint32_t bin) { atomicAdd(&hist[bin * COPIES + (tid & (COPIES - 1))], 1); };
 
   // the m-th largest word, 11 bits and then twice their rest; `left` of the words equal to it stay
   uint32_t T = 0;
   int left = m;
   for (int shift = 21, bits = 11; shift >= 0; bits = shift == 10 ? 10 : 11, shift -= bits) {
-#pragma unroll 4
-    for (int j = tid; j < len; j += SEL_T) {
-      uint32_t w;
-      if (shift == 21) {
-        w = fresh(j);
-        if (IN_LDS) words[j] = w;
-      } else {
-        w = word(j);
-        if (w >> (shift + bits) != T >> (shift + bits)) continue;
+    if (KEPT && shift == 21) {
+#pragma unroll
+      for (int i = 0; i < FOURS; ++i) {
+        const int j = (i * SEL_T + tid) * 4;
+        if (j < len) {
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          if (there[i])
+            w = make_uint4(rank(kp[i].x, kw[i].x), rank(kp[i].y, kw[i].y), rank(kp[i].z, kw[i].z), rank(kp[i].w, kw[i].w));
+          *(uint4*)(words + j) = w;
+          count(w.x >> 21);
+          if (j + 1 < len) count(w.y >> 21);
+          if (j + 2 < len) count(w.z >> 21);
+          if (j + 3 < len) count(w.w >> 21);
+        }
       }
-      atomicAdd(&hist[(w >> shift) & ((1u << bits) - 1)], 1);
+    } else {
+#pragma unroll 4
+      for (int j = tid; j < len; j += SEL_T) {
+        const uint32_t w = word(j);
+        if (shift == 21 || w >> (shift + bits) == T >> (shift + bits)) count((w >> shift) & ((1u << bits) - 1));
+      }
     }
     __syncthreads();
     // the bins from the top, BINS / SEL_T a thread: the one in which the left-th word lies
     int mine[BINS / SEL_T], sum = 0, total;
 #pragma unroll
     for (int i = 0; i < BINS / SEL_T; ++i) {
-      mine[i] = hist[BINS - 1 - (tid * (BINS / SEL_T) + i)];
+      int4* h = (int4*)&hist[(BINS - 1 - (tid * (BINS / SEL_T) + i)) * COPIES];
+      mine[i] = (h->x + h->y) + (h->z + h->w);
       sum += mine[i];
+      *h = make_int4(0, 0, 0, 0);
     }
     int above = block_prefix(sum, scan, total);
 #pragma unroll
     for (int i = 0; i < BINS / SEL_T; ++i) {
-      const int d = BINS - 1 - (tid * (BINS / SEL_T) + i);
       if (above < left && above + mine[i] >= left) {
-        pick[0] = d;
+        pick[0] = BINS - 1 - (tid * (BINS / SEL_T) + i);
         pick[1] = left - above;
       }
       above += mine[i];
-      hist[d] = 0;
     }
     __syncthreads();
     T |= (uint32_t)pick[0] << shift;
@@ -205,21 +250,25 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
   move_rows(a, hk, b, a.counts[b * a.c.Hkv + hk], blockIdx.x * per, gridDim.x * per, threadIdx.x);
 }
 
-template <bool IN_LDS, bool INLINE>
+template <bool KEPT, bool INLINE>
 hipError_t launch_select(const EvictArgs& a, size_t lds, hipStream_t st) {
-  hipError_t e = hipFuncSetAttribute((const void*)evict_select_kernel<IN_LDS, INLINE>,
-                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  if (e != hipSuccess) return e;
-  evict_select_kernel<IN_LDS, INLINE><<<dim3(a.c.Hkv, a.c.B), SEL_T, lds, st>>>(a);
+  if (lds > 24 * 1024) {                               // with the static tables beyond the 64 KB of any launch
+    hipError_t e = hipFuncSetAttribute((const void*)evict_select_kernel<KEPT, INLINE>,
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  evict_select_kernel<KEPT, INLINE><<<dim3(a.c.Hkv, a.c.B), SEL_T, lds, st>>>(a);
   return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_evict(const EvictArgs& a, hipStream_t st) {
-  const bool in_lds = a.c.cap <= LDS_KEYS, few = a.moves <= INLINE_MOVES;
-  const size_t lds = in_lds ? (size_t)a.c.cap * 4 : 0;
-  hipError_t e = in_lds ? (few ? launch_select<true, true>(a, lds, st) : launch_select<true, false>(a, lds, st))
+  const bool fours = a.c.shift >= 2 && ((a.c.w_ps | a.c.w_hs | a.c.p_ps | a.c.p_hs) & 3) == 0 &&
+                     (((uintptr_t)a.c.weight | (uintptr_t)a.c.pos) & 15) == 0;
+  const bool kept = a.c.cap <= LDS_KEYS && fours, few = a.moves <= INLINE_MOVES;
+  const size_t lds = kept ? (size_t)(a.c.cap + 3) / 4 * 16 : 0;
+  hipError_t e = kept ? (few ? launch_select<true, true>(a, lds, st) : launch_select<true, false>(a, lds, st))
                         : (few ? launch_select<false, true>(a, lds, st) : launch_select<false, false>(a, lds, st));
   if (e != hipSuccess || few) return e;
   const int per = 256 / (a.row_bytes / 16);
