@@ -48,15 +48,15 @@ __device__ __forceinline__ int block_prefix(int x, int* lds, int& total) {
   return before + incl - x;
 }
 
-// A row's worth of lanes moves a key's row and its value's, r-th of n, with weight and pos.
-__device__ __forceinline__ void move_rows(const EvictArgs& a, int hk, int b, int n, int r0, int step, int tid) {
+// A row's worth of lanes moves a key's row and its value's, r-th of n, with weight and pos; from and to: the slots.
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int hk, int b, const int* from, const int* to, int n,
+                                          int r0, int step, int tid) {
   const CacheView& c = a.c;
   const int chunks = a.row_bytes / 16, at = tid % chunks * 16;
-  const int64_t list = (int64_t)(b * c.Hkv + hk) * a.moves;
   const int32_t* table = c.table + (int64_t)b * c.t_stride;
   const int32_t* out_table = a.dst_table ? a.dst_table + (int64_t)b * a.dst_stride : table;
   for (int r = r0 + tid / chunks; r < n; r += step) {
-    const int j = a.from[list + r], i = a.dst_table ? r : a.to[list + r];
+    const int j = from[r], i = a.dst_table ? r : to[r];
     if (a.dst_table && i >= a.dst_cap) break;
     const int p = c.page_of(table, j), g = c.page_of(out_table, i);
     if (p < 0 || g < 0) continue;
@@ -82,6 +82,32 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
   __shared__ int hist[BINS * COPIES], scan[SEL_T / 64], pick[2];
   const CacheView& c = a.c;
   const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  __shared__ int moved[2][INLINE ? INLINE_MOVES : 1];
+  const int32_t* table = c.table + (int64_t)b * c.t_stride;
+  const float* weight = c.weight + hk * c.w_hs;
+  const int32_t* posp = c.pos + hk * c.p_hs;
+  int last = INT32_MIN;
+  int4 kp[KEPT ? FOURS : 1];
+  float4 kw[KEPT ? FOURS : 1];
+  bool there[KEPT ? FOURS : 1];
+  if constexpr (KEPT) {
+    // not waiting for the length: what a page holds behind it can be read
+#pragma unroll
+    for (int i = 0; i < FOURS; ++i) {
+      const int j = (i * SEL_T + tid) * 4;
+      there[i] = false;
+      if (i * SEL_T * 4 < c.cap) {
+        const int p = j < c.cap ? c.page_of(table, j) : -1;
+        const int s = c.slot_of(j);
+        there[i] = p >= 0;
+        if (there[i]) {
+          kp[i] = *(const int4*)(posp + p * c.p_ps + s);
+          kw[i] = *(const float4*)(weight + p * c.w_ps + s);
+        }
+      }
+    }
+  }
+  for (int i = tid; i < BINS * COPIES; i += SEL_T) hist[i] = 0;
   const int len = c.len(b), m = min(len, a.budget);
   const int seg = b * c.Hkv + hk;
   if (hk == 0 && tid == 0) a.new_lens[b] = m;
@@ -90,33 +116,11 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
     if (tid == 0) a.counts[seg] = 0;
     return;
   }
-  const int32_t* table = c.table + (int64_t)b * c.t_stride;
-  const float* weight = c.weight + hk * c.w_hs;
-  const int32_t* posp = c.pos + hk * c.p_hs;
-  for (int i = tid; i < BINS * COPIES; i += SEL_T) hist[i] = 0;
-  int last = INT32_MIN;
-  int4 kp[KEPT ? FOURS : 1];
-  float4 kw[KEPT ? FOURS : 1];
-  bool there[KEPT ? FOURS : 1];
   if constexpr (KEPT) {
 #pragma unroll
     for (int i = 0; i < FOURS; ++i) {
       const int j = (i * SEL_T + tid) * 4;
-      there[i] = false;
-      if (i * SEL_T * 4 < len) {
-        const int p = c.page_of(table, min(j, len - 1));
-        there[i] = p >= 0 && j < len;
-        const int s = c.slot_of(j);
-        if (there[i]) {
-          kp[i] = *(const int4*)(posp + p * c.p_ps + s);
-          kw[i] = *(const float4*)(weight + p * c.w_ps + s);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < FOURS; ++i) {
-      const int j = (i * SEL_T + tid) * 4;
-      if (there[i]) {
+      if (there[i] && j < len) {
         last = max(last, kp[i].x);
         if (j + 1 < len) last = max(last, kp[i].y);
         if (j + 2 < len) last = max(last, kp[i].z);
@@ -202,8 +206,8 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
 
   // who stays, in the order of the slots, PER consecutive ones a thread
   int ties = 0, n_from = 0, n_to = 0;
-  int32_t* from = a.from + (int64_t)seg * a.moves;
-  int32_t* to = a.to + (int64_t)seg * a.moves;
+  int32_t* from = INLINE ? moved[0] : a.from + (int64_t)seg * a.moves;
+  int32_t* to = INLINE ? moved[1] : a.to + (int64_t)seg * a.moves;
   for (int j0 = 0; j0 < len; j0 += SEL_T * PER) {
     const int j = j0 + tid * PER;
     uint32_t above = 0, equal = 0;                     // a bit a key
@@ -237,9 +241,8 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
   }
   n_from = min(n_from, a.moves);
   if (INLINE) {
-    __threadfence_block();
     __syncthreads();
-    move_rows(a, hk, b, n_from, 0, SEL_T / (a.row_bytes / 16), tid);
+    move_rows(a, hk, b, from, to, n_from, 0, SEL_T / (a.row_bytes / 16), tid);
   } else if (tid == 0) {
     a.counts[seg] = n_from;
   }
@@ -247,7 +250,9 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
 
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
   const int hk = blockIdx.y, b = blockIdx.z, per = 256 / (a.row_bytes / 16);
-  move_rows(a, hk, b, a.counts[b * a.c.Hkv + hk], blockIdx.x * per, gridDim.x * per, threadIdx.x);
+  const int64_t seg = (int64_t)b * a.c.Hkv + hk;
+  move_rows(a, hk, b, a.from + seg * a.moves, a.to + seg * a.moves, a.counts[seg], blockIdx.x * per, gridDim.x * per,
+            threadIdx.x);
 }
 
 template <bool KEPT, bool INLINE>

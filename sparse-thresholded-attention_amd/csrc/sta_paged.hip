@@ -745,55 +745,60 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
   if (lane == 0) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l * (1.f / T::P_SCALE));
 }
 
-// The weights that a step's rows give the keys of a kv head: a workgroup takes 256 keys, its waves the rows in
-// turn, four keys a lane; the waves' sums are added in order.  Reads each score once.
+// The weights that a step's rows give the keys of a kv head, from their scores: four keys a lane, 256 a wave.  SHARED: the
+// four waves of a workgroup take the rows of 256 keys in turn, and their sums are added in order (many rows); else each
+// has keys of its own.
+template <bool SHARED>
 __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
-  constexpr int ROWS = 256;
-  __shared__ float lse[ROWS];
-  __shared__ floatx4 sums[4][64];
+  __shared__ floatx4 sums[SHARED ? 4 : 1][64];
   const CacheView& c = a.c;
-  const int b = blockIdx.z, hk = blockIdx.y, j0 = blockIdx.x * 256, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int len = c.len(b);
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int b = blockIdx.z, hk = blockIdx.y, j0 = SHARED ? blockIdx.x * 256 : (blockIdx.x * 4 + wave) * 256;
+  const int len = uniform(c.len(b));
   if (j0 >= len) return;
   const int rows = a.H / c.Hkv * a.Q;
   const int64_t row0 = ((int64_t)b * c.Hkv + hk) * rows;
   const int j = j0 + lane * 4;
   const bool all = j0 + 256 <= common(a, b);           // every row sees every key
+  const float* s = a.scores + row0 * a.score_stride + j;
   floatx4 sum = floatx4{0.f, 0.f, 0.f, 0.f};
-  for (int r0 = 0; r0 < rows; r0 += ROWS) {
-    const int n = min(rows - r0, ROWS);
-    __syncthreads();
-    // a row that saw nothing has lse -inf: 0 for every key
-    if (tid < n) lse[tid] = a.lse[row0 + r0 + tid];
-    __syncthreads();
-    const float* s = a.scores + (row0 + r0) * a.score_stride + j;
-    if (all) {
+  constexpr int STEP = SHARED ? 4 : 1;
+  const int first = SHARED ? wave : 0;
+  if (all) {
 #pragma unroll 4
-      for (int r = wave; r < n; r += 4) {
-        const floatx4 x = *(const floatx4*)(s + r * a.score_stride);
-        const float z = lse[r];
+    for (int r = first; r < rows; r += STEP) {
+      const floatx4 x = *(const floatx4*)(s + r * a.score_stride);
+      const float z = a.lse[row0 + r];                 // -inf: the row saw nothing, and gives nothing
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += z == -INFINITY ? 0.f : exp_of(x[e] - z);
-      }
-    } else {
-      for (int r = wave; r < n; r += 4) {
-        const int end = len - (a.Q - 1 - (r0 + r) % a.Q);
-        if (j >= end) continue;                        // beyond: not written
-        const floatx4 x = *(const floatx4*)(s + r * a.score_stride);
-        const float z = lse[r];
+      for (int e = 0; e < 4; ++e) sum[e] += z == -INFINITY ? 0.f : exp_of(x[e] - z);
+    }
+  } else {
+    for (int r = first; r < rows; r += STEP) {
+      const int end = len - (a.Q - 1 - r % a.Q);
+      if (j >= end) continue;                          // beyond: not written
+      const floatx4 x = *(const floatx4*)(s + r * a.score_stride);
+      const float z = a.lse[row0 + r];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += j + e >= end || z == -INFINITY ? 0.f : exp_of(x[e] - z);
-      }
+      for (int e = 0; e < 4; ++e) sum[e] += j + e >= end || z == -INFINITY ? 0.f : exp_of(x[e] - z);
     }
   }
-  sums[wave][lane] = sum;
-  __syncthreads();
-  const int mine = j0 + tid;
-  if (mine >= len) return;
-  const int p = c.page_of(c.table + (int64_t)b * c.t_stride, mine);
-  if (p < 0) return;
-  const float* w = (const float*)sums;
-  c.weight[p * c.w_ps + hk * c.w_hs + c.slot_of(mine)] += (w[tid] + w[256 + tid]) + (w[512 + tid] + w[768 + tid]);
+  const int32_t* table = c.table + (int64_t)b * c.t_stride;
+  if constexpr (SHARED) {
+    sums[wave][lane] = sum;
+    __syncthreads();
+    const int mine = j0 + tid;
+    if (mine >= len) return;
+    const int p = c.page_of(table, mine);
+    const float* w = (const float*)sums;
+    if (p >= 0)
+      c.weight[p * c.w_ps + hk * c.w_hs + c.slot_of(mine)] += (w[tid] + w[256 + tid]) + (w[512 + tid] + w[768 + tid]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int p = j + e < len ? c.page_of(table, j + e) : -1;
+      if (p >= 0) c.weight[p * c.w_ps + hk * c.w_hs + c.slot_of(j + e)] += sum[e];
+    }
+  }
 }
 
 // The same from the scores formed again, where a kv head has many rows (PagedCut::reform): a wave holds 64 keys
@@ -908,7 +913,8 @@ hipError_t launch_attend(const PagedArgs& a, const PagedCut& cut, hipStream_t st
       return hipGetLastError();
     }
   }
-  paged_weight_kernel<<<dim3((a.c.cap + 255) / 256, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
+  if (a.H / a.c.Hkv * a.Q > 16) paged_weight_kernel<true><<<dim3((a.c.cap + 255) / 256, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
+  else paged_weight_kernel<false><<<dim3((a.c.cap + 1023) / 1024, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
   return hipGetLastError();
 }
 
