@@ -3,7 +3,7 @@
 // Every kv head of a sequence keeps m = min(len, budget) keys.  A key's rank is one 32-bit word,
 // larger first: all ones for a forced key (pos < n_global or pos > largest pos - n_local), else
 // its weight's bits in an order-preserving form (NaN above +inf, -0 as +0), 0 for a key without a
-// page.  The m-th largest word T comes from three counting passes over 11, 11 and 10 bits; a key stays if
+// page.  The m-th largest word T comes from three counting passes over 10, 11 and 11 bits; a key stays if
 // its word is above T, or equal to T and among the first of those by slot.
 //
 // The kept keys need no order in a cache that stores rotated keys, so in place only the kept keys
@@ -19,7 +19,7 @@ namespace {
 constexpr int SEL_T = 1024;
 constexpr int BINS = 2048;             // of a counting pass
 constexpr int PER = 8;                 // consecutive keys of a thread
-constexpr int COPIES = 4;              // of the counting table, one int4 a bin
+constexpr int COPIES = 4;              // of the counting table
 constexpr int LDS_KEYS = 28672;        // 112 KB of words
 constexpr int FOURS = LDS_KEYS / 4 / SEL_T;
 constexpr int INLINE_MOVES = 64;       // rows a head that the selecting workgroup moves itself
@@ -150,14 +150,17 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
     return rank(posp[p * c.p_ps + s], weight[p * c.w_ps + s]);
   };
   auto word = [&](int j) { return KEPT ? words[j] : fresh(j); };
-  // weights crowd into few bins: lanes count in COPIES tables side by side
-  auto count = [&](uint32_t bin) { atomicAdd(&hist[bin * COPIES + (tid & (COPIES - 1))], 1); };
+  // weights crowd into few bins of the first pass: lanes count in 8 tables side by side, then in 4 of twice the bins
+  auto count = [&](uint32_t bin, int copies) { atomicAdd(&hist[bin * copies + (tid & (copies - 1))], 1); };
 
-  // the m-th largest word, 11 bits and then twice their rest; `left` of the words equal to it stay
+  // the m-th largest word, 10 bits, 11 and 11; `left` of the words equal to it stay
   uint32_t T = 0;
   int left = m;
-  for (int shift = 21, bits = 11; shift >= 0; bits = shift == 10 ? 10 : 11, shift -= bits) {
-    if (KEPT && shift == 21) {
+#pragma unroll
+  for (int shift = 22; shift >= 0; shift -= 11) {
+    const bool top = shift == 22;
+    const int copies = top ? 2 * COPIES : COPIES, bins = top ? BINS / 2 : BINS;
+    if (KEPT && top) {
 #pragma unroll
       for (int i = 0; i < FOURS; ++i) {
         const int j = (i * SEL_T + tid) * 4;
@@ -166,34 +169,31 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
           if (there[i])
             w = make_uint4(rank(kp[i].x, kw[i].x), rank(kp[i].y, kw[i].y), rank(kp[i].z, kw[i].z), rank(kp[i].w, kw[i].w));
           *(uint4*)(words + j) = w;
-          count(w.x >> 21);
-          if (j + 1 < len) count(w.y >> 21);
-          if (j + 2 < len) count(w.z >> 21);
-          if (j + 3 < len) count(w.w >> 21);
+          count(w.x >> 22, copies);
+          if (j + 1 < len) count(w.y >> 22, copies);
+          if (j + 2 < len) count(w.z >> 22, copies);
+          if (j + 3 < len) count(w.w >> 22, copies);
         }
       }
     } else {
 #pragma unroll 4
       for (int j = tid; j < len; j += SEL_T) {
         const uint32_t w = word(j);
-        if (shift == 21 || w >> (shift + bits) == T >> (shift + bits)) count((w >> shift) & ((1u << bits) - 1));
+        if (top || w >> (shift + 11) == T >> (shift + 11)) count((w >> shift) & (bins - 1), copies);
       }
     }
     __syncthreads();
-    // the bins from the top, BINS / SEL_T a thread: the one in which the left-th word lies
-    int mine[BINS / SEL_T], sum = 0, total;
+    // 8 numbers a thread, from the top: one bin of 8 copies or two of 4; the bin in which the left-th word lies
+    int4* h = (int4*)&hist[(SEL_T - 1 - tid) * 8];
+    const int4 low = h[0], high = h[1];
+    h[0] = h[1] = make_int4(0, 0, 0, 0);
+    int mine[2] = {(high.x + high.y) + (high.z + high.w), (low.x + low.y) + (low.z + low.w)}, total;
+    if (top) mine[0] += mine[1], mine[1] = 0;
+    int above = block_prefix(mine[0] + mine[1], scan, total);
 #pragma unroll
-    for (int i = 0; i < BINS / SEL_T; ++i) {
-      int4* h = (int4*)&hist[(BINS - 1 - (tid * (BINS / SEL_T) + i)) * COPIES];
-      mine[i] = (h->x + h->y) + (h->z + h->w);
-      sum += mine[i];
-      *h = make_int4(0, 0, 0, 0);
-    }
-    int above = block_prefix(sum, scan, total);
-#pragma unroll
-    for (int i = 0; i < BINS / SEL_T; ++i) {
+    for (int i = 0; i < 2; ++i) {
       if (above < left && above + mine[i] >= left) {
-        pick[0] = BINS - 1 - (tid * (BINS / SEL_T) + i);
+        pick[0] = top ? SEL_T - 1 - tid : 2 * (SEL_T - 1 - tid) + 1 - i;
         pick[1] = left - above;
       }
       above += mine[i];
