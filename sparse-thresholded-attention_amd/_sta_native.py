@@ -1471,7 +1471,7 @@ def _ints(x, dev):
     """A device int32 tensor with unit stride in its last dim."""
     if x.dtype != torch.int32 or x.device != dev:
         x = x.to(device=dev, dtype=torch.int32)
-    return x if x.stride(-1) == 1 else x.contiguous()
+    return x if x.stride(-1) == 1 else x.contiguous()      # lens of stride 0 (expanded) too
 
 
 class PagedCache:
@@ -1535,15 +1535,21 @@ class PagedCache:
         return most if max_len is None else min(int(max_len), most)
 
 
+def _empty_as(x):
+    """A contiguous tensor of x's shape, dtype and device (empty_like, the cheaper call, keeps strides)."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1.0, inverse=False):
     """sta_rotary of q (T, H, D) and k (T, Hkv, D) or None -> their rotations."""
     _device_input(q, "q")
     dev = q.device
-    _require(q.dim() == 3, f"q must be (T, heads, D), not {tuple(q.shape)}")
+    if q.dim() != 3:
+        raise ValueError(f"q must be (T, heads, D), not {tuple(q.shape)}")
     q = _rows(q)
     T, H, D = q.shape
     a = RotaryArgsC()
-    q_out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+    q_out = _empty_as(q)
     a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
     a.q_tok_stride, a.q_head_stride, _ = q.stride()
     a.q_out_tok_stride, a.q_out_head_stride = H * D, D
@@ -1551,30 +1557,36 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
     if k is not None:
         if k.dtype != q.dtype:
             raise TypeError("q and k must share one dtype")
-        _require(k.dim() == 3 and k.shape[0] == T and k.shape[2] == D, f"k must be ({T}, kv heads, {D})")
-        k = _rows(k.to(dev))
-        a.Hkv = k.shape[1]
-        k_out = torch.empty((T, a.Hkv, D), dtype=q.dtype, device=dev)
+        if k.dim() != 3 or k.shape[0] != T or k.shape[2] != D:
+            raise ValueError(f"k must be ({T}, kv heads, {D}), not {tuple(k.shape)}")
+        k = _rows(k if k.device == dev else k.to(dev))
+        a.Hkv = Hkv = k.shape[1]
+        k_out = _empty_as(k)
         a.k, a.k_out = k.data_ptr(), k_out.data_ptr()
         a.k_tok_stride, a.k_head_stride, _ = k.stride()
-        a.k_out_tok_stride, a.k_out_head_stride = a.Hkv * D, D
-    if positions.dtype not in POS_TYPES:
+        a.k_out_tok_stride, a.k_out_head_stride = Hkv * D, D
+    a.pos_type = pos_type = POS_TYPES.get(positions.dtype, -1)
+    if pos_type < 0:
         raise TypeError(f"positions must be int32, int64 or float32, not {positions.dtype}")
-    positions = positions.to(dev)
-    if positions.dim() == 1:
-        positions = positions[None]
+    if positions.device != dev:
+        positions = positions.to(dev)
     if inv_freq.dtype != torch.float32 or inv_freq.device != dev or not inv_freq.is_contiguous():
         inv_freq = inv_freq.to(device=dev, dtype=torch.float32).contiguous()
-    sections = (inv_freq.numel(),) if sections is None else tuple(int(s) for s in sections)
-    _require(len(sections) <= 4, "at most 4 axes")
-    _require(tuple(positions.shape) == (len(sections), T), f"positions must be ({len(sections)}, {T})")
-    _require(sum(sections) == inv_freq.numel(), f"sections {sections} do not share out {inv_freq.numel()} frequencies")
-    a.dtype, a.T, a.H, a.D, a.axes = DTYPES[q.dtype], T, H, D, len(sections)
-    a.section[:len(sections)] = sections
-    a.positions, a.pos_type = positions.data_ptr(), POS_TYPES[positions.dtype]
-    a.pos_axis_stride, a.pos_tok_stride = positions.stride()
-    a.inv_freq, a.pos_scale, a.rope_scale = inv_freq.data_ptr(), float(pos_scale), float(rope_scale)
-    a.inverse = int(inverse)
+    half = inv_freq.numel()
+    sections = (half,) if sections is None else tuple(int(s) for s in sections)
+    axes = len(sections)
+    _require(1 <= axes <= 4, "1 to 4 axes")
+    _require(sum(sections) == half, f"sections {sections} do not share out {half} frequencies")
+    if positions.dim() == 1 and axes == 1 and positions.shape[0] == T:
+        a.pos_tok_stride = positions.stride(0)
+    elif tuple(positions.shape) == (axes, T):
+        a.pos_axis_stride, a.pos_tok_stride = positions.stride()
+    else:
+        raise ValueError(f"positions must be ({axes}, {T}), not {tuple(positions.shape)}")
+    a.dtype, a.T, a.H, a.D, a.axes = DTYPES[q.dtype], T, H, D, axes
+    a.section[:axes] = sections
+    a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
+    a.pos_scale, a.rope_scale, a.inverse = float(pos_scale), float(rope_scale), int(inverse)
     _launch(lib().sta_rotary, a, dev, "sta_rotary")
     return q_out, k_out
 
@@ -1585,9 +1597,9 @@ def cache_append(cache, k, v, table, lens, starts=None, seen=None):
     dev = cache.device
     if k.dtype != cache.k.dtype or v.dtype != cache.k.dtype:
         raise TypeError("k, v and the cache must share one dtype")
-    _require(k.dim() == 3 and k.shape[1:] == (cache.kv_heads, cache.head_dim) and v.shape == k.shape,
-             f"k and v must be (T, {cache.kv_heads}, {cache.head_dim})")
-    k, v = _rows(k.to(dev)), _rows(v.to(dev))
+    if k.dim() != 3 or k.shape[1:] != (cache.kv_heads, cache.head_dim) or v.shape != k.shape:
+        raise ValueError(f"k and v must be (T, {cache.kv_heads}, {cache.head_dim})")
+    k, v = _rows(k if k.device == dev else k.to(dev)), _rows(v if v.device == dev else v.to(dev))
     a = AppendArgsC()
     keep = cache._fill(a, table, lens)
     B = a.cache.B
@@ -1602,7 +1614,7 @@ def cache_append(cache, k, v, table, lens, starts=None, seen=None):
         seen = _ints(seen, dev)
         _require(tuple(seen.shape) == (B,), f"seen must be ({B},)")
         a.seen = seen.data_ptr()
-    new_lens = torch.empty(B, dtype=torch.int32, device=dev)
+    new_lens = torch.empty_like(keep[1])
     a.new_lens = new_lens.data_ptr()
     _launch(lib().sta_cache_append, a, dev, "sta_cache_append")
     del keep
@@ -1616,18 +1628,22 @@ def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want
     dev = cache.device
     if q.dtype != cache.k.dtype:
         raise TypeError("q and the cache must share one dtype")
-    _require(q.dim() in (3, 4) and q.shape[-1] == cache.head_dim,
-             f"q must be (B, heads, {cache.head_dim}) or (B, heads, queries, {cache.head_dim})")
+    if q.dim() not in (3, 4) or q.shape[-1] != cache.head_dim:
+        raise ValueError(f"q must be (B, heads, {cache.head_dim}) or (B, heads, queries, {cache.head_dim})")
     shape = q.shape
-    q = _rows((q if q.dim() == 4 else q.unsqueeze(2)).to(dev))
+    q = _rows(q if q.device == dev else q.to(dev))
     a = PagedArgsC()
     table, lens = cache._fill(a, table, lens)
-    _require(shape[0] == a.cache.B, f"q holds {shape[0]} sequences, table {a.cache.B}")
-    a.q, a.H, a.Q = q.data_ptr(), q.shape[1], q.shape[2]
-    a.q_batch_stride, a.q_head_stride, a.q_tok_stride, _ = q.stride()
+    _require(shape[0] == a.cache.B, "q and table must hold the same number of sequences")
+    a.q, a.H, a.Q = q.data_ptr(), shape[1], 1
+    if len(shape) == 4:
+        a.Q = shape[2]
+        a.q_batch_stride, a.q_head_stride, a.q_tok_stride, _ = q.stride()
+    else:
+        a.q_batch_stride, a.q_head_stride, _ = q.stride()
     a.sm_scale = 1.0 / math.sqrt(cache.head_dim) if sm_scale is None else float(sm_scale)
     a.max_len, a.accumulate = cache._max_len(table, max_len), int(bool(accumulate))
-    out = torch.empty(shape, dtype=q.dtype, device=dev)
+    out = _empty_as(q)
     a.out = out.data_ptr()
     lse = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if want_lse else None
     a.lse = _ptr(lse)
@@ -1652,7 +1668,7 @@ def cache_evict(cache, table, lens, budget, n_global=32, n_local=32, dst_table=N
         _require(dst_table.dim() == 2 and dst_table.shape[0] == a.cache.B, "dst_table must have a row a sequence")
         a.dst_table, a.dst_width = dst_table.data_ptr(), dst_table.shape[1]
         a.dst_stride = dst_table.stride(0)
-    new_lens = torch.empty(a.cache.B, dtype=torch.int32, device=dev)
+    new_lens = torch.empty_like(lens)
     a.new_lens = new_lens.data_ptr()
     n = lib().sta_evict_workspace_size(ctypes.byref(a))
     if n == 0:
