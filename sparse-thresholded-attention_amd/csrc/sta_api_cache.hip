@@ -247,7 +247,7 @@ int sta_cache_append(const sta_append_args* a, void* stream) {
   d.v_ts = a->v_tok_stride * es;
   d.v_hs = a->v_head_stride * es;
   d.T = a->T;
-  d.row_bytes = (int)(a->cache.D * es);
+  while ((16 << d.row_shift) < a->cache.D * es) ++d.row_shift;
   d.starts = a->starts;
   d.seen = a->seen;
   d.new_lens = a->new_lens;

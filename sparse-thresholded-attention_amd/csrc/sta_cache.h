@@ -36,7 +36,7 @@ struct AppendArgs {
   const char* k;
   const char* v;
   int64_t k_ts, k_hs, v_ts, v_hs;   // bytes
-  int T, row_bytes;
+  int T, row_shift;                 // a row is 16 << row_shift bytes
   const int32_t* starts;
   const int32_t* seen;
   int32_t* new_lens;

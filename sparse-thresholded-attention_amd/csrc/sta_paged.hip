@@ -12,46 +12,75 @@ namespace sta {
 
 namespace {
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
+
 // ------------------------------------------------------------------------------------------
-// append: one thread moves 16 bytes of a key and of its value
+// append: a wave per token moves the rows of all kv heads, 16 bytes a lane, two keys' and two values' in flight.  Bound
+// by memory.
 // ------------------------------------------------------------------------------------------
+// the last sequence that starts at or before t (64 candidates at once), -1: none
+__device__ __forceinline__ int sequence_of(const int32_t* starts, int B, int t) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = B;
+  for (;;) {
+    const int step = (n + 63) / 64, at = lo + lane * step;
+    const int below = __popcll(__ballot(at < lo + n && starts[min(at, B)] <= t));
+    if (below == 0) return lo - 1;
+    const int end = lo + n;
+    lo += (below - 1) * step;
+    if (step == 1) return lo;
+    n = min(step, end - lo);
+  }
+}
+
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const CacheView& c = a.c;
-  const int chunks = a.row_bytes / 16;
   if (blockIdx.x == 0) {
     for (int b = threadIdx.x; b < c.B; b += 256) {
       const int n = a.starts ? max(a.starts[b + 1] - a.starts[b], 0) : 1;
       a.new_lens[b] = (int)min((int64_t)c.len(b) + n, (int64_t)c.cap);
     }
   }
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = gid / chunks;
-  if (row >= (int64_t)a.T * c.Hkv) return;
-  const int at = (int)(gid - row * chunks) * 16;
-  const int t = (int)(row / c.Hkv), h = (int)(row - (int64_t)t * c.Hkv);
+  const int t = blockIdx.x * 4 + uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (t >= a.T) return;
   int b = t, i = 0;
   if (a.starts) {
-    // the last sequence that starts at or before t
-    int lo = 0, hi = c.B;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (a.starts[mid] <= t) lo = mid + 1;
-      else hi = mid;
-    }
-    b = lo - 1;
+    b = uniform(sequence_of(a.starts, c.B, t));
     if (b < 0 || t >= a.starts[b + 1]) return;
     i = t - a.starts[b];
   }
-  const int64_t j = (int64_t)c.len(b) + i;
-  if (j >= c.cap) return;
-  const int p = c.page_of(c.table + (int64_t)b * c.t_stride, (int)j);
+  const int64_t at = (int64_t)c.len(b) + i;
+  if (i < 0 || at >= c.cap) return;
+  const int j = (int)at, p = uniform(c.page_of(c.table + (int64_t)b * c.t_stride, j));
   if (p < 0) return;
-  const int s = c.slot_of((int)j);
-  *(u32x4*)(c.k + p * c.k_ps + h * c.k_hs + s * c.k_ss + at) = *(const u32x4*)(a.k + t * a.k_ts + h * a.k_hs + at);
-  *(u32x4*)(c.v + p * c.v_ps + h * c.v_hs + s * c.v_ss + at) = *(const u32x4*)(a.v + t * a.v_ts + h * a.v_hs + at);
-  if (at == 0) {
+  const int s = c.slot_of(j), shift = a.row_shift, all = c.Hkv << shift;
+  const char* k = a.k + t * a.k_ts;
+  const char* v = a.v + t * a.v_ts;
+  char* ko = c.k + p * c.k_ps + s * c.k_ss;
+  char* vo = c.v + p * c.v_ps + s * c.v_ss;
+  const int mask = (1 << shift) - 1;
+  for (int x = lane; x < all; x += 128) {
+    const int h0 = x >> shift, h1 = min(x + 64, all - 1) >> shift, w = (x & mask) * 16, w1 = ((x + 64) & mask) * 16;
+    const bool more = x + 64 < all;
+    const u32x4 k0 = *(const u32x4*)(k + h0 * a.k_hs + w), v0 = *(const u32x4*)(v + h0 * a.v_hs + w);
+    u32x4 k1, v1;
+    if (more) {
+      k1 = *(const u32x4*)(k + h1 * a.k_hs + w1);
+      v1 = *(const u32x4*)(v + h1 * a.v_hs + w1);
+    }
+    *(u32x4*)(ko + h0 * c.k_hs + w) = k0;
+    *(u32x4*)(vo + h0 * c.v_hs + w) = v0;
+    if (more) {
+      *(u32x4*)(ko + h1 * c.k_hs + w1) = k1;
+      *(u32x4*)(vo + h1 * c.v_hs + w1) = v1;
+    }
+  }
+  for (int h = lane; h < c.Hkv; h += 64) {
     if (c.weight) c.weight[p * c.w_ps + h * c.w_hs + s] = 0.f;
-    if (c.pos) c.pos[p * c.p_ps + h * c.p_hs + s] = (a.seen ? a.seen[b] : (int)j - i) + i;
+    if (c.pos) c.pos[p * c.p_ps + h * c.p_hs + s] = (a.seen ? a.seen[b] : j - i) + i;
   }
 }
 
@@ -88,11 +117,6 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
 // whole part of x / y, 0 <= x < 2^40, 1 <= y < 2^40 (the quotient's distance from a whole number above it is
 // at least 1 / y, beyond the rounding of the division)
 __device__ __forceinline__ int div40(int64_t x, int64_t y) { return (int)((double)x / (double)y); }
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
-}
-
 __device__ __forceinline__ int units_of(int keys, int unit) { return max(1, (keys + unit - 1) / unit); }
 
 // keys that every query of sequence b sees
@@ -927,8 +951,7 @@ hipError_t launch_rows(const PagedArgs& a, const PagedCut& cut, hipStream_t st) 
 }  // namespace
 
 hipError_t launch_append(const AppendArgs& a, hipStream_t st) {
-  const int64_t threads = (int64_t)a.T * a.c.Hkv * (a.row_bytes / 16);
-  const unsigned blocks = (unsigned)((threads + 255) / 256);
+  const unsigned blocks = ((unsigned)a.T + 3) / 4;
   append_kernel<<<blocks ? blocks : 1, 256, 0, st>>>(a);
   return hipGetLastError();
 }
