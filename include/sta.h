@@ -638,6 +638,7 @@ typedef struct sta_paged_args {
   size_t workspace_bytes;
 } sta_paged_args;
 
+/* 1: the call needs none, and workspace may be NULL */
 size_t sta_paged_workspace_size(const sta_paged_args* args);
 int sta_paged_attention(const sta_paged_args* args, void* stream);
 

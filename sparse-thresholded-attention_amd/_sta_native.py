@@ -1440,11 +1440,14 @@ POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}   # STA_POS_*
 
 def _launch(fn, args, dev, what):
     """fn on dev's current stream, with dev current while it launches."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        _check(fn(ctypes.byref(args), _stream(dev)), what)
+    index = dev.index
+    if index is None or index == torch._C._cuda_getDevice():
+        rc = fn(ctypes.byref(args), _stream(dev))
     else:
         with torch.cuda.device(dev):
-            _check(fn(ctypes.byref(args), _stream(dev)), what)
+            rc = fn(ctypes.byref(args), _stream(dev))
+    if rc != STA_OK:
+        _check(rc, what)
 
 
 def _require(ok, what):
@@ -1460,11 +1463,12 @@ def _device_input(x, name):
 
 
 def _rows(x):
-    """x with unit stride in its last dim, and 16-byte rows at strides that are not negative."""
-    esz = x.element_size()
-    if (x.stride(-1) != 1 and x.shape[-1] != 1) or x.data_ptr() % 16 or any(s * esz % 16 for s in x.stride()[:-1]):
-        x = x.contiguous()
-    return x
+    """x with unit stride in its last dim and 16-byte aligned rows."""
+    *strides, last = x.stride()
+    esz, bits = x.element_size(), x.data_ptr()
+    for s in strides:
+        bits |= s * esz
+    return x if last == 1 and not bits & 15 else x.contiguous()
 
 
 def _ints(x, dev):
@@ -1650,8 +1654,9 @@ def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want
     n = lib().sta_paged_workspace_size(ctypes.byref(a))
     if n == 0:
         _check(-1, "sta_paged_workspace_size")
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    if n > 1:                                          # 1: the call needs none
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
     _launch(lib().sta_paged_attention, a, dev, "sta_paged_attention")
     return (out, lse) if want_lse else out
 

@@ -133,8 +133,8 @@ PagedLayout paged_layout(const sta_paged_args* a) {
   off = align256(off + part_rows * a->cache.D * 4);
   L.ml_off = off;                                     // their maxima and sums
   off = align256(off + part_rows * 8);
-  L.lse_off = off;                                    // (B, H, Q) when not an output
-  off = align256(off + rows * 4);
+  L.lse_off = off;                                    // (B, H, Q) for the weights when not an output
+  if (a->accumulate && !L.cut.small) off = align256(off + rows * 4);
   L.scores_off = off;                                 // (B, H, Q, score_stride)
   if (a->accumulate && !L.cut.reform) off = align256(off + rows * L.score_stride * 4);
   L.total = off;
@@ -257,7 +257,8 @@ int sta_cache_append(const sta_append_args* a, void* stream) {
 
 size_t sta_paged_workspace_size(const sta_paged_args* a) {
   if (paged_check(a) != STA_OK) return 0;
-  return paged_layout(a).total;
+  const size_t total = paged_layout(a).total;
+  return total ? total : 1;
 }
 
 int sta_paged_attention(const sta_paged_args* a, void* stream) {
@@ -269,7 +270,7 @@ int sta_paged_attention(const sta_paged_args* a, void* stream) {
   if (!a->out || !aligned16(a->out)) return fail(STA_ERR_INVALID_ARG, "out must be non-NULL and 16-byte aligned");
   if (a->accumulate && !a->cache.weight) return fail(STA_ERR_INVALID_ARG, "accumulate needs cache.weight");
   const PagedLayout L = paged_layout(a);
-  if ((rc = check_ws(a->workspace, a->workspace_bytes, L.total)) != STA_OK) return rc;
+  if (L.total && (rc = check_ws(a->workspace, a->workspace_bytes, L.total)) != STA_OK) return rc;
   char* ws = (char*)a->workspace;
   PagedArgs d{};
   d.c = view_of(a->cache, a->max_len);
@@ -282,7 +283,7 @@ int sta_paged_attention(const sta_paged_args* a, void* stream) {
   d.sm_scale = a->sm_scale;
   d.accumulate = a->accumulate != 0;
   d.out = a->out;
-  d.lse = a->lse ? a->lse : (float*)(ws + L.lse_off);
+  d.lse = a->lse ? a->lse : a->accumulate && !L.cut.small ? (float*)(ws + L.lse_off) : nullptr;
   d.scores = a->accumulate && !L.cut.reform ? (float*)(ws + L.scores_off) : nullptr;
   d.score_stride = L.score_stride;
   d.part_o = (float*)(ws + L.part_off);

@@ -50,7 +50,7 @@ struct PagedArgs {
   float sm_scale;
   int accumulate;
   void* out;
-  float* lse;                       // (B, H, Q), the caller's or in the workspace
+  float* lse;                       // (B, H, Q), the caller's or in the workspace; NULL: not stored
   float* scores;                    // (B, H, Q, score_stride); NULL: not stored
   int64_t score_stride;
   float* part_o;                    // (records, rows, D) unnormalised outputs of unfinished row tiles, permuted

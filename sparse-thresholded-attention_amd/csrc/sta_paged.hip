@@ -479,7 +479,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
       lds.sum[row] = ll;
       lds.lse[row] = lse;
       if (!done) a.part_ml[record * T::ROWS + row] = make_float2(mm, ll);
-      else if (rr < R) a.lse[(int64_t)b * a.H + hk * G + rr] = lse;          // done: one query
+      else if (rr < R && a.lse) a.lse[(int64_t)b * a.H + hk * G + rr] = lse;   // done: one query
     }
     for (int w = 0; w < NW; w += 4) {                  // four waves' sums at a time
       if (wave / 4 == w / 4) {
@@ -661,7 +661,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
   const int64_t row_out = (int64_t)b * a.H + h;
   if (tid < D)
     store_elem<DT>(a.out, row_out * D + tid, l == 0.f ? 0.f : ((o[0][tid] + o[1][tid]) + (o[2][tid] + o[3][tid])) / l);
-  if (tid == 0) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l * (1.f / T::P_SCALE));
+  if (tid == 0 && a.lse) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l * (1.f / T::P_SCALE));
 }
 
 // Several queries: a wave per row takes its records and then the keys behind the common ones.  The waves of a workgroup
@@ -766,7 +766,7 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
   for (int s = 32; s; s >>= 1) l += __shfl_xor(l, s, 64);
 #pragma unroll
   for (int e = 0; e < W; ++e) store_elem<DT>(a.out, row_out * D + lane * W + e, l == 0.f ? 0.f : y[e] / l);
-  if (lane == 0) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l * (1.f / T::P_SCALE));
+  if (lane == 0 && a.lse) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l * (1.f / T::P_SCALE));
 }
 
 // The weights that a step's rows give the keys of a kv head, from their scores: four keys a lane, 256 a wave.  SHARED: the

@@ -21,7 +21,7 @@ def _cache(native, p):
     c.k_slot_stride = c.v_slot_stride = 128
     c.weight_page_stride = c.pos_page_stride = 8 * 16
     c.weight_head_stride = c.pos_head_stride = 16
-    c.table_stride, c.table_width, c.B = 32, 32, 4
+    c.table_stride, c.table_width, c.B = 512, 512, 4
     return c
 
 
@@ -43,7 +43,7 @@ def _paged(native, p):
     a.cache = _cache(native, p)
     a.q = a.out = p
     a.q_batch_stride, a.q_head_stride, a.q_tok_stride = 32 * 128, 128, 128
-    a.H, a.Q, a.sm_scale, a.max_len = 32, 1, 0.1, 512
+    a.H, a.Q, a.sm_scale, a.max_len = 32, 1, 0.1, 8192
     return a
 
 
@@ -87,10 +87,31 @@ def test_attention_refuses_a_small_workspace_and_missing_weights():
     assert native.lib().sta_paged_workspace_size(None) == 0
 
 
+def test_attention_workspace_sizes():
+    """Short calls need none; long ones two records a run; stored scores only below 65 rows a kv head."""
+    import _sta_native as native
+    buf, p = _host(native)
+
+    def size(**kw):
+        a = _paged(native, p)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return native.lib().sta_paged_workspace_size(ctypes.byref(a))
+    assert size(max_len=1024) == 1
+    records = 2 * 512 * 16 * (128 * 4 + 8)
+    assert records <= size() < records + 1024
+    scores = 4 * 32 * 8192 * 4
+    assert records + scores <= size(accumulate=1) < records + scores + 4 * 32 * 4 + 1024
+    assert size(accumulate=1, max_len=1024) == 4 * 32 * 1024 * 4
+    # 32 queries: 128 rows, four tiles, a fourth of the runs, and a record a kv head
+    rows = 4 * (2 * 128 + 8 * 4) * 32 * (128 * 4 + 8)
+    assert rows <= size(Q=32) <= size(Q=32, accumulate=1) < rows + 4 * 32 * 32 * 4 + 2048
+
+
 def _evict(native, p):
     a = native.EvictArgsC()
     a.cache = _cache(native, p)
-    a.budget, a.n_global, a.n_local, a.max_len = 100, 4, 32, 512
+    a.budget, a.n_global, a.n_local, a.max_len = 100, 4, 32, 8192
     a.new_lens = p + 1024
     a.workspace, a.workspace_bytes = p, 1 << 40
     return a
