@@ -207,6 +207,12 @@ ATTEND = [
     ([600, 33, 5], 28, 4, 32, 128, 32, F16, "slot"),
     ([170], 24, 1, 33, 128, 128, BF16, "head"),
     ([5000, 4097], 8, 2, 1, 128, 64, BF16, "head"),
+    ([1500, 7], 4, 2, 40, 128, 16, F32, "head"),              # 80 rows a kv head, fp32
+    ([3, 900], 40, 1, 1, 128, 16, F16, "slot"),               # three row tiles, one query
+    ([1024, 1023], 4, 4, 1, 64, 16, F32, "head"),
+] + [([100 + 13 * i] * 3 + [0] * (i % 2), 4, 2, 1 + i % 2, 64, 16, BF16, "head") for i in range(2)] + [
+    ([1 + (37 * i) % 90 for i in range(150)], 4, 2, 1, 64, 16, BF16, "head"),      # more sequences than lanes
+    ([1 + (37 * i) % 90 for i in range(150)] + [1200], 4, 2, 1, 64, 16, BF16, "head"),
 ]
 
 
@@ -250,7 +256,7 @@ def test_attention_of_strided_queries_scales_and_a_short_bound():
     _check_attend(made, odd, pc.paged_attention(odd, made.cache, made.table, made.lens), made.attend_ref(odd, 0.125))
 
 
-@pytest.mark.parametrize("Q,dtype", [(1, BF16), (4, BF16), (3, F32), (1, F16)])
+@pytest.mark.parametrize("Q,dtype", [(1, BF16), (4, BF16), (3, F32), (1, F16), (40, BF16), (20, F16), (40, F32)])
 def test_attention_ignores_what_it_does_not_see(Q, dtype):
     """NaN and infinities behind the sequences, in pages of no table, and in keys that the earlier
     queries of a call do not see; entries that are no page."""
@@ -271,9 +277,10 @@ def test_attention_ignores_what_it_does_not_see(Q, dtype):
         if n % 32 and int(table[i, n // 32]) >= 0 and int(table[i, n // 32]) < made.cache.pages:
             made.cache.k[int(table[i, n // 32]), :, n % 32:] = bad[i % 3]
             made.cache.v[int(table[i, n // 32]), :, n % 32:] = bad[(i + 1) % 3]
+    weight0 = made.cache.weight.clone()
     again, lse = pc.paged_attention(q, made.cache, table, made.lens, accumulate=True, want_lse=True)
     assert torch.equal(again, clean)
-    _check_attend(made, q, again, want, lse)
+    _check_attend(made, q, again, want, lse, made.cache.weight, weight0)
     # the newest key of sequence 1 is NaN: only its own query sees it
     p = int(table[1, 69 // 32])
     made.cache.v[p, :, 69 % 32] = bad[0]
@@ -417,6 +424,8 @@ EVICT = [
     ([2049, 1025], 1, 128, 1, BF16, 1, 0, 1, "head"),
     ([300, 290], 2, 64, 128, BF16, 200, 150, 150, "pair"),    # more forced keys than the budget holds
     ([5000], 1, 64, 64, F32, 4096, 16, 16, "head"),
+    ([30011, 12], 1, 64, 16, BF16, 700, 4, 32, "head"),       # words beyond LDS
+    ([20000], 2, 64, 128, BF16, 19990, 0, 5, "head"),         # few moves, found in a long sequence
 ]
 
 
@@ -448,6 +457,46 @@ def test_eviction_against_the_definition(case, move):
     assert got.tolist() == left and made.lens.tolist() == lens
     for name, x, y in zip(("k", "v", "weight", "pos"), (made.cache.k, made.cache.v, w, made.cache.pos), want):
         assert torch.equal(x.cpu().view(torch.uint8), y.view(torch.uint8)), name
+
+
+def test_eviction_with_weights_and_positions_of_any_alignment():
+    import paged_cache as pc
+    made = Made(580, [300, 64], 3, 64, 16, BF16)
+    c = made.cache
+    wide_w = torch.zeros((c.pages, 4, 19), device=DEV)
+    wide_p = torch.zeros((c.pages, 5, 17), dtype=torch.int32, device=DEV)
+    w, p = wide_w[:, 1:, 3:], wide_p[:, :3, 1:]               # strides and bases off 16 bytes
+    w.copy_(c.weight)
+    p.copy_(c.pos)
+    want = ref.evict(c.k, c.v, w, p, made.table, [300, 64], 100, 4, 8, made.cap)
+    other = pc.PagedCache(c.k, c.v, w, p)
+    pc.cache_evict(other, made.table, made.lens, 100, 4, 8)
+    for x, y in zip((c.k, c.v, w, p), want):
+        assert torch.equal(x.cpu(), y)
+    assert torch.all(wide_w[:, 0] == 0) and torch.all(wide_w[:, :, :3] == 0) and torch.all(wide_p[:, 3:] == 0)
+
+
+def test_a_long_eviction_in_a_graph():
+    import paged_cache as pc
+    made, other = Made(585, [20000, 900], 2, 64, 16, BF16), Made(585, [20000, 900], 2, 64, 16, BF16)
+    left = pc.cache_evict(made.cache, made.table, made.lens, 600, 4, 8)
+    fields = lambda m: (m.cache.k, m.cache.v, m.cache.weight, m.cache.pos)           # noqa: E731
+    start = [x.clone() for x in fields(other)]
+    pc.cache_evict(other.cache, other.table, other.lens, 600, 4, 8)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = pc.cache_evict(other.cache, other.table, other.lens, 600, 4, 8)
+    for _ in range(3):
+        for x, y in zip(fields(other), start):
+            x.copy_(y)
+        got.zero_()
+        pc.cache_evict(made.cache, made.table, left, 600, 4, 8)                      # eager work in between: no moves
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, left)
+        for x, y in zip(fields(other), fields(made)):
+            assert torch.equal(x, y)
 
 
 def test_eviction_of_missing_pages():
