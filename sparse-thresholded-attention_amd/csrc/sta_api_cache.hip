@@ -125,7 +125,8 @@ int paged_cap(const sta_paged_args* a) {
 PagedLayout paged_layout(const sta_paged_args* a) {
   PagedLayout L{};
   const size_t rows = (size_t)a->cache.B * a->H * a->Q;
-  L.cut = paged_cut(a->cache.dtype, a->cache.D, a->H, a->cache.Hkv, a->Q, a->cache.B, paged_cap(a));
+  L.cut = paged_cut(a->cache.dtype, a->cache.D, a->H, a->cache.Hkv, a->Q, a->cache.B, paged_cap(a),
+                    a->cache.page_size);
   L.score_stride = ((int64_t)paged_cap(a) + 255) / 256 * 256;   // whole units, and 256 keys of the weights
   const size_t part_rows = (size_t)L.cut.records * L.cut.rows;
   size_t off = 0;

@@ -53,7 +53,7 @@ struct PagedArgs {
   float* lse;                       // (B, H, Q), the caller's or in the workspace; NULL: not stored
   float* scores;                    // (B, H, Q, score_stride); NULL: not stored
   int64_t score_stride;
-  float* part_o;                    // (records, rows, D) unnormalised outputs of unfinished row tiles, permuted
+  float* part_o;                    // (records, rows, D) unnormalised outputs of unfinished row tiles
   float2* part_ml;                  // (records, rows) their maxima and sums
   int runs;
 };
@@ -62,11 +62,12 @@ struct PagedArgs {
 // kv head; `runs` runs of units of keys; `grid` workgroups, one a run and row tile
 struct PagedCut {
   int rows, tiles, runs, grid;
+  bool many;                        // 128 rows a workgroup, keys through LDS
   bool reform;                      // weights from scores formed again, not from stored ones
   bool small;                       // short sequences, one query each: one launch, nothing to join
   int64_t records;                  // of unfinished row tiles, in the workspace
 };
-PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap);
+PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap, int page_size);
 
 struct EvictArgs {
   CacheView c;

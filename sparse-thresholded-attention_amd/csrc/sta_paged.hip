@@ -234,10 +234,9 @@ __device__ __forceinline__ void load_words(int64_t p, uint32_t* w) {
   }
 }
 
-// where element (row, dim) of a 16-row tile lies in a piece's record: the accumulators of a wave as
-// they are, so that records are written 16 bytes a lane without a transpose
+// where element (row, dim) of a 16-row tile lies in a wave's accumulators, stored 16 bytes a lane as they are
 template <int VE>
-__device__ __forceinline__ int part_index(int row, int dim) {
+__device__ __forceinline__ int acc_index(int row, int dim) {
   const int e = dim % VE, m = dim / VE;                // m = 4 (lane / 16) + slot
   return ((e * 4 + m / 4) * 16 + row) * 4 + m % 4;
 }
@@ -259,6 +258,72 @@ struct MergeLds {
   floatx4 acc[4][VE * 4 * 16];
   float m[16][16 * NT], l[16][16 * NT], sum[16 * NT], lse[16 * NT];
 };
+
+// The keys of a turn into a wave's states: sc holds their scores, v their values.  EXACT: P.V in fp32 throughout.
+template <int DT, int D, int NT, bool EXACT, typename Scores, typename Values, typename State, typename Acc>
+__device__ __forceinline__ void attend_keys(Scores& sc, Values& v, State& m, State& l, Acc& acc) {
+  using T = Tile<DT, D, NT>;
+  constexpr int SUB = T::SUB, VE = T::VE;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    float top = fmaxf(fmaxf(sc[t][0][0], sc[t][0][1]), fmaxf(sc[t][0][2], sc[t][0][3]));
+    if (SUB == 2) top = fmaxf(top, fmaxf(fmaxf(sc[t][SUB - 1][0], sc[t][SUB - 1][1]), fmaxf(sc[t][SUB - 1][2], sc[t][SUB - 1][3])));
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (__any(top > m[t])) {
+      const float m1 = fmaxf(m[t], top), f = exp_of(m[t] - at_least(m1));
+      m[t] = m1;
+      l[t] *= f;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[t][e] *= f;
+    }
+    const float m0 = at_least(m[t]);
+#pragma unroll
+    for (int s = 0; s < SUB; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = T::P_SCALE * exp_of(sc[t][s][i] - m0);
+        sc[t][s][i] = p;
+        l[t] += p;
+      }
+  }
+  if constexpr (EXACT) {
+#pragma unroll
+    for (int s = 0; s < SUB; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float ve = v_elem<DT>(v[s][i], e);
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(ve, sc[t][s][i], acc[t][e], 0, 0, 0);
+        }
+  } else {
+    u32x4 hi[NT], lo[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float p0 = sc[t][x / 2][x % 2 * 2], p1 = sc[t][x / 2][x % 2 * 2 + 1];
+        hi[t][x] = pack2_dt<DT>(p0, p1);
+        lo[t][x] = pack2_dt<DT>(p0 - half_of<DT>(hi[t][x], 0), p1 - half_of<DT>(hi[t][x], 1));
+      }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      u32x4 ve;                                      // element e of the lane's eight keys
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        ve[x] = __builtin_amdgcn_perm(v[x / 2][x % 2 * 2 + 1][e / 2], v[x / 2][x % 2 * 2][e / 2],
+                                      e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        acc[t][e] = mfma_qk<DT>(ve, hi[t], acc[t][e]);
+        acc[t][e] = mfma_qk<DT>(ve, lo[t], acc[t][e]);
+      }
+    }
+  }
+}
 
 // A workgroup of NW waves takes the units u0 .. u1 - 1 of a row tile: out and lse where that is all of it
 // (done), else a record.
@@ -319,7 +384,6 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
   };
   int next_entry;
   uint32_t there;
-  // EXACT: P.V in fp32 throughout
   auto turn = [&](int u, auto last_turn, auto exact) {
     constexpr bool LAST = decltype(last_turn)::value, EXACT = decltype(exact)::value;
     uint32_t v[SUB][4][VW];
@@ -362,65 +426,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
       load_k();
       next_entry = entry_at(u + 2);
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float top = fmaxf(fmaxf(sc[t][0][0], sc[t][0][1]), fmaxf(sc[t][0][2], sc[t][0][3]));
-      if (SUB == 2) top = fmaxf(top, fmaxf(fmaxf(sc[t][SUB - 1][0], sc[t][SUB - 1][1]), fmaxf(sc[t][SUB - 1][2], sc[t][SUB - 1][3])));
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      if (__any(top > m[t])) {
-        const float m1 = fmaxf(m[t], top), f = exp_of(m[t] - at_least(m1));
-        m[t] = m1;
-        l[t] *= f;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[t][e] *= f;
-      }
-      const float m0 = at_least(m[t]);
-#pragma unroll
-      for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = T::P_SCALE * exp_of(sc[t][s][i] - m0);
-          sc[t][s][i] = p;
-          l[t] += p;
-        }
-    }
-    if constexpr (EXACT) {
-#pragma unroll
-      for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const float ve = v_elem<DT>(v[s][i], e);
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-              acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(ve, sc[t][s][i], acc[t][e], 0, 0, 0);
-          }
-    } else {
-      u32x4 hi[NT], lo[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float p0 = sc[t][x / 2][x % 2 * 2], p1 = sc[t][x / 2][x % 2 * 2 + 1];
-          hi[t][x] = pack2_dt<DT>(p0, p1);
-          lo[t][x] = pack2_dt<DT>(p0 - half_of<DT>(hi[t][x], 0), p1 - half_of<DT>(hi[t][x], 1));
-        }
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        u32x4 ve;                                      // element e of the lane's eight keys
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          ve[x] = __builtin_amdgcn_perm(v[x / 2][x % 2 * 2 + 1][e / 2], v[x / 2][x % 2 * 2][e / 2],
-                                        e & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          acc[t][e] = mfma_qk<DT>(ve, hi[t], acc[t][e]);
-          acc[t][e] = mfma_qk<DT>(ve, lo[t], acc[t][e]);
-        }
-      }
-    }
+    attend_keys<DT, D, NT, EXACT>(sc, v, m, l, acc);
   };
   auto sweep = [&](auto exact) {
 #pragma unroll
@@ -491,23 +497,23 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
       }
       __syncthreads();
     }
-    if (!done) {
-      floatx4* part = (floatx4*)(a.part_o + (record * T::ROWS + t * 16) * D);
-      for (int i = tid; i < VE * 64; i += 64 * NW)
-        part[i] = (lds.acc[0][i] + lds.acc[1][i]) + (lds.acc[2][i] + lds.acc[3][i]);
-    } else if (tid < 256) {
+    if (tid < 256) {
       // thread: one 16th of a row
       const int orow = tid / 16, m16 = tid % 16, rr = row0 + t * 16 + orow;
-      const float sum = lds.sum[t * 16 + orow], inv = sum == 0.f ? 0.f : 1.f / sum;
-      if (rr < R) {
-        float y[VE];
+      float y[VE];
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const int at = part_index<VE>(orow, m16 * VE + e);
-          const float* p0 = (const float*)lds.acc[0];
-          constexpr int W = VE * 64 * 4;
-          y[e] = sum == 0.f ? 0.f : ((p0[at] + p0[W + at]) + (p0[2 * W + at] + p0[3 * W + at])) * inv;
-        }
+      for (int e = 0; e < VE; ++e) {
+        const int at = acc_index<VE>(orow, m16 * VE + e);
+        const float* p0 = (const float*)lds.acc[0];
+        constexpr int W = VE * 64 * 4;
+        y[e] = (p0[at] + p0[W + at]) + (p0[2 * W + at] + p0[3 * W + at]);
+      }
+      if (!done) {
+        store_out<DT_F32, VE>((char*)(a.part_o + (record * T::ROWS + t * 16 + orow) * D + m16 * VE), y);
+      } else if (rr < R) {
+        const float sum = lds.sum[t * 16 + orow], inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) y[e] = sum == 0.f ? 0.f : y[e] * inv;
         store_out<DT, VE>((char*)a.out + (((int64_t)b * a.H + hk * G + rr) * D + m16 * VE) * T::E, y);
       }
     }
@@ -544,6 +550,202 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
     const bool whole = u1 - u0 == units;               // the kv head's keys are this run's alone
     const int64_t record = (whole ? whole_record(a, b, hk) : 2 * (int64_t)run + (at != run0)) * tiles + tile;
     attend_tile<DT, D, NT, ACC, MULTI, 4>(a, lds, b, len, hk, tile * T::ROWS, u0, u1, !MULTI && whole, record);
+    at = first + u1;
+    ++hk;
+  }
+}
+
+// Many rows a kv head (PagedCut::many): 128 of them a workgroup, 32 a wave, over the same keys.  A turn's 32 keys and
+// values go to LDS by asynchronous copies, two turns ahead in three buffers, each wave fetching 8 keys whose page is
+// uniform; a row's 16-byte chunks lie permuted by its number, so that the reads of 16 rows' equal chunks and of one row's
+// chunks both spread over the banks.  Against 32 rows a workgroup, whose waves read the keys for themselves (32 queries of
+// 32 heads over 8 kv heads x 128, 4 sequences up to 12288 keys): 51 -> MANY_US us.
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int tiles) {
+  using T = Tile<DT, D, 2>;
+  constexpr int NT = 2, KS = T::KS, VE = T::VE, VW = T::VW, ROWS = Tile<DT, D, 8>::ROWS;
+  constexpr int CH = T::RB / 16, PER = 64 / CH, COPIES = 8 / PER;    // chunks of a row, rows of a copy, copies of 8 rows
+  __shared__ u32x4 staged[2][3][32 * CH];
+  __shared__ int again;
+  u32x4 (&keys)[3][32 * CH] = staged[0], (&values)[3][32 * CH] = staged[1];
+  const CacheView& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, g4 = lane >> 4;
+  const int G = a.H / c.Hkv, R = G * a.Q;
+  const int x = blockIdx.x / 8, tile = tiles == 1 ? 0 : x % tiles;
+  const int run = tiles == 1 ? blockIdx.x : x / tiles * 8 + blockIdx.x % 8;
+  const int64_t each = units_each(a, T::UNIT);
+  const int64_t run0 = run * each, run1 = run0 + each;
+  int64_t base = 0;
+  int b = find_seq(a, T::UNIT, run0, -1, base);
+  if (b < 0) return;
+  int len = uniform(common(a, b)), units = units_of(len, T::UNIT);
+  int hk = uniform(div40(run0 - base, units));
+  for (int64_t at = run0; at < run1;) {
+    if (hk == c.Hkv) {
+      if (++b == c.B) return;
+      base = at;
+      hk = 0;
+      len = uniform(common(a, b));
+      units = units_of(len, T::UNIT);
+    }
+    const int64_t first = base + (int64_t)hk * units;
+    const int u0 = (int)(at - first), u1 = (int)min((int64_t)units, run1 - first);
+    const int64_t record = (u1 - u0 == units ? whole_record(a, b, hk) : 2 * (int64_t)run + (at != run0)) * tiles + tile;
+    const int t0 = u0 * 4, t1 = min(u1 * 4, (len + 31) / 32);         // turns
+    const int32_t* table = c.table + (int64_t)b * c.t_stride;
+    const int last = max(len - 1, 0);
+
+    u32x4 q[NT][KS];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int row = tile * ROWS + wave * 32 + t * 16 + r, g = row / a.Q, i = row - g * a.Q;
+      const bool real = row < R;
+      const char* qp = (const char*)a.q + (b * a.q_bs + (real ? hk * G + g : 0) * a.q_hs + (real ? i : 0) * a.q_ts) * T::E + g4 * 16;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        q[t][s] = *(const u32x4*)(qp + s * 64);
+        if (!real) q[t][s] = u32x4{0, 0, 0, 0};
+      }
+    }
+    struct Entries { int page[4]; };                   // of a turn's four eights of keys, through the scalar cache
+    auto entries_of = [&](int t) {
+      Entries e;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        e.page[w] = *(const __attribute__((address_space(4))) int32_t*)(int64_t)(table + (min(t * 32 + w * 8, last) >> c.shift));
+      return e;
+    };
+    // copies this wave's keys of turn t, whose entries these are; which keys of the turn exist
+    auto stage = [&](int t, int buf, const Entries& e) {
+      uint32_t is = 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        if ((unsigned)e.page[w] < (unsigned)c.pages) is |= 0xffu << (8 * w);
+      if (t * 32 + 32 > len) is &= (1u << (len - t * 32)) - 1;         // a turn has a key: len - t * 32 in [1, 31]
+      const int page = wave == 0 ? e.page[0] : wave == 1 ? e.page[1] : wave == 2 ? e.page[2] : e.page[3];
+#pragma unroll
+      for (int y = 0; y < COPIES; ++y) {
+        const int row = wave * 8 + y * PER + lane / CH, slot = c.slot_of(t * 32 + row);
+        const int chunk = ((lane % CH) ^ (row & (CH - 1))) * 16;
+        const bool have = is >> row & 1;
+        const char* kp = have ? c.k + hk * c.k_hs + page * c.k_ps + slot * c.k_ss : (const char*)zero_row;
+        const char* vp = have ? c.v + hk * c.v_hs + page * c.v_ps + slot * c.v_ss : (const char*)zero_row;
+        copy16_to_lds(kp + chunk, uniform((int)lds_addr(&keys[buf][(wave * 8 + y * PER) * CH])));
+        copy16_to_lds(vp + chunk, uniform((int)lds_addr(&values[buf][(wave * 8 + y * PER) * CH])));
+      }
+      return is;
+    };
+    floatx4 acc[NT][VE];
+    float m[NT], l[NT];
+    auto sweep = [&](auto exact) {
+      constexpr bool EXACT = decltype(exact)::value;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[t][e] = floatx4{0.f, 0.f, 0.f, 0.f};
+      }
+      uint32_t there = 0, next = 0, after = 0;
+      if (t0 < t1) there = stage(t0, 0, entries_of(t0));
+      if (t0 + 1 < t1) next = stage(t0 + 1, 1, entries_of(t0 + 1));
+      Entries ahead = entries_of(t0 + 2);
+      int buf = 0;
+      for (int t = t0; t < t1; ++t) {
+        // this wave's copies of turn t are done, and with the barrier everyone's, and everyone is done with turn t - 1
+        if (t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * COPIES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (t + 2 < t1) {
+          after = stage(t + 2, buf == 0 ? 2 : buf - 1, ahead);
+          ahead = entries_of(t + 3);
+        }
+        floatx4 sc[NT][2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int row = s * 16 + r;
+          u32x4 k[KS];
+#pragma unroll
+          for (int i = 0; i < KS; ++i) k[i] = keys[buf][row * CH + ((i * 4 + g4) ^ (row & (CH - 1)))];
+#pragma unroll
+          for (int y = 0; y < NT; ++y) {
+            floatx4 z = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) z = mfma_qk<DT>(k[i], q[y][i], z);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[y][s][i] = z[i] * a.sm_scale;
+          }
+        }
+        uint32_t v[2][4][VW];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = s * 16 + g4 * 4 + i;
+            if constexpr (VW == 4) {
+              const u32x4 w = values[buf][row * CH + (r ^ (row & (CH - 1)))];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) v[s][i][y] = w[y];
+            } else {
+              const u32x2 w = ((const u32x2*)values[buf])[(row * CH + ((r >> 1) ^ (row & (CH - 1)))) * 2 + (r & 1)];
+              v[s][i][0] = w[0], v[s][i][1] = w[1];
+            }
+          }
+        if (there != ~0u) {
+#pragma unroll
+          for (int y = 0; y < NT; ++y)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (!(there >> (g4 * 4) & 1u << (s * 16 + i))) sc[y][s][i] = -INFINITY;
+        }
+        attend_keys<DT, D, NT, EXACT>(sc, v, m, l, acc);
+        there = next;
+        next = after;
+        buf = buf == 2 ? 0 : buf + 1;
+      }
+    };
+    if (tid == 0) again = 0;
+    __syncthreads();
+    sweep(std::integral_constant<bool, false>());
+    bool nan = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) nan |= acc[t][e][i] != acc[t][e][i];
+    if (nan) again = 1;
+    __syncthreads();
+    if (again) {
+      sweep(std::integral_constant<bool, true>());
+      __syncthreads();                                 // staged is free
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      l[t] += __shfl_xor(l[t], 16, 64);
+      l[t] += __shfl_xor(l[t], 32, 64);
+      const int64_t row = record * ROWS + wave * 32 + t * 16;
+      if (g4 == 0) a.part_ml[row + r] = make_float2(m[t], l[t]);
+      // rows whole, through LDS
+      float* mine = (float*)staged + wave * (16 * (D + 4));
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine[r * (D + 4) + (g4 * 4 + i) * VE + e] = acc[t][e][i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int y = 0; y < D / 16; ++y) {
+        const int word = (y * 64 + lane) * 4;
+        *(float4*)(a.part_o + row * D + word) = *(const float4*)(mine + word / D * (D + 4) + word % D);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();                                   // the buffers and `again` are free for the next kv head
     at = first + u1;
     ++hk;
   }
@@ -647,13 +849,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
   float y[W];
 #pragma unroll
   for (int e = 0; e < W; ++e) y[e] = 0.f;
-  const float* part = a.part_o + rr / 16 * 16 * D;
+  const float* part = a.part_o + rr * D + lane * W;
 #pragma unroll 4
   for (int p = wave; p < rec.n; p += 4) {
     const int64_t at = record(p);
     const float f = exp_of(ml[at].x - m0);
 #pragma unroll
-    for (int e = 0; e < W; ++e) y[e] += f * part[at * D + part_index<T::VE>(rr % 16, lane * W + e)];
+    for (int e = 0; e < W; ++e) y[e] += f * part[at * D + e];
   }
 #pragma unroll
   for (int e = 0; e < W; ++e) o[wave][lane * W + e] = y[e];
@@ -690,13 +892,13 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
   float y[W];
 #pragma unroll
   for (int e = 0; e < W; ++e) y[e] = 0.f;
-  const float* part = a.part_o + rr / 16 * 16 * D;
+  const float* part = a.part_o + rr * D + lane * W;
 #pragma unroll 4
   for (int p = 0; p < rec.n; ++p) {
     const int64_t at = record(p);
     const float f = exp_of(ml[at].x - m0);
 #pragma unroll
-    for (int e = 0; e < W; ++e) y[e] += f * part[at * D + part_index<T::VE>(rr % 16, lane * W + e)];
+    for (int e = 0; e < W; ++e) y[e] += f * part[at * D + e];
   }
   const int64_t row_out = ((int64_t)b * a.H + h) * a.Q + i;
   const int n0 = common(a, b), end = c.len(b) - (a.Q - 1 - i);
@@ -922,6 +1124,17 @@ hipError_t launch_attend(const PagedArgs& a, const PagedCut& cut, hipStream_t st
       return hipGetLastError();
     }
   }
+  if constexpr (MULTI && NT == 2 && DT != DT_F32) {
+    if (cut.many) {
+      paged_many_kernel<DT, D><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
+      hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      paged_join_rows_kernel<DT, D, 8><<<dim3((a.H * a.Q + 3) / 4, a.c.B), 256, 0, st>>>(a, cut.tiles);
+      if ((e = hipGetLastError()) != hipSuccess || !a.accumulate) return e;
+      paged_reform_kernel<DT, D><<<dim3((a.c.cap + 255) / 256, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
+      return hipGetLastError();
+    }
+  }
   if (a.scores) paged_attend_kernel<DT, D, NT, true, MULTI><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
   else paged_attend_kernel<DT, D, NT, false, MULTI><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
   hipError_t e = hipGetLastError();
@@ -944,7 +1157,7 @@ hipError_t launch_attend(const PagedArgs& a, const PagedCut& cut, hipStream_t st
 
 template <int DT, int D>
 hipError_t launch_rows(const PagedArgs& a, const PagedCut& cut, hipStream_t st) {
-  if (cut.rows == 32) return a.Q == 1 ? launch_attend<DT, D, 2, false>(a, cut, st) : launch_attend<DT, D, 2, true>(a, cut, st);
+  if (cut.rows > 16) return a.Q == 1 ? launch_attend<DT, D, 2, false>(a, cut, st) : launch_attend<DT, D, 2, true>(a, cut, st);
   return a.Q == 1 ? launch_attend<DT, D, 1, false>(a, cut, st) : launch_attend<DT, D, 1, true>(a, cut, st);
 }
 
@@ -956,13 +1169,14 @@ hipError_t launch_append(const AppendArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap) {
+PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap, int page_size) {
   PagedCut cut;
   const int R = H / Hkv * Q;
-  cut.rows = R > 16 ? 32 : 16;
+  cut.many = Q > 1 && R > 64 && dtype != STA_DTYPE_F32 && page_size >= 8;
+  cut.rows = cut.many ? 128 : R > 16 ? 32 : 16;
   cut.tiles = (R + cut.rows - 1) / cut.rows;
   const int unit = dtype == STA_DTYPE_F32 ? Tile<DT_F32, 64, 1>::UNIT : Tile<DT_BF16, 64, 1>::UNIT;
-  const int waves = cut.rows == 32 ? 2 : (D == 64 ? Tile<DT_BF16, 64, 1>::WAVES : Tile<DT_BF16, 128, 1>::WAVES);
+  const int waves = cut.rows > 16 ? 2 : (D == 64 ? Tile<DT_BF16, 64, 1>::WAVES : Tile<DT_BF16, 128, 1>::WAVES);
   const int64_t most = cap <= unit ? 1 : (cap + unit - 1) / unit;
   const int64_t all = (int64_t)Hkv * B * most;
   int runs = 256 * waves;
@@ -979,7 +1193,7 @@ PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap) {
 }
 
 hipError_t launch_paged(int dtype, int D, const PagedArgs& a, hipStream_t st) {
-  const PagedCut cut = paged_cut(dtype, D, a.H, a.c.Hkv, a.Q, a.c.B, a.c.cap);
+  const PagedCut cut = paged_cut(dtype, D, a.H, a.c.Hkv, a.Q, a.c.B, a.c.cap, 1 << a.c.shift);
   if (dtype == STA_DTYPE_F32) return D == 64 ? launch_rows<DT_F32, 64>(a, cut, st) : launch_rows<DT_F32, 128>(a, cut, st);
   if (dtype == STA_DTYPE_BF16) return D == 64 ? launch_rows<DT_BF16, 64>(a, cut, st) : launch_rows<DT_BF16, 128>(a, cut, st);
   return D == 64 ? launch_rows<DT_F16, 64>(a, cut, st) : launch_rows<DT_F16, 128>(a, cut, st);

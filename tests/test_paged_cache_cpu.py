@@ -103,8 +103,8 @@ def test_attention_workspace_sizes():
     scores = 4 * 32 * 8192 * 4
     assert records + scores <= size(accumulate=1) < records + scores + 4 * 32 * 4 + 1024
     assert size(accumulate=1, max_len=1024) == 4 * 32 * 1024 * 4
-    # 32 queries: 128 rows, four tiles, a fourth of the runs, and a record a kv head
-    rows = 4 * (2 * 128 + 8 * 4) * 32 * (128 * 4 + 8)
+    # 32 queries: 128 rows in one tile, and a record a kv head
+    rows = (2 * 512 + 8 * 4) * 128 * (128 * 4 + 8)
     assert rows <= size(Q=32) <= size(Q=32, accumulate=1) < rows + 4 * 32 * 32 * 4 + 2048
 
 
