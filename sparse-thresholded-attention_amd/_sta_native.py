@@ -1468,7 +1468,8 @@ def _rows(x):
     esz, bits = x.element_size(), x.data_ptr()
     for s in strides:
         bits |= s * esz
-    return x if last == 1 and not bits & 15 else x.contiguous()
+    # a copy even of a contiguous one: it may begin anywhere, and a dim of size 1 have any stride
+    return x if last == 1 and not bits & 15 else x.clone(memory_format=torch.contiguous_format)
 
 
 def _ints(x, dev):
@@ -1482,7 +1483,7 @@ class PagedCache:
     """The pages of one layer's key-value cache: k, v (pages, Hkv, page_size, D), and, for each key and kv head,
     the attention weight it has drawn (weight, fp32) and its token's number in the sequence (pos,
     int32), both (pages, Hkv, page_size) or None.  The tensors are used as they are, whatever their
-    strides over pages, heads and slots."""
+    strides over pages, heads and slots; other tensors make another PagedCache."""
 
     def __init__(self, k, v, weight=None, pos=None):
         for name, x in (("k", k), ("v", v)):
@@ -1500,7 +1501,7 @@ class PagedCache:
             _require(x.shape == k.shape[:3] and x.device == k.device,
                      f"cache {name} must be {tuple(k.shape[:3])} on the device of k")
             _require(x.stride(2) == 1 or x.shape[2] == 1, f"cache {name} needs unit stride in its last dim")
-        self.k, self.v, self.weight, self.pos, self.device = k, v, weight, pos, k.device
+        self._k, self._v, self._weight, self._pos, self.device = k, v, weight, pos, k.device
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self._c = c = CacheC()
         c.k, c.v = k.data_ptr(), v.data_ptr()
@@ -1512,6 +1513,12 @@ class PagedCache:
             c.pos, c.pos_page_stride, c.pos_head_stride = pos.data_ptr(), pos.stride(0), pos.stride(1)
         c.dtype, c.pages, c.page_size = DTYPES[k.dtype], self.pages, self.page_size
         c.Hkv, c.D = self.kv_heads, self.head_dim
+
+    # the calls use the addresses taken above
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    weight = property(lambda self: self._weight)
+    pos = property(lambda self: self._pos)
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda", evictable=True):

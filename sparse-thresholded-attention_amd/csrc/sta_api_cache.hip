@@ -28,7 +28,7 @@ int check_rows(const char* name, const void* p, int dtype, int64_t s0, int64_t s
   return STA_OK;
 }
 
-// the cache; need_lens: also what a call reads (the workspace sizes take shapes alone)
+// the shapes, all that the workspace sizes take
 int check_cache_shape(const sta_cache& c) {
   if (!dtype_ok(c.dtype)) return fail(STA_ERR_INVALID_ARG, "dtype %d is not one of STA_DTYPE_F32/BF16/F16", c.dtype);
   if (c.D != 64 && c.D != 128) return fail(STA_ERR_UNSUPPORTED, "head_dim %d not in {64, 128}", c.D);

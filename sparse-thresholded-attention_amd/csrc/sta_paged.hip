@@ -18,8 +18,9 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
 }
 
 // ------------------------------------------------------------------------------------------
-// append: a wave per token moves the rows of all kv heads, 16 bytes a lane, two keys' and two values' in flight.  Bound
-// by memory.
+// append: a wave per token moves the rows of all kv heads, 16 bytes a lane, two keys' and two values' in flight.  A wave
+// finds its token's sequence and page once (a wave per token and head had each search again: 12 prompts of up to 4001
+// tokens, 8 heads x 128, bf16: 57 -> 45 us).  Bound by memory: 224 MB there, 5.0 TB/s.
 // ------------------------------------------------------------------------------------------
 // the last sequence that starts at or before t (64 candidates at once), -1: none
 __device__ __forceinline__ int sequence_of(const int32_t* starts, int B, int t) {
@@ -527,7 +528,7 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
   __shared__ MergeLds<D, NT, T::VE> lds;
   const CacheView& c = a.c;
   // workgroups go to the XCDs in turn: the row tiles of a run are 8 apart, on one XCD, and find each other's keys in
-  // its L2 (32 queries of 32 heads over 8 kv heads, 4 sequences up to 12288 keys: 69 -> 52 us)
+  // its L2 (16 queries of 32 heads over 8 kv heads x 128, bf16, 8 sequences up to 8192 keys: 58 -> 50 us)
   const int x = blockIdx.x / 8, tile = tiles == 1 ? 0 : x % tiles;
   const int run = tiles == 1 ? blockIdx.x : x / tiles * 8 + blockIdx.x % 8;
   const int64_t each = units_each(a, T::UNIT);
@@ -559,7 +560,7 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
 // values go to LDS by asynchronous copies, two turns ahead in three buffers, each wave fetching 8 keys whose page is
 // uniform; a row's 16-byte chunks lie permuted by its number, so that the reads of 16 rows' equal chunks and of one row's
 // chunks both spread over the banks.  Against 32 rows a workgroup, whose waves read the keys for themselves (32 queries of
-// 32 heads over 8 kv heads x 128, 4 sequences up to 12288 keys): 51 -> MANY_US us.
+// 32 heads over 8 kv heads x 128, 4 sequences up to 12288 keys): 51 -> 42 us.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int tiles) {
   using T = Tile<DT, D, 2>;
@@ -973,7 +974,9 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
 
 // The weights that a step's rows give the keys of a kv head, from their scores: four keys a lane, 256 a wave.  SHARED: the
 // four waves of a workgroup take the rows of 256 keys in turn, and their sums are added in order (many rows); else each
-// has keys of its own.
+// has keys of its own.  Without SHARED, keys that lie fours to 16 aligned bytes of a page have their weights loaded before
+// the scores and written back together (32 sequences of 4096 keys, 32q / 8kv heads, pages of 16: 11.0 -> 9.6 us; 17 MB of
+// scores and 8 of weights, bound by the chain length, page, weight and the launch).
 template <bool SHARED>
 __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
   __shared__ floatx4 sums[SHARED ? 4 : 1][64];
@@ -987,6 +990,16 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
   const int j = j0 + lane * 4;
   const bool all = j0 + 256 <= common(a, b);           // every row sees every key
   const float* s = a.scores + row0 * a.score_stride + j;
+  const int32_t* table = c.table + (int64_t)b * c.t_stride;
+  const bool fours = !SHARED && c.shift >= 2 && ((c.w_ps | c.w_hs) & 3) == 0 && ((uintptr_t)c.weight & 15) == 0;
+  int page = -1;
+  float* drawn = nullptr;
+  floatx4 had = floatx4{0.f, 0.f, 0.f, 0.f};
+  if (fours && j + 4 <= len) {
+    page = c.page_of(table, j);
+    drawn = c.weight + (page >= 0 ? page * c.w_ps + hk * c.w_hs + c.slot_of(j) : 0);
+    if (page >= 0) had = *(const floatx4*)drawn;
+  }
   floatx4 sum = floatx4{0.f, 0.f, 0.f, 0.f};
   constexpr int STEP = SHARED ? 4 : 1;
   const int first = SHARED ? wave : 0;
@@ -1008,7 +1021,6 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
       for (int e = 0; e < 4; ++e) sum[e] += j + e >= end || z == -INFINITY ? 0.f : exp_of(x[e] - z);
     }
   }
-  const int32_t* table = c.table + (int64_t)b * c.t_stride;
   if constexpr (SHARED) {
     sums[wave][lane] = sum;
     __syncthreads();
@@ -1018,6 +1030,8 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
     const float* w = (const float*)sums;
     if (p >= 0)
       c.weight[p * c.w_ps + hk * c.w_hs + c.slot_of(mine)] += (w[tid] + w[256 + tid]) + (w[512 + tid] + w[768 + tid]);
+  } else if (fours && j + 4 <= len) {                  // in one page, 16 aligned bytes
+    if (page >= 0) *(floatx4*)drawn = had + sum;
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -1172,6 +1186,8 @@ hipError_t launch_append(const AppendArgs& a, hipStream_t st) {
 PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap, int page_size) {
   PagedCut cut;
   const int R = H / Hkv * Q;
+  // 128 rows a workgroup past 64 (32q / 8kv heads x 128, bf16, 8 sequences up to 8192 keys, R = 48 / 64 / 80 / 96 / 128: 56 /
+  // 56 / 57 / 58 / 53 us, 32 rows a workgroup 51 / 51 / 65 / 66 / 67); an eight of keys has to lie in one page
   cut.many = Q > 1 && R > 64 && dtype != STA_DTYPE_F32 && page_size >= 8;
   cut.rows = cut.many ? 128 : R > 16 ? 32 : 16;
   cut.tiles = (R + cut.rows - 1) / cut.rows;

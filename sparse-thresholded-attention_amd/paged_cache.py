@@ -19,7 +19,8 @@ A decoding step of a batch, held at `budget` keys a head:
 
 All of them launch on the current stream of the tensors' device, allocate their results and their
 workspace from torch's allocator, and neither synchronise nor keep anything between calls, so a HIP
-graph can capture them.  There is no fallback: a CPU tensor, an unsupported shape or a missing
+graph can capture them (a captured training step calls rotary_grad itself).  rotary alone takes part
+in autograd.  There is no fallback: a CPU tensor, an unsupported shape or a missing
 library raises.
 """
 import torch
@@ -83,7 +84,7 @@ def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want
     A query that sees no key gets zeros and -inf.
 
     accumulate: add every key's probability, summed over the queries and the heads of its kv head, to
-    cache.weight; the pages of such a call belong to one sequence each.  max_len: a bound on lens known
+    cache.weight; a page of such a call stands in one place of one sequence's table.  max_len: a bound on lens known
     to the host (default: the table's); it sizes the workspace, 4 bytes a query row and key with
     accumulate, and lengths past it count as max_len."""
     return native.paged_attention(q, cache, table, lens, sm_scale, accumulate, want_lse, max_len)
@@ -96,6 +97,8 @@ def cache_evict(cache, table, lens, budget, n_global=32, n_local=32, dst_table=N
 
     In place (dst_table None) the kept keys in slots from budget on move into the dropped ones' slots, so
     that the keys of a sequence are no longer in the order of their tokens; cache.pos says which they
-    are.  With dst_table (B, pages) the kept keys are copied, in order, to that table's pages and the
-    source pages, which may be shared, stay as they are."""
+    are; a page stands in one place of one sequence's table.  With dst_table (B, pages) the kept keys
+    are copied, in order, to that table's pages, others than the source's, which may be shared and stay
+    as they are.  Keys without a page rank last; one that is kept all the same leaves its slot of
+    dst_table unwritten."""
     return native.cache_evict(cache, table, lens, budget, n_global, n_local, dst_table, max_len)

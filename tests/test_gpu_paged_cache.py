@@ -93,6 +93,30 @@ def test_rotary_position_types_strides_and_one_input(dtype):
     assert empty.shape == (0, 1, 64)
 
 
+def test_rows_that_begin_anywhere_and_dims_of_size_one():
+    """Tensors that count as contiguous and whose address or strides are no multiples of 16 bytes."""
+    import paged_cache as pc
+    inv = (10000.0 ** -(torch.arange(64) / 64.0)).to(DEV)
+    flat = _randn(5, (4 * 2 * 128 + 1,), BF16)
+    shifted = flat[1:].view(4, 2, 128)                       # 2 bytes behind an aligned address
+    single = _randn(6, (3, 2 * 128 + 4), BF16)[1:2, :256].unflatten(1, (2, 128))     # one token, rows of 260 elements
+    pos4, pos1 = torch.arange(4, device=DEV), torch.arange(1, device=DEV) + 9
+    for x, pos in ((shifted, pos4), (single, pos1)):
+        assert x.is_contiguous()
+        y, none = pc.rotary(x, None, pos, inv)
+        assert none is None
+        _check_rotary(x, y, pos[None], inv, (64,))
+    made = Made(7, [40], 2, 128, 16, BF16)
+    q = _randn(8, (2, 128 + 2), BF16)[:, :128].unsqueeze(0)
+    odd = _randn(9, (2 * 128 + 1,), BF16)[1:].view(1, 2, 128)
+    for x in (q, odd):
+        got = pc.paged_attention(x, made.cache, made.table, made.lens)
+        assert torch.equal(got, pc.paged_attention(x.clone(memory_format=torch.contiguous_format), made.cache, made.table,
+                                                   made.lens))
+    with pytest.raises(AttributeError):
+        made.cache.k = made.cache.v
+
+
 def test_rotary_gradients_through_autograd():
     """Against the formula's gradient and against differences of the formula in 64 bits."""
     import paged_cache as pc
@@ -235,6 +259,24 @@ def test_attention_against_the_definition(case, accumulate):
     _check_attend(made, q, got, want, lse, made.cache.weight if accumulate else None, weight0)
     if not accumulate:
         assert torch.equal(made.cache.weight, weight0)
+
+
+@pytest.mark.parametrize("Q", [1, 3])
+def test_weights_of_any_alignment(Q):
+    import paged_cache as pc
+    made = Made(90, [1500, 3, 2049], 2, 64, 16, BF16)
+    c = made.cache
+    flat = torch.zeros(c.weight.numel() + 1, device=DEV)
+    shifted = flat[1:].view(c.weight.shape)
+    shifted.copy_(c.weight)
+    made.cache = pc.PagedCache(c.k, c.v, shifted, c.pos)
+    q = _randn(91, (3, 8, Q, 64), BF16)
+    before = shifted.clone()
+    got, lse = pc.paged_attention(q, made.cache, made.table, made.lens, accumulate=True, want_lse=True)
+    _check_attend(made, q, got, made.attend_ref(q, 0.125), lse, shifted, before)
+    aligned = pc.PagedCache(c.k, c.v, before.clone(), c.pos)
+    pc.paged_attention(q, aligned, made.table, made.lens, accumulate=True)
+    assert torch.equal(aligned.weight, shifted)
 
 
 def test_attention_of_strided_queries_scales_and_a_short_bound():
