@@ -653,9 +653,9 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
       Entries ahead = entries_of(t0 + 2);
       int buf = 0;
       for (int t = t0; t < t1; ++t) {
-        // this wave's copies of turn t are done, and with the barrier everyone's, and everyone is done with turn t - 1
-        if (t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * COPIES) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // this wave's copies of turn t are done, and its reads of turn t - 1, and with the barrier everyone's
+        if (t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * COPIES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         if (t + 2 < t1) {
