@@ -58,7 +58,8 @@ template <int DT>
 __global__ __launch_bounds__(256) void rotary_kernel(sta_rotary_args a, int half) {
   constexpr int V = ROT_V<DT>;
   extern __shared__ float2 trig[];                 // [half]
-  const int64_t t = blockIdx.x;
+  const int64_t t = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  if (t >= a.T) return;
   for (int f = threadIdx.x; f < half; f += 256) {
     int axis = 0, first = 0;
     while (axis + 1 < a.axes && f >= first + a.section[axis]) first += a.section[axis++];
@@ -105,7 +106,9 @@ template <int DT>
 hipError_t launch_dt(const sta_rotary_args& a, hipStream_t st) {
   int half = 0;
   for (int i = 0; i < a.axes; ++i) half += a.section[i];
-  rotary_kernel<DT><<<a.T, 256, (size_t)half * sizeof(float2), st>>>(a, half);
+  // a dimension of a grid holds below 2^32 threads
+  const int most = 1 << 20, blocks = a.T < most ? a.T : most;
+  rotary_kernel<DT><<<dim3(blocks, (a.T - 1) / most + 1), 256, (size_t)half * sizeof(float2), st>>>(a, half);
   return hipGetLastError();
 }
 

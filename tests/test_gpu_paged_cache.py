@@ -117,6 +117,18 @@ def test_rows_that_begin_anywhere_and_dims_of_size_one():
         made.cache.k = made.cache.v
 
 
+def test_rotary_of_more_tokens_than_one_grid_dimension_holds():
+    """2^24 workgroups of 256 threads are 2^32 of them."""
+    import paged_cache as pc
+    T = (1 << 24) + 3
+    q = torch.arange(T * 16, device=DEV, dtype=torch.int32).remainder_(509).to(BF16).view(T, 1, 16)
+    positions, inv_freq = torch.arange(T, device=DEV, dtype=torch.int32), torch.ones(8, device=DEV)
+    got, _ = pc.rotary(q, None, positions, inv_freq)
+    for at in (0, (1 << 20) - 2, (1 << 23) + 5, T - 7):
+        part, _ = pc.rotary(q[at:at + 7], None, positions[at:at + 7], inv_freq)
+        assert torch.equal(got[at:at + 7], part)
+
+
 def test_rotary_gradients_through_autograd():
     """Against the formula's gradient and against differences of the formula in 64 bits."""
     import paged_cache as pc

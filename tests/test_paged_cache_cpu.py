@@ -142,7 +142,7 @@ def test_eviction_refuses_lengths_in_place_and_a_short_destination():
 
 
 @pytest.mark.parametrize("field,value,code", CACHE_FAULTS + POINTER_FAULTS + [
-    ("T", -1, -1), ("T", 5, -1), ("k", None, -1), ("v_tok_stride", 2, -2), ("new_lens", None, -1)])
+    ("T", -1, -1), ("T", 5, -1), ("T", 1 << 26, -2), ("k", None, -1), ("v_tok_stride", 2, -2), ("new_lens", None, -1)])
 def test_append_refuses(field, value, code):
     import _sta_native as native
     buf, p = _host(native)
