@@ -1042,8 +1042,10 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
 }
 
 // The same from the scores formed again, where a kv head has many rows (PagedCut::reform): a wave holds 64 keys
-// in registers, the rows come 64 at a time through LDS, and each lane adds up its row's p of four keys a subtile over
-// the row tiles; the 16 lanes of those keys meet at the end.
+// in registers, the rows come 64 at a time through LDS, fetched during the 64 before, and each lane adds up its row's p of
+// four keys a subtile over the row tiles; the 16 lanes of those keys meet at the end.  Bound by the keys' bytes, a second
+// time, and the latencies before them (128 rows a kv head x 128, bf16, 4 sequences up to 12288 keys: 24 us, 28 with the
+// rows fetched in their own turn; 50 MB of keys are 10; 32 or 16 keys a wave: the same or slower).
 template <int DT, int D>
 __global__ __launch_bounds__(256) void paged_reform_kernel(PagedArgs a) {
   using T = Tile<DT, D, 1>;
@@ -1054,7 +1056,7 @@ __global__ __launch_bounds__(256) void paged_reform_kernel(PagedArgs a) {
   const CacheView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, g4 = lane >> 4;
   const int b = blockIdx.z, hk = blockIdx.y, block0 = blockIdx.x * (64 * SUBS), key0 = block0 + wave * (16 * SUBS);
-  const int len = uniform(c.len(b)), R = a.H / c.Hkv * a.Q;
+  const int len = uniform(c.len(b)), G = a.H / c.Hkv, R = G * a.Q;
   if (block0 >= len) return;
   const int32_t* table = c.table + (int64_t)b * c.t_stride;
   // the lane's key of the wave's, and all of them in their lanes
@@ -1069,46 +1071,63 @@ __global__ __launch_bounds__(256) void paged_reform_kernel(PagedArgs a) {
 #pragma unroll
     for (int i = 0; i < KS; ++i) k[s][i] = *(global4)(p + i * 64);
   }
-  const bool all = key0 + 16 * SUBS <= common(a, b);   // every row sees every key of the wave
+  const float scale = a.sm_scale * LOG2E;
   floatx4 w[SUBS];
 #pragma unroll
   for (int s = 0; s < SUBS; ++s) w[s] = floatx4{0.f, 0.f, 0.f, 0.f};
+  // the rows of a turn are fetched during the one before
+  constexpr int CH = T::RB / 16, PER = ROWS * CH / 256;
+  u32x4 held[PER];
+  float held_z;
+  int held_end;
+  auto fetch = [&](int r0) {
+#pragma unroll
+    for (int x = 0; x < PER; ++x) {
+      const int rr = min(r0 + (x * 256 + tid) / CH, R - 1), g = rr / a.Q, i = rr - g * a.Q;
+      held[x] = *(global4)((int64_t)((const char*)a.q + (b * a.q_bs + (hk * G + g) * a.q_hs + i * a.q_ts) * T::E + tid % CH * 16));
+    }
+    const int rr = min(r0 + tid % ROWS, R - 1), g = rr / a.Q, i = rr - g * a.Q;
+    held_z = a.lse[((int64_t)b * a.H + hk * G + g) * a.Q + i];
+    // a row that saw nothing, or is none, sees no key here
+    held_end = r0 + tid % ROWS < R && held_z != -INFINITY ? len - (a.Q - 1 - i) : 0;
+  };
+  fetch(0);
   for (int r0 = 0; r0 < R; r0 += ROWS) {
     const int n = min(R - r0, ROWS);
     __syncthreads();
-    for (int x = tid; x < ROWS * (T::RB / 16); x += 256) {
-      const int row = x / (T::RB / 16), at = x - row * (T::RB / 16), rr = r0 + row;
-      const int h = hk * (a.H / c.Hkv) + rr / a.Q, i = rr % a.Q;
-      if (row < n)
-        rows[row * STRIDE + at] = *(global4)((int64_t)((const char*)a.q + (b * a.q_bs + h * a.q_hs + i * a.q_ts) * T::E + at * 16));
-      else
-        rows[row * STRIDE + at] = u32x4{0, 0, 0, 0};
-    }
+#pragma unroll
+    for (int x = 0; x < PER; ++x) rows[(x * 256 + tid) / CH * STRIDE + tid % CH] = held[x];
     if (tid < ROWS) {
-      const int rr = r0 + tid, i = rr % a.Q;
-      // a row that saw nothing, or is none, gives nothing: exp(s - inf)
-      const float z = tid < n ? a.lse[((int64_t)b * a.H + hk * (a.H / c.Hkv) + rr / a.Q) * a.Q + i] : INFINITY;
-      minus[tid] = z == -INFINITY ? INFINITY : z;
-      ends[tid] = len - (a.Q - 1 - i);
+      minus[tid] = held_z * LOG2E;
+      ends[tid] = held_end;
     }
     __syncthreads();
+    if (r0 + ROWS < R) fetch(r0 + ROWS);
     for (int t = 0; t < n; t += 16) {
       u32x4 q[KS];
 #pragma unroll
       for (int i = 0; i < KS; ++i) q[i] = rows[(t + r) * STRIDE + i * 4 + g4];
       const float z = minus[t + r];
       const int end = ends[t + r];
-      const bool live = z != INFINITY;
+      floatx4 x[SUBS];
 #pragma unroll
       for (int s = 0; s < SUBS; ++s) {
-        floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
+        x[s] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < KS; ++i) x = mfma_qk<DT>(k[s][i], q[i], x);
+        for (int i = 0; i < KS; ++i) x[s] = mfma_qk<DT>(k[s][i], q[i], x[s]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = exp_of(x[i] * a.sm_scale - z);
-          w[s][i] += live && (all || key0 + s * 16 + g4 * 4 + i < end) ? p : 0.f;
-        }
+        for (int i = 0; i < 4; ++i) x[s][i] = __builtin_amdgcn_exp2f(fmaf(x[s][i], scale, -z));
+      }
+      if (__all(key0 + 16 * SUBS <= end)) {
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[s][i] += x[s][i];
+      } else {
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[s][i] += key0 + s * 16 + g4 * 4 + i < end ? x[s][i] : 0.f;
       }
     }
   }
