@@ -1219,10 +1219,11 @@ PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap, int 
   cut.runs = (int)(all < runs ? all : runs);
   cut.grid = cut.tiles == 1 ? cut.runs : (cut.runs + 7) / 8 * 8 * cut.tiles;
   // stored scores cost 8 bytes a row and key, reformed ones the keys once more and their products: 32q / 8kv heads
-  // x 128, bf16, 8 sequences up to 8192 keys, R = 32 / 64 rows: 56 / 87 us stored, 66 / 86 reformed, and 117 / 97 at
-  // R = 128 (4 up to 12288); fp32 97 / 147 and 118 / 184
+  // x 128, bf16, 8 sequences up to 8192 keys, R = 24 / 48 / 56 / 64 rows: 48 / 68 / 74 / 80 us stored, 59 / 72 / 74 / 75
+  // reformed, and 117 / 93 at R = 128 (4 up to 12288); x 64, R = 32 / 64: 40 / 60 and 40 / 52; fp32, R = 32 / 64, 97 / 147
+  // and 118 / 184
   cut.small = Q == 1 && cut.tiles == 1 && cap <= SMALL_KEYS;
-  cut.reform = !cut.small && R > 64 && dtype != STA_DTYPE_F32;
+  cut.reform = !cut.small && R >= 64 && dtype != STA_DTYPE_F32;
   cut.records = cut.small ? 0 : cut.tiles * (2 * (int64_t)cut.runs + (Q > 1 ? (int64_t)Hkv * B : 0));
   return cut;
 }

@@ -249,6 +249,9 @@ ATTEND = [
 ] + [([100 + 13 * i] * 3 + [0] * (i % 2), 4, 2, 1 + i % 2, 64, 16, BF16, "head") for i in range(2)] + [
     ([1 + (37 * i) % 90 for i in range(150)], 4, 2, 1, 64, 16, BF16, "head"),      # more sequences than lanes
     ([1 + (37 * i) % 90 for i in range(150)] + [1200], 4, 2, 1, 64, 16, BF16, "head"),
+    ([700, 9, 0, 1301], 8, 2, 16, 128, 16, BF16, "head"),      # 64 rows a kv head
+    ([333, 40], 16, 4, 16, 64, 8, F16, "pair"),
+    ([610, 90], 8, 2, 20, 128, 4, BF16, "slot"),               # 80 rows, pages of less than 8
 ]
 
 
