@@ -1472,6 +1472,11 @@ def _rows(x):
     return x if last == 1 and not bits & 15 else x.clone(memory_format=torch.contiguous_format)
 
 
+def _int32(x):
+    """A number for an int32 field, which would keep its low 32 bits: one beyond them stays as far beyond as it can."""
+    return max(-2 ** 31, min(int(x), 2 ** 31 - 1))
+
+
 def _ints(x, dev):
     """A device int32 tensor with unit stride in its last dim."""
     if x.dtype != torch.int32 or x.device != dev:
@@ -1543,7 +1548,7 @@ class PagedCache:
 
     def _max_len(self, table, max_len):
         most = table.shape[1] * self.page_size
-        return most if max_len is None else min(int(max_len), most)
+        return _int32(most if max_len is None else min(int(max_len), most))
 
 
 def _empty_as(x):
@@ -1614,7 +1619,7 @@ def cache_append(cache, k, v, table, lens, starts=None, seen=None):
     a = AppendArgsC()
     keep = cache._fill(a, table, lens)
     B = a.cache.B
-    a.k, a.v, a.T = k.data_ptr(), v.data_ptr(), k.shape[0]
+    a.k, a.v, a.T = k.data_ptr(), v.data_ptr(), _int32(k.shape[0])
     a.k_tok_stride, a.k_head_stride, _ = k.stride()
     a.v_tok_stride, a.v_head_stride, _ = v.stride()
     if starts is not None:
@@ -1673,7 +1678,7 @@ def cache_evict(cache, table, lens, budget, n_global=32, n_local=32, dst_table=N
     dev = cache.device
     a = EvictArgsC()
     table, lens = cache._fill(a, table, lens)
-    a.budget, a.n_global, a.n_local = int(budget), int(n_global), int(n_local)
+    a.budget, a.n_global, a.n_local = _int32(budget), _int32(n_global), _int32(n_local)
     a.max_len = cache._max_len(table, max_len)
     if dst_table is not None:
         dst_table = _ints(dst_table, dev)

@@ -516,6 +516,19 @@ def test_eviction_against_the_definition(case, move):
         assert torch.equal(x.cpu().view(torch.uint8), y.view(torch.uint8)), name
 
 
+def test_eviction_of_numbers_beyond_32_bits():
+    """A budget or window that no length reaches keeps everything, and one below zero is refused."""
+    import paged_cache as pc
+    made = Made(700, [90, 20], 2, 64, 16, BF16)
+    before = made.cache.k.clone(), made.cache.weight.clone()
+    for kw in ({"budget": 2 ** 32 + 5}, {"budget": 2 ** 31}, {"budget": 95, "n_local": 2 ** 32 + 1, "max_len": 2 ** 33}):
+        assert pc.cache_evict(made.cache, made.table, made.lens, **kw).tolist() == [90, 20]
+    assert torch.equal(made.cache.k, before[0]) and torch.equal(made.cache.weight, before[1])
+    for kw in ({"budget": -2 ** 32 + 5}, {"budget": 5, "n_global": -2 ** 32 + 5}, {"budget": 5, "max_len": -2 ** 32 + 5}):
+        with pytest.raises(RuntimeError):
+            pc.cache_evict(made.cache, made.table, made.lens, **kw)
+
+
 def test_eviction_with_weights_and_positions_of_any_alignment():
     import paged_cache as pc
     made = Made(580, [300, 64], 3, 64, 16, BF16)
