@@ -24,25 +24,38 @@ in autograd.  There is no fallback: a CPU tensor, an unsupported shape or a miss
 library raises.
 """
 import torch
+from torch.autograd import forward_ad
 
 import _sta_native as native
 from _sta_native import PagedCache  # noqa: F401
 
 
+def _tangents():
+    """Whether a forward-mode level is open, in which a tensor may carry a tangent."""
+    return forward_ad._current_level >= 0
+
+
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, sections, pos_scale, rope_scale, inverse):
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.how = (sections, pos_scale, rope_scale)
-        ctx.inverse = inverse
+    def forward(q, k, positions, inv_freq, sections, pos_scale, rope_scale, inverse):
         return native.rotary(q, k, positions, inv_freq, sections, pos_scale, rope_scale, inverse)
 
     @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, _, positions, inv_freq, *ctx.how, ctx.inverse = inputs
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.save_for_forward(positions, inv_freq)
+
+    # linear in q and k: the gradient is the rotation the other way, the tangent the rotation of theirs; both are
+    # differentiable themselves
+    @staticmethod
     def backward(ctx, dq, dk):
-        positions, inv_freq = ctx.saved_tensors
-        # linear in q and k: the gradient is the rotation the other way, itself differentiable
-        return (*_Rotary.apply(dq, dk, positions, inv_freq, *ctx.how, not ctx.inverse),
+        return (*_Rotary.apply(dq, dk, *ctx.saved_tensors, *ctx.how, not ctx.inverse),
                 None, None, None, None, None, None)
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        return _Rotary.apply(tq, tk, *ctx.saved_tensors, *ctx.how, ctx.inverse)
 
 
 def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1.0):
@@ -53,15 +66,17 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
     row turns by positions[axis of i] * pos_scale * inv_freq[i], the angle formed in 64 bits, and is
     scaled by rope_scale; elements from R on are copied.  sections: how many frequencies each axis
     owns, in order (default: all of them one axis).  D a multiple of 8 up to 512, R / 2 a multiple of
-    8.  Gradients flow to q and k, not to positions or frequencies."""
-    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+    8.  Gradients and forward-mode tangents flow to and from q and k, not positions or frequencies."""
+    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad) or _tangents():
         return _Rotary.apply(q, k, positions, inv_freq, sections, pos_scale, rope_scale, False)
     return native.rotary(q, k, positions, inv_freq, sections, pos_scale, rope_scale)
 
 
 def rotary_grad(dq, dk, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1.0):
     """The gradients of rotary's inputs from those of its outputs, without an autograd graph: the
-    rotation the other way round, with the same scale."""
+    rotation the other way round, with the same scale.  Inputs with forward-mode tangents are refused."""
+    if _tangents() and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in (dq, dk)):
+        raise RuntimeError("rotary_grad keeps no graph and no forward-mode tangents: differentiate rotary")
     return native.rotary(dq, dk, positions, inv_freq, sections, pos_scale, rope_scale, inverse=True)
 
 
