@@ -1516,8 +1516,8 @@ class PagedCache:
             c.weight, c.weight_page_stride, c.weight_head_stride = weight.data_ptr(), weight.stride(0), weight.stride(1)
         if pos is not None:
             c.pos, c.pos_page_stride, c.pos_head_stride = pos.data_ptr(), pos.stride(0), pos.stride(1)
-        c.dtype, c.pages, c.page_size = DTYPES[k.dtype], self.pages, self.page_size
-        c.Hkv, c.D = self.kv_heads, self.head_dim
+        c.dtype, c.pages, c.page_size = DTYPES[k.dtype], _int32(self.pages), _int32(self.page_size)
+        c.Hkv, c.D = _int32(self.kv_heads), _int32(self.head_dim)
 
     # the calls use the addresses taken above
     k = property(lambda self: self._k)
@@ -1542,7 +1542,8 @@ class PagedCache:
                  "table must be (B, pages of a sequence) and lens (B,)")
         a.cache = self._c
         c = a.cache
-        c.table, c.table_stride, (c.B, c.table_width) = table.data_ptr(), table.stride(0), table.shape
+        c.table, c.table_stride = table.data_ptr(), table.stride(0)
+        c.B, c.table_width = _int32(table.shape[0]), _int32(table.shape[1])
         c.lens = lens.data_ptr()
         return table, lens
 
@@ -1564,6 +1565,7 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
         raise ValueError(f"q must be (T, heads, D), not {tuple(q.shape)}")
     q = _rows(q)
     T, H, D = q.shape
+    _require(T < 2 ** 31, f"{T} tokens: a call takes below 2^31")
     a = RotaryArgsC()
     q_out = _empty_as(q)
     a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
@@ -1576,7 +1578,8 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
         if k.dim() != 3 or k.shape[0] != T or k.shape[2] != D:
             raise ValueError(f"k must be ({T}, kv heads, {D}), not {tuple(k.shape)}")
         k = _rows(k if k.device == dev else k.to(dev))
-        a.Hkv = Hkv = k.shape[1]
+        Hkv = k.shape[1]
+        a.Hkv = _int32(Hkv)
         k_out = _empty_as(k)
         a.k, a.k_out = k.data_ptr(), k_out.data_ptr()
         a.k_tok_stride, a.k_head_stride, _ = k.stride()
@@ -1599,8 +1602,8 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
         a.pos_axis_stride, a.pos_tok_stride = positions.stride()
     else:
         raise ValueError(f"positions must be ({axes}, {T}), not {tuple(positions.shape)}")
-    a.dtype, a.T, a.H, a.D, a.axes = DTYPES[q.dtype], T, H, D, axes
-    a.section[:axes] = sections
+    a.dtype, a.T, a.H, a.D, a.axes = DTYPES[q.dtype], T, _int32(H), _int32(D), axes
+    a.section[:axes] = [_int32(s) for s in sections]
     a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
     a.pos_scale, a.rope_scale, a.inverse = float(pos_scale), float(rope_scale), int(inverse)
     _launch(lib().sta_rotary, a, dev, "sta_rotary")
@@ -1618,7 +1621,7 @@ def cache_append(cache, k, v, table, lens, starts=None, seen=None):
     k, v = _rows(k if k.device == dev else k.to(dev)), _rows(v if v.device == dev else v.to(dev))
     a = AppendArgsC()
     keep = cache._fill(a, table, lens)
-    B = a.cache.B
+    B = keep[0].shape[0]
     a.k, a.v, a.T = k.data_ptr(), v.data_ptr(), _int32(k.shape[0])
     a.k_tok_stride, a.k_head_stride, _ = k.stride()
     a.v_tok_stride, a.v_head_stride, _ = v.stride()
@@ -1650,10 +1653,10 @@ def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want
     q = _rows(q if q.device == dev else q.to(dev))
     a = PagedArgsC()
     table, lens = cache._fill(a, table, lens)
-    _require(shape[0] == a.cache.B, "q and table must hold the same number of sequences")
-    a.q, a.H, a.Q = q.data_ptr(), shape[1], 1
+    _require(shape[0] == table.shape[0], "q and table must hold the same number of sequences")
+    a.q, a.H, a.Q = q.data_ptr(), _int32(shape[1]), 1
     if len(shape) == 4:
-        a.Q = shape[2]
+        a.Q = _int32(shape[2])
         a.q_batch_stride, a.q_head_stride, a.q_tok_stride, _ = q.stride()
     else:
         a.q_batch_stride, a.q_head_stride, _ = q.stride()
@@ -1682,8 +1685,8 @@ def cache_evict(cache, table, lens, budget, n_global=32, n_local=32, dst_table=N
     a.max_len = cache._max_len(table, max_len)
     if dst_table is not None:
         dst_table = _ints(dst_table, dev)
-        _require(dst_table.dim() == 2 and dst_table.shape[0] == a.cache.B, "dst_table must have a row a sequence")
-        a.dst_table, a.dst_width = dst_table.data_ptr(), dst_table.shape[1]
+        _require(dst_table.dim() == 2 and dst_table.shape[0] == table.shape[0], "dst_table must have a row a sequence")
+        a.dst_table, a.dst_width = dst_table.data_ptr(), _int32(dst_table.shape[1])
         a.dst_stride = dst_table.stride(0)
     new_lens = torch.empty_like(lens)
     a.new_lens = new_lens.data_ptr()

@@ -66,7 +66,7 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
     row turns by positions[axis of i] * pos_scale * inv_freq[i], the angle formed in 64 bits, and is
     scaled by rope_scale; elements from R on are copied.  sections: how many frequencies each axis
     owns, in order (default: all of them one axis).  D a multiple of 8 up to 512, R / 2 a multiple of
-    8.  Gradients and forward-mode tangents flow to and from q and k, not positions or frequencies."""
+    8, T below 2^31.  Gradients and forward-mode tangents flow to and from q and k, not positions or frequencies."""
     if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad) or _tangents():
         return _Rotary.apply(q, k, positions, inv_freq, sections, pos_scale, rope_scale, False)
     return native.rotary(q, k, positions, inv_freq, sections, pos_scale, rope_scale)

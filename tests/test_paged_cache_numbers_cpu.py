@@ -1,0 +1,93 @@
+"""CPU checks of sizes and numbers beyond 32 bits at the paged cache's entry points, whose C structs hold 32: nothing is
+launched, and tensors that would not fit here stand on the meta device."""
+import ctypes
+
+import pytest
+import torch
+
+BIG = 2 ** 32
+
+
+@pytest.fixture
+def native(monkeypatch):
+    import _sta_native as native
+
+    def launch(fn, args, dev, what):
+        launched.append((what, args))
+    launched = native_launched
+    launched.clear()
+    monkeypatch.setattr(native, "_device_input", lambda x, name: None)
+    monkeypatch.setattr(native, "_launch", launch)
+    return native
+
+
+native_launched = []
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("T", [BIG + 1, BIG, 2 ** 31])
+def test_rotary_refuses_more_tokens_than_32_bits_hold(native, T):
+    pos, inv = _meta(T, dtype=torch.int32), _meta(8, dtype=torch.float32)
+    for q, k in ((_meta(T, 1, 16), None), (_meta(T, 1, 16), _meta(T, 2, 16))):
+        with pytest.raises(ValueError, match="tokens"):
+            native.rotary(q, k, pos, inv)
+    assert not native_launched
+
+
+def test_rotary_keeps_the_sizes_it_takes(native):
+    T = 2 ** 31 - 1
+    native.rotary(_meta(T, 1, 16), None, _meta(T, dtype=torch.int32), _meta(8, dtype=torch.float32))
+    (_, a), = native_launched
+    assert (a.T, a.H, a.Hkv, a.D, list(a.section)) == (T, 1, 0, 16, [8, 0, 0, 0])
+
+
+@pytest.mark.parametrize("q,k,half,sections", [
+    ((3, BIG + 4, 16), None, 8, None), ((3, 4, 16), (3, BIG + 4, 16), 8, None), ((3, 4, BIG + 16), None, 8, None),
+    ((3, 4, 16), None, 8, (BIG + 8, -BIG))])
+def test_rotary_does_not_fold_large_sizes_into_small_ones(native, q, k, half, sections):
+    """A number that 32 bits do not hold reaches the library as one that it refuses."""
+    axes = len(sections) if sections else 1
+    pos, inv = _meta(axes, 3, dtype=torch.int32), _meta(half, dtype=torch.float32)
+    native.rotary(_meta(*q), None if k is None else _meta(*k), pos, inv, sections)
+    (_, a), = native_launched
+    a.positions = a.inv_freq = 256                            # refused before any address is used
+    a.q = a.q_out = a.k = a.k_out = 256
+    assert native.lib().sta_rotary(ctypes.byref(a), None) in (-1, -2)
+
+
+def _cache(native, pages=4, heads=2, slots=16, d=64):
+    return native.PagedCache(_meta(pages, heads, slots, d), _meta(pages, heads, slots, d))
+
+
+@pytest.mark.parametrize("shape", [{"heads": BIG + 2}, {"slots": BIG + 16}, {"d": BIG + 64}])
+def test_a_cache_does_not_fold_large_sizes_into_small_ones(native, shape):
+    c = _cache(native, **shape)
+    with pytest.raises(RuntimeError):
+        native.paged_attention(_meta(3, 2 * c.kv_heads, c.head_dim), c, _meta(3, 5, dtype=torch.int32),
+                               _meta(3, dtype=torch.int32), max_len=64)
+    assert not native_launched
+
+
+@pytest.mark.parametrize("q", [(BIG + 3, 4, 64), (3, BIG + 4, 64), (3, 4, BIG + 1, 64)])
+def test_attention_refuses_more_sequences_heads_or_queries(native, q):
+    with pytest.raises(RuntimeError):
+        native.paged_attention(_meta(*q), _cache(native), _meta(q[0], 5, dtype=torch.int32),
+                               _meta(q[0], dtype=torch.int32), max_len=64)
+    assert not native_launched
+
+
+def test_wide_tables_and_many_pages_stay_as_large_as_they_can(native):
+    c = _cache(native, pages=BIG + 4)
+    assert c._c.pages == 2 ** 31 - 1
+    native.paged_attention(_meta(3, 4, 64), c, _meta(3, BIG + 5, dtype=torch.int32), _meta(3, dtype=torch.int32),
+                           max_len=64)
+    (_, a), = native_launched
+    assert a.cache.table_width == 2 ** 31 - 1 and a.max_len == 64
+    evictable = native.PagedCache(c.k, c.v, _meta(BIG + 4, 2, 16, dtype=torch.float32),
+                                  _meta(BIG + 4, 2, 16, dtype=torch.int32))
+    native.cache_evict(evictable, _meta(3, 5, dtype=torch.int32), _meta(3, dtype=torch.int32), 64, max_len=70,
+                       dst_table=_meta(3, BIG + 1, dtype=torch.int32))
+    assert native_launched[1][1].dst_width == 2 ** 31 - 1
