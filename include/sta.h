@@ -604,7 +604,7 @@ int sta_rotary(const sta_rotary_args* args, void* stream);
 /* Write T new keys and values behind the sequences' keys: rows starts[b] .. starts[b + 1] - 1 of k
  * and v go to the slots lens[b] .. of sequence b (starts NULL: one row a sequence, T = B; rows
  * outside [starts[0], starts[B]) are not read).  A cache with weight gets 0 there, one with pos
- * seen[b] + i (seen NULL: the slot).  Keys past the table's end are dropped.  new_lens[b], not the
+ * seen[b] + i, at most 2^31 - 1 (seen NULL: the slot).  Keys past the table's end are dropped.  new_lens[b], not the
  * lens array itself, receives the new length. */
 typedef struct sta_append_args {
   sta_cache cache;

@@ -1478,7 +1478,9 @@ def _int32(x):
 
 
 def _ints(x, dev):
-    """A device int32 tensor with unit stride in its last dim."""
+    """A device int32 tensor with unit stride in its last dim; 64-bit numbers beyond 32 bits as _int32."""
+    if x.dtype == torch.int64:
+        x = x.clamp(-2 ** 31, 2 ** 31 - 1)
     if x.dtype != torch.int32 or x.device != dev:
         x = x.to(device=dev, dtype=torch.int32)
     return x if x.stride(-1) == 1 else x.contiguous()      # lens of stride 0 (expanded) too

@@ -79,9 +79,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       *(u32x4*)(vo + h1 * c.v_hs + w1) = v1;
     }
   }
+  const int seen = a.seen ? a.seen[b] : j - i, pos = seen > INT32_MAX - i ? INT32_MAX : seen + i;
   for (int h = lane; h < c.Hkv; h += 64) {
     if (c.weight) c.weight[p * c.w_ps + h * c.w_hs + s] = 0.f;
-    if (c.pos) c.pos[p * c.p_ps + h * c.p_hs + s] = (a.seen ? a.seen[b] : j - i) + i;
+    if (c.pos) c.pos[p * c.p_ps + h * c.p_hs + s] = pos;
   }
 }
 

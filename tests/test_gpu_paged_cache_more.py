@@ -37,3 +37,42 @@ def test_rotary_forward_mode_on_the_device():
     assert torch.equal(a.primal, plain[0]) and torch.equal(b.primal, plain[1])
     _check_rotary(tq, a.tangent, positions, inv_freq, (16, 16), 0.5, 1.25)
     assert b.tangent is None or torch.all(b.tangent == 0)
+
+
+# ------------------------------------------------------------------------------- numbers beyond 32 bits
+def test_lengths_and_pages_of_64_bits():
+    """Lengths beyond 32 bits count as the table's end, pages beyond them as none, tokens seen stay the largest number."""
+    import paged_cache as pc
+    made = Made(900, [90, 40], 2, 64, 16, BF16)
+    q = _randn(901, (2, 4, 64), BF16)
+    far = torch.tensor([2 ** 32 + 5, -2 ** 32 + 5], device=DEV)
+    table = made.table.long()
+    holes = table.clone()
+    holes[0, 1], holes[0, 2] = holes[0, 1] + 2 ** 32, holes[0, 2] - 2 ** 32
+    want = pc.paged_attention(q, made.cache, made.table, torch.tensor([made.cap, 0], dtype=torch.int32, device=DEV))
+    assert torch.equal(pc.paged_attention(q, made.cache, table, far), want)
+    gone = made.table.clone()
+    gone[0, 1:3] = -1
+    want = pc.paged_attention(q, made.cache, gone, made.lens)
+    assert torch.equal(pc.paged_attention(q, made.cache, holes, made.lens.long()), want)
+    assert pc.cache_evict(made.cache, table, far, 2 ** 20).tolist() == [made.cap, 0]
+    k = _randn(902, (2, 2, 64), BF16)
+    before = made.cache.k.clone()
+    assert pc.cache_append(made.cache, k, k, table, far).tolist() == [made.cap, 1]
+    p = made.rows[1][0]
+    assert torch.equal(made.cache.k[p, :, 0], k[1])
+    before[p, :, 0] = k[1]
+    assert torch.equal(made.cache.k, before)
+
+
+def test_tokens_seen_stop_at_the_largest_number():
+    """pos is seen + i as far as 32 bits go; it does not wrap into the first tokens, which eviction always keeps."""
+    import paged_cache as pc
+    made = Made(910, [0, 0], 1, 64, 16, BF16, room=16)
+    k = _randn(911, (8, 1, 64), BF16)
+    starts = torch.tensor([0, 4, 8], dtype=torch.int32, device=DEV)
+    seen = torch.tensor([2 ** 31 - 3, 2 ** 32 + 9], device=DEV)
+    pc.cache_append(made.cache, k, k, made.table, made.lens, starts, seen)
+    most = 2 ** 31 - 1
+    assert made.cache.pos[made.rows[0][0], 0, :4].tolist() == [most - 2, most - 1, most, most]
+    assert made.cache.pos[made.rows[1][0], 0, :4].tolist() == [most] * 4

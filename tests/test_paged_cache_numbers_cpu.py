@@ -91,3 +91,15 @@ def test_wide_tables_and_many_pages_stay_as_large_as_they_can(native):
     native.cache_evict(evictable, _meta(3, 5, dtype=torch.int32), _meta(3, dtype=torch.int32), 64, max_len=70,
                        dst_table=_meta(3, BIG + 1, dtype=torch.int32))
     assert native_launched[1][1].dst_width == 2 ** 31 - 1
+
+
+def test_index_tensors_of_64_bits_are_clamped(native):
+    """A length, page or offset beyond 32 bits stays as far beyond as it can: it does not become a small one."""
+    x = torch.tensor([2 ** 32 + 5, -2 ** 32 + 3, 2 ** 31, -2 ** 31 - 1, 7, -1, 2 ** 31 - 1, -2 ** 31])
+    got = native._ints(x, x.device)
+    most, least = 2 ** 31 - 1, -2 ** 31
+    assert got.dtype == torch.int32 and got.tolist() == [most, least, most, least, 7, -1, most, least]
+    table = native._ints(x.reshape(2, 4).t(), x.device)
+    assert table.stride(-1) == 1 and table.tolist() == got.reshape(2, 4).t().tolist()
+    same = torch.tensor([1, 2], dtype=torch.int32)
+    assert native._ints(same, same.device) is same
