@@ -603,9 +603,10 @@ int sta_rotary(const sta_rotary_args* args, void* stream);
 
 /* Write T new keys and values behind the sequences' keys: rows starts[b] .. starts[b + 1] - 1 of k
  * and v go to the slots lens[b] .. of sequence b (starts NULL: one row a sequence, T = B; rows
- * outside [starts[0], starts[B]) are not read).  A cache with weight gets 0 there, one with pos
- * seen[b] + i, at most 2^31 - 1 (seen NULL: the slot).  Keys past the table's end are dropped.  new_lens[b], not the
- * lens array itself, receives the new length. */
+ * outside [starts[0], starts[B]) are not read, and an offset below 0 or past T counts as 0 or T).
+ * A cache with weight gets 0 there, one with pos seen[b] + i, at most 2^31 - 1 (seen NULL: the slot).
+ * Keys past the table's end are dropped.  new_lens[b], not the lens array itself, receives the new
+ * length. */
 typedef struct sta_append_args {
   sta_cache cache;
   const void* k;           /* (T, Hkv, D) in the cache's dtype, 16-byte rows */

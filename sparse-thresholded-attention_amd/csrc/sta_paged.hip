@@ -37,11 +37,14 @@ __device__ __forceinline__ int sequence_of(const int32_t* starts, int B, int t) 
   }
 }
 
+// where sequence b begins among the rows that there are
+__device__ __forceinline__ int row_of(const AppendArgs& a, int b) { return min(max(a.starts[b], 0), a.T); }
+
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const CacheView& c = a.c;
   if (blockIdx.x == 0) {
     for (int b = threadIdx.x; b < c.B; b += 256) {
-      const int n = a.starts ? max(a.starts[b + 1] - a.starts[b], 0) : 1;
+      const int n = a.starts ? max(row_of(a, b + 1) - row_of(a, b), 0) : 1;
       a.new_lens[b] = (int)min((int64_t)c.len(b) + n, (int64_t)c.cap);
     }
   }
@@ -51,10 +54,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   if (a.starts) {
     b = uniform(sequence_of(a.starts, c.B, t));
     if (b < 0 || t >= a.starts[b + 1]) return;
-    i = t - a.starts[b];
+    i = t - row_of(a, b);
   }
   const int64_t at = (int64_t)c.len(b) + i;
-  if (i < 0 || at >= c.cap) return;
+  if (at >= c.cap) return;
   const int j = (int)at, p = uniform(c.page_of(c.table + (int64_t)b * c.t_stride, j));
   if (p < 0) return;
   const int s = c.slot_of(j), shift = a.row_shift, all = c.Hkv << shift;

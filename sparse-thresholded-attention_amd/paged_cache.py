@@ -86,9 +86,9 @@ def cache_append(cache, k, v, table, lens, starts=None, seen=None):
 
     table (B, pages of a sequence) int32, -1 where there is no page; lens (B,) int32.  Without starts
     every sequence gets one row (T = B); with starts (B + 1,) int32 the rows starts[b] ..
-    starts[b + 1] - 1 are sequence b's, and rows outside all of them are not read.  seen (B,): how many
-    tokens the sequence has had before these, the first new key's cache.pos (default: its slot, right
-    while nothing has been evicted).  New keys start with weight 0."""
+    starts[b + 1] - 1 are sequence b's, as far as k has them, and rows outside all of them are not
+    read.  seen (B,): how many tokens the sequence has had before these, the first new key's cache.pos
+    (default: its slot, right while nothing has been evicted).  New keys start with weight 0."""
     return native.cache_append(cache, k, v, table, lens, starts, seen)
 
 

@@ -76,3 +76,16 @@ def test_tokens_seen_stop_at_the_largest_number():
     most = 2 ** 31 - 1
     assert made.cache.pos[made.rows[0][0], 0, :4].tolist() == [most - 2, most - 1, most, most]
     assert made.cache.pos[made.rows[1][0], 0, :4].tolist() == [most] * 4
+
+
+def test_offsets_of_rows_that_are_not_there():
+    """Offsets outside the rows of k and v add no length: only rows that were written count."""
+    import paged_cache as pc
+    made = Made(920, [3, 5, 0], 2, 64, 16, BF16, room=16)
+    k = _randn(921, (6, 2, 64), BF16)
+    for starts, new in (([0, 4, 9, 9], [7, 7, 0]), ([0, 2, 6, 20], [5, 9, 0]), ([6, 6, 7, 8], [3, 5, 0]),
+                        ([2 ** 31 - 1] * 4, [3, 5, 0]), ([-3, 2, 6, 6], [5, 9, 0])):
+        got = pc.cache_append(made.cache, k, k, made.table, made.lens, torch.tensor(starts, device=DEV))
+        assert got.tolist() == new, starts
+    p = made.rows[0][0]                                       # the last call: rows 0 and 1 behind the three keys
+    assert torch.equal(made.cache.k[p, :, 3:5].transpose(0, 1), k[:2])
