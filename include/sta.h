@@ -612,7 +612,7 @@ typedef struct sta_append_args {
   const void* k;           /* (T, Hkv, D) in the cache's dtype, 16-byte rows */
   const void* v;
   int64_t k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
-  int32_t T;               /* below 2^26, and T * Hkv below 2^31 */
+  int32_t T;               /* at most 2^26 - 4, and T * Hkv below 2^31 */
   const int32_t* starts;   /* (B + 1,) ascending, or NULL */
   const int32_t* seen;     /* (B,) or NULL */
   int32_t* new_lens;       /* (B,) */

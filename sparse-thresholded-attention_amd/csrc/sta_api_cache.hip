@@ -227,8 +227,9 @@ int sta_cache_append(const sta_append_args* a, void* stream) {
   int rc = check_cache_shape(a->cache);
   if (rc != STA_OK) return rc;
   if (a->T < 0) return fail(STA_ERR_INVALID_ARG, "T=%d must be >= 0", a->T);
-  if ((int64_t)a->T * a->cache.Hkv >= ((int64_t)1 << 31) || a->T >= 1 << 26)
-    return fail(STA_ERR_UNSUPPORTED, "T=%d must be below 2^26, and times Hkv=%d below 2^31", a->T, a->cache.Hkv);
+  // four tokens a workgroup of 256 threads, below 2^32 threads
+  if ((int64_t)a->T * a->cache.Hkv >= ((int64_t)1 << 31) || a->T > (1 << 26) - 4)
+    return fail(STA_ERR_UNSUPPORTED, "T=%d must be at most 2^26 - 4, and times Hkv=%d below 2^31", a->T, a->cache.Hkv);
   if (!a->starts && a->T != a->cache.B)
     return fail(STA_ERR_INVALID_ARG, "without starts T=%d must be B=%d", a->T, a->cache.B);
   if ((rc = check_cache(a->cache)) != STA_OK) return rc;

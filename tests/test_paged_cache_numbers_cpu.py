@@ -103,3 +103,26 @@ def test_index_tensors_of_64_bits_are_clamped(native):
     assert table.stride(-1) == 1 and table.tolist() == got.reshape(2, 4).t().tolist()
     same = torch.tensor([1, 2], dtype=torch.int32)
     assert native._ints(same, same.device) is same
+
+
+def _append_args(native, T):
+    """Arguments that are refused for k at the latest, so that nothing is launched."""
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    a = native.AppendArgsC()
+    c = a.cache
+    c.k = c.v = c.table = c.lens = p
+    c.dtype, c.pages, c.page_size, c.Hkv, c.D = 1, 64, 16, 1, 64
+    for x in ("k", "v"):
+        setattr(c, x + "_page_stride", 16 * 64), setattr(c, x + "_head_stride", 16 * 64), setattr(c, x + "_slot_stride", 64)
+    c.table_stride, c.table_width, c.B = 4, 4, 2
+    a.T, a.starts, a.new_lens = T, p, p + 1024
+    return buf, a
+
+
+@pytest.mark.parametrize("T,code", [(2 ** 26 - 4, -1), (2 ** 26 - 3, -2), (2 ** 26 - 1, -2)])
+def test_append_takes_as_many_tokens_as_a_grid_holds(T, code):
+    """Four tokens a workgroup of 256 threads: a grid holds below 2^32 threads, so 2^24 - 1 workgroups."""
+    import _sta_native as native
+    buf, a = _append_args(native, T)
+    assert native.lib().sta_cache_append(ctypes.byref(a), None) == code
