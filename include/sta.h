@@ -652,7 +652,7 @@ int sta_paged_attention(const sta_paged_args* args, void* stream);
  * the pages of dst_table, none of which the tables of this call may hold otherwise; the source stays.
  * new_lens[b], not the lens array itself, receives min(lens[b], budget). */
 typedef struct sta_evict_args {
-  sta_cache cache;         /* weight and pos required */
+  sta_cache cache;         /* weight and pos required; B * Hkv below 2^31 */
   int32_t budget, n_global, n_local; /* budget >= 1 */
   int32_t max_len;         /* lengths are at most this */
   const int32_t* dst_table; /* (B, dst_width), dst_width * page_size >= min(budget, max_len) */

@@ -147,6 +147,9 @@ int evict_check(const sta_evict_args* a) {
   if (!a) return fail(STA_ERR_INVALID_ARG, "args is NULL");
   int rc = check_cache_shape(a->cache);
   if (rc != STA_OK) return rc;
+  // the kernel numbers the pairs in an int
+  if ((int64_t)a->cache.B * a->cache.Hkv > INT_MAX)
+    return fail(STA_ERR_INVALID_ARG, "B=%d times Hkv=%d must be below 2^31", a->cache.B, a->cache.Hkv);
   if (a->budget < 1) return fail(STA_ERR_INVALID_ARG, "budget=%d must be >= 1", a->budget);
   if (a->n_global < 0 || a->n_local < 0)
     return fail(STA_ERR_INVALID_ARG, "n_global=%d / n_local=%d must be >= 0", a->n_global, a->n_local);

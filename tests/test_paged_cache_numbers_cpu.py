@@ -126,3 +126,16 @@ def test_append_takes_as_many_tokens_as_a_grid_holds(T, code):
     import _sta_native as native
     buf, a = _append_args(native, T)
     assert native.lib().sta_cache_append(ctypes.byref(a), None) == code
+
+
+@pytest.mark.parametrize("B,Hkv,ok", [(32768, 65535, True), (32769, 65535, False), (65535, 65535, False)])
+def test_eviction_numbers_its_heads_in_32_bits(B, Hkv, ok):
+    """The kernel numbers the (sequence, kv head) pairs in an int."""
+    import _sta_native as native
+    a = native.EvictArgsC()
+    c = a.cache
+    c.dtype, c.pages, c.page_size, c.Hkv, c.D = 1, 4, 1, Hkv, 64
+    c.table_stride, c.table_width, c.B = 1, 1, B
+    a.budget, a.max_len = 1, 1
+    assert (native.lib().sta_evict_workspace_size(ctypes.byref(a)) > 0) == ok
+    assert ok or native.lib().sta_cache_evict(ctypes.byref(a), None) == -1
