@@ -89,3 +89,199 @@ def test_offsets_of_rows_that_are_not_there():
         assert got.tolist() == new, starts
     p = made.rows[0][0]                                       # the last call: rows 0 and 1 behind the three keys
     assert torch.equal(made.cache.k[p, :, 3:5].transpose(0, 1), k[:2])
+
+
+# --------------------------------------------------------------------------- runs of several units
+def _attend_f64(made, q, sm_scale):
+    """As paged_ref.attend, in matrix products over a kv head's rows: out, lse, rel (B, H, Q), reach like out, and a
+    kv head's weights with the bound of their error: {(b, h): (drawn, tol)}."""
+    q4 = (q if q.dim() == 4 else q[:, :, None]).double()
+    B, H, Q, D = q4.shape
+    c, ps = made.cache, made.ps
+    G, n_max = H // c.kv_heads, max(max(made.lens_host), 1)
+    out, reach = torch.zeros_like(q4), torch.zeros_like(q4)
+    lse = torch.full(q4.shape[:3], float("-inf"), dtype=torch.float64, device=DEV)
+    rel, drawn = torch.zeros_like(lse), {}
+    for b, n in enumerate(made.lens_host):
+        if n == 0:
+            continue
+        ids = made.table[b, :-(-n // ps)].long()
+        ends = (n - (Q - 1) + torch.arange(Q, device=DEV)).repeat(G)              # rows are (head of the group, query)
+        unseen = torch.arange(n, device=DEV) >= ends[:, None]
+        some = (ends > 0)[:, None]
+        for h in range(c.kv_heads):
+            k = c.k[ids, h].reshape(-1, D)[:n].double()
+            v = c.v[ids, h].reshape(-1, D)[:n].double()
+            rows = q4[b, h * G:(h + 1) * G].reshape(-1, D)
+            s = (rows @ k.t().contiguous() * sm_scale).masked_fill(unseen, float("-inf"))
+            p = torch.where(some, torch.softmax(torch.where(some, s, 0.0), dim=-1), 0.0)
+            size = (rows.abs() @ k.abs().t().contiguous() * abs(sm_scale)).masked_fill(unseen, 0.0).amax(dim=-1)
+            r = 2 * (D + 8) * U * size + (n_max + 64) * U
+            part = slice(h * G, (h + 1) * G)
+            out[b, part] = (p @ v).view(G, Q, D)
+            reach[b, part] = (p @ v.abs()).view(G, Q, D)
+            lse[b, part] = torch.where(some[:, 0], torch.logsumexp(torch.where(some, s, 0.0), dim=-1),
+                                       float("-inf")).view(G, Q)
+            rel[b, part] = r.view(G, Q)
+            # each probability off by its row's rel, their sum over the rows by a rounding each
+            drawn[b, h] = p.sum(0), (r[:, None] * p).sum(0) + rows.shape[0] * U * p.sum(0)
+    return out, lse, rel, reach, drawn
+
+
+def _check_attend_f64(made, q, got, lse, weight=None, weight0=None, sm_scale=None):
+    out, want_lse, rel, reach, drawn = _attend_f64(made, q, 1 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale)
+    half, tiny = _half_step(q.dtype), torch.finfo(q.dtype).smallest_normal
+    tol = (rel[..., None] * reach + half * out.abs()) * 1.01 + tiny * half
+    err = (got.double().reshape(out.shape) - out).abs()
+    assert torch.all(err <= tol), f"out: {(err / tol).max().item():.2f} of the bound"
+    if lse is not None:
+        lse, fine = lse.double().reshape(want_lse.shape), torch.isfinite(want_lse)
+        assert torch.equal(torch.isfinite(lse), fine) and torch.all(lse[~fine] == float("-inf"))
+        off = (lse - want_lse).abs()[fine] / (rel + 4 * U * (1 + want_lse.abs()))[fine]
+        assert torch.all(off <= 1), f"lse: {off.max().item():.2f} of the bound"
+    if weight is None:
+        return
+    grow, bound = weight0.double(), torch.zeros_like(weight0, dtype=torch.float64)
+    touched = torch.zeros_like(weight0, dtype=torch.bool)
+    for (b, h), (w, t) in drawn.items():
+        ids = made.table[b, :-(-len(w) // made.ps)].long()
+        pad = len(ids) * made.ps - len(w)
+        w, t = (torch.nn.functional.pad(x, (0, pad)).view(-1, made.ps) for x in (w, t))
+        grow[ids, h] += w
+        bound[ids, h] += t
+        touched[ids, h] = (torch.arange(len(ids) * made.ps, device=DEV) < len(ids) * made.ps - pad).view(-1, made.ps)
+    # one addition in fp32; a probability below the normal range may go
+    tol = bound * 1.01 + 2 * U * grow.abs() + 2.0 ** -120
+    off = ((weight.double() - grow).abs() / tol)[touched]
+    assert torch.all(off <= 1), f"weight: {off.max().item():.2f} of the bound, {int((off > 1).sum())} keys"
+    assert torch.equal(weight[~touched], weight0[~touched]), "a weight outside the sequences changed"
+
+
+def _ragged(seed, B, low, high):
+    """Lengths of low to high with empty and very short sequences among them."""
+    g = torch.Generator().manual_seed(seed)
+    lens = torch.randint(low, high, (B,), generator=g).tolist()
+    for i in range(2, B, 5):
+        lens[i] = (0, 1, 33, 0, 127)[i // 5 % 5]
+    return lens
+
+
+RUNS = [
+    # B, lengths, H, Hkv, Q, D, page size, dtype: each gives the chip's workgroups three units and more
+    (26, (900, 3600), 16, 8, 1, 64, 16, BF16),
+    (30, (900, 3600), 8, 8, 1, 128, 64, F16),
+    (20, (900, 2100), 8, 8, 1, 64, 32, F32),
+    (24, (1200, 3600), 320, 8, 1, 128, 16, F16),               # two row tiles, one query
+    (24, (1200, 3600), 512, 8, 1, 64, 16, BF16),               # the same with weights from scores formed again
+    (26, (900, 3600), 32, 8, 3, 128, 16, BF16),
+    (26, (900, 3600), 16, 8, 7, 64, 8, F16),
+    (18, (900, 2200), 16, 8, 5, 128, 16, F32),
+    (26, (900, 3600), 32, 8, 16, 128, 32, BF16),               # 64 rows, two tiles of 32
+    (26, (900, 3600), 32, 8, 20, 128, 16, BF16),               # 80 rows: keys through LDS
+    (26, (900, 3600), 32, 8, 40, 64, 8, F16),                  # 160 rows: two tiles of 128
+    (30, (900, 3600), 24, 8, 33, 128, 64, F16),
+]
+
+
+@pytest.mark.parametrize("case", range(len(RUNS)))
+def test_attention_in_runs_of_several_units_and_heads(case):
+    """Runs that hold several units, that end one kv head and begin the next, or that hold whole ones."""
+    import paged_cache as pc
+    B, (low, high), H, Hkv, Q, D, ps, dtype = RUNS[case]
+    lens = _ragged(case, B, low, high)
+    print(f"[case] runs {RUNS[case]}", flush=True)
+    unit = 64 if dtype == F32 else 128
+    units = Hkv * sum(max(1, -(-max(n - (Q - 1), 0) // unit)) for n in lens)
+    assert units >= 3 * (768 if D == 64 and H // Hkv * Q <= 16 else 512), units    # at most as many runs, so three each
+    made = Made(1000 + 10 * case, lens, Hkv, D, ps, dtype, layout=("head", "slot", "pair")[case % 3])
+    made.cache.weight.zero_()
+    if case % 2:                                              # additions to weights that keys have
+        made.cache.weight.add_(0.25)
+    q = _randn(1001 + 10 * case, (B, H, Q, D) if Q > 1 else (B, H, D), dtype, 1.5)
+    weight0 = made.cache.weight.clone()
+    plain = pc.paged_attention(q, made.cache, made.table, made.lens)
+    got, lse = pc.paged_attention(q, made.cache, made.table, made.lens, accumulate=True, want_lse=True)
+    _check_attend_f64(made, q, got, lse, made.cache.weight, weight0)
+    assert torch.equal(plain, got)
+    before = made.cache.weight.clone()
+    made.cache.weight.copy_(weight0)
+    again = pc.paged_attention(q, made.cache, made.table, made.lens, accumulate=True)
+    assert torch.equal(again, got) and torch.equal(made.cache.weight, before)
+
+
+WEIGHTS = [
+    # lens, H, Hkv, Q, D, page size, dtype
+    ([5000, 4097], 8, 2, 1, 128, 64, BF16), ([1000, 0, 257, 511], 32, 8, 1, 128, 16, BF16),
+    ([2500], 16, 1, 1, 128, 256, F16), ([3000, 77], 6, 2, 1, 128, 1, F32), ([2513, 90], 71, 1, 1, 64, 8, BF16),
+    ([1500, 7], 4, 2, 40, 128, 16, F32), ([4000, 9, 0, 1301], 8, 2, 16, 128, 16, BF16),
+    ([6000, 33, 5], 28, 4, 32, 128, 32, F16), ([610, 90], 8, 2, 20, 128, 4, BF16), ([4000, 40], 8, 2, 3, 64, 16, F32),
+]
+
+
+@pytest.mark.parametrize("case", range(len(WEIGHTS)))
+def test_weights_of_many_keys(case):
+    """What each key draws, from weights of zero: a key of thousands draws little, and all of it counts."""
+    import paged_cache as pc
+    lens, H, Hkv, Q, D, ps, dtype = WEIGHTS[case]
+    print(f"[case] weights {WEIGHTS[case]}", flush=True)
+    made = Made(1300 + 10 * case, lens, Hkv, D, ps, dtype)
+    made.cache.weight.zero_()
+    q = _randn(1301 + 10 * case, (len(lens), H, Q, D), dtype, 1.5)
+    weight0 = made.cache.weight.clone()
+    got, lse = pc.paged_attention(q, made.cache, made.table, made.lens, accumulate=True, want_lse=True)
+    _check_attend_f64(made, q, got, lse, made.cache.weight, weight0)
+
+
+def test_weights_of_two_streams_at_once():
+    import paged_cache as pc
+    a, b = Made(1400, [3000, 100], 4, 128, 16, BF16), Made(1420, [700, 2900], 2, 64, 32, F16)
+    qa, qb = _randn(1401, (2, 16, 128), BF16), _randn(1421, (2, 16, 40, 64), F16)
+    ones = [pc.PagedCache(m.cache.k, m.cache.v, m.cache.weight.clone(), m.cache.pos) for m in (a, b)]
+    for _ in range(4):
+        pc.paged_attention(qa, ones[0], a.table, a.lens, accumulate=True)
+        pc.paged_attention(qb, ones[1], b.table, b.lens, accumulate=True)
+    torch.cuda.synchronize()
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(4):
+        with torch.cuda.stream(s):
+            pc.paged_attention(qa, a.cache, a.table, a.lens, accumulate=True)
+        with torch.cuda.stream(t):
+            pc.paged_attention(qb, b.cache, b.table, b.lens, accumulate=True)
+    torch.cuda.synchronize()
+    assert torch.equal(a.cache.weight, ones[0].weight) and torch.equal(b.cache.weight, ones[1].weight)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, BF16), (64, F16), (128, F16)])
+@pytest.mark.parametrize("Q", [20, 40])
+def test_infinite_values_among_many_rows(Q, D, dtype):
+    """A workgroup of 128 rows repeats a kv head whose values are infinite, and not the next one of its run."""
+    import paged_cache as pc
+    inf = float("inf")
+    # one page a sequence and kv head of 8, so that a run holds several heads; and one long sequence, cut into runs
+    for lens in ([100] * 90 + [0, 33] * 10, [5000, 250]):
+        made = Made(1500, lens, 8, D, 128, dtype)
+        made.cache.weight.zero_()
+        other = made.cache.weight.clone()
+        q = _randn(1501, (len(lens), 32, Q, D), dtype)
+        clean, lse = pc.paged_attention(q, made.cache, made.table, made.lens, accumulate=True, want_lse=True)
+        v, was = made.cache.v, made.cache.v.clone()
+        p = made.rows[1][0]
+        v[p, 2, 5, 7], v[p, 2, 6, 9], v[p, 2, 7, 9], v[p, 2, 8, 11] = inf, inf, -inf, -inf
+        v[made.rows[0][0], 5, 0, 0] = -inf
+        marked = pc.PagedCache(made.cache.k, v, other, made.cache.pos)
+        got, same = pc.paged_attention(q, marked, made.table, made.lens, accumulate=True, want_lse=True)
+        assert torch.all(got[1, 8:12, :, 7] == inf) and torch.isnan(got[1, 8:12, :, 9]).all()
+        assert torch.all(got[1, 8:12, :, 11] == -inf) and torch.all(got[0, 20:24, :, 0] == -inf)
+        keep = torch.ones_like(got, dtype=torch.bool)
+        keep[1, 8:12, :, [7, 9, 11]] = False
+        keep[0, 20:24, :, 0] = False
+        assert torch.isfinite(got[keep]).all()
+        # rows of other kv heads are not repeated in fp32: the same bits; the repeated ones within the bound
+        v.copy_(was)
+        full = torch.where(keep, got, clean)
+        _check_attend_f64(made, q, full, same, other, torch.zeros_like(other))
+        _check_attend_f64(made, q, clean, lse, made.cache.weight, torch.zeros_like(other))
+        if len(lens) > 2:                                     # whole heads: others' rows see no repeat
+            rest = torch.ones(got.shape[:2], dtype=torch.bool, device=DEV)
+            rest[1, 8:12] = rest[0, 20:24] = False
+            assert torch.equal(got[rest], clean[rest])
