@@ -113,7 +113,7 @@ int paged_check(const sta_paged_args* a) {
 
 struct PagedLayout {
   PagedCut cut;
-  size_t part_off, ml_off, lse_off, scores_off, total;
+  size_t part_off, ml_off, stats_off, scores_off, total;
   int64_t score_stride;
 };
 
@@ -134,8 +134,10 @@ PagedLayout paged_layout(const sta_paged_args* a) {
   off = align256(off + part_rows * a->cache.D * 4);
   L.ml_off = off;                                     // their maxima and sums
   off = align256(off + part_rows * 8);
-  L.lse_off = off;                                    // (B, H, Q) for the weights when not an output
-  if (a->accumulate && !L.cut.small) off = align256(off + rows * 4);
+  // the rows' maxima and sums for the weights: several queries leave them in the whole kv heads' records, which the
+  // join has read by then
+  L.stats_off = a->Q > 1 ? L.ml_off + (size_t)2 * L.cut.runs * L.cut.tiles * L.cut.rows * 8 : off;
+  if (a->accumulate && !L.cut.small && a->Q == 1) off = align256(off + rows * 8);
   L.scores_off = off;                                 // (B, H, Q, score_stride)
   if (a->accumulate && !L.cut.reform) off = align256(off + rows * L.score_stride * 4);
   L.total = off;
@@ -288,7 +290,9 @@ int sta_paged_attention(const sta_paged_args* a, void* stream) {
   d.sm_scale = a->sm_scale;
   d.accumulate = a->accumulate != 0;
   d.out = a->out;
-  d.lse = a->lse ? a->lse : a->accumulate && !L.cut.small ? (float*)(ws + L.lse_off) : nullptr;
+  d.lse = a->lse;
+  d.stats = a->accumulate && !L.cut.small ? (float2*)(ws + L.stats_off) : nullptr;
+  d.stat_stride = a->Q > 1 ? (int64_t)L.cut.tiles * L.cut.rows : a->H / a->cache.Hkv;
   d.scores = a->accumulate && !L.cut.reform ? (float*)(ws + L.scores_off) : nullptr;
   d.score_stride = L.score_stride;
   d.part_o = (float*)(ws + L.part_off);

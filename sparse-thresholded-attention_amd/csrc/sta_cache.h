@@ -50,7 +50,11 @@ struct PagedArgs {
   float sm_scale;
   int accumulate;
   void* out;
-  float* lse;                       // (B, H, Q), the caller's or in the workspace; NULL: not stored
+  float* lse;                       // (B, H, Q); NULL: not stored
+  // accumulate: of each row its scores' maximum and 1 / the sum of exp(score - maximum), 0 where it saw nothing;
+  // row g Q + i of a kv head at (b Hkv + kv head) stat_stride + row
+  float2* stats;
+  int64_t stat_stride;
   float* scores;                    // (B, H, Q, score_stride); NULL: not stored
   int64_t score_stride;
   float* part_o;                    // (records, rows, D) unnormalised outputs of unfinished row tiles

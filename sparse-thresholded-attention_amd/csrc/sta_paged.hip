@@ -165,6 +165,11 @@ __device__ __forceinline__ int64_t whole_record(const PagedArgs& a, int b, int h
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 __device__ __forceinline__ float at_least(float m) { return m == -INFINITY ? 0.f : m; }   // what p is relative to
+// What the weights' probabilities are formed from, as exp(score - x) y: a maximum (at_least) and a sum.  Not exp(score -
+// lse): near a log-sum-exp of 1000 its rounding alone is 3e-5 of every weight.
+__device__ __forceinline__ float2 stats_of(float m, float l) { return make_float2(m, l == 0.f ? 0.f : 1.f / l); }
+// nothing from a row that saw nothing, whatever its scores hold
+__device__ __forceinline__ float prob(float score, float2 z) { return z.y == 0.f ? 0.f : exp_of(score - z.x) * z.y; }
 
 // waves of a workgroup in a call of short sequences: four a SIMD where a wave gets by with 128 registers
 template <int D, int NT>
@@ -261,7 +266,8 @@ __device__ __forceinline__ void store_out(char* out, const float* y) {   // N = 
 template <int D, int NT, int VE>
 struct MergeLds {
   floatx4 acc[4][VE * 4 * 16];
-  float m[16][16 * NT], l[16][16 * NT], sum[16 * NT], lse[16 * NT];
+  float m[16][16 * NT], l[16][16 * NT], sum[16 * NT];
+  float2 stats[16 * NT];
 };
 
 // The keys of a turn into a wave's states: sc holds their scores, v their values.  EXACT: P.V in fp32 throughout.
@@ -486,11 +492,15 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
 #pragma unroll
     for (int w = 0; w < NW; ++w) ll += lds.l[w][row] * exp_of(lds.m[w][row] - m0);
     if (wave == 0 && g4 == 0) {
-      const float lse = ll == 0.f ? -INFINITY : m0 + logf(ll * (1.f / T::P_SCALE));
+      const float l1 = ll * (1.f / T::P_SCALE);
       lds.sum[row] = ll;
-      lds.lse[row] = lse;
-      if (!done) a.part_ml[record * T::ROWS + row] = make_float2(mm, ll);
-      else if (rr < R && a.lse) a.lse[(int64_t)b * a.H + hk * G + rr] = lse;   // done: one query
+      if (ACC) lds.stats[row] = stats_of(m0, l1);
+      if (!done) {
+        a.part_ml[record * T::ROWS + row] = make_float2(mm, ll);
+      } else if (rr < R) {                             // one query
+        if (a.lse) a.lse[(int64_t)b * a.H + hk * G + rr] = ll == 0.f ? -INFINITY : m0 + logf(l1);
+        if (a.stats) a.stats[((int64_t)b * c.Hkv + hk) * a.stat_stride + rr] = stats_of(m0, l1);
+      }
     }
     for (int w = 0; w < NW; w += 4) {                  // four waves' sums at a time
       if (wave / 4 == w / 4) {
@@ -774,10 +784,7 @@ __global__ __launch_bounds__((64 * SMALL_WAVES<D, NT>), (SMALL_WAVES<D, NT> / 4)
     const float* s = a.scores + ((int64_t)b * a.H + hk * R) * a.score_stride;
     for (int j = threadIdx.x; j < len; j += 64 * NW) {
       float sum = 0.f;
-      for (int r = 0; r < R; ++r) {
-        const float z = lds.lse[r];
-        sum += z == -INFINITY ? 0.f : exp_of(s[r * a.score_stride + j] - z);
-      }
+      for (int r = 0; r < R; ++r) sum += prob(s[r * a.score_stride + j], lds.stats[r]);
       const int p = c.page_of(c.table + (int64_t)b * c.t_stride, j);
       if (p >= 0) c.weight[p * c.w_ps + hk * c.w_hs + c.slot_of(j)] += sum;
     }
@@ -868,7 +875,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
   const int64_t row_out = (int64_t)b * a.H + h;
   if (tid < D)
     store_elem<DT>(a.out, row_out * D + tid, l == 0.f ? 0.f : ((o[0][tid] + o[1][tid]) + (o[2][tid] + o[3][tid])) / l);
-  if (tid == 0 && a.lse) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l * (1.f / T::P_SCALE));
+  if (tid == 0) {
+    const float l1 = l * (1.f / T::P_SCALE);
+    if (a.lse) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l1);
+    if (a.stats) a.stats[((int64_t)b * a.c.Hkv + hk) * a.stat_stride + row] = stats_of(m0, l1);
+  }
 }
 
 // Several queries: a wave per row takes its records and then the keys behind the common ones.  The waves of a workgroup
@@ -973,7 +984,12 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
   for (int s = 32; s; s >>= 1) l += __shfl_xor(l, s, 64);
 #pragma unroll
   for (int e = 0; e < W; ++e) store_elem<DT>(a.out, row_out * D + lane * W + e, l == 0.f ? 0.f : y[e] / l);
-  if (lane == 0 && a.lse) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l * (1.f / T::P_SCALE));
+  if (lane == 0) {
+    const float l1 = l * (1.f / T::P_SCALE);
+    if (a.lse) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l1);
+    // the row's own record of the whole kv head, which this wave has read by now
+    if (a.stats) a.stats[((int64_t)b * c.Hkv + hk) * a.stat_stride + row] = stats_of(m0, l1);
+  }
 }
 
 // The weights that a step's rows give the keys of a kv head, from their scores: four keys a lane, 256 a wave.  SHARED: the
@@ -994,6 +1010,7 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
   const int j = j0 + lane * 4;
   const bool all = j0 + 256 <= common(a, b);           // every row sees every key
   const float* s = a.scores + row0 * a.score_stride + j;
+  const float2* stats = a.stats + ((int64_t)b * c.Hkv + hk) * a.stat_stride;
   const int32_t* table = c.table + (int64_t)b * c.t_stride;
   const bool fours = !SHARED && c.shift >= 2 && ((c.w_ps | c.w_hs) & 3) == 0 && ((uintptr_t)c.weight & 15) == 0;
   int page = -1;
@@ -1011,18 +1028,18 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
 #pragma unroll 4
     for (int r = first; r < rows; r += STEP) {
       const floatx4 x = *(const floatx4*)(s + r * a.score_stride);
-      const float z = a.lse[row0 + r];                 // -inf: the row saw nothing, and gives nothing
+      const float2 z = stats[r];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += z == -INFINITY ? 0.f : exp_of(x[e] - z);
+      for (int e = 0; e < 4; ++e) sum[e] += prob(x[e], z);
     }
   } else {
     for (int r = first; r < rows; r += STEP) {
       const int end = len - (a.Q - 1 - r % a.Q);
       if (j >= end) continue;                          // beyond: not written
       const floatx4 x = *(const floatx4*)(s + r * a.score_stride);
-      const float z = a.lse[row0 + r];
+      const float2 z = stats[r];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += j + e >= end || z == -INFINITY ? 0.f : exp_of(x[e] - z);
+      for (int e = 0; e < 4; ++e) sum[e] += j + e >= end ? 0.f : prob(x[e], z);
     }
   }
   if constexpr (SHARED) {
@@ -1055,7 +1072,7 @@ __global__ __launch_bounds__(256) void paged_reform_kernel(PagedArgs a) {
   using T = Tile<DT, D, 1>;
   constexpr int KS = T::KS, SUBS = 4, ROWS = 64, STRIDE = T::RB / 16 + 1;   // 16-byte words, padded
   __shared__ u32x4 rows[ROWS * STRIDE];
-  __shared__ float minus[ROWS];
+  __shared__ float2 stats[ROWS];
   __shared__ int ends[ROWS];
   const CacheView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, g4 = lane >> 4;
@@ -1075,14 +1092,13 @@ __global__ __launch_bounds__(256) void paged_reform_kernel(PagedArgs a) {
 #pragma unroll
     for (int i = 0; i < KS; ++i) k[s][i] = *(global4)(p + i * 64);
   }
-  const float scale = a.sm_scale * LOG2E;
   floatx4 w[SUBS];
 #pragma unroll
   for (int s = 0; s < SUBS; ++s) w[s] = floatx4{0.f, 0.f, 0.f, 0.f};
   // the rows of a turn are fetched during the one before
   constexpr int CH = T::RB / 16, PER = ROWS * CH / 256;
   u32x4 held[PER];
-  float held_z;
+  float2 held_z;
   int held_end;
   auto fetch = [&](int r0) {
 #pragma unroll
@@ -1091,9 +1107,9 @@ __global__ __launch_bounds__(256) void paged_reform_kernel(PagedArgs a) {
       held[x] = *(global4)((int64_t)((const char*)a.q + (b * a.q_bs + (hk * G + g) * a.q_hs + i * a.q_ts) * T::E + tid % CH * 16));
     }
     const int rr = min(r0 + tid % ROWS, R - 1), g = rr / a.Q, i = rr - g * a.Q;
-    held_z = a.lse[((int64_t)b * a.H + hk * G + g) * a.Q + i];
+    held_z = a.stats[((int64_t)b * c.Hkv + hk) * a.stat_stride + rr];
     // a row that saw nothing, or is none, sees no key here
-    held_end = r0 + tid % ROWS < R && held_z != -INFINITY ? len - (a.Q - 1 - i) : 0;
+    held_end = r0 + tid % ROWS < R && held_z.y != 0.f ? len - (a.Q - 1 - i) : 0;
   };
   fetch(0);
   for (int r0 = 0; r0 < R; r0 += ROWS) {
@@ -1102,7 +1118,7 @@ __global__ __launch_bounds__(256) void paged_reform_kernel(PagedArgs a) {
 #pragma unroll
     for (int x = 0; x < PER; ++x) rows[(x * 256 + tid) / CH * STRIDE + tid % CH] = held[x];
     if (tid < ROWS) {
-      minus[tid] = held_z * LOG2E;
+      stats[tid] = held_z;
       ends[tid] = held_end;
     }
     __syncthreads();
@@ -1111,7 +1127,7 @@ __global__ __launch_bounds__(256) void paged_reform_kernel(PagedArgs a) {
       u32x4 q[KS];
 #pragma unroll
       for (int i = 0; i < KS; ++i) q[i] = rows[(t + r) * STRIDE + i * 4 + g4];
-      const float z = minus[t + r];
+      const float2 z = stats[t + r];
       const int end = ends[t + r];
       floatx4 x[SUBS];
 #pragma unroll
@@ -1120,7 +1136,7 @@ __global__ __launch_bounds__(256) void paged_reform_kernel(PagedArgs a) {
 #pragma unroll
         for (int i = 0; i < KS; ++i) x[s] = mfma_qk<DT>(k[s][i], q[i], x[s]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[s][i] = __builtin_amdgcn_exp2f(fmaf(x[s][i], scale, -z));
+        for (int i = 0; i < 4; ++i) x[s][i] = exp_of(x[s][i] * a.sm_scale - z.x) * z.y;
       }
       if (__all(key0 + 16 * SUBS <= end)) {
 #pragma unroll

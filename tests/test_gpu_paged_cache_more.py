@@ -285,3 +285,44 @@ def test_infinite_values_among_many_rows(Q, D, dtype):
             rest = torch.ones(got.shape[:2], dtype=torch.bool, device=DEV)
             rest[1, 8:12] = rest[0, 20:24] = False
             assert torch.equal(got[rest], clean[rest])
+
+
+# ------------------------------------------------------------------------------ large scores and values
+LARGE = [
+    # H, Hkv, Q, D, dtype, width of the table in keys
+    (8, 2, 1, 64, BF16, 512), (8, 2, 1, 128, F32, 512),       # one launch
+    (8, 2, 1, 64, F16, 4096), (8, 2, 1, 128, F32, 4096),      # split
+    (40, 1, 1, 64, BF16, 4096), (96, 1, 1, 64, BF16, 4096),   # several row tiles, from stored scores and formed again
+    (8, 2, 5, 128, BF16, 4096), (8, 2, 5, 64, F32, 4096), (8, 2, 16, 64, F16, 4096), (8, 2, 20, 128, BF16, 4096),
+]
+
+
+@pytest.mark.parametrize("case", range(len(LARGE)))
+def test_weights_at_large_scores(case):
+    """Scores that are whole numbers near 1024, with no rounding in them: a weight is off by what its softmax and its sums
+    round, not by what a logarithm near 1024 would (2^-14 of it)."""
+    import paged_cache as pc
+    H, Hkv, Q, D, dtype, width = LARGE[case]
+    print(f"[case] large scores {LARGE[case]}", flush=True)
+    lens = [50, 37, 51 + Q]
+    made = Made(1600, lens, Hkv, D, 16, dtype, extra_width=width // 16 - 6)
+    c = made.cache
+    c.weight.zero_()
+    small = torch.randint(0, 3, c.k.shape, generator=torch.Generator().manual_seed(1601)).to(dtype).to(DEV)
+    c.k.zero_()
+    c.k[..., 0], c.k[..., 1] = 32.0, small[..., 1]
+    q = torch.zeros((3, H, Q, D), dtype=dtype, device=DEV)
+    q[..., 0] = 32.0
+    q[..., 1] = torch.randint(0, 3, (3, H, Q), generator=torch.Generator().manual_seed(1602)).to(dtype).to(DEV)
+    weight0 = c.weight.clone()
+    pc.paged_attention(q, c, made.table, made.lens, sm_scale=1.0, accumulate=True)
+    _, _, _, _, drawn = _attend_f64(made, q, 1.0)
+    for (b, h), (w, _) in drawn.items():
+        ids = made.table[b, :-(-len(w) // 16)].long()
+        got = c.weight[ids, h].reshape(-1)[:len(w)].double()
+        # The differences of scores, down to -4, are whole.  exp: the argument times log2(e), at most 6, rounds by 6 u and
+        # log2(e) itself by 4 u in the exponent, and the result by a step; n of them are summed, the sum inverted, the two
+        # multiplied and the rows summed; twice the first, for p and its sum, and 16 u for what is left
+        n, rows = len(w), H // Hkv * Q
+        assert torch.all((got - w).abs() <= (2 * 12 + n + 2 * rows + 16) * U * w), f"{((got - w).abs() / w).max().item():.2e}"
+    assert torch.equal(c.weight[made.free], weight0[made.free])
