@@ -1472,16 +1472,19 @@ def _rows(x):
     return x if last == 1 and not bits & 15 else x.clone(memory_format=torch.contiguous_format)
 
 
+_MOST = 2 ** 31 - 1      # the largest number of an int32 field; sizes beyond it count as it
+
+
 def _int32(x):
     """A number for an int32 field, which would keep its low 32 bits: one beyond them stays as far beyond as it can."""
-    return max(-2 ** 31, min(int(x), 2 ** 31 - 1))
+    return max(-2 ** 31, min(int(x), _MOST))
 
 
 def _ints(x, dev):
     """A device int32 tensor with unit stride in its last dim; 64-bit numbers beyond 32 bits as _int32."""
-    if x.dtype == torch.int64:
-        x = x.clamp(-2 ** 31, 2 ** 31 - 1)
     if x.dtype != torch.int32 or x.device != dev:
+        if x.dtype == torch.int64:
+            x = x.clamp(-2 ** 31, _MOST)
         x = x.to(device=dev, dtype=torch.int32)
     return x if x.stride(-1) == 1 else x.contiguous()      # lens of stride 0 (expanded) too
 
@@ -1518,8 +1521,8 @@ class PagedCache:
             c.weight, c.weight_page_stride, c.weight_head_stride = weight.data_ptr(), weight.stride(0), weight.stride(1)
         if pos is not None:
             c.pos, c.pos_page_stride, c.pos_head_stride = pos.data_ptr(), pos.stride(0), pos.stride(1)
-        c.dtype, c.pages, c.page_size = DTYPES[k.dtype], _int32(self.pages), _int32(self.page_size)
-        c.Hkv, c.D = _int32(self.kv_heads), _int32(self.head_dim)
+        c.dtype, c.pages, c.page_size = DTYPES[k.dtype], min(self.pages, _MOST), min(self.page_size, _MOST)
+        c.Hkv, c.D = min(self.kv_heads, _MOST), min(self.head_dim, _MOST)
 
     # the calls use the addresses taken above
     k = property(lambda self: self._k)
@@ -1544,8 +1547,8 @@ class PagedCache:
                  "table must be (B, pages of a sequence) and lens (B,)")
         a.cache = self._c
         c = a.cache
-        c.table, c.table_stride = table.data_ptr(), table.stride(0)
-        c.B, c.table_width = _int32(table.shape[0]), _int32(table.shape[1])
+        c.table, c.table_stride, (B, width) = table.data_ptr(), table.stride(0), table.shape
+        c.B, c.table_width = B if B < _MOST else _MOST, width if width < _MOST else _MOST
         c.lens = lens.data_ptr()
         return table, lens
 
@@ -1567,7 +1570,8 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
         raise ValueError(f"q must be (T, heads, D), not {tuple(q.shape)}")
     q = _rows(q)
     T, H, D = q.shape
-    _require(T < 2 ** 31, f"{T} tokens: a call takes below 2^31")
+    if T > _MOST:                                        # clamped, the others' output would stay unwritten
+        raise ValueError(f"{T} tokens: a call takes below 2^31")
     a = RotaryArgsC()
     q_out = _empty_as(q)
     a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
@@ -1581,7 +1585,7 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
             raise ValueError(f"k must be ({T}, kv heads, {D}), not {tuple(k.shape)}")
         k = _rows(k if k.device == dev else k.to(dev))
         Hkv = k.shape[1]
-        a.Hkv = _int32(Hkv)
+        a.Hkv = Hkv if Hkv < _MOST else _MOST
         k_out = _empty_as(k)
         a.k, a.k_out = k.data_ptr(), k_out.data_ptr()
         a.k_tok_stride, a.k_head_stride, _ = k.stride()
@@ -1604,8 +1608,8 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
         a.pos_axis_stride, a.pos_tok_stride = positions.stride()
     else:
         raise ValueError(f"positions must be ({axes}, {T}), not {tuple(positions.shape)}")
-    a.dtype, a.T, a.H, a.D, a.axes = DTYPES[q.dtype], T, _int32(H), _int32(D), axes
-    a.section[:axes] = [_int32(s) for s in sections]
+    a.dtype, a.T, a.H, a.D, a.axes = DTYPES[q.dtype], T, H if H < _MOST else _MOST, D if D < _MOST else _MOST, axes
+    a.section[:axes] = sections if axes == 1 else [_int32(s) for s in sections]
     a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
     a.pos_scale, a.rope_scale, a.inverse = float(pos_scale), float(rope_scale), int(inverse)
     _launch(lib().sta_rotary, a, dev, "sta_rotary")
@@ -1624,7 +1628,7 @@ def cache_append(cache, k, v, table, lens, starts=None, seen=None):
     a = AppendArgsC()
     keep = cache._fill(a, table, lens)
     B = keep[0].shape[0]
-    a.k, a.v, a.T = k.data_ptr(), v.data_ptr(), _int32(k.shape[0])
+    a.k, a.v, a.T = k.data_ptr(), v.data_ptr(), min(k.shape[0], _MOST)
     a.k_tok_stride, a.k_head_stride, _ = k.stride()
     a.v_tok_stride, a.v_head_stride, _ = v.stride()
     if starts is not None:
@@ -1656,9 +1660,10 @@ def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want
     a = PagedArgsC()
     table, lens = cache._fill(a, table, lens)
     _require(shape[0] == table.shape[0], "q and table must hold the same number of sequences")
-    a.q, a.H, a.Q = q.data_ptr(), _int32(shape[1]), 1
+    H = shape[1]
+    a.q, a.H, a.Q = q.data_ptr(), H if H < _MOST else _MOST, 1
     if len(shape) == 4:
-        a.Q = _int32(shape[2])
+        a.Q = min(shape[2], _MOST)
         a.q_batch_stride, a.q_head_stride, a.q_tok_stride, _ = q.stride()
     else:
         a.q_batch_stride, a.q_head_stride, _ = q.stride()
@@ -1688,7 +1693,7 @@ def cache_evict(cache, table, lens, budget, n_global=32, n_local=32, dst_table=N
     if dst_table is not None:
         dst_table = _ints(dst_table, dev)
         _require(dst_table.dim() == 2 and dst_table.shape[0] == table.shape[0], "dst_table must have a row a sequence")
-        a.dst_table, a.dst_width = dst_table.data_ptr(), _int32(dst_table.shape[1])
+        a.dst_table, a.dst_width = dst_table.data_ptr(), min(dst_table.shape[1], _MOST)
         a.dst_stride = dst_table.stride(0)
     new_lens = torch.empty_like(lens)
     a.new_lens = new_lens.data_ptr()

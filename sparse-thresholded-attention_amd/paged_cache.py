@@ -30,11 +30,6 @@ import _sta_native as native
 from _sta_native import PagedCache  # noqa: F401
 
 
-def _tangents():
-    """Whether a forward-mode level is open, in which a tensor may carry a tangent."""
-    return forward_ad._current_level >= 0
-
-
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(q, k, positions, inv_freq, sections, pos_scale, rope_scale, inverse):
@@ -67,7 +62,8 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
     scaled by rope_scale; elements from R on are copied.  sections: how many frequencies each axis
     owns, in order (default: all of them one axis).  D a multiple of 8 up to 512, R / 2 a multiple of
     8, T below 2^31.  Gradients and forward-mode tangents flow to and from q and k, not positions or frequencies."""
-    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad) or _tangents():
+    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad) \
+            or forward_ad._current_level >= 0:               # a level in which a tensor may carry a tangent
         return _Rotary.apply(q, k, positions, inv_freq, sections, pos_scale, rope_scale, False)
     return native.rotary(q, k, positions, inv_freq, sections, pos_scale, rope_scale)
 
@@ -75,7 +71,7 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
 def rotary_grad(dq, dk, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1.0):
     """The gradients of rotary's inputs from those of its outputs, without an autograd graph: the
     rotation the other way round, with the same scale.  Inputs with forward-mode tangents are refused."""
-    if _tangents() and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in (dq, dk)):
+    if forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in (dq, dk)):
         raise RuntimeError("rotary_grad keeps no graph and no forward-mode tangents: differentiate rotary")
     return native.rotary(dq, dk, positions, inv_freq, sections, pos_scale, rope_scale, inverse=True)
 
