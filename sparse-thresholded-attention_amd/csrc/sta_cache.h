@@ -57,7 +57,7 @@ struct PagedArgs {
   int64_t stat_stride;
   float* scores;                    // (B, H, Q, score_stride); NULL: not stored
   int64_t score_stride;
-  float* part_o;                    // (records, rows, D) unnormalised outputs of unfinished row tiles
+  float* part_o;                    // (records, rows, D) sums of unfinished row tiles, scaled by sum_scale
   float2* part_ml;                  // (records, rows) their maxima and sums
   int runs;
 };

@@ -102,8 +102,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 //                   operand B, and lane l loads 1/16 of the V rows of those keys, whose elements e are operand
 //                   A of the dims (l % 16) * VE + e
 //
-// so neither P nor V moves between lanes.  P goes in two 16-bit parts, P = hi + lo within 2^-17 of itself, two
-// instructions for each; fp32 caches use the fp32 instruction of depth 4, whose operands P and V are as well.
+// so neither P nor V moves between lanes.  P goes in two 16-bit parts, P = hi + lo within 2^-17 of itself (fp16: down to
+// 2^-22), two instructions for each: beside the 2^-8 or 2^-11 of the output's own rounding, which it does not move.  Its
+// sum is of the whole P.  fp32 caches use the fp32 instruction of depth 4, whose operands P and V are as well.
 //
 // Work.  The sequences' lengths are known to the device alone, and differ.  Every wave sums their units (of
 // 4 KT keys; an empty sequence counts one, which writes its zeros) over the kv heads, and the call's runs, as many
@@ -168,8 +169,6 @@ __device__ __forceinline__ float at_least(float m) { return m == -INFINITY ? 0.f
 // What the weights' probabilities are formed from, as exp(score - x) y: a maximum (at_least) and a sum.  Not exp(score -
 // lse): near a log-sum-exp of 1000 its rounding alone is 3e-5 of every weight.
 __device__ __forceinline__ float2 stats_of(float m, float l) { return make_float2(m, l == 0.f ? 0.f : 1.f / l); }
-// nothing from a row that saw nothing, whatever its scores hold
-__device__ __forceinline__ float prob(float score, float2 z) { return z.y == 0.f ? 0.f : exp_of(score - z.x) * z.y; }
 
 // waves of a workgroup in a call of short sequences: four a SIMD where a wave gets by with 128 registers
 template <int D, int NT>
@@ -190,7 +189,8 @@ struct Tile {
   static constexpr int VE = D / 16;                    // V elements of a lane
   static constexpr int VW = VE * E / 4;                // their words
   static constexpr int NT = NT_, ROWS = 16 * NT;
-  // P is below 1: times 2^14 its fp16 halves stay clear of the subnormal range down to 2^-28
+  // P is at most 1: times 2^14 its high fp16 half is normal down to 2^-28, and both hold it within 2^-17 of itself down to
+  // 2^-22, within 2^-39 below
   static constexpr float P_SCALE = DT == DT_F16 ? 16384.f : 1.f;
   // Waves of a SIMD, and so workgroups of a CU (256 a grid and wave): what the registers hold without spills.
   // Three at D = 64 (bf16, 32q / 8kv heads, up to 8192 keys: 37 us, with two 41), two at D = 128 (two sequences of up
@@ -270,9 +270,11 @@ struct MergeLds {
   float2 stats[16 * NT];
 };
 
-// The keys of a turn into a wave's states: sc holds their scores, v their values.  EXACT: P.V in fp32 throughout.
+// The keys of a turn into a wave's states: sc holds their scores, v their values; P is scaled by p_scale.  EXACT: P.V in
+// fp32 throughout.
 template <int DT, int D, int NT, bool EXACT, typename Scores, typename Values, typename State, typename Acc>
-__device__ __forceinline__ void attend_keys(Scores& sc, Values& v, State& m, State& l, Acc& acc) {
+__device__ __forceinline__ void attend_keys(Scores& sc, Values& v, State& m, State& l, Acc& acc,
+                                            float p_scale) {
   using T = Tile<DT, D, NT>;
   constexpr int SUB = T::SUB, VE = T::VE;
 #pragma unroll
@@ -293,7 +295,7 @@ __device__ __forceinline__ void attend_keys(Scores& sc, Values& v, State& m, Sta
     for (int s = 0; s < SUB; ++s)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = T::P_SCALE * exp_of(sc[t][s][i] - m0);
+        const float p = p_scale * exp_of(sc[t][s][i] - m0);
         sc[t][s][i] = p;
         l[t] += p;
       }
@@ -334,6 +336,28 @@ __device__ __forceinline__ void attend_keys(Scores& sc, Values& v, State& m, Sta
       }
     }
   }
+}
+
+// The sums of a kv head's waves and runs are added scaled by this, a power of two at most 1 over the number of its keys
+// (those that all queries see and the last Q - 1): no sum of theirs exceeds the largest value.
+__device__ __forceinline__ float sum_scale(const PagedArgs& a, int common) {
+  return __uint_as_float((uint32_t)(127 - (32 - __clz(common + a.Q - 1))) << 23);
+}
+
+// Whether a sum is no finite number: one of large values may have passed the type's largest, and an infinite value times
+// a part of P that is 0 or below 0 is NaN where the formula says infinity.  Then the keys are taken again, P whole and scaled
+// so that no sum of up to 2^28 values exceeds the largest of them.
+constexpr float AGAIN_SCALE = 0x1p-28f;
+template <int NT, int VE, typename Acc>
+__device__ __forceinline__ bool beyond(const Acc& acc) {
+  floatx4 zero = floatx4{0.f, 0.f, 0.f, 0.f};            // an infinity or a NaN times 0 is NaN
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) zero[i] = fmaf(acc[t][e][i], 0.f, zero[i]);
+  return (zero[0] + zero[1]) + (zero[2] + zero[3]) != 0.f;
 }
 
 // A workgroup of NW waves takes the units u0 .. u1 - 1 of a row tile: out and lse where that is all of it
@@ -395,7 +419,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
   };
   int next_entry;
   uint32_t there;
-  auto turn = [&](int u, auto last_turn, auto exact) {
+  auto turn = [&](int u, auto last_turn, auto exact, float p_scale) {
     constexpr bool LAST = decltype(last_turn)::value, EXACT = decltype(exact)::value;
     uint32_t v[SUB][4][VW];
 #pragma unroll
@@ -437,9 +461,9 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
       load_k();
       next_entry = entry_at(u + 2);
     }
-    attend_keys<DT, D, NT, EXACT>(sc, v, m, l, acc);
+    attend_keys<DT, D, NT, EXACT>(sc, v, m, l, acc, p_scale);
   };
-  auto sweep = [&](auto exact) {
+  auto sweep = [&](auto exact, float p_scale) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t] = -INFINITY;
@@ -451,30 +475,23 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
     next_entry = entry_at(u0 + 1);
     load_k();
     int u = u0;
-    while (u + 1 < u1) turn(u++, std::integral_constant<bool, false>(), exact);
-    turn(u, std::integral_constant<bool, true>(), exact);
+    while (u + 1 < u1) turn(u++, std::integral_constant<bool, false>(), exact, p_scale);
+    turn(u, std::integral_constant<bool, true>(), exact, p_scale);
   };
-  if constexpr (DT == DT_F32) {
-    sweep(std::integral_constant<bool, true>());
-  } else {
-    sweep(std::integral_constant<bool, false>());
-    // an infinite value times a part of P that is 0 or below 0 is NaN where the formula says infinity: then once
-    // more with P whole
-    bool nan = false;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < VE; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) nan |= acc[t][e][i] != acc[t][e][i];
-    if (__any(nan)) sweep(std::integral_constant<bool, true>());
+  float unit = 1.f / T::P_SCALE;                       // of the sums
+  sweep(std::integral_constant<bool, DT == DT_F32>(), T::P_SCALE);
+  if (__builtin_expect(__any(beyond<NT, VE>(acc)), 0)) {
+    sweep(std::integral_constant<bool, true>(), AGAIN_SCALE);
+    unit = 1.f / AGAIN_SCALE;
   }
 
   // the waves' states into one
+  const float small = sum_scale(a, len);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     l[t] += __shfl_xor(l[t], 16, 64);
     l[t] += __shfl_xor(l[t], 32, 64);
+    l[t] *= unit;
     if (g4 == 0) {
       lds.m[wave][t * 16 + r] = m[t];
       lds.l[wave][t * 16 + r] = l[t];
@@ -491,15 +508,15 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
     float ll = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) ll += lds.l[w][row] * exp_of(lds.m[w][row] - m0);
+    const float scale = f * (unit * small);
     if (wave == 0 && g4 == 0) {
-      const float l1 = ll * (1.f / T::P_SCALE);
-      lds.sum[row] = ll;
-      if (ACC) lds.stats[row] = stats_of(m0, l1);
+      lds.sum[row] = ll * small;
+      if (ACC) lds.stats[row] = stats_of(m0, ll);
       if (!done) {
         a.part_ml[record * T::ROWS + row] = make_float2(mm, ll);
       } else if (rr < R) {                             // one query
-        if (a.lse) a.lse[(int64_t)b * a.H + hk * G + rr] = ll == 0.f ? -INFINITY : m0 + logf(l1);
-        if (a.stats) a.stats[((int64_t)b * c.Hkv + hk) * a.stat_stride + rr] = stats_of(m0, l1);
+        if (a.lse) a.lse[(int64_t)b * a.H + hk * G + rr] = ll == 0.f ? -INFINITY : m0 + logf(ll);
+        if (a.stats) a.stats[((int64_t)b * c.Hkv + hk) * a.stat_stride + rr] = stats_of(m0, ll);
       }
     }
     for (int w = 0; w < NW; w += 4) {                  // four waves' sums at a time
@@ -507,7 +524,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           floatx4& at = lds.acc[wave % 4][(e * 4 + g4) * 16 + r];
-          at = w == 0 ? acc[t][e] * f : at + acc[t][e] * f;
+          at = w == 0 ? acc[t][e] * scale : at + acc[t][e] * scale;
         }
       }
       __syncthreads();
@@ -652,7 +669,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
     };
     floatx4 acc[NT][VE];
     float m[NT], l[NT];
-    auto sweep = [&](auto exact) {
+    auto sweep = [&](auto exact, float p_scale) {
       constexpr bool EXACT = decltype(exact)::value;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -716,7 +733,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
               for (int i = 0; i < 4; ++i)
                 if (!(there >> (g4 * 4) & 1u << (s * 16 + i))) sc[y][s][i] = -INFINITY;
         }
-        attend_keys<DT, D, NT, EXACT>(sc, v, m, l, acc);
+        attend_keys<DT, D, NT, EXACT>(sc, v, m, l, acc, p_scale);
         there = next;
         next = after;
         buf = buf == 2 ? 0 : buf + 1;
@@ -724,24 +741,21 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
     };
     if (tid == 0) again = 0;
     __syncthreads();
-    sweep(std::integral_constant<bool, false>());
-    bool nan = false;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < VE; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) nan |= acc[t][e][i] != acc[t][e][i];
-    if (nan) again = 1;
+    sweep(std::integral_constant<bool, false>(), T::P_SCALE);
+    if (beyond<NT, VE>(acc)) again = 1;
     __syncthreads();
+    float unit = 1.f / T::P_SCALE;                     // of the sums
     if (again) {
-      sweep(std::integral_constant<bool, true>());
+      unit = 1.f / AGAIN_SCALE;
+      sweep(std::integral_constant<bool, true>(), AGAIN_SCALE);
       __syncthreads();                                 // staged is free
     }
+    const float scale = unit * sum_scale(a, len);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       l[t] += __shfl_xor(l[t], 16, 64);
       l[t] += __shfl_xor(l[t], 32, 64);
+      l[t] *= unit;
       const int64_t row = record * ROWS + wave * 32 + t * 16;
       if (g4 == 0) a.part_ml[row + r] = make_float2(m[t], l[t]);
       // rows whole, through LDS
@@ -749,7 +763,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
 #pragma unroll
       for (int e = 0; e < VE; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine[r * (D + 4) + (g4 * 4 + i) * VE + e] = acc[t][e][i];
+        for (int i = 0; i < 4; ++i) mine[r * (D + 4) + (g4 * 4 + i) * VE + e] = acc[t][e][i] * scale;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -784,7 +798,10 @@ __global__ __launch_bounds__((64 * SMALL_WAVES<D, NT>), (SMALL_WAVES<D, NT> / 4)
     const float* s = a.scores + ((int64_t)b * a.H + hk * R) * a.score_stride;
     for (int j = threadIdx.x; j < len; j += 64 * NW) {
       float sum = 0.f;
-      for (int r = 0; r < R; ++r) sum += prob(s[r * a.score_stride + j], lds.stats[r]);
+      for (int r = 0; r < R; ++r) {
+        const float2 z = lds.stats[r];
+        sum = fmaf(exp_of(s[r * a.score_stride + j] - z.x), z.y, sum);
+      }
       const int p = c.page_of(c.table + (int64_t)b * c.t_stride, j);
       if (p >= 0) c.weight[p * c.w_ps + hk * c.w_hs + c.slot_of(j)] += sum;
     }
@@ -874,11 +891,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
   __syncthreads();
   const int64_t row_out = (int64_t)b * a.H + h;
   if (tid < D)
-    store_elem<DT>(a.out, row_out * D + tid, l == 0.f ? 0.f : ((o[0][tid] + o[1][tid]) + (o[2][tid] + o[3][tid])) / l);
+    store_elem<DT>(a.out, row_out * D + tid, l == 0.f ? 0.f : ((o[0][tid] + o[1][tid]) + (o[2][tid] + o[3][tid])) / (l * sum_scale(a, common(a, b))));
   if (tid == 0) {
-    const float l1 = l * (1.f / T::P_SCALE);
-    if (a.lse) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l1);
-    if (a.stats) a.stats[((int64_t)b * a.c.Hkv + hk) * a.stat_stride + row] = stats_of(m0, l1);
+    if (a.lse) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l);
+    if (a.stats) a.stats[((int64_t)b * a.c.Hkv + hk) * a.stat_stride + row] = stats_of(m0, l);
   }
 }
 
@@ -905,6 +921,8 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
     const float2 s = ml[record(p)];
     l += s.y * exp_of(s.x - m0);
   }
+  const int n0 = common(a, b), end = c.len(b) - (a.Q - 1 - i);
+  const float p_scale = sum_scale(a, n0);
   float y[W];
 #pragma unroll
   for (int e = 0; e < W; ++e) y[e] = 0.f;
@@ -916,8 +934,8 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
 #pragma unroll
     for (int e = 0; e < W; ++e) y[e] += f * part[at * D + e];
   }
+  l *= p_scale;
   const int64_t row_out = ((int64_t)b * a.H + h) * a.Q + i;
-  const int n0 = common(a, b), end = c.len(b) - (a.Q - 1 - i);
   const int32_t* table = c.table + (int64_t)b * c.t_stride;
   uint32_t q[VW];
   load_words<VW>((int64_t)((const char*)a.q + (b * a.q_bs + h * a.q_hs + i * a.q_ts) * T::E + l16 * (VW * 4)), q);
@@ -954,7 +972,7 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
     if (a.scores && key < keys) a.scores[row_out * a.score_stride + j0 + key] = mine;
     const float m1 = fmaxf(wave_max_f32(mine), m);
     m0 = at_least(m1);
-    const float f = exp_of(m - m0), p = T::P_SCALE * exp_of(mine - m0);
+    const float f = exp_of(m - m0), p = p_scale * exp_of(mine - m0);
     m = m1;
     l = l * f + p;
 #pragma unroll
@@ -985,7 +1003,7 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
 #pragma unroll
   for (int e = 0; e < W; ++e) store_elem<DT>(a.out, row_out * D + lane * W + e, l == 0.f ? 0.f : y[e] / l);
   if (lane == 0) {
-    const float l1 = l * (1.f / T::P_SCALE);
+    const float l1 = l * (1.f / p_scale);
     if (a.lse) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l1);
     // the row's own record of the whole kv head, which this wave has read by now
     if (a.stats) a.stats[((int64_t)b * c.Hkv + hk) * a.stat_stride + row] = stats_of(m0, l1);
@@ -1030,7 +1048,7 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
       const floatx4 x = *(const floatx4*)(s + r * a.score_stride);
       const float2 z = stats[r];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += prob(x[e], z);
+      for (int e = 0; e < 4; ++e) sum[e] = fmaf(exp_of(x[e] - z.x), z.y, sum[e]);
     }
   } else {
     for (int r = first; r < rows; r += STEP) {
@@ -1039,7 +1057,7 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
       const floatx4 x = *(const floatx4*)(s + r * a.score_stride);
       const float2 z = stats[r];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += j + e >= end ? 0.f : prob(x[e], z);
+      for (int e = 0; e < 4; ++e) sum[e] += j + e >= end ? 0.f : exp_of(x[e] - z.x) * z.y;
     }
   }
   if constexpr (SHARED) {

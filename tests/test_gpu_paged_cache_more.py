@@ -326,3 +326,34 @@ def test_weights_at_large_scores(case):
         n, rows = len(w), H // Hkv * Q
         assert torch.all((got - w).abs() <= (2 * 12 + n + 2 * rows + 16) * U * w), f"{((got - w).abs() / w).max().item():.2e}"
     assert torch.equal(c.weight[made.free], weight0[made.free])
+
+
+@pytest.mark.parametrize("D,dtype,H,Hkv", [(64, F32, 8, 2), (128, F32, 8, 2), (64, BF16, 8, 2), (128, BF16, 8, 2),
+                                           (64, BF16, 40, 1), (128, BF16, 160, 2)])
+@pytest.mark.parametrize("Q", [1, 5, 20])
+@pytest.mark.parametrize("lens", [[900, 2, 40], [6000, 31, 700]])
+def test_attention_of_values_near_the_largest(D, dtype, H, Hkv, Q, lens):
+    """A mean of values near the type's largest is finite, however many keys it is of: no sum exceeds it."""
+    import paged_cache as pc
+    print(f"[case] large values {D} {dtype} {H}/{Hkv} Q={Q} {lens}", flush=True)
+    made = Made(1700, lens, Hkv, D, 16, dtype)
+    v = made.cache.v
+    v[..., 3], v[..., 5] = 3.0e38, -3.0e38
+    v[..., 7] = torch.where(v[..., 7].float() > 0, 3.0e38, -3.0e38).to(dtype)
+    q = _randn(1701, (len(lens), H, Q, D), dtype)
+    got, lse = pc.paged_attention(q, made.cache, made.table, made.lens, want_lse=True)
+    assert torch.isfinite(got).all()
+    _check_attend_f64(made, q, got, lse)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Q", [1, 5, 20])
+def test_attention_of_small_values(dtype, Q):
+    """Values far below 1 keep their precision beside large ones of other dims."""
+    import paged_cache as pc
+    for lens in ([900, 40], [5000, 200]):
+        made = Made(1800, lens, 2, 64, 16, dtype)
+        made.cache.v[..., :32] *= 1e-30
+        q = _randn(1801, (2, 8, Q, 64), dtype)
+        got, lse = pc.paged_attention(q, made.cache, made.table, made.lens, want_lse=True)
+        _check_attend_f64(made, q, got, lse)
