@@ -79,8 +79,9 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int hk, int b, con
 // INLINE: the few rows that can move are moved here.
 template <bool KEPT, bool INLINE>
 __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictArgs a) {
-  extern __shared__ uint32_t words[];
-  __shared__ int hist[BINS * COPIES], scan[SEL_T / 64], pick[3];
+  extern __shared__ __align__(16) uint32_t words[];
+  __shared__ __align__(16) int hist[BINS * COPIES];
+  __shared__ int scan[SEL_T / 64], pick[3];
   const CacheView& c = a.c;
   const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   __shared__ int moved[2][INLINE ? INLINE_MOVES : 1];

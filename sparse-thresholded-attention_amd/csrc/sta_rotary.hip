@@ -57,7 +57,7 @@ __device__ __forceinline__ double position(const sta_rotary_args& a, int axis, i
 template <int DT>
 __global__ __launch_bounds__(256) void rotary_kernel(sta_rotary_args a, int half) {
   constexpr int V = ROT_V<DT>;
-  extern __shared__ float2 trig[];                 // [half]
+  extern __shared__ __align__(16) float2 trig[];   // [half]
   const int64_t t = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
   if (t >= a.T) return;
   for (int f = threadIdx.x; f < half; f += 256) {
