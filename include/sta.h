@@ -647,7 +647,8 @@ int sta_paged_attention(const sta_paged_args* args, void* stream);
  * pos < n_global or pos > (the head's largest pos) - n_local, then the others by weight, the
  * largest first (NaN before all), equal ones by slot, the lower first.
  * dst_table NULL: the kept keys in slots >= budget move, with weight and pos, into the dropped ones'
- * slots < budget, both in ascending order; the others stay.  Nothing moves where lens[b] <= budget.
+ * slots < budget, both in ascending order; the others stay.  A key that moves to a slot without a
+ * page is lost.  Nothing moves where lens[b] <= budget.
  * dst_table: the kept keys are copied in ascending order of their slots to the slots 0, 1, ... of
  * the pages of dst_table, none of which the tables of this call may hold otherwise; the source stays.
  * new_lens[b], not the lens array itself, receives min(lens[b], budget). */

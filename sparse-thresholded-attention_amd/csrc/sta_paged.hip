@@ -273,8 +273,7 @@ struct MergeLds {
 // The keys of a turn into a wave's states: sc holds their scores, v their values; P is scaled by p_scale.  EXACT: P.V in
 // fp32 throughout.
 template <int DT, int D, int NT, bool EXACT, typename Scores, typename Values, typename State, typename Acc>
-__device__ __forceinline__ void attend_keys(Scores& sc, Values& v, State& m, State& l, Acc& acc,
-                                            float p_scale) {
+__device__ __forceinline__ void attend_keys(Scores& sc, Values& v, State& m, State& l, Acc& acc, float p_scale) {
   using T = Tile<DT, D, NT>;
   constexpr int SUB = T::SUB, VE = T::VE;
 #pragma unroll
@@ -345,8 +344,8 @@ __device__ __forceinline__ float sum_scale(const PagedArgs& a, int common) {
 }
 
 // Whether a sum is no finite number: one of large values may have passed the type's largest, and an infinite value times
-// a part of P that is 0 or below 0 is NaN where the formula says infinity.  Then the keys are taken again, P whole and scaled
-// so that no sum of up to 2^28 values exceeds the largest of them.
+// a part of P that is 0 or below 0 is NaN where the formula says infinity.  Then the keys are taken again, P whole and
+// scaled so that no sum of up to 2^28 values exceeds the largest of them.
 constexpr float AGAIN_SCALE = 0x1p-28f;
 template <int NT, int VE, typename Acc>
 __device__ __forceinline__ bool beyond(const Acc& acc) {
@@ -890,8 +889,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
   for (int e = 0; e < W; ++e) o[wave][lane * W + e] = y[e];
   __syncthreads();
   const int64_t row_out = (int64_t)b * a.H + h;
-  if (tid < D)
-    store_elem<DT>(a.out, row_out * D + tid, l == 0.f ? 0.f : ((o[0][tid] + o[1][tid]) + (o[2][tid] + o[3][tid])) / (l * sum_scale(a, common(a, b))));
+  if (tid < D) {
+    const float sum = (o[0][tid] + o[1][tid]) + (o[2][tid] + o[3][tid]);
+    store_elem<DT>(a.out, row_out * D + tid, l == 0.f ? 0.f : sum / (l * sum_scale(a, common(a, b))));
+  }
   if (tid == 0) {
     if (a.lse) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l);
     if (a.stats) a.stats[((int64_t)b * a.c.Hkv + hk) * a.stat_stride + row] = stats_of(m0, l);

@@ -20,8 +20,8 @@ A decoding step of a batch, held at `budget` keys a head:
 All of them launch on the current stream of the tensors' device, allocate their results and their
 workspace from torch's allocator, and neither synchronise nor keep anything between calls, so a HIP
 graph can capture them (a captured training step calls rotary_grad itself).  rotary alone takes part
-in autograd.  There is no fallback: a CPU tensor, an unsupported shape or a missing
-library raises.
+in automatic differentiation, in both modes; the others keep neither gradients nor tangents.  There is
+no fallback: a CPU tensor, an unsupported shape or a missing library raises.
 """
 import torch
 from torch.autograd import forward_ad
@@ -58,10 +58,11 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
     their dtype.
 
     positions (T,) or (axes, T): int32, int64 or float32.  inv_freq (R / 2,): pair (i, R / 2 + i) of a
-    row turns by positions[axis of i] * pos_scale * inv_freq[i], the angle formed in 64 bits, and is
-    scaled by rope_scale; elements from R on are copied.  sections: how many frequencies each axis
-    owns, in order (default: all of them one axis).  D a multiple of 8 up to 512, R / 2 a multiple of
-    8, T below 2^31.  Gradients and forward-mode tangents flow to and from q and k, not positions or frequencies."""
+    row turns by positions[axis of i] * pos_scale * inv_freq[i], the angle formed in 64 bits from the
+    scale and the frequency in 32, and is scaled by rope_scale; elements from R on are copied.
+    sections: how many frequencies each axis owns, in order (default: all of them one axis).  D a
+    multiple of 8 up to 512, R / 2 a multiple of 8, T below 2^31.  Gradients and forward-mode tangents
+    pass through q and k, not through positions or frequencies."""
     if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad) \
             or forward_ad._current_level >= 0:               # a level in which a tensor may carry a tangent
         return _Rotary.apply(q, k, positions, inv_freq, sections, pos_scale, rope_scale, False)
@@ -71,7 +72,8 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
 def rotary_grad(dq, dk, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1.0):
     """The gradients of rotary's inputs from those of its outputs, without an autograd graph: the
     rotation the other way round, with the same scale.  Inputs with forward-mode tangents are refused."""
-    if forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in (dq, dk)):
+    if forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None
+                                              for x in (dq, dk)):
         raise RuntimeError("rotary_grad keeps no graph and no forward-mode tangents: differentiate rotary")
     return native.rotary(dq, dk, positions, inv_freq, sections, pos_scale, rope_scale, inverse=True)
 
@@ -80,7 +82,8 @@ def cache_append(cache, k, v, table, lens, starts=None, seen=None):
     """Write new keys and values k, v (T, Hkv, D) behind the sequences' cached ones; returns the new
     lengths (B,) int32 (lens itself is not changed).
 
-    table (B, pages of a sequence) int32, -1 where there is no page; lens (B,) int32.  Without starts
+    table (B, pages of a sequence) int32, -1 where there is no page; lens (B,) int32 (64-bit numbers of
+    either are clamped to 32).  Without starts
     every sequence gets one row (T = B); with starts (B + 1,) int32 the rows starts[b] ..
     starts[b + 1] - 1 are sequence b's, as far as k has them, and rows outside all of them are not
     read.  seen (B,): how many tokens the sequence has had before these, the first new key's cache.pos
@@ -95,9 +98,10 @@ def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want
     A query that sees no key gets zeros and -inf.
 
     accumulate: add every key's probability, summed over the queries and the heads of its kv head, to
-    cache.weight; a page of such a call stands in one place of one sequence's table.  max_len: a bound on lens known
-    to the host (default: the table's); it sizes the workspace, 4 bytes a query row and key with
-    accumulate, and lengths past it count as max_len."""
+    cache.weight; a page of such a call stands in one place of one sequence's table.  max_len: a bound
+    on lens known to the host (default: the table's); lengths past it count as max_len.  It sizes the
+    workspace of accumulate, 4 bytes a query row and key for fp32 and below 64 rows (queries times heads
+    of a kv head).  Meant for a few new tokens: the last Q - 1 keys are taken row by row."""
     return native.paged_attention(q, cache, table, lens, sm_scale, accumulate, want_lse, max_len)
 
 
@@ -108,7 +112,8 @@ def cache_evict(cache, table, lens, budget, n_global=32, n_local=32, dst_table=N
 
     In place (dst_table None) the kept keys in slots from budget on move into the dropped ones' slots, so
     that the keys of a sequence are no longer in the order of their tokens; cache.pos says which they
-    are; a page stands in one place of one sequence's table.  With dst_table (B, pages) the kept keys
+    are; a page stands in one place of one sequence's table, and a kept key whose new slot has no page is
+    lost.  With dst_table (B, pages) the kept keys
     are copied, in order, to that table's pages, others than the source's, which may be shared and stay
     as they are.  Keys without a page rank last; one that is kept all the same leaves its slot of
     dst_table unwritten."""

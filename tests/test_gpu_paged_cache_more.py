@@ -357,3 +357,58 @@ def test_attention_of_small_values(dtype, Q):
         q = _randn(1801, (2, 8, Q, 64), dtype)
         got, lse = pc.paged_attention(q, made.cache, made.table, made.lens, want_lse=True)
         _check_attend_f64(made, q, got, lse)
+
+
+@pytest.mark.parametrize("case", [0, 2, 5, 7, 8, 9])
+def test_large_values_in_runs_of_several_heads(case):
+    """Some heads of a run repeat their keys for their large values, the others do not."""
+    import paged_cache as pc
+    B, (low, high), H, Hkv, Q, D, ps, dtype = RUNS[case]
+    lens = _ragged(case, B, low, high)
+    print(f"[case] large values in runs {RUNS[case]}", flush=True)
+    made = Made(1900 + case, lens, Hkv, D, ps, dtype)
+    made.cache.weight.zero_()
+    for b in range(0, B, 3):
+        for p in made.rows[b]:
+            if p >= 0:
+                made.cache.v[p, b % Hkv, :, 1:9] = 3.0e38 if b % 2 else -3.0e38
+    q = _randn(1901 + case, (B, H, Q, D), dtype, 1.5)
+    weight0 = made.cache.weight.clone()
+    got, lse = pc.paged_attention(q, made.cache, made.table, made.lens, accumulate=True, want_lse=True)
+    assert torch.isfinite(got).all()
+    _check_attend_f64(made, q, got, lse, made.cache.weight, weight0)
+
+
+@pytest.mark.parametrize("H,Hkv,Q,D,dtype", [(16, 8, 1, 64, BF16), (512, 8, 1, 64, F16), (8, 8, 1, 128, F32), (16, 8, 3, 128, BF16),
+                                             (32, 8, 16, 64, F16), (32, 8, 20, 128, BF16)])
+def test_split_calls_with_weights_in_two_graphs(H, Hkv, Q, D, dtype):
+    """Two captured calls, replayed in turn with eager work between them, give the eager call's bits each time."""
+    import paged_cache as pc
+    print(f"[case] graphs {H}/{Hkv} Q={Q} D={D} {dtype}", flush=True)
+    made = [Made(2000 + i, lens, Hkv, D, 16, dtype) for i, lens in enumerate(([3000, 17, 0, 1900], [1200, 2600, 5, 64]))]
+    q = [_randn(2010 + i, (4, H, Q, D), dtype) for i in range(2)]
+    start = [m.cache.weight.clone() for m in made]
+
+    def call(i):
+        return pc.paged_attention(q[i], made[i].cache, made[i].table, made[i].lens, accumulate=True, want_lse=True)
+    want = []
+    for i in range(2):
+        out, lse = call(i)
+        want.append((out, lse, made[i].cache.weight.clone()))
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(i))
+        graphs.append(g)
+    for turn in range(3):
+        for i in (turn % 2, 1 - turn % 2):
+            made[i].cache.weight.copy_(start[i])
+            for x in outs[i]:
+                x.fill_(7.0)
+            pc.paged_attention(q[1 - i], made[1 - i].cache, made[1 - i].table, made[1 - i].lens)    # eager work
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            for x, w in zip((*outs[i], made[i].cache.weight), want[i]):
+                assert torch.equal(x, w), f"replay {turn} of graph {i}"

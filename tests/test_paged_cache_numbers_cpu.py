@@ -139,3 +139,22 @@ def test_eviction_numbers_its_heads_in_32_bits(B, Hkv, ok):
     a.budget, a.max_len = 1, 1
     assert (native.lib().sta_evict_workspace_size(ctypes.byref(a)) > 0) == ok
     assert ok or native.lib().sta_cache_evict(ctypes.byref(a), None) == -1
+
+
+def test_workspace_of_stored_and_reformed_weights():
+    """Scores are stored for fp32 and below 64 rows a kv head; from 64 on, 16-bit weights are formed again without them."""
+    import _sta_native as native
+
+    def size(H, Q, dtype, accumulate):
+        a = native.PagedArgsC()
+        c = a.cache
+        c.dtype, c.pages, c.page_size, c.Hkv, c.D = native.DTYPES[dtype], 64, 16, 8, 64
+        c.table_stride, c.table_width, c.B = 512, 512, 4
+        a.H, a.Q, a.sm_scale, a.max_len, a.accumulate = H, Q, 0.1, 8192, accumulate
+        return native.lib().sta_paged_workspace_size(ctypes.byref(a))
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        for H, Q in ((56, 9), (32, 16), (512, 1), (504, 1)):  # 63, 64, 64 and 63 rows a kv head
+            more = size(H, Q, dtype, 1) - size(H, Q, dtype, 0)
+            stats = 4 * H * 8 if Q == 1 else 0                # a maximum and a sum a row; several queries have room for them
+            scores = 4 * H * Q * 8192 * 4 if dtype == torch.float32 or H // 8 * Q < 64 else 0
+            assert stats + scores <= more < stats + scores + 512
