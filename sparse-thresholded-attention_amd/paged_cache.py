@@ -99,7 +99,7 @@ def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want
 
     accumulate: add every key's probability, summed over the queries and the heads of its kv head, to
     cache.weight; a page of such a call stands in one place of one sequence's table.  max_len: a bound
-    on lens known to the host (default: the table's); lengths past it count as max_len.  It sizes the
+    on lens known to the host, at least 1 (default: the table's); lengths past it count as max_len.  It sizes the
     workspace of accumulate, 4 bytes a query row and key for fp32 and below 64 rows (queries times heads
     of a kv head).  Meant for a few new tokens: the last Q - 1 keys are taken row by row."""
     return native.paged_attention(q, cache, table, lens, sm_scale, accumulate, want_lse, max_len)
