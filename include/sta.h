@@ -601,6 +601,77 @@ typedef struct sta_rotary_args {
 
 int sta_rotary(const sta_rotary_args* args, void* stream);
 
+/* Each head's row divided by its root mean square, times a weight of D elements shared by the heads, and
+ * rotated: y = R(x / sqrt(mean(x^2) + eps) * w), R as sta_rotary's with inverse = 0.  In 32 bits (angles in
+ * 64), rounded once.  Outputs may be the inputs. */
+typedef struct sta_norm_rotary_args {
+  sta_rotary_args rot;     /* tensors, positions and frequencies; inverse must be 0 */
+  const void* q_weight;    /* (D,) of weight_dtype; NULL: ones */
+  const void* k_weight;
+  int32_t weight_dtype;    /* STA_DTYPE_* */
+  float eps;               /* finite, not negative */
+} sta_norm_rotary_args;
+
+int sta_norm_rotary(const sta_norm_rotary_args* args, void* stream);
+
+/* Its gradients.  fwd.rot.q and k are the inputs of sta_norm_rotary, fwd.rot.q_out and k_out receive their
+ * gradients, dq_out and dk_out hold those of its outputs.  dq_weight and dk_weight receive the weights'
+ * gradients in weight_dtype (NULL: not wanted), summed over the tokens and heads in one order. */
+typedef struct sta_norm_rotary_grad_args {
+  sta_norm_rotary_args fwd;
+  const void* dq_out;      /* (T, H, D) */
+  const void* dk_out;      /* (T, Hkv, D) */
+  int64_t dq_out_tok_stride, dq_out_head_stride, dk_out_tok_stride, dk_out_head_stride;
+  void* dq_weight;         /* (D,) */
+  void* dk_weight;
+  void* workspace;         /* needed for the weights' gradients only */
+  size_t workspace_bytes;
+} sta_norm_rotary_grad_args;
+
+/* 1: the call needs none, and workspace may be NULL */
+size_t sta_norm_rotary_grad_workspace_size(const sta_norm_rotary_grad_args* args);
+int sta_norm_rotary_grad(const sta_norm_rotary_grad_args* args, void* stream);
+
+/* Attention over packed sequences, causal, with a sliding window and first keys that stay visible.
+ * Sequence b has the rows starts[b] .. starts[b + 1] - 1 of q and out and k_starts[b] .. k_starts[b + 1] - 1
+ * of k and v; row i of its nq is at position p = nk - nq + i among its nk keys and sees the keys j <= p with
+ * j > p - window or j < sinks.  out = sum_j p_j v_j with p the softmax of sm_scale * q . k_j over them; a row
+ * that sees no key, or whose scores are all -inf, gets zeros and lse -inf, and so do rows of no sequence.
+ * Offsets below 0 or past T (S) count as 0 or T (S). */
+typedef struct sta_window_args {
+  const void* q;           /* (T, H, D), 16-byte rows, element strides */
+  const void* k;           /* (S, Hkv, D) */
+  const void* v;
+  int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+  int32_t dtype, T, S, H, Hkv, D; /* D in {64, 128} */
+  int32_t B;
+  const int32_t* starts;   /* (B + 1,) ascending; NULL: one sequence (B = 1) of all T rows */
+  const int32_t* k_starts; /* (B + 1,) ascending; NULL: one sequence of all S keys */
+  int32_t window;          /* keys of a window, the row's own among them; 0: all earlier keys */
+  int32_t sinks;
+  float sm_scale;          /* finite */
+  void* out;               /* (T, H, D) contiguous */
+  float* lse;              /* (H, T): log sum exp of the scaled scores */
+} sta_window_args;
+
+int sta_window_attention(const sta_window_args* args, void* stream);
+
+/* The gradients of q, k and v from out's, without atomics.  fwd.out and fwd.lse hold what
+ * sta_window_attention left.  Rows and keys of no sequence get zeros. */
+typedef struct sta_window_grad_args {
+  sta_window_args fwd;
+  const void* dout;        /* (T, H, D), 16-byte rows */
+  int64_t dout_tok_stride, dout_head_stride;
+  void* dq;                /* (T, H, D) contiguous */
+  void* dk;                /* (S, Hkv, D) contiguous */
+  void* dv;
+  void* workspace;
+  size_t workspace_bytes;
+} sta_window_grad_args;
+
+size_t sta_window_grad_workspace_size(const sta_window_grad_args* args);
+int sta_window_attention_grad(const sta_window_grad_args* args, void* stream);
+
 /* Write T new keys and values behind the sequences' keys: rows starts[b] .. starts[b + 1] - 1 of k
  * and v go to the slots lens[b] .. of sequence b (starts NULL: one row a sequence, T = B; rows
  * outside [starts[0], starts[B]) are not read, and an offset below 0 or past T counts as 0 or T).
@@ -642,6 +713,30 @@ typedef struct sta_paged_args {
 /* 1: the call needs none, and workspace may be NULL */
 size_t sta_paged_workspace_size(const sta_paged_args* args);
 int sta_paged_attention(const sta_paged_args* args, void* stream);
+
+/* The same with a sliding window: query i, at position p = lens[b] - (Q - i), sees the keys j <= p with
+ * j > p - window or j < sinks.  Pages that no query sees may be gone from the table (-1). */
+typedef struct sta_paged_window_args {
+  sta_paged_args paged;    /* accumulate must be 0 */
+  int32_t window;          /* keys of a window, the query's own among them; 0: all earlier keys */
+  int32_t sinks;
+} sta_paged_window_args;
+
+size_t sta_paged_window_workspace_size(const sta_paged_window_args* args);
+int sta_paged_window_attention(const sta_paged_window_args* args, void* stream);
+
+/* The same for sequences that begin with the same keys: every query sees the prefix_len keys of the pages of
+ * prefix and then its sequence's own, which table and lens of the cache stand for, as in
+ * sta_paged_attention.  The prefix's keys are read once for all sequences. */
+typedef struct sta_prefix_args {
+  sta_paged_args own;      /* accumulate must be 0; B * H * Q at most 2^22 */
+  const int32_t* prefix;   /* (prefix_width,) pages */
+  int32_t prefix_width;
+  int32_t prefix_len;      /* 1 to prefix_width * page_size */
+} sta_prefix_args;
+
+size_t sta_prefix_workspace_size(const sta_prefix_args* args);
+int sta_prefix_attention(const sta_prefix_args* args, void* stream);
 
 /* Keep the min(lens[b], budget) keys of each kv head that come first in this order: those with
  * pos < n_global or pos > (the head's largest pos) - n_local, then the others by weight, the

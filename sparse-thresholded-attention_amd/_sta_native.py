@@ -26,7 +26,11 @@ EXPORTS = ["sta_abi_version", "sta_last_error", "sta_shared_workspace_size", "st
            "sta_dca_decode", "sta_decode_workspace_size", "sta_decode_scores",
            "sta_decode_build_sets", "sta_decode_build_sets_chunk", "sta_decode_attend", "sta_decode_attention",
            "sta_rotary", "sta_cache_append", "sta_paged_workspace_size", "sta_paged_attention",
-           "sta_evict_workspace_size", "sta_cache_evict"]
+           "sta_evict_workspace_size", "sta_cache_evict",
+           "sta_norm_rotary", "sta_norm_rotary_grad_workspace_size", "sta_norm_rotary_grad",
+           "sta_paged_window_workspace_size", "sta_paged_window_attention",
+           "sta_prefix_workspace_size", "sta_prefix_attention",
+           "sta_window_attention", "sta_window_grad_workspace_size", "sta_window_attention_grad"]
 SCORES = {"freq": 0, "margin": 1, "expmass": 2}
 
 
@@ -248,6 +252,61 @@ class EvictArgsC(ctypes.Structure):
     ]
 
 
+class NormRotaryArgsC(ctypes.Structure):
+    """Mirror of sta_norm_rotary_args (include/sta.h)."""
+    _fields_ = [
+        ("rot", RotaryArgsC), ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+        ("weight_dtype", ctypes.c_int32), ("eps", ctypes.c_float),
+    ]
+
+
+class NormRotaryGradArgsC(ctypes.Structure):
+    """Mirror of sta_norm_rotary_grad_args (include/sta.h)."""
+    _fields_ = [
+        ("fwd", NormRotaryArgsC), ("dq_out", ctypes.c_void_p), ("dk_out", ctypes.c_void_p),
+        ("dq_out_tok_stride", ctypes.c_int64), ("dq_out_head_stride", ctypes.c_int64),
+        ("dk_out_tok_stride", ctypes.c_int64), ("dk_out_head_stride", ctypes.c_int64),
+        ("dq_weight", ctypes.c_void_p), ("dk_weight", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PagedWindowArgsC(ctypes.Structure):
+    """Mirror of sta_paged_window_args (include/sta.h)."""
+    _fields_ = [("paged", PagedArgsC), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32)]
+
+
+class PrefixArgsC(ctypes.Structure):
+    """Mirror of sta_prefix_args (include/sta.h)."""
+    _fields_ = [("own", PagedArgsC), ("prefix", ctypes.c_void_p), ("prefix_width", ctypes.c_int32),
+                ("prefix_len", ctypes.c_int32)]
+
+
+class WindowArgsC(ctypes.Structure):
+    """Mirror of sta_window_args (include/sta.h)."""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("q_tok_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("k_tok_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("v_tok_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("T", ctypes.c_int32), ("S", ctypes.c_int32), ("H", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32), ("B", ctypes.c_int32),
+        ("starts", ctypes.c_void_p), ("k_starts", ctypes.c_void_p),
+        ("window", ctypes.c_int32), ("sinks", ctypes.c_int32), ("sm_scale", ctypes.c_float),
+        ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+    ]
+
+
+class WindowGradArgsC(ctypes.Structure):
+    """Mirror of sta_window_grad_args (include/sta.h)."""
+    _fields_ = [
+        ("fwd", WindowArgsC), ("dout", ctypes.c_void_p),
+        ("dout_tok_stride", ctypes.c_int64), ("dout_head_stride", ctypes.c_int64),
+        ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 RULES = {"shared": 0, "pq": 1, "stream": 2}    # STA_RULE_SHARED / STA_RULE_PQ / STA_RULE_STREAM
 
 
@@ -316,11 +375,18 @@ def lib():
         L.sta_dca_decode.restype = ctypes.c_int
         L.sta_dca_decode.argtypes = [ctypes.POINTER(DcaDecodeArgsC), ctypes.c_void_p]
         for name, args in (("sta_rotary", RotaryArgsC), ("sta_cache_append", AppendArgsC),
-                           ("sta_paged_attention", PagedArgsC), ("sta_cache_evict", EvictArgsC)):
+                           ("sta_paged_attention", PagedArgsC), ("sta_cache_evict", EvictArgsC),
+                           ("sta_norm_rotary", NormRotaryArgsC), ("sta_norm_rotary_grad", NormRotaryGradArgsC),
+                           ("sta_paged_window_attention", PagedWindowArgsC), ("sta_prefix_attention", PrefixArgsC),
+                           ("sta_window_attention", WindowArgsC), ("sta_window_attention_grad", WindowGradArgsC)):
             fn = getattr(L, name)
             fn.restype = ctypes.c_int
             fn.argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
-        for name, args in (("sta_paged_workspace_size", PagedArgsC), ("sta_evict_workspace_size", EvictArgsC)):
+        for name, args in (("sta_paged_workspace_size", PagedArgsC), ("sta_evict_workspace_size", EvictArgsC),
+                           ("sta_norm_rotary_grad_workspace_size", NormRotaryGradArgsC),
+                           ("sta_paged_window_workspace_size", PagedWindowArgsC),
+                           ("sta_prefix_workspace_size", PrefixArgsC),
+                           ("sta_window_grad_workspace_size", WindowGradArgsC)):
             fn = getattr(L, name)
             fn.restype = ctypes.c_size_t
             fn.argtypes = [ctypes.POINTER(args)]
@@ -1562,8 +1628,8 @@ def _empty_as(x):
     return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
-def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1.0, inverse=False):
-    """sta_rotary of q (T, H, D) and k (T, Hkv, D) or None -> their rotations."""
+def _fill_rotary(a, q, k, positions, inv_freq, sections, pos_scale, rope_scale, inverse):
+    """a for rotating q (T, H, D) and k (T, Hkv, D) or None: the outputs, and the tensors that a points to."""
     _device_input(q, "q")
     dev = q.device
     if q.dim() != 3:
@@ -1572,7 +1638,6 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
     T, H, D = q.shape
     if T > _MOST:                                        # clamped, the others' output would stay unwritten
         raise ValueError(f"{T} tokens: a call takes below 2^31")
-    a = RotaryArgsC()
     q_out = _empty_as(q)
     a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
     a.q_tok_stride, a.q_head_stride, _ = q.stride()
@@ -1612,8 +1677,88 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
     a.section[:axes] = sections if axes == 1 else [_int32(s) for s in sections]
     a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
     a.pos_scale, a.rope_scale, a.inverse = float(pos_scale), float(rope_scale), int(inverse)
-    _launch(lib().sta_rotary, a, dev, "sta_rotary")
+    return q_out, k_out, (q, k, positions, inv_freq)
+
+
+def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1.0, inverse=False):
+    """sta_rotary of q (T, H, D) and k (T, Hkv, D) or None -> their rotations."""
+    a = RotaryArgsC()
+    q_out, k_out, keep = _fill_rotary(a, q, k, positions, inv_freq, sections, pos_scale, rope_scale, inverse)
+    _launch(lib().sta_rotary, a, q.device, "sta_rotary")
+    del keep
     return q_out, k_out
+
+
+def _norm_weight(w, x, name):
+    """A norm weight of x's heads, (D,), on its device; None stays None."""
+    if w is None:
+        return None
+    _require(x is not None, f"{name} without its tensor")
+    if w.dtype not in DTYPES:
+        raise TypeError(f"unsupported dtype {w.dtype} of {name}")
+    _require(tuple(w.shape) == (x.shape[-1],), f"{name} must be ({x.shape[-1]},), not {tuple(w.shape)}")
+    w = w if w.device == x.device else w.to(x.device)
+    return w if w.is_contiguous() else w.contiguous()
+
+
+def _fill_norm_rotary(a, q, k, q_weight, k_weight, positions, inv_freq, sections, eps, pos_scale, rope_scale):
+    q_out, k_out, keep = _fill_rotary(a.rot, q, k, positions, inv_freq, sections, pos_scale, rope_scale, False)
+    q_weight, k_weight = _norm_weight(q_weight, q, "q_weight"), _norm_weight(k_weight, k, "k_weight")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise TypeError("q_weight and k_weight must share one dtype")
+    given = q_weight if q_weight is not None else k_weight
+    a.weight_dtype = 0 if given is None else DTYPES[given.dtype]
+    a.q_weight = None if q_weight is None else q_weight.data_ptr()
+    a.k_weight = None if k_weight is None else k_weight.data_ptr()
+    a.eps = float(eps)
+    return q_out, k_out, (*keep, q_weight, k_weight)
+
+
+def norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, sections=None, eps=1e-6, pos_scale=1.0, rope_scale=1.0):
+    """sta_norm_rotary of q (T, H, D) and k (T, Hkv, D) or None -> both normed and rotated."""
+    a = NormRotaryArgsC()
+    q_out, k_out, keep = _fill_norm_rotary(a, q, k, q_weight, k_weight, positions, inv_freq, sections, eps, pos_scale,
+                                           rope_scale)
+    _launch(lib().sta_norm_rotary, a, q.device, "sta_norm_rotary")
+    del keep
+    return q_out, k_out
+
+
+def norm_rotary_grad(dq, dk, q, k, q_weight, k_weight, positions, inv_freq, sections=None, eps=1e-6, pos_scale=1.0,
+                     rope_scale=1.0, want_weights=True):
+    """sta_norm_rotary_grad -> (dq, dk, dq_weight, dk_weight) of the inputs, None for what was None."""
+    a = NormRotaryGradArgsC()
+    q_grad, k_grad, keep = _fill_norm_rotary(a.fwd, q, k, q_weight, k_weight, positions, inv_freq, sections, eps,
+                                             pos_scale, rope_scale)
+    dev, rows = q.device, []
+    for name, d, x in (("dq", dq, q), ("dk", dk, k)):
+        _require((d is None) == (x is None), f"{name} must be given with its tensor")
+        if d is None:
+            rows.append(None)
+            continue
+        if d.dtype != x.dtype:
+            raise TypeError(f"{name} must have its tensor's dtype")
+        _require(d.shape == x.shape, f"{name} must be {tuple(x.shape)}, not {tuple(d.shape)}")
+        rows.append(_rows(d if d.device == dev else d.to(dev)))
+    dq, dk = rows
+    a.dq_out = dq.data_ptr()
+    a.dq_out_tok_stride, a.dq_out_head_stride, _ = dq.stride()
+    if dk is not None:
+        a.dk_out = dk.data_ptr()
+        a.dk_out_tok_stride, a.dk_out_head_stride, _ = dk.stride()
+    weights = [None, None]
+    if want_weights:
+        weights = [None if w is None else torch.empty_like(w) for w in keep[-2:]]
+        a.dq_weight, a.dk_weight = (None if w is None else w.data_ptr() for w in weights)
+    n = lib().sta_norm_rotary_grad_workspace_size(ctypes.byref(a))
+    if n == 0:
+        _check(-1, "sta_norm_rotary_grad_workspace_size")
+    if n > 1 or weights[0] is not None or weights[1] is not None:
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    _launch(lib().sta_norm_rotary_grad, a, dev, "sta_norm_rotary_grad")
+    del keep
+    return q_grad, k_grad, weights[0], weights[1]
 
 
 def cache_append(cache, k, v, table, lens, starts=None, seen=None):
@@ -1646,9 +1791,8 @@ def cache_append(cache, k, v, table, lens, starts=None, seen=None):
     return new_lens
 
 
-def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want_lse=False, max_len=None):
-    """sta_paged_attention of q (B, H, D) or (B, H, Q, D) -> out like q, and with want_lse the
-    log-sum-exp (B, H) or (B, H, Q) fp32."""
+def _fill_paged(a, q, cache, table, lens, sm_scale, accumulate, want_lse, max_len):
+    """a for the attention of q over the cache: out, lse or None, and the tensors that a points to."""
     _device_input(q, "q")
     dev = cache.device
     if q.dtype != cache.k.dtype:
@@ -1657,7 +1801,6 @@ def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want
         raise ValueError(f"q must be (B, heads, {cache.head_dim}) or (B, heads, queries, {cache.head_dim})")
     shape = q.shape
     q = _rows(q if q.device == dev else q.to(dev))
-    a = PagedArgsC()
     table, lens = cache._fill(a, table, lens)
     _require(shape[0] == table.shape[0], "q and table must hold the same number of sequences")
     H = shape[1]
@@ -1673,13 +1816,48 @@ def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want
     a.out = out.data_ptr()
     lse = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if want_lse else None
     a.lse = _ptr(lse)
-    n = lib().sta_paged_workspace_size(ctypes.byref(a))
+    return out, lse, (q, table, lens)
+
+
+def _run_paged(size, call, a, paged, dev, what):
+    n = size(ctypes.byref(a))
     if n == 0:
-        _check(-1, "sta_paged_workspace_size")
+        _check(-1, what + " workspace")
     if n > 1:                                          # 1: the call needs none
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), n
-    _launch(lib().sta_paged_attention, a, dev, "sta_paged_attention")
+        paged.workspace, paged.workspace_bytes = ws.data_ptr(), n
+    _launch(call, a, dev, what)
+
+
+def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want_lse=False, max_len=None, window=None,
+                    sinks=0):
+    """sta_paged_attention of q (B, H, D) or (B, H, Q, D) -> out like q, and with want_lse the
+    log-sum-exp (B, H) or (B, H, Q) fp32; with a window sta_paged_window_attention."""
+    L = lib()
+    if window is None:
+        a = paged = PagedArgsC()
+        size, call, what = L.sta_paged_workspace_size, L.sta_paged_attention, "sta_paged_attention"
+    else:
+        _require(int(window) >= 1, "a window holds at least the query's own key")
+        a = PagedWindowArgsC()
+        a.window, a.sinks, paged = _int32(window), _int32(sinks), a.paged
+        size, call, what = L.sta_paged_window_workspace_size, L.sta_paged_window_attention, "sta_paged_window_attention"
+    out, lse, keep = _fill_paged(paged, q, cache, table, lens, sm_scale, accumulate, want_lse, max_len)
+    _run_paged(size, call, a, paged, cache.device, what)
+    del keep
+    return (out, lse) if want_lse else out
+
+
+def prefix_attention(q, cache, prefix, prefix_len, table, lens, sm_scale=None, want_lse=False, max_len=None):
+    """sta_prefix_attention of q (B, H, D) or (B, H, Q, D) -> out like q, and with want_lse the log-sum-exp."""
+    a = PrefixArgsC()
+    out, lse, keep = _fill_paged(a.own, q, cache, table, lens, sm_scale, False, want_lse, max_len)
+    prefix = _ints(prefix, cache.device)
+    _require(prefix.dim() == 1, "prefix must be (pages,)")
+    a.prefix, a.prefix_width, a.prefix_len = prefix.data_ptr(), min(prefix.shape[0], _MOST), _int32(prefix_len)
+    _run_paged(lib().sta_prefix_workspace_size, lib().sta_prefix_attention, a, a.own, cache.device,
+               "sta_prefix_attention")
+    del keep
     return (out, lse) if want_lse else out
 
 
@@ -1704,3 +1882,87 @@ def cache_evict(cache, table, lens, budget, n_global=32, n_local=32, dst_table=N
     a.workspace, a.workspace_bytes = ws.data_ptr(), n
     _launch(lib().sta_cache_evict, a, dev, "sta_cache_evict")
     return new_lens
+
+
+# ---------------------------------------------------------------------------------------------
+# attention over packed sequences with a sliding window and sinks (window_attention.py)
+# ---------------------------------------------------------------------------------------------
+def _fill_window(a, q, k, v, window, sinks, starts, k_starts, sm_scale):
+    """a for the attention of q over k, v; the tensors that it points to."""
+    _device_input(q, "q")
+    dev = q.device
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        if x.dtype != q.dtype:
+            raise TypeError("q, k and v must share one dtype")
+        _require(x.dim() == 3, f"{name} must be (tokens, heads, D), not {tuple(x.shape)}")
+    _require(k.shape == v.shape and k.shape[2] == q.shape[2], "k and v must share one shape, and q their last dim")
+    q = _rows(q)
+    k, v = _rows(k if k.device == dev else k.to(dev)), _rows(v if v.device == dev else v.to(dev))
+    (T, H, D), (S, Hkv, _) = q.shape, k.shape
+    if starts is None:
+        _require(k_starts is None, "k_starts without starts")
+        a.B = 1
+    else:
+        starts = _ints(starts, dev)
+        _require(starts.dim() == 1 and starts.shape[0] >= 2, "starts must be (sequences + 1,)")
+        if k_starts is None:
+            _require(S == T, f"{T} queries and {S} keys: k_starts says where the keys' sequences begin")
+            k_starts = starts
+        else:
+            k_starts = _ints(k_starts, dev)
+            _require(k_starts.shape == starts.shape, "starts and k_starts must share one shape")
+        a.B = min(starts.shape[0] - 1, _MOST)
+        a.starts, a.k_starts = starts.data_ptr(), k_starts.data_ptr()
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_tok_stride, a.q_head_stride, _ = q.stride()
+    a.k_tok_stride, a.k_head_stride, _ = k.stride()
+    a.v_tok_stride, a.v_head_stride, _ = v.stride()
+    a.dtype, a.T, a.S, a.H, a.Hkv, a.D = (DTYPES[q.dtype], *(min(x, _MOST) for x in (T, S, H, Hkv, D)))
+    if window is not None:
+        _require(int(window) >= 1, "a window holds at least the query's own key")
+        a.window = _int32(window)
+    a.sinks = _int32(sinks)
+    a.sm_scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    return q, k, v, starts, k_starts
+
+
+def window_attention(q, k, v, window=None, sinks=0, starts=None, k_starts=None, sm_scale=None):
+    """sta_window_attention of q (T, H, D) over k, v (S, Hkv, D) -> out like q, and the log-sum-exp (H, T)."""
+    a = WindowArgsC()
+    keep = _fill_window(a, q, k, v, window, sinks, starts, k_starts, sm_scale)
+    out = _empty_as(keep[0])
+    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+    a.out, a.lse = out.data_ptr(), lse.data_ptr()
+    _launch(lib().sta_window_attention, a, q.device, "sta_window_attention")
+    del keep
+    return out, lse
+
+
+def window_attention_grad(dout, q, k, v, out, lse, window=None, sinks=0, starts=None, k_starts=None, sm_scale=None):
+    """sta_window_attention_grad from window_attention's out and lse (H, T) -> (dq, dk, dv)."""
+    a = WindowGradArgsC()
+    keep = _fill_window(a.fwd, q, k, v, window, sinks, starts, k_starts, sm_scale)
+    dev = q.device
+    for name, x in (("dout", dout), ("out", out)):
+        if x.dtype != q.dtype:
+            raise TypeError(f"{name} must have the dtype of q")
+        _require(x.shape == q.shape, f"{name} must be {tuple(q.shape)}, not {tuple(x.shape)}")
+    _require(tuple(lse.shape) == (q.shape[1], q.shape[0]) and lse.dtype == torch.float32 and lse.device == dev,
+             "lse must be what the forward pass returned")
+    dout = _rows(dout if dout.device == dev else dout.to(dev))
+    out = out if out.device == dev else out.to(dev)
+    out = out if out.is_contiguous() and not out.data_ptr() & 15 else out.clone(memory_format=torch.contiguous_format)
+    lse = lse.contiguous()
+    a.fwd.out, a.fwd.lse = out.data_ptr(), lse.data_ptr()
+    a.dout = dout.data_ptr()
+    a.dout_tok_stride, a.dout_head_stride, _ = dout.stride()
+    dq, dk, dv = _empty_as(keep[0]), _empty_as(keep[1]), _empty_as(keep[2])
+    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    n = lib().sta_window_grad_workspace_size(ctypes.byref(a))
+    if n == 0:
+        _check(-1, "sta_window_grad_workspace_size")
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    _launch(lib().sta_window_attention_grad, a, dev, "sta_window_attention_grad")
+    del keep
+    return dq, dk, dv

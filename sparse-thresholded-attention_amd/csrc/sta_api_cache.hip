@@ -1,5 +1,6 @@
 // sta_api_cache.hip -- the C ABI of the paged cache and its operators (include/sta.h: sta_rotary,
-// sta_cache_append, sta_paged_attention, sta_cache_evict).
+// sta_norm_rotary, sta_cache_append, sta_paged_attention, sta_paged_window_attention, sta_prefix_attention,
+// sta_cache_evict).
 #include <limits.h>
 #include <math.h>
 
@@ -96,6 +97,60 @@ int check_ws(const void* ws, size_t bytes, size_t need) {
   return STA_OK;
 }
 
+// -------------------------------------------------------------------------------- rotation
+// the shapes, all that a workspace size takes
+int check_rotary_shape(const sta_rotary_args* a) {
+  if (!a) return fail(STA_ERR_INVALID_ARG, "args is NULL");
+  if (!dtype_ok(a->dtype)) return fail(STA_ERR_INVALID_ARG, "dtype %d is not one of STA_DTYPE_F32/BF16/F16", a->dtype);
+  if (a->T < 0 || a->H < 0 || a->Hkv < 0 || a->H + (int64_t)a->Hkv < 1 || a->H + (int64_t)a->Hkv > (1 << 20))
+    return fail(STA_ERR_INVALID_ARG, "T=%d, H=%d, Hkv=%d: need T >= 0 and 1 to 2^20 heads", a->T, a->H, a->Hkv);
+  if (a->D < 8 || a->D > 512 || a->D % 8 != 0)
+    return fail(STA_ERR_UNSUPPORTED, "head_dim %d is not a multiple of 8 up to 512", a->D);
+  if (a->axes < 1 || a->axes > STA_ROTARY_MAX_AXES)
+    return fail(STA_ERR_INVALID_ARG, "axes=%d outside [1, %d]", a->axes, STA_ROTARY_MAX_AXES);
+  int64_t half = 0;
+  for (int i = 0; i < a->axes; ++i) {
+    if (a->section[i] < 0) return fail(STA_ERR_INVALID_ARG, "section[%d]=%d is negative", i, a->section[i]);
+    half += a->section[i];
+  }
+  if (half < 1 || 2 * half > a->D || half % 8 != 0)
+    return fail(STA_ERR_UNSUPPORTED, "the sections sum to %lld: need a multiple of 8 up to head_dim / 2 = %d",
+                (long long)half, a->D / 2);
+  if (a->pos_type < STA_POS_I32 || a->pos_type > STA_POS_F32)
+    return fail(STA_ERR_INVALID_ARG, "pos_type %d is not one of STA_POS_*", a->pos_type);
+  return STA_OK;
+}
+
+int check_rotary(const sta_rotary_args* a) {
+  int rc = check_rotary_shape(a);
+  if (rc != STA_OK) return rc;
+  if (a->T == 0) return STA_OK;
+  if (!a->positions || !a->inv_freq) return fail(STA_ERR_INVALID_ARG, "positions and inv_freq must be non-NULL");
+  if (a->H) {
+    if ((rc = check_rows("q", a->q, a->dtype, a->q_tok_stride, a->q_head_stride)) != STA_OK) return rc;
+    if ((rc = check_rows("q_out", a->q_out, a->dtype, a->q_out_tok_stride, a->q_out_head_stride)) != STA_OK) return rc;
+  }
+  if (a->Hkv) {
+    if ((rc = check_rows("k", a->k, a->dtype, a->k_tok_stride, a->k_head_stride)) != STA_OK) return rc;
+    if ((rc = check_rows("k_out", a->k_out, a->dtype, a->k_out_tok_stride, a->k_out_head_stride)) != STA_OK) return rc;
+  }
+  return STA_OK;
+}
+
+int check_norm_rotary(const sta_norm_rotary_args* a) {
+  if (!a) return fail(STA_ERR_INVALID_ARG, "args is NULL");
+  const int rc = check_rotary(&a->rot);
+  if (rc != STA_OK) return rc;
+  if (a->rot.inverse) return fail(STA_ERR_INVALID_ARG, "the normed rotation has no inverse form");
+  if (!dtype_ok(a->weight_dtype))
+    return fail(STA_ERR_INVALID_ARG, "weight_dtype %d is not one of STA_DTYPE_F32/BF16/F16", a->weight_dtype);
+  const uintptr_t low = (uintptr_t)esize(a->weight_dtype) - 1;
+  if (((uintptr_t)a->q_weight | (uintptr_t)a->k_weight) & low)
+    return fail(STA_ERR_UNSUPPORTED, "a weight is not aligned to its elements");
+  if (!(a->eps >= 0.f) || !isfinite(a->eps)) return fail(STA_ERR_INVALID_ARG, "eps must be finite and not negative");
+  return STA_OK;
+}
+
 // -------------------------------------------------------------------------------- attention
 int paged_check(const sta_paged_args* a) {
   if (!a) return fail(STA_ERR_INVALID_ARG, "args is NULL");
@@ -122,11 +177,11 @@ int paged_cap(const sta_paged_args* a) {
   return (int)(cap < a->max_len ? cap : a->max_len);
 }
 
-PagedLayout paged_layout(const sta_paged_args* a) {
+PagedLayout paged_layout(const sta_paged_args* a, int window = 0, int sinks = 0, bool joined = false) {
   PagedLayout L{};
   const size_t rows = (size_t)a->cache.B * a->H * a->Q;
-  L.cut = paged_cut(a->cache.dtype, a->cache.D, a->H, a->cache.Hkv, a->Q, a->cache.B, paged_cap(a),
-                    a->cache.page_size);
+  L.cut = paged_cut(a->cache.dtype, a->cache.D, a->H, a->cache.Hkv, a->Q, a->cache.B,
+                    window_cap(paged_cap(a), window, sinks), a->cache.page_size, joined);
   L.score_stride = ((int64_t)paged_cap(a) + 255) / 256 * 256;   // whole units, and 256 keys of the weights
   const size_t part_rows = (size_t)L.cut.records * L.cut.rows;
   size_t off = 0;
@@ -142,6 +197,83 @@ PagedLayout paged_layout(const sta_paged_args* a) {
   if (a->accumulate && !L.cut.reform) off = align256(off + rows * L.score_stride * 4);
   L.total = off;
   return L;
+}
+
+// what a call needs beyond its shapes
+int paged_check_pointers(const sta_paged_args* a) {
+  int rc = check_cache(a->cache);
+  if (rc != STA_OK) return rc;
+  if ((rc = check_rows("q", a->q, a->cache.dtype, a->q_batch_stride, a->q_head_stride, a->q_tok_stride)) != STA_OK)
+    return rc;
+  if (!a->out || !aligned16(a->out)) return fail(STA_ERR_INVALID_ARG, "out must be non-NULL and 16-byte aligned");
+  if (a->accumulate && !a->cache.weight) return fail(STA_ERR_INVALID_ARG, "accumulate needs cache.weight");
+  return STA_OK;
+}
+
+PagedArgs paged_args(const sta_paged_args* a, const PagedLayout& L, char* ws) {
+  PagedArgs d{};
+  d.c = view_of(a->cache, a->max_len);
+  d.q = a->q;
+  d.q_bs = a->q_batch_stride;
+  d.q_hs = a->q_head_stride;
+  d.q_ts = a->q_tok_stride;
+  d.H = a->H;
+  d.Q = a->Q;
+  d.sm_scale = a->sm_scale;
+  d.accumulate = a->accumulate != 0;
+  d.out = a->out;
+  d.lse = a->lse;
+  d.stats = a->accumulate && !L.cut.small ? (float2*)(ws + L.stats_off) : nullptr;
+  d.stat_stride = a->Q > 1 ? (int64_t)L.cut.tiles * L.cut.rows : a->H / a->cache.Hkv;
+  d.scores = a->accumulate && !L.cut.reform ? (float*)(ws + L.scores_off) : nullptr;
+  d.score_stride = L.score_stride;
+  d.part_o = (float*)(ws + L.part_off);
+  d.part_ml = (float2*)(ws + L.ml_off);
+  d.runs = L.cut.runs;
+  return d;
+}
+
+// -------------------------------------------------------------------------------- windows and prefixes
+int window_check(const sta_paged_window_args* a) {
+  if (!a) return fail(STA_ERR_INVALID_ARG, "args is NULL");
+  const int rc = paged_check(&a->paged);
+  if (rc != STA_OK) return rc;
+  if (a->window < 0 || a->sinks < 0)
+    return fail(STA_ERR_INVALID_ARG, "window=%d and sinks=%d must not be negative", a->window, a->sinks);
+  if (a->paged.accumulate) return fail(STA_ERR_UNSUPPORTED, "accumulate and a window do not go together");
+  return STA_OK;
+}
+// as the kernels take them: 0 where the window reaches every key
+int window_of(const sta_paged_window_args* a) { return a->window < paged_cap(&a->paged) ? a->window : 0; }
+int sinks_of(const sta_paged_window_args* a) {
+  const int cap = paged_cap(&a->paged);
+  return a->sinks < cap ? a->sinks : cap;
+}
+
+// the call over the prefix: one sequence, whose queries are all of the batch's
+sta_paged_args prefix_call(const sta_prefix_args* a) {
+  sta_paged_args p = a->own;
+  p.cache.B = 1;
+  p.cache.table = a->prefix;
+  p.cache.table_stride = 0;
+  p.cache.table_width = a->prefix_width;
+  p.Q = a->own.cache.B * a->own.Q;
+  p.max_len = a->prefix_len;
+  return p;
+}
+
+int prefix_check(const sta_prefix_args* a) {
+  if (!a) return fail(STA_ERR_INVALID_ARG, "args is NULL");
+  int rc = paged_check(&a->own);
+  if (rc != STA_OK) return rc;
+  if (a->own.accumulate) return fail(STA_ERR_UNSUPPORTED, "accumulate and a prefix do not go together");
+  if (a->prefix_width < 1 || a->prefix_len < 1 || a->prefix_len >= (1 << 28) ||
+      (int64_t)a->prefix_width * a->own.cache.page_size < a->prefix_len)
+    return fail(STA_ERR_INVALID_ARG, "prefix_len=%d must lie in [1, 2^28) and within the prefix's %d pages",
+                a->prefix_len, a->prefix_width);
+  if ((int64_t)a->own.H * a->own.Q * a->own.cache.B > (1 << 22))
+    return fail(STA_ERR_INVALID_ARG, "B * H * Q must be at most 2^22 behind a prefix");
+  return STA_OK;
 }
 
 // -------------------------------------------------------------------------------- eviction
@@ -194,37 +326,47 @@ EvictLayout evict_layout(const sta_evict_args* a) {
 extern "C" {
 
 int sta_rotary(const sta_rotary_args* a, void* stream) {
-  if (!a) return fail(STA_ERR_INVALID_ARG, "args is NULL");
-  if (!dtype_ok(a->dtype)) return fail(STA_ERR_INVALID_ARG, "dtype %d is not one of STA_DTYPE_F32/BF16/F16", a->dtype);
-  if (a->T < 0 || a->H < 0 || a->Hkv < 0 || a->H + (int64_t)a->Hkv < 1 || a->H + (int64_t)a->Hkv > (1 << 20))
-    return fail(STA_ERR_INVALID_ARG, "T=%d, H=%d, Hkv=%d: need T >= 0 and 1 to 2^20 heads", a->T, a->H, a->Hkv);
-  if (a->D < 8 || a->D > 512 || a->D % 8 != 0)
-    return fail(STA_ERR_UNSUPPORTED, "head_dim %d is not a multiple of 8 up to 512", a->D);
-  if (a->axes < 1 || a->axes > STA_ROTARY_MAX_AXES)
-    return fail(STA_ERR_INVALID_ARG, "axes=%d outside [1, %d]", a->axes, STA_ROTARY_MAX_AXES);
-  int64_t half = 0;
-  for (int i = 0; i < a->axes; ++i) {
-    if (a->section[i] < 0) return fail(STA_ERR_INVALID_ARG, "section[%d]=%d is negative", i, a->section[i]);
-    half += a->section[i];
-  }
-  if (half < 1 || 2 * half > a->D || half % 8 != 0)
-    return fail(STA_ERR_UNSUPPORTED, "the sections sum to %lld: need a multiple of 8 up to head_dim / 2 = %d",
-                (long long)half, a->D / 2);
-  if (a->pos_type < STA_POS_I32 || a->pos_type > STA_POS_F32)
-    return fail(STA_ERR_INVALID_ARG, "pos_type %d is not one of STA_POS_*", a->pos_type);
-  if (a->T == 0) return STA_OK;
-  if (!a->positions || !a->inv_freq) return fail(STA_ERR_INVALID_ARG, "positions and inv_freq must be non-NULL");
-  int rc;
-  if (a->H) {
-    if ((rc = check_rows("q", a->q, a->dtype, a->q_tok_stride, a->q_head_stride)) != STA_OK) return rc;
-    if ((rc = check_rows("q_out", a->q_out, a->dtype, a->q_out_tok_stride, a->q_out_head_stride)) != STA_OK) return rc;
-  }
-  if (a->Hkv) {
-    if ((rc = check_rows("k", a->k, a->dtype, a->k_tok_stride, a->k_head_stride)) != STA_OK) return rc;
-    if ((rc = check_rows("k_out", a->k_out, a->dtype, a->k_out_tok_stride, a->k_out_head_stride)) != STA_OK) return rc;
-  }
+  const int rc = check_rotary(a);
+  if (rc != STA_OK || a->T == 0) return rc;
   hipError_t e = launch_rotary(*a, (hipStream_t)stream);
   return e == hipSuccess ? STA_OK : hip_fail(e, "rotary");
+}
+
+int sta_norm_rotary(const sta_norm_rotary_args* a, void* stream) {
+  const int rc = check_norm_rotary(a);
+  if (rc != STA_OK || a->rot.T == 0) return rc;
+  hipError_t e = launch_norm_rotary(*a, (hipStream_t)stream);
+  return e == hipSuccess ? STA_OK : hip_fail(e, "norm and rotary");
+}
+
+size_t sta_norm_rotary_grad_workspace_size(const sta_norm_rotary_grad_args* a) {
+  // the shapes alone
+  if (!a || check_rotary_shape(&a->fwd.rot) != STA_OK) return 0;
+  if (!a->dq_weight && !a->dk_weight) return 1;
+  const size_t n = (size_t)norm_grad_blocks(a->fwd.rot) * 2 * a->fwd.rot.D * sizeof(float);
+  return n ? n : 1;
+}
+
+int sta_norm_rotary_grad(const sta_norm_rotary_grad_args* a, void* stream) {
+  if (!a) return fail(STA_ERR_INVALID_ARG, "args is NULL");
+  int rc = check_norm_rotary(&a->fwd);
+  if (rc != STA_OK) return rc;
+  const sta_rotary_args& r = a->fwd.rot;
+  if (r.T) {
+    if (r.H && (rc = check_rows("dq_out", a->dq_out, r.dtype, a->dq_out_tok_stride, a->dq_out_head_stride)) != STA_OK)
+      return rc;
+    if (r.Hkv && (rc = check_rows("dk_out", a->dk_out, r.dtype, a->dk_out_tok_stride, a->dk_out_head_stride)) != STA_OK)
+      return rc;
+  }
+  sta_norm_rotary_grad_args d = *a;
+  if (!a->dq_weight && !a->dk_weight) {
+    d.workspace = nullptr;
+    if (!r.T) return STA_OK;
+  } else if ((rc = check_ws(a->workspace, a->workspace_bytes, sta_norm_rotary_grad_workspace_size(a))) != STA_OK) {
+    return rc;
+  }
+  hipError_t e = launch_norm_rotary_grad(d, (hipStream_t)stream);
+  return e == hipSuccess ? STA_OK : hip_fail(e, "norm and rotary gradient");
 }
 
 int sta_cache_append(const sta_append_args* a, void* stream) {
@@ -270,36 +412,52 @@ size_t sta_paged_workspace_size(const sta_paged_args* a) {
 
 int sta_paged_attention(const sta_paged_args* a, void* stream) {
   int rc = paged_check(a);
-  if (rc != STA_OK) return rc;
-  if ((rc = check_cache(a->cache)) != STA_OK) return rc;
-  if ((rc = check_rows("q", a->q, a->cache.dtype, a->q_batch_stride, a->q_head_stride, a->q_tok_stride)) != STA_OK)
-    return rc;
-  if (!a->out || !aligned16(a->out)) return fail(STA_ERR_INVALID_ARG, "out must be non-NULL and 16-byte aligned");
-  if (a->accumulate && !a->cache.weight) return fail(STA_ERR_INVALID_ARG, "accumulate needs cache.weight");
+  if (rc != STA_OK || (rc = paged_check_pointers(a)) != STA_OK) return rc;
   const PagedLayout L = paged_layout(a);
   if (L.total && (rc = check_ws(a->workspace, a->workspace_bytes, L.total)) != STA_OK) return rc;
-  char* ws = (char*)a->workspace;
-  PagedArgs d{};
-  d.c = view_of(a->cache, a->max_len);
-  d.q = a->q;
-  d.q_bs = a->q_batch_stride;
-  d.q_hs = a->q_head_stride;
-  d.q_ts = a->q_tok_stride;
-  d.H = a->H;
-  d.Q = a->Q;
-  d.sm_scale = a->sm_scale;
-  d.accumulate = a->accumulate != 0;
-  d.out = a->out;
-  d.lse = a->lse;
-  d.stats = a->accumulate && !L.cut.small ? (float2*)(ws + L.stats_off) : nullptr;
-  d.stat_stride = a->Q > 1 ? (int64_t)L.cut.tiles * L.cut.rows : a->H / a->cache.Hkv;
-  d.scores = a->accumulate && !L.cut.reform ? (float*)(ws + L.scores_off) : nullptr;
-  d.score_stride = L.score_stride;
-  d.part_o = (float*)(ws + L.part_off);
-  d.part_ml = (float2*)(ws + L.ml_off);
-  d.runs = L.cut.runs;
+  const PagedArgs d = paged_args(a, L, (char*)a->workspace);
   hipError_t e = launch_paged(a->cache.dtype, a->cache.D, d, (hipStream_t)stream);
   return e == hipSuccess ? STA_OK : hip_fail(e, "paged attention");
+}
+
+size_t sta_paged_window_workspace_size(const sta_paged_window_args* a) {
+  if (window_check(a) != STA_OK) return 0;
+  const size_t total = paged_layout(&a->paged, window_of(a), sinks_of(a)).total;
+  return total ? total : 1;
+}
+
+int sta_paged_window_attention(const sta_paged_window_args* a, void* stream) {
+  int rc = window_check(a);
+  if (rc != STA_OK || (rc = paged_check_pointers(&a->paged)) != STA_OK) return rc;
+  const sta_paged_args& p = a->paged;
+  const PagedLayout L = paged_layout(&p, window_of(a), sinks_of(a));
+  if (L.total && (rc = check_ws(p.workspace, p.workspace_bytes, L.total)) != STA_OK) return rc;
+  PagedArgs d = paged_args(&p, L, (char*)p.workspace);
+  d.window = window_of(a);
+  d.sinks = sinks_of(a);
+  hipError_t e = launch_paged(p.cache.dtype, p.cache.D, d, (hipStream_t)stream);
+  return e == hipSuccess ? STA_OK : hip_fail(e, "paged window attention");
+}
+
+size_t sta_prefix_workspace_size(const sta_prefix_args* a) {
+  if (prefix_check(a) != STA_OK) return 0;
+  const sta_paged_args p = prefix_call(a);
+  return paged_layout(&a->own, 0, 0, true).total + paged_layout(&p, 0, 0, true).total;
+}
+
+int sta_prefix_attention(const sta_prefix_args* a, void* stream) {
+  int rc = prefix_check(a);
+  if (rc != STA_OK || (rc = paged_check_pointers(&a->own)) != STA_OK) return rc;
+  if (!a->prefix) return fail(STA_ERR_INVALID_ARG, "prefix must be non-NULL");
+  const sta_paged_args p = prefix_call(a);
+  const PagedLayout L = paged_layout(&a->own, 0, 0, true), P = paged_layout(&p, 0, 0, true);
+  if ((rc = check_ws(a->own.workspace, a->own.workspace_bytes, L.total + P.total)) != STA_OK) return rc;
+  char* ws = (char*)a->own.workspace;
+  const PagedArgs d = paged_args(&a->own, L, ws);
+  PagedArgs shared = paged_args(&p, P, ws + L.total);
+  shared.per = a->own.Q;
+  hipError_t e = launch_prefix(a->own.cache.dtype, a->own.cache.D, d, shared, (hipStream_t)stream);
+  return e == hipSuccess ? STA_OK : hip_fail(e, "attention behind a prefix");
 }
 
 size_t sta_evict_workspace_size(const sta_evict_args* a) {

@@ -60,6 +60,8 @@ struct PagedArgs {
   float* part_o;                    // (records, rows, D) sums of unfinished row tiles, scaled by sum_scale
   float2* part_ml;                  // (records, rows) their maxima and sums
   int runs;
+  int window, sinks;                // keys of a window (0: all) and first keys that stay visible
+  int per;                          // queries of a sequence in a call over a shared prefix
 };
 
 // how a call of the attention is cut (host): a row tile is `rows` query rows of one kv head, `tiles` of them a
@@ -71,7 +73,14 @@ struct PagedCut {
   bool small;                       // short sequences, one query each: one launch, nothing to join
   int64_t records;                  // of unfinished row tiles, in the workspace
 };
-PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap, int page_size);
+// joined: records of every row tile, for a join of more than this call's
+PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap, int page_size, bool joined);
+// a bound on the numbers of the keys that all queries see (Common): the lengths', or the window's and the sinks'
+inline int window_cap(int cap, int window, int sinks) {
+  if (!window) return cap;
+  const int64_t most = (int64_t)window + sinks + 16;
+  return most < cap ? (int)most : cap;
+}
 
 struct EvictArgs {
   CacheView c;
@@ -87,8 +96,14 @@ struct EvictArgs {
 };
 
 hipError_t launch_rotary(const sta_rotary_args& a, hipStream_t st);
+hipError_t launch_norm_rotary(const sta_norm_rotary_args& a, hipStream_t st);
+// the weights' gradients only with a workspace, of 2 D floats a block
+hipError_t launch_norm_rotary_grad(const sta_norm_rotary_grad_args& a, hipStream_t st);
+int norm_grad_blocks(const sta_rotary_args& a);
 hipError_t launch_append(const AppendArgs& a, hipStream_t st);
 hipError_t launch_paged(int dtype, int D, const PagedArgs& a, hipStream_t st);
+// behind a shared prefix: p's rows are those of all sequences of a, a.Q each
+hipError_t launch_prefix(int dtype, int D, const PagedArgs& a, const PagedArgs& p, hipStream_t st);
 hipError_t launch_evict(const EvictArgs& a, hipStream_t st);
 
 }  // namespace sta

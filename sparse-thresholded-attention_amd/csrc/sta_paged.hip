@@ -125,19 +125,59 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
 __device__ __forceinline__ int div40(int64_t x, int64_t y) { return (int)((double)x / (double)y); }
 __device__ __forceinline__ int units_of(int keys, int unit) { return max(1, (keys + unit - 1) / unit); }
 
-// keys that every query of sequence b sees
-__device__ __forceinline__ int common(const PagedArgs& a, int b) { return max(a.c.len(b) - (a.Q - 1), 0); }
+// What a call's queries see.  PLAIN: query i of Q the first len - (Q - 1 - i) keys.  WINDOWED: of those the latest a.window
+// and the first a.sinks.  SHARED: the rows of all sequences, a.per queries each, as the queries of the one sequence that is
+// their common prefix, whose a.c.cap keys all of them see.
+enum Form { PLAIN, WINDOWED, SHARED };
+
+// The keys that every query of a sequence sees, numbered without those between the sinks and the last query's window; both
+// sides of the gap lie on multiples of 8, so that eights of numbers are eights of keys.  The numbers in front of the window
+// and behind the sinks up to there are no keys.
+template <Form F>
+struct Common {
+  int n;                                   // numbers
+  __device__ __forceinline__ int key(int u) const { return u; }
+  __device__ __forceinline__ bool sees(int) const { return true; }
+};
+template <>
+struct Common<WINDOWED> {
+  int n, head, skip, sinks, lo;            // numbers below head are keys, those from it on are skip behind; the window's first key
+  __device__ __forceinline__ int key(int u) const { return u < head ? u : u + skip; }
+  __device__ __forceinline__ bool sees(int j) const { return j < sinks || j >= lo; }
+};
+template <Form F>
+__device__ __forceinline__ Common<F> common_of(const PagedArgs& a, int b) {
+  if constexpr (F == SHARED) {
+    return {a.c.cap};
+  } else if constexpr (F == WINDOWED) {
+    const int len = a.c.len(b), end = max(len - (a.Q - 1), 0);
+    Common<WINDOWED> c;
+    c.sinks = a.sinks;
+    c.lo = max(len - a.window, 0);
+    const int lo8 = c.lo & ~7, head = min((int)(((unsigned)a.sinks + 7u) & ~7u), lo8);
+    c.head = head;
+    c.skip = lo8 - head;
+    c.n = min(end, head) + max(end - lo8, 0);
+    return c;
+  } else {
+    return {max(a.c.len(b) - (a.Q - 1), 0)};
+  }
+}
+template <Form F>
+__device__ __forceinline__ int common(const PagedArgs& a, int b) { return common_of<F>(a, b).n; }
 
 // units of a run (at least one); every lane of the wave takes part
+template <Form F>
 __device__ __forceinline__ int64_t units_each(const PagedArgs& a, int unit) {
   int64_t sum = 0;
-  for (int b = threadIdx.x & 63; b < a.c.B; b += 64) sum += units_of(common(a, b), unit);
+  for (int b = threadIdx.x & 63; b < a.c.B; b += 64) sum += units_of(common<F>(a, b), unit);
   const int64_t all = uniform(wave_sum64(sum)) * a.c.Hkv;
   return all <= a.runs ? 1 : uniform(div40(all + a.runs - 1, a.runs));
 }
 
 // The sequence that holds unit `at` (or, at < 0, sequence b) and the number of its first unit; -1: behind
 // the last.  Uniform; every lane takes part.
+template <Form F>
 __device__ __forceinline__ int find_seq(const PagedArgs& a, int unit, int64_t at, int b, int64_t& base) {
   const CacheView& c = a.c;
   const int lane = threadIdx.x & 63;
@@ -145,7 +185,7 @@ __device__ __forceinline__ int find_seq(const PagedArgs& a, int unit, int64_t at
   for (int b0 = 0; b0 < c.B; b0 += 64) {
     const int mine = b0 + lane;
     // up to 64 * 2^22 units of a row tile
-    const int n = mine < c.B ? units_of(common(a, mine), unit) : 0;
+    const int n = mine < c.B ? units_of(common<F>(a, mine), unit) : 0;
     const int incl = wave_incl_sum(n);
     const unsigned long long hit = at < 0 ? __ballot(mine == b) : __ballot(run + (int64_t)incl * c.Hkv > at);
     if (hit) {
@@ -338,9 +378,22 @@ __device__ __forceinline__ void attend_keys(Scores& sc, Values& v, State& m, Sta
 }
 
 // The sums of a kv head's waves and runs are added scaled by this, a power of two at most 1 over the number of its keys
-// (those that all queries see and the last Q - 1): no sum of theirs exceeds the largest value.
+// (those that all queries see and the last Q - 1; behind a window as many in front of it): no sum of theirs exceeds the
+// largest value.
+template <Form F>
 __device__ __forceinline__ float sum_scale(const PagedArgs& a, int common) {
-  return __uint_as_float((uint32_t)(127 - (32 - __clz(common + a.Q - 1))) << 23);
+  return __uint_as_float((uint32_t)(127 - (32 - __clz(common + (F == WINDOWED ? 2 : 1) * (a.Q - 1)))) << 23);
+}
+
+// where the row of query i of head h begins
+template <Form F, int E>
+__device__ __forceinline__ const char* query_row(const PagedArgs& a, int b, int h, int i) {
+  if constexpr (F == SHARED) {
+    const int seq = i / a.per;
+    return (const char*)a.q + (seq * a.q_bs + h * a.q_hs + (i - seq * a.per) * a.q_ts) * E;
+  } else {
+    return (const char*)a.q + (b * a.q_bs + h * a.q_hs + i * a.q_ts) * E;
+  }
 }
 
 // Whether a sum is no finite number: one of large values may have passed the type's largest, and an infinite value times
@@ -365,9 +418,10 @@ __device__ __forceinline__ bool beyond(const Acc& acc) {
 // paged_join_kernel adds the last Q - 1 keys, of which each query sees others, row by row, so that the rows
 // of an instruction always see the same keys (0 times a NaN or an infinity would reach rows that do not
 // see its key).
-template <int DT, int D, int NT, bool ACC, bool MULTI, int NW>
-__device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, D / 16>& lds, int b, int len, int hk,
+template <int DT, int D, int NT, bool ACC, bool MULTI, int NW, Form F>
+__device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, D / 16>& lds, int b, Common<F> keys, int hk,
                                             int row0, int u0, int u1, bool done, int64_t record) {
+  const int len = keys.n;
   using T = Tile<DT, D, NT>;
   constexpr int KS = T::KS, VE = T::VE, VW = T::VW, SUB = T::SUB, KT = T::KT;
   const CacheView& c = a.c;
@@ -382,7 +436,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
     const int row = row0 + t * 16 + r;
     const int g = MULTI ? row / a.Q : row, i = MULTI ? row - g * a.Q : 0, h = hk * G + g;
     const bool real = row < R;
-    const char* qp = (const char*)a.q + (b * a.q_bs + (real ? h : 0) * a.q_hs + (real ? i : 0) * a.q_ts) * T::E + g4 * 16;
+    const char* qp = query_row<F, T::E>(a, b, real ? h : 0, real ? i : 0) + g4 * 16;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       q[t][s] = *(const u32x4*)(qp + s * 64);
@@ -397,12 +451,12 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
   // A turn's rows: lane l knows those of key l % KT, and the others ask it.  The table entry is loaded two turns
   // ahead, K one turn, V at its turn's beginning.  The last turn, which loads nothing for a next one, is a copy of
   // its own: past a branch that may skip loads the compiler would wait for all loads in flight.
-  const int last = max(len - 1, 0) >> c.shift;
-  auto entry_at = [&](int u) { return table[min(((u * NW + wave) * KT + (lane & (KT - 1))) >> c.shift, last)]; };
+  const int last = keys.key(max(len - 1, 0)) >> c.shift;
+  auto entry_at = [&](int u) { return table[min(keys.key((u * NW + wave) * KT + (lane & (KT - 1))) >> c.shift, last)]; };
   int64_t krow, vrow;                                  // a key that does not exist is a row of zeros
   auto rows_of = [&](int u, int entry) {               // and which keys exist; lanes beyond KT repeat the first ones
-    const int j = (u * NW + wave) * KT + (lane & (KT - 1)), slot = c.slot_of(j);
-    const bool is = j < len && (unsigned)entry < (unsigned)c.pages;
+    const int j = (u * NW + wave) * KT + (lane & (KT - 1)), key = keys.key(j), slot = c.slot_of(key);
+    const bool is = j < len && keys.sees(key) && (unsigned)entry < (unsigned)c.pages;
     krow = (int64_t)(is ? c.k + hk * c.k_hs + entry * c.k_ps + slot * c.k_ss : (const char*)zero_row);
     vrow = (int64_t)(is ? c.v + hk * c.v_hs + entry * c.v_ps + slot * c.v_ss : (const char*)zero_row);
     return (uint32_t)__ballot(is);
@@ -485,7 +539,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
   }
 
   // the waves' states into one
-  const float small = sum_scale(a, len);
+  const float small = sum_scale<F>(a, len);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     l[t] += __shfl_xor(l[t], 16, 64);
@@ -552,7 +606,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
   }
 }
 
-template <int DT, int D, int NT, bool ACC, bool MULTI>
+template <int DT, int D, int NT, bool ACC, bool MULTI, Form F>
 __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_kernel(PagedArgs a, int tiles) {
   using T = Tile<DT, D, NT>;
   __shared__ MergeLds<D, NT, T::VE> lds;
@@ -561,26 +615,26 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
   // its L2 (16 queries of 32 heads over 8 kv heads x 128, bf16, 8 sequences up to 8192 keys: 58 -> 50 us)
   const int x = blockIdx.x / 8, tile = tiles == 1 ? 0 : x % tiles;
   const int run = tiles == 1 ? blockIdx.x : x / tiles * 8 + blockIdx.x % 8;
-  const int64_t each = units_each(a, T::UNIT);
+  const int64_t each = units_each<F>(a, T::UNIT);
   const int64_t run0 = run * each, run1 = run0 + each;
   int64_t base = 0;
-  int b = find_seq(a, T::UNIT, run0, -1, base);
+  int b = find_seq<F>(a, T::UNIT, run0, -1, base);
   if (b < 0) return;
-  int len = uniform(common(a, b)), units = units_of(len, T::UNIT);
+  int len = uniform(common<F>(a, b)), units = units_of(len, T::UNIT);
   int hk = uniform(div40(run0 - base, units));
   for (int64_t at = run0; at < run1;) {
     if (hk == c.Hkv) {
       if (++b == c.B) return;
       base = at;
       hk = 0;
-      len = uniform(common(a, b));
+      len = uniform(common<F>(a, b));
       units = units_of(len, T::UNIT);
     }
     const int64_t first = base + (int64_t)hk * units;
     const int u0 = (int)(at - first), u1 = (int)min((int64_t)units, run1 - first);
     const bool whole = u1 - u0 == units;               // the kv head's keys are this run's alone
     const int64_t record = (whole ? whole_record(a, b, hk) : 2 * (int64_t)run + (at != run0)) * tiles + tile;
-    attend_tile<DT, D, NT, ACC, MULTI, 4>(a, lds, b, len, hk, tile * T::ROWS, u0, u1, !MULTI && whole, record);
+    attend_tile<DT, D, NT, ACC, MULTI, 4, F>(a, lds, b, common_of<F>(a, b), hk, tile * T::ROWS, u0, u1, !MULTI && whole, record);
     at = first + u1;
     ++hk;
   }
@@ -591,7 +645,7 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
 // uniform; a row's 16-byte chunks lie permuted by its number, so that the reads of 16 rows' equal chunks and of one row's
 // chunks both spread over the banks.  Against 32 rows a workgroup, whose waves read the keys for themselves (32 queries of
 // 32 heads over 8 kv heads x 128, 4 sequences up to 12288 keys): 51 -> 42 us.
-template <int DT, int D>
+template <int DT, int D, Form F>
 __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int tiles) {
   using T = Tile<DT, D, 2>;
   constexpr int NT = 2, KS = T::KS, VE = T::VE, VW = T::VW, ROWS = Tile<DT, D, 8>::ROWS;
@@ -604,19 +658,19 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
   const int G = a.H / c.Hkv, R = G * a.Q;
   const int x = blockIdx.x / 8, tile = tiles == 1 ? 0 : x % tiles;
   const int run = tiles == 1 ? blockIdx.x : x / tiles * 8 + blockIdx.x % 8;
-  const int64_t each = units_each(a, T::UNIT);
+  const int64_t each = units_each<F>(a, T::UNIT);
   const int64_t run0 = run * each, run1 = run0 + each;
   int64_t base = 0;
-  int b = find_seq(a, T::UNIT, run0, -1, base);
+  int b = find_seq<F>(a, T::UNIT, run0, -1, base);
   if (b < 0) return;
-  int len = uniform(common(a, b)), units = units_of(len, T::UNIT);
+  int len = uniform(common<F>(a, b)), units = units_of(len, T::UNIT);
   int hk = uniform(div40(run0 - base, units));
   for (int64_t at = run0; at < run1;) {
     if (hk == c.Hkv) {
       if (++b == c.B) return;
       base = at;
       hk = 0;
-      len = uniform(common(a, b));
+      len = uniform(common<F>(a, b));
       units = units_of(len, T::UNIT);
     }
     const int64_t first = base + (int64_t)hk * units;
@@ -624,6 +678,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
     const int64_t record = (u1 - u0 == units ? whole_record(a, b, hk) : 2 * (int64_t)run + (at != run0)) * tiles + tile;
     const int t0 = u0 * 4, t1 = min(u1 * 4, (len + 31) / 32);         // turns
     const int32_t* table = c.table + (int64_t)b * c.t_stride;
+    const Common<F> numbers = common_of<F>(a, b);
     const int last = max(len - 1, 0);
 
     u32x4 q[NT][KS];
@@ -631,7 +686,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
     for (int t = 0; t < NT; ++t) {
       const int row = tile * ROWS + wave * 32 + t * 16 + r, g = row / a.Q, i = row - g * a.Q;
       const bool real = row < R;
-      const char* qp = (const char*)a.q + (b * a.q_bs + (real ? hk * G + g : 0) * a.q_hs + (real ? i : 0) * a.q_ts) * T::E + g4 * 16;
+      const char* qp = query_row<F, T::E>(a, b, real ? hk * G + g : 0, real ? i : 0) + g4 * 16;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         q[t][s] = *(const u32x4*)(qp + s * 64);
@@ -643,7 +698,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
       Entries e;
 #pragma unroll
       for (int w = 0; w < 4; ++w)
-        e.page[w] = *(const __attribute__((address_space(4))) int32_t*)(int64_t)(table + (min(t * 32 + w * 8, last) >> c.shift));
+        e.page[w] = *(const __attribute__((address_space(4))) int32_t*)(int64_t)(table + (numbers.key(min(t * 32 + w * 8, last)) >> c.shift));
       return e;
     };
     // copies this wave's keys of turn t, whose entries these are; which keys of the turn exist
@@ -653,10 +708,11 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
       for (int w = 0; w < 4; ++w)
         if ((unsigned)e.page[w] < (unsigned)c.pages) is |= 0xffu << (8 * w);
       if (t * 32 + 32 > len) is &= (1u << (len - t * 32)) - 1;         // a turn has a key: len - t * 32 in [1, 31]
+      if constexpr (F == WINDOWED) is &= (uint32_t)__ballot(numbers.sees(numbers.key(t * 32 + (lane & 31))));
       const int page = wave == 0 ? e.page[0] : wave == 1 ? e.page[1] : wave == 2 ? e.page[2] : e.page[3];
 #pragma unroll
       for (int y = 0; y < COPIES; ++y) {
-        const int row = wave * 8 + y * PER + lane / CH, slot = c.slot_of(t * 32 + row);
+        const int row = wave * 8 + y * PER + lane / CH, slot = c.slot_of(numbers.key(t * 32 + row));
         const int chunk = ((lane % CH) ^ (row & (CH - 1))) * 16;
         const bool have = is >> row & 1;
         const char* kp = have ? c.k + hk * c.k_hs + page * c.k_ps + slot * c.k_ss : (const char*)zero_row;
@@ -749,7 +805,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
       sweep(std::integral_constant<bool, true>(), AGAIN_SCALE);
       __syncthreads();                                 // staged is free
     }
-    const float scale = unit * sum_scale(a, len);
+    const float scale = unit * sum_scale<F>(a, len);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       l[t] += __shfl_xor(l[t], 16, 64);
@@ -781,15 +837,15 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
 
 // Calls whose sequences are all short: one launch.  A workgroup of 8 waves (16 where the registers allow) takes a kv
 // head's whole row tile, and adds the weights it gives itself.
-template <int DT, int D, int NT, bool ACC>
+template <int DT, int D, int NT, bool ACC, Form F>
 __global__ __launch_bounds__((64 * SMALL_WAVES<D, NT>), (SMALL_WAVES<D, NT> / 4)) void paged_small_kernel(PagedArgs a) {
   using T = Tile<DT, D, NT>;
   constexpr int NW = SMALL_WAVES<D, NT>;
   __shared__ MergeLds<D, NT, T::VE> lds;
   const CacheView& c = a.c;
   const int hk = blockIdx.x, b = blockIdx.y;
-  const int len = uniform(c.len(b)), R = a.H / c.Hkv;
-  attend_tile<DT, D, NT, ACC, false, NW>(a, lds, b, len, hk, 0, 0, units_of(len, NW * T::KT), true, 0);
+  const int len = uniform(common<F>(a, b)), R = a.H / c.Hkv;
+  attend_tile<DT, D, NT, ACC, false, NW, F>(a, lds, b, common_of<F>(a, b), hk, 0, 0, units_of(len, NW * T::KT), true, 0);
   if constexpr (ACC) {
     // the scores are this workgroup's own: its barriers order them, and its L1 has never held them before
     __threadfence_block();
@@ -813,11 +869,12 @@ struct Records {
   int64_t w0, first;
   __device__ __forceinline__ int64_t at(int p) const { return p ? 2 * (w0 + p) : first; }
 };
+template <Form F>
 __device__ __forceinline__ Records records_of(const PagedArgs& a, int unit, int b, int hk) {
-  const int64_t each = units_each(a, unit);
+  const int64_t each = units_each<F>(a, unit);
   int64_t base = 0;
-  find_seq(a, unit, -1, b, base);
-  const int units = units_of(common(a, b), unit);
+  find_seq<F>(a, unit, -1, b, base);
+  const int units = units_of(common<F>(a, b), unit);
   const int64_t first = base + (int64_t)hk * units;
   Records r;
   r.w0 = div40(first, each);
@@ -850,8 +907,32 @@ __device__ __forceinline__ void store_elem(void* out, int64_t at, float x) {
   else ((uint16_t*)out)[at] = (uint16_t)(DT == DT_F16 ? f32_to_f16_bits(x) : f32_to_bf16_bits(x));
 }
 
+// the keys of query i that are not common, counted from n0 to end
+template <Form F>
+struct Others {
+  __device__ __forceinline__ void set(const PagedArgs&, int, int, int&, int&) {}
+  __device__ __forceinline__ int key(int x) const { return x; }
+  __device__ __forceinline__ bool sees(int) const { return true; }
+};
+template <>
+struct Others<WINDOWED> {
+  int front, from, behind, lo, sinks;      // keys from + x, x < front, then behind + x - front
+  __device__ __forceinline__ void set(const PagedArgs& a, int b, int i, int& n0, int& end) {
+    const int len = a.c.len(b), common_end = max(len - (a.Q - 1), 0), row_end = max(end, 0);
+    lo = max(row_end - a.window, 0);
+    sinks = a.sinks;
+    from = max(lo, sinks);
+    front = max(min(max(len - a.window, 0), common_end) - from, 0);
+    behind = common_end;
+    n0 = 0;
+    end = front + max(row_end - common_end, 0);
+  }
+  __device__ __forceinline__ int key(int x) const { return x < front ? from + x : behind + x - front; }
+  __device__ __forceinline__ bool sees(int j) const { return j >= lo || j < sinks; }
+};
+
 // One query: a workgroup per row takes its records, a wave each in turn.
-template <int DT, int D, int NT>
+template <int DT, int D, int NT, Form F>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles) {
   using T = Tile<DT, D, NT>;
   constexpr int W = D / 64;                            // a lane's dims
@@ -859,7 +940,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int h = blockIdx.x, b = blockIdx.y, G = a.H / a.c.Hkv, hk = h / G, row = h - hk * G;
   const int tile = row / T::ROWS, rr = row - tile * T::ROWS;
-  const Records rec = records_of(a, T::UNIT, b, hk);
+  const Records rec = records_of<F>(a, T::UNIT, b, hk);
   if (rec.n == 1) return;                              // written by its workgroup
   auto record = [&](int p) { return (rec.at(p) * tiles + tile) * T::ROWS; };
   const float2* ml = a.part_ml + rr;
@@ -891,7 +972,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
   const int64_t row_out = (int64_t)b * a.H + h;
   if (tid < D) {
     const float sum = (o[0][tid] + o[1][tid]) + (o[2][tid] + o[3][tid]);
-    store_elem<DT>(a.out, row_out * D + tid, l == 0.f ? 0.f : sum / (l * sum_scale(a, common(a, b))));
+    store_elem<DT>(a.out, row_out * D + tid, l == 0.f ? 0.f : sum / (l * sum_scale<F>(a, common<F>(a, b))));
   }
   if (tid == 0) {
     if (a.lse) a.lse[row_out] = l == 0.f ? -INFINITY : m0 + logf(l);
@@ -899,10 +980,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int tiles)
   }
 }
 
-// Several queries: a wave per row takes its records and then the keys behind the common ones.  The waves of a workgroup
-// are rows of one query and kv head where there are four, so that those keys are fetched once.
-template <int DT, int D, int NT>
-__global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int tiles) {
+// Several queries: a wave per row takes its records and then the keys behind the common ones (and, with a window, those in
+// front of it that an earlier query sees).  The waves of a workgroup are rows of one query and kv head where there are
+// four, so that those keys are fetched once.
+// BEHIND: also the records that its row of p left, p being the call over the prefix that all sequences share.
+template <int DT, int D, int NT, Form F, bool BEHIND>
+__device__ __forceinline__ void join_row(const PagedArgs& a, int tiles, const PagedArgs& p, int p_tiles, int p_rows) {
   using T = Tile<DT, D, NT>;
   constexpr int W = D / 64, VW = T::VW;
   const CacheView& c = a.c;
@@ -911,40 +994,66 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
   if (x >= a.H * a.Q) return;
   const int g = x % G, i = x / G % a.Q, hk = x / (G * a.Q), h = hk * G + g, row = g * a.Q + i;
   const int tile = row / T::ROWS, rr = row - tile * T::ROWS;
-  const Records rec = records_of(a, T::UNIT, b, hk);
+  const Records rec = records_of<F>(a, T::UNIT, b, hk);
   auto record = [&](int p) { return (rec.at(p) * tiles + tile) * T::ROWS; };
   const float2* ml = a.part_ml + rr;
+  const int shared_row = BEHIND ? g * p.Q + b * a.Q + i : 0, shared_tile = BEHIND ? shared_row / p_rows : 0;
+  const int shared_in = shared_row - shared_tile * p_rows;
+  Records shared{0, 0, 0};
+  if constexpr (BEHIND) shared = records_of<SHARED>(p, T::UNIT, 0, hk);
+  auto shared_record = [&](int x) { return (shared.at(x) * p_tiles + shared_tile) * p_rows + shared_in; };
   float m = -INFINITY;
-  for (int p = lane; p < rec.n; p += 64) m = fmaxf(m, ml[record(p)].x);
+  for (int x = lane; x < rec.n; x += 64) m = fmaxf(m, ml[record(x)].x);
+  if constexpr (BEHIND)
+    for (int x = lane; x < shared.n; x += 64) m = fmaxf(m, p.part_ml[shared_record(x)].x);
   m = wave_max_f32(m);
   float m0 = at_least(m), l = 0.f;
-  for (int p = lane; p < rec.n; p += 64) {
-    const float2 s = ml[record(p)];
+  for (int x = lane; x < rec.n; x += 64) {
+    const float2 s = ml[record(x)];
     l += s.y * exp_of(s.x - m0);
   }
-  const int n0 = common(a, b), end = c.len(b) - (a.Q - 1 - i);
-  const float p_scale = sum_scale(a, n0);
+  if constexpr (BEHIND)
+    for (int x = lane; x < shared.n; x += 64) {
+      const float2 s = p.part_ml[shared_record(x)];
+      l += s.y * exp_of(s.x - m0);
+    }
+  int n0 = common<F>(a, b), end = c.len(b) - (a.Q - 1 - i);
+  // what the sums are scaled by: own records by own_scale, the prefix's by shared_scale, all of them together by the smaller
+  const float own_scale = sum_scale<F>(a, n0), shared_scale = BEHIND ? sum_scale<SHARED>(p, p.c.cap) : 1.f;
+  const float p_scale = BEHIND ? fminf(own_scale, shared_scale) * 0.5f : own_scale;
+  // the row's other keys, from n0 to end; with a window numbered so that the ones in front of it come first
+  Others<F> others;
+  others.set(a, b, i, n0, end);
   float y[W];
 #pragma unroll
   for (int e = 0; e < W; ++e) y[e] = 0.f;
   const float* part = a.part_o + rr * D + lane * W;
 #pragma unroll 4
-  for (int p = 0; p < rec.n; ++p) {
-    const int64_t at = record(p);
-    const float f = exp_of(ml[at].x - m0);
+  for (int x = 0; x < rec.n; ++x) {
+    const int64_t at = record(x);
+    const float f = BEHIND ? exp_of(ml[at].x - m0) * (p_scale / own_scale) : exp_of(ml[at].x - m0);
 #pragma unroll
     for (int e = 0; e < W; ++e) y[e] += f * part[at * D + e];
+  }
+  if constexpr (BEHIND) {
+#pragma unroll 4
+    for (int x = 0; x < shared.n; ++x) {
+      const int64_t at = shared_record(x);
+      const float f = exp_of(p.part_ml[at].x - m0) * (p_scale / shared_scale);
+#pragma unroll
+      for (int e = 0; e < W; ++e) y[e] += f * p.part_o[at * D + lane * W + e];
+    }
   }
   l *= p_scale;
   const int64_t row_out = ((int64_t)b * a.H + h) * a.Q + i;
   const int32_t* table = c.table + (int64_t)b * c.t_stride;
   uint32_t q[VW];
-  load_words<VW>((int64_t)((const char*)a.q + (b * a.q_bs + h * a.q_hs + i * a.q_ts) * T::E + l16 * (VW * 4)), q);
+  load_words<VW>((int64_t)(query_row<F, T::E>(a, b, h, i) + l16 * (VW * 4)), q);
   for (int j0 = n0; j0 < end; j0 += 64) {
     const int keys = min(end - j0, 64);
     // lane 16 i + j has key 4 j + i: its rows and, at last, its score; lanes behind the keys have rows of zeros
-    const int key = l16 * 4 + (lane >> 4);
-    const int page = key < keys ? c.page_of(table, j0 + key) : -1, slot = c.slot_of(j0 + key);
+    const int key = l16 * 4 + (lane >> 4), at = others.key(j0 + key);
+    const int page = key < keys && others.sees(at) ? c.page_of(table, at) : -1, slot = c.slot_of(at);
     const int64_t krow = (int64_t)(page < 0 ? (const char*)zero_row : c.k + hk * c.k_hs + page * c.k_ps + slot * c.k_ss);
     const int64_t vrow = (int64_t)(page < 0 ? (const char*)zero_row : c.v + hk * c.v_hs + page * c.v_ps + slot * c.v_ss);
     float mine = -INFINITY;
@@ -973,9 +1082,9 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
     if (a.scores && key < keys) a.scores[row_out * a.score_stride + j0 + key] = mine;
     const float m1 = fmaxf(wave_max_f32(mine), m);
     m0 = at_least(m1);
-    const float f = exp_of(m - m0), p = p_scale * exp_of(mine - m0);
+    const float f = exp_of(m - m0), prob = p_scale * exp_of(mine - m0);
     m = m1;
-    l = l * f + p;
+    l = l * f + prob;
 #pragma unroll
     for (int e = 0; e < W; ++e) y[e] *= f;
     // a key that does not exist has p = 0 and a row of zeros
@@ -993,7 +1102,7 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
 #pragma unroll
       for (int x = 0; x < 8; ++x) {
         const int from = ((t0 + x) & 3) * 16 + ((t0 + x) >> 2);
-        const float pt = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), from));
+        const float pt = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(prob), from));
 #pragma unroll
         for (int e = 0; e < W; ++e) y[e] = fmaf(pt, v_elem<DT>(w[x], e), y[e]);
       }
@@ -1009,6 +1118,15 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int t
     // the row's own record of the whole kv head, which this wave has read by now
     if (a.stats) a.stats[((int64_t)b * c.Hkv + hk) * a.stat_stride + row] = stats_of(m0, l1);
   }
+}
+
+template <int DT, int D, int NT, Form F>
+__global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int tiles) {
+  join_row<DT, D, NT, F, false>(a, tiles, a, 0, 0);
+}
+template <int DT, int D, int NT>
+__global__ __launch_bounds__(256) void prefix_join_kernel(PagedArgs a, int tiles, PagedArgs p, int p_tiles, int p_rows) {
+  join_row<DT, D, NT, PLAIN, true>(a, tiles, p, p_tiles, p_rows);
 }
 
 // The weights that a step's rows give the keys of a kv head, from their scores: four keys a lane, 256 a wave.  SHARED: the
@@ -1027,7 +1145,7 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedArgs a) {
   const int rows = a.H / c.Hkv * a.Q;
   const int64_t row0 = ((int64_t)b * c.Hkv + hk) * rows;
   const int j = j0 + lane * 4;
-  const bool all = j0 + 256 <= common(a, b);           // every row sees every key
+  const bool all = j0 + 256 <= common<PLAIN>(a, b);           // every row sees every key
   const float* s = a.scores + row0 * a.score_stride + j;
   const float2* stats = a.stats + ((int64_t)b * c.Hkv + hk) * a.stat_stride;
   const int32_t* table = c.table + (int64_t)b * c.t_stride;
@@ -1186,51 +1304,96 @@ __global__ __launch_bounds__(256) void paged_reform_kernel(PagedArgs a) {
   }
 }
 
-template <int DT, int D, int NT, bool MULTI>
+template <int DT, int D, int NT, bool MULTI, Form F>
 hipError_t launch_attend(const PagedArgs& a, const PagedCut& cut, hipStream_t st) {
   if constexpr (!MULTI) {
     if (cut.small) {
       constexpr int threads = 64 * SMALL_WAVES<D, NT>;
-      if (a.accumulate) paged_small_kernel<DT, D, NT, true><<<dim3(a.c.Hkv, a.c.B), threads, 0, st>>>(a);
-      else paged_small_kernel<DT, D, NT, false><<<dim3(a.c.Hkv, a.c.B), threads, 0, st>>>(a);
+      if constexpr (F == PLAIN) {
+        if (a.accumulate) {
+          paged_small_kernel<DT, D, NT, true, F><<<dim3(a.c.Hkv, a.c.B), threads, 0, st>>>(a);
+          return hipGetLastError();
+        }
+      }
+      paged_small_kernel<DT, D, NT, false, F><<<dim3(a.c.Hkv, a.c.B), threads, 0, st>>>(a);
       return hipGetLastError();
     }
   }
   if constexpr (MULTI && NT == 2 && DT != DT_F32) {
     if (cut.many) {
-      paged_many_kernel<DT, D><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
+      paged_many_kernel<DT, D, F><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
       hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
-      paged_join_rows_kernel<DT, D, 8><<<dim3((a.H * a.Q + 3) / 4, a.c.B), 256, 0, st>>>(a, cut.tiles);
+      paged_join_rows_kernel<DT, D, 8, F><<<dim3((a.H * a.Q + 3) / 4, a.c.B), 256, 0, st>>>(a, cut.tiles);
       if ((e = hipGetLastError()) != hipSuccess || !a.accumulate) return e;
       paged_reform_kernel<DT, D><<<dim3((a.c.cap + 255) / 256, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
       return hipGetLastError();
     }
   }
-  if (a.scores) paged_attend_kernel<DT, D, NT, true, MULTI><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
-  else paged_attend_kernel<DT, D, NT, false, MULTI><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
+  bool scores = false;
+  if constexpr (F == PLAIN) {
+    scores = a.scores != nullptr;
+    if (scores) paged_attend_kernel<DT, D, NT, true, MULTI, F><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
+  }
+  if (!scores) paged_attend_kernel<DT, D, NT, false, MULTI, F><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess) {
-    if constexpr (MULTI) paged_join_rows_kernel<DT, D, NT><<<dim3((a.H * a.Q + 3) / 4, a.c.B), 256, 0, st>>>(a, cut.tiles);
-    else paged_join_kernel<DT, D, NT><<<dim3(a.H, a.c.B), 256, 0, st>>>(a, cut.tiles);
+    if constexpr (MULTI) paged_join_rows_kernel<DT, D, NT, F><<<dim3((a.H * a.Q + 3) / 4, a.c.B), 256, 0, st>>>(a, cut.tiles);
+    else paged_join_kernel<DT, D, NT, F><<<dim3(a.H, a.c.B), 256, 0, st>>>(a, cut.tiles);
     e = hipGetLastError();
   }
-  if (e != hipSuccess || !a.accumulate) return e;
+  if constexpr (F == PLAIN) {
+    if (e != hipSuccess || !a.accumulate) return e;
+    if constexpr (DT != DT_F32) {
+      if (cut.reform) {
+        paged_reform_kernel<DT, D><<<dim3((a.c.cap + 255) / 256, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
+        return hipGetLastError();
+      }
+    }
+    if (a.H / a.c.Hkv * a.Q > 16) paged_weight_kernel<true><<<dim3((a.c.cap + 255) / 256, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
+    else paged_weight_kernel<false><<<dim3((a.c.cap + 1023) / 1024, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
+    e = hipGetLastError();
+  }
+  return e;
+}
+
+template <int DT, int D, Form F>
+hipError_t launch_rows(const PagedArgs& a, const PagedCut& cut, hipStream_t st) {
+  if (cut.rows > 16) return a.Q == 1 ? launch_attend<DT, D, 2, false, F>(a, cut, st) : launch_attend<DT, D, 2, true, F>(a, cut, st);
+  return a.Q == 1 ? launch_attend<DT, D, 1, false, F>(a, cut, st) : launch_attend<DT, D, 1, true, F>(a, cut, st);
+}
+
+// records of every row tile, for a join that adds others
+template <int DT, int D, Form F>
+hipError_t launch_records(const PagedArgs& a, const PagedCut& cut, hipStream_t st) {
   if constexpr (DT != DT_F32) {
-    if (cut.reform) {
-      paged_reform_kernel<DT, D><<<dim3((a.c.cap + 255) / 256, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
+    if (cut.many) {
+      paged_many_kernel<DT, D, F><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
       return hipGetLastError();
     }
   }
-  if (a.H / a.c.Hkv * a.Q > 16) paged_weight_kernel<true><<<dim3((a.c.cap + 255) / 256, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
-  else paged_weight_kernel<false><<<dim3((a.c.cap + 1023) / 1024, a.c.Hkv, a.c.B), 256, 0, st>>>(a);
+  if (cut.rows > 16) paged_attend_kernel<DT, D, 2, false, true, F><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
+  else paged_attend_kernel<DT, D, 1, false, true, F><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
+  return hipGetLastError();
+}
+
+// Behind a prefix that all sequences share: its keys once for the rows of all sequences, 128 or fewer of them a workgroup,
+// each sequence's own keys as in a call without one, and a join of both.
+template <int DT, int D>
+hipError_t launch_prefix_dt(const PagedArgs& a, const PagedCut& cut, const PagedArgs& p, const PagedCut& p_cut, hipStream_t st) {
+  hipError_t e = launch_records<DT, D, SHARED>(p, p_cut, st);
+  if (e == hipSuccess) e = launch_records<DT, D, PLAIN>(a, cut, st);
+  if (e != hipSuccess) return e;
+  const dim3 grid((a.H * a.Q + 3) / 4, a.c.B);
+  if (cut.rows == 128) prefix_join_kernel<DT, D, 8><<<grid, 256, 0, st>>>(a, cut.tiles, p, p_cut.tiles, p_cut.rows);
+  else if (cut.rows > 16) prefix_join_kernel<DT, D, 2><<<grid, 256, 0, st>>>(a, cut.tiles, p, p_cut.tiles, p_cut.rows);
+  else prefix_join_kernel<DT, D, 1><<<grid, 256, 0, st>>>(a, cut.tiles, p, p_cut.tiles, p_cut.rows);
   return hipGetLastError();
 }
 
 template <int DT, int D>
-hipError_t launch_rows(const PagedArgs& a, const PagedCut& cut, hipStream_t st) {
-  if (cut.rows > 16) return a.Q == 1 ? launch_attend<DT, D, 2, false>(a, cut, st) : launch_attend<DT, D, 2, true>(a, cut, st);
-  return a.Q == 1 ? launch_attend<DT, D, 1, false>(a, cut, st) : launch_attend<DT, D, 1, true>(a, cut, st);
+hipError_t launch_form(const PagedArgs& a, const PagedCut& cut, hipStream_t st) {
+  return a.window ? launch_rows<DT, D, WINDOWED>(a, cut, st) : launch_rows<DT, D, PLAIN>(a, cut, st);
 }
 
 }  // namespace
@@ -1241,7 +1404,7 @@ hipError_t launch_append(const AppendArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap, int page_size) {
+PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap, int page_size, bool joined) {
   PagedCut cut;
   const int R = H / Hkv * Q;
   // 128 rows a workgroup past 64 (32q / 8kv heads x 128, bf16, 8 sequences up to 8192 keys, R = 48 / 64 / 80 / 96 / 128: 56 /
@@ -1261,17 +1424,27 @@ PagedCut paged_cut(int dtype, int D, int H, int Hkv, int Q, int B, int cap, int 
   // x 128, bf16, 8 sequences up to 8192 keys, R = 24 / 48 / 56 / 64 rows: 48 / 68 / 74 / 80 us stored, 59 / 72 / 74 / 75
   // reformed, and 117 / 93 at R = 128 (4 up to 12288); x 64, R = 32 / 64: 40 / 60 and 40 / 52; fp32, R = 32 / 64, 97 / 147
   // and 118 / 184
-  cut.small = Q == 1 && cut.tiles == 1 && cap <= SMALL_KEYS;
+  cut.small = !joined && Q == 1 && cut.tiles == 1 && cap <= SMALL_KEYS;
   cut.reform = !cut.small && R >= 64 && dtype != STA_DTYPE_F32;
-  cut.records = cut.small ? 0 : cut.tiles * (2 * (int64_t)cut.runs + (Q > 1 ? (int64_t)Hkv * B : 0));
+  cut.records = cut.small ? 0 : cut.tiles * (2 * (int64_t)cut.runs + (Q > 1 || joined ? (int64_t)Hkv * B : 0));
   return cut;
 }
 
 hipError_t launch_paged(int dtype, int D, const PagedArgs& a, hipStream_t st) {
-  const PagedCut cut = paged_cut(dtype, D, a.H, a.c.Hkv, a.Q, a.c.B, a.c.cap, 1 << a.c.shift);
-  if (dtype == STA_DTYPE_F32) return D == 64 ? launch_rows<DT_F32, 64>(a, cut, st) : launch_rows<DT_F32, 128>(a, cut, st);
-  if (dtype == STA_DTYPE_BF16) return D == 64 ? launch_rows<DT_BF16, 64>(a, cut, st) : launch_rows<DT_BF16, 128>(a, cut, st);
-  return D == 64 ? launch_rows<DT_F16, 64>(a, cut, st) : launch_rows<DT_F16, 128>(a, cut, st);
+  const PagedCut cut = paged_cut(dtype, D, a.H, a.c.Hkv, a.Q, a.c.B, window_cap(a.c.cap, a.window, a.sinks), 1 << a.c.shift, false);
+  if (dtype == STA_DTYPE_F32) return D == 64 ? launch_form<DT_F32, 64>(a, cut, st) : launch_form<DT_F32, 128>(a, cut, st);
+  if (dtype == STA_DTYPE_BF16) return D == 64 ? launch_form<DT_BF16, 64>(a, cut, st) : launch_form<DT_BF16, 128>(a, cut, st);
+  return D == 64 ? launch_form<DT_F16, 64>(a, cut, st) : launch_form<DT_F16, 128>(a, cut, st);
+}
+
+hipError_t launch_prefix(int dtype, int D, const PagedArgs& a, const PagedArgs& p, hipStream_t st) {
+  const PagedCut cut = paged_cut(dtype, D, a.H, a.c.Hkv, a.Q, a.c.B, a.c.cap, 1 << a.c.shift, true);
+  const PagedCut p_cut = paged_cut(dtype, D, p.H, p.c.Hkv, p.Q, 1, p.c.cap, 1 << p.c.shift, true);
+  if (dtype == STA_DTYPE_F32)
+    return D == 64 ? launch_prefix_dt<DT_F32, 64>(a, cut, p, p_cut, st) : launch_prefix_dt<DT_F32, 128>(a, cut, p, p_cut, st);
+  if (dtype == STA_DTYPE_BF16)
+    return D == 64 ? launch_prefix_dt<DT_BF16, 64>(a, cut, p, p_cut, st) : launch_prefix_dt<DT_BF16, 128>(a, cut, p, p_cut, st);
+  return D == 64 ? launch_prefix_dt<DT_F16, 64>(a, cut, p, p_cut, st) : launch_prefix_dt<DT_F16, 128>(a, cut, p, p_cut, st);
 }
 
 }  // namespace sta

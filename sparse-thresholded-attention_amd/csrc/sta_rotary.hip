@@ -10,49 +10,11 @@
 // all of its heads, so a workgroup takes a token: it computes them once into LDS and then streams the
 // token's rows, 16 bytes of both rotation halves a thread.  16384 tokens of
 // 32 + 32 heads x 128, bf16: 537 MB in 94 us, 5.7 TB/s; 32 tokens: 5 us, most of it the launch and the angles.
-#include "sta_cache.h"
-#include "sta_device.h"
+#include "sta_rotary.h"
 
 namespace sta {
 
 namespace {
-
-template <int DT>
-constexpr int ROT_V = DT == DT_F32 ? 4 : 8;       // elements in 16 bytes
-
-template <int DT>
-__device__ __forceinline__ void unpack16(const u32x4& w, float* o) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if constexpr (DT == DT_F32) {
-      o[e] = __uint_as_float(w[e]);
-    } else if constexpr (DT == DT_BF16) {
-      o[2 * e] = __uint_as_float(w[e] << 16);
-      o[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-    } else {
-      o[2 * e] = f16_bits_to_f32(w[e] & 0xffffu);
-      o[2 * e + 1] = f16_bits_to_f32(w[e] >> 16);
-    }
-  }
-}
-
-template <int DT>
-__device__ __forceinline__ u32x4 pack16(const float* o) {
-  u32x4 w;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if constexpr (DT == DT_F32) w[e] = __float_as_uint(o[e]);
-    else w[e] = pack2_dt<DT>(o[2 * e], o[2 * e + 1]);
-  }
-  return w;
-}
-
-__device__ __forceinline__ double position(const sta_rotary_args& a, int axis, int64_t t) {
-  const int64_t i = axis * a.pos_axis_stride + t * a.pos_tok_stride;
-  if (a.pos_type == STA_POS_I64) return (double)((const int64_t*)a.positions)[i];
-  if (a.pos_type == STA_POS_F32) return (double)((const float*)a.positions)[i];
-  return (double)((const int32_t*)a.positions)[i];
-}
 
 template <int DT>
 __global__ __launch_bounds__(256) void rotary_kernel(sta_rotary_args a, int half) {
@@ -60,16 +22,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(sta_rotary_args a, int half
   extern __shared__ __align__(16) float2 trig[];   // [half]
   const int64_t t = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
   if (t >= a.T) return;
-  for (int f = threadIdx.x; f < half; f += 256) {
-    int axis = 0, first = 0;
-    while (axis + 1 < a.axes && f >= first + a.section[axis]) first += a.section[axis++];
-    double turns = position(a, axis, t) * (double)a.pos_scale * (double)a.inv_freq[f];
-    turns *= 0.15915494309189533577;
-    turns -= rint(turns);
-    float s, c;
-    sincospif((float)(2.0 * turns), &s, &c);
-    trig[f] = make_float2(c * a.rope_scale, (a.inverse ? -s : s) * a.rope_scale);
-  }
+  for (int f = threadIdx.x; f < half; f += 256) trig[f] = turn_of(a, f, t);
   __syncthreads();
   const int rot = half / V, chunks = rot + (a.D - 2 * half) / V;     // of a row
   const int rows = a.H + a.Hkv;

@@ -1,0 +1,141 @@
+// sta_window.hip -- the forward pass of attention with a sliding window and sinks (sta_window.h).
+//
+// A workgroup takes 128 rows of one head, a wave 32 of them, and walks the keys that they see in stages of 64 (fp32: 32)
+// through two LDS buffers, the next one copied while this one is worked on.
+//
+//   S^T = K Q^T     K rows of the stage as operand A, the wave's Q rows in registers as B; the result holds
+//                   row l % 32, keys 8 (i / 4) + 4 (l / 32) + i % 4 in slot i of lane l
+//   O^T += V^T P^T  those slots are, as they stand, contraction elements of operand B; operand A is read transposed
+//                   from the stage's V rows (ds_read_b64_tr_b16), in the same order of keys
+//
+// so P never moves between lanes.  The running maximum and sum of a row are fp32, a lane pair's own; a maximum that rises
+// by less than 2^8 leaves the sums as they are.  P is rounded once to 16 bits for the second product (its sum is of the
+// unrounded one): an error of 2^-9 (fp16 2^-12) of each probability, which adds up at random over the keys to about
+// what rounding the output itself costs.
+#include "sta_window.h"
+
+namespace sta {
+
+namespace {
+
+using namespace window;
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_kernel(WindowArgs a) {
+  using T = Tile<DT, D>;
+  constexpr int KT = T::KT, SUB = T::SUB;
+  __shared__ u32x4 lds[2][2][KT * T::CH];
+  const int G = a.H / a.Hkv, lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), r = lane & 31, h4 = (lane >> 5) * 4;
+  const int id = xcd_order(), hk = id / (a.q_tiles * G), rest = id - hk * (a.q_tiles * G);
+  if (hk >= a.Hkv) return;
+  // late tiles see more keys: first
+  const int tile_all = a.q_tiles - 1 - rest / G, h = hk * G + rest % G;
+  int base, none;
+  const int e = find_entry(a.B + 2, tile_all, [&](int x) { return (entry_of(a.starts, x, a.B, a.T).n + ROWS - 1) / ROWS; },
+                           [](int) { return 0; }, base, none);
+  if (e < 0) return;
+  const Span sq = entry_of(a.starts, e, a.B, a.T);
+  const int row0 = (tile_all - base) * ROWS, row = row0 + wave * 32 + r;
+  if (row0 < 0 || row0 >= sq.n) return;    // starts that do not ascend
+  const bool real = row < sq.n;
+  char* out = a.out + ((int64_t)(sq.at + row) * a.H + h) * T::RB;
+  float* lse = a.lse + (int64_t)h * a.T + sq.at + row;
+  floatx16 acc[T::DB];
+#pragma unroll
+  for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+  if (e == 0 || e > a.B) {                 // rows of no sequence
+    if (real) {
+      store_rows<DT, T>(out, acc, 0.f);
+      if (lane < 32) *lse = -INFINITY;
+    }
+    return;
+  }
+  const Span sk = span_of(a.k_starts, e - 1, a.S);
+  const int off = sk.n - sq.n, p0 = off + row0, pw = p0 + wave * 32;
+  const bool idle = row0 + wave * 32 >= sq.n;
+  const KeyRange keys = keys_of<KT>(a, p0, min(p0 + ROWS, sk.n) - 1);
+  const char* kb = a.k + sk.at * a.k_ts + hk * a.k_hs;
+  const char* vb = a.v + sk.at * a.v_ts + hk * a.v_hs;
+  const Row me = row_at(a, off + row);
+
+  u32x4 q[T::KD];
+  load_rows<T>(q, a.q + sq.at * a.q_ts + h * a.q_hs, a.q_ts, row, sq.n);
+  signed_rows<DT>(q, a.flip, a.keep);
+  // P times 2^shift: an fp16 P below 2^-14 of 2^8 would lose bits
+  constexpr float SHIFT = DT == DT_F16 ? 7.f : 0.f, RISE = 8.f;
+  float m = -INFINITY, l = 0.f;
+  if (keys.n) {
+    stage<T>(lds[0][0], kb, a.k_ts, keys.at(0) * KT, sk.n);
+    stage<T>(lds[0][1], vb, a.v_ts, keys.at(0) * KT, sk.n);
+  }
+  for (int t = 0; t < keys.n; ++t) {
+    next_stage();
+    if (t + 1 < keys.n) {
+      stage<T>(lds[t + 1 & 1][0], kb, a.k_ts, keys.at(t + 1) * KT, sk.n);
+      stage<T>(lds[t + 1 & 1][1], vb, a.v_ts, keys.at(t + 1) * KT, sk.n);
+    }
+    const int k0 = keys.at(t) * KT, k1 = k0 + KT - 1;
+    const u32x4 *kt = lds[t & 1][0], *vt = lds[t & 1][1];
+    const int lo_first = max(pw, 0) - a.window + 1, lo_last = max(pw + 31, 0) - a.window + 1;
+    if (idle || k0 > pw + 31 || (k1 < lo_first && k0 >= a.sinks)) continue;
+    const bool all = k1 <= pw && (k0 >= lo_last || k1 < a.sinks);
+    floatx16 s[SUB];
+#pragma unroll
+    for (int y = 0; y < SUB; ++y) s[y] = rows_product<DT, T>(kt, y * 32, q);
+    if (!all) {
+#pragma unroll
+      for (int y = 0; y < SUB; ++y)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!me.sees(k0 + y * 32 + 8 * (i / 4) + h4 + i % 4)) s[y][i] = -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int y = 0; y < SUB; ++y)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[y][i]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
+    if (__any(top > m + RISE)) {
+      const float m1 = fmaxf(m, top), f = exp2_of(m - at_least(m1));
+      m = m1;
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < T::DB; ++b) acc[b] *= f;
+    }
+    const float m0 = at_least(m) - SHIFT;
+#pragma unroll
+    for (int y = 0; y < SUB; ++y) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[y][i] = exp2_of(fmaf(s[y][i], a.c, -m0));
+        l += s[y][i];
+      }
+      Weights<DT> p;
+      p.set(s[y]);
+      transposed_product<DT, T>(vt, y * 32, p, acc);
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!real) return;
+  store_rows<DT, T>(out, acc, l == 0.f ? 0.f : 1.f / l);
+  if (lane < 32) *lse = l == 0.f ? -INFINITY : (at_least(m) - SHIFT + log2f(l)) * 0.693147180559945309f;
+}
+
+template <int DT, int D>
+hipError_t launch_dt(const WindowArgs& a, hipStream_t st) {
+  const unsigned grid = ((unsigned)a.q_tiles * a.H + 7) / 8 * 8;
+  window_kernel<DT, D><<<grid, 256, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_window(int dtype, int D, const WindowArgs& a, hipStream_t st) {
+  if (dtype == DT_F32) return D == 64 ? launch_dt<DT_F32, 64>(a, st) : launch_dt<DT_F32, 128>(a, st);
+  if (dtype == DT_BF16) return D == 64 ? launch_dt<DT_BF16, 64>(a, st) : launch_dt<DT_BF16, 128>(a, st);
+  return D == 64 ? launch_dt<DT_F16, 64>(a, st) : launch_dt<DT_F16, 128>(a, st);
+}
+
+}  // namespace sta

@@ -1,0 +1,431 @@
+// sta_window_grad.hip -- the backward pass of attention with a sliding window and sinks (sta_window.h).
+//
+//   dv_j = sum_i p_ij dout_i,  dp_ij = dout_i . v_j,  ds_ij = p_ij (dp_ij - delta_i),  delta_i = out_i . dout_i,
+//   dq_i = sm_scale sum_j ds_ij k_j,  dk_j = sm_scale sum_i ds_ij q_i
+//
+// with p formed again from the scores and the row's log-sum-exp.  Two passes without atomics, so that sums have one
+// order: one over the keys of 128 rows for dq (three products a pair), one over the rows of 128 keys for dk and dv
+// (four), the heads of a kv head one after the other.  Both keep the layouts of the forward pass: the 128 rows or
+// keys in registers as operand B, the others in stages through LDS, read as they lie for the scores and dp, and
+// transposed for the sums.  p and ds are rounded once to 16 bits for those, as p is in the forward pass.
+#include "sta_window.h"
+
+namespace sta {
+
+namespace {
+
+using namespace window;
+
+// An fp16 ds would pass the type's range: it is scaled by a power of two that keeps |ds| <= p 2 |dout| |v| below 2^14, from
+// the largest row of each.
+__device__ __forceinline__ float ds_scale(const WindowArgs& a, float* shared) {
+  const int tid = threadIdx.x;
+  float x = 0.f, y = 0.f;
+  for (int i = tid; i < a.norm_blocks; i += 256) {
+    x = fmaxf(x, a.norms[2 * i]);
+    y = fmaxf(y, a.norms[2 * i + 1]);
+  }
+  x = wave_max_f32(x);
+  y = wave_max_f32(y);
+  if ((tid & 63) == 0) shared[tid >> 6] = x, shared[4 + (tid >> 6)] = y;
+  __syncthreads();
+  x = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
+  y = fmaxf(fmaxf(shared[4], shared[5]), fmaxf(shared[6], shared[7]));
+  __syncthreads();
+  const float most = 2.f * sqrtf(x) * sqrtf(y);
+  if (!(most > 0.f && most < INFINITY)) return 1.f;
+  return __uint_as_float((uint32_t)(127 + min(max(13 - ilogbf(most), -100), 100)) << 23);
+}
+
+// delta and the base-2 log of the sum, +inf for rows that see nothing (their p is 0 then); CH lanes a row
+template <int DT, int D>
+__global__ __launch_bounds__(256) void window_delta_kernel(WindowArgs a) {
+  using T = Tile<DT, D>;
+  constexpr int V = 16 / T::E, PER = 256 / T::CH;
+  __shared__ float most[2][4];
+  const int c = threadIdx.x % T::CH, mine = threadIdx.x / T::CH;
+  auto elements = [](const char* p, float* x) {
+    const u32x4 w = *(const u32x4*)p;
+    if constexpr (DT == DT_F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+    } else {
+      Raw8<DT> raw;
+      raw.w = w;
+      raw.to_f32(x);
+    }
+  };
+  auto row_sum = [](float x) {
+#pragma unroll
+    for (int s = 1; s < T::CH; s *= 2) x += __shfl_xor(x, s, 64);
+    return x;
+  };
+  float do2 = 0.f, v2 = 0.f;
+  const int64_t rows = (int64_t)a.T * a.H;
+  for (int64_t i = (int64_t)blockIdx.x * PER + mine; i < rows; i += (int64_t)gridDim.x * PER) {
+    const int64_t t = i / a.H;
+    const int h = (int)(i - t * a.H);
+    float x[V], y[V];
+    elements(a.out + i * T::RB + c * 16, x);
+    elements(a.dout + t * a.do_ts + h * a.do_hs + c * 16, y);
+    float dot = 0.f, sq = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      dot = fmaf(x[e], y[e], dot);
+      sq = fmaf(y[e], y[e], sq);
+    }
+    dot = row_sum(dot);
+    if constexpr (DT == DT_F16) do2 = fmaxf(do2, row_sum(sq));
+    if (c == 0) {
+      const float lse = a.lse_in[h * (int64_t)a.T + t];
+      a.row_lse[h * (int64_t)a.T + t] = lse == -INFINITY ? INFINITY : lse * 1.44269504088896340736f;
+      a.row_delta[h * (int64_t)a.T + t] = dot;
+    }
+  }
+  if constexpr (DT == DT_F16) {
+    const int64_t keys = (int64_t)a.S * a.Hkv;
+    for (int64_t i = (int64_t)blockIdx.x * PER + mine; i < keys; i += (int64_t)gridDim.x * PER) {
+      const int64_t t = i / a.Hkv;
+      float x[V], sq = 0.f;
+      elements(a.v + t * a.v_ts + (i - t * a.Hkv) * a.v_hs + c * 16, x);
+#pragma unroll
+      for (int e = 0; e < V; ++e) sq = fmaf(x[e], x[e], sq);
+      v2 = fmaxf(v2, row_sum(sq));
+    }
+    do2 = wave_max_f32(do2);
+    v2 = wave_max_f32(v2);
+    if ((threadIdx.x & 63) == 0) most[0][threadIdx.x >> 6] = do2, most[1][threadIdx.x >> 6] = v2;
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      const float* x = most[threadIdx.x];
+      a.norms[2 * blockIdx.x + threadIdx.x] = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// dq: the forward pass' walk
+// ------------------------------------------------------------------------------------------
+template <int DT, int D>
+__global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dq_kernel(WindowArgs a) {
+  using T = Tile<DT, D>;
+  constexpr int KT = T::KT, SUB = T::SUB;
+  __shared__ u32x4 lds[2][2][KT * T::CH];
+  __shared__ float shared[8];
+  const int G = a.H / a.Hkv, lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), r = lane & 31, h4 = (lane >> 5) * 4;
+  const int id = xcd_order(), hk = id / (a.q_tiles * G), rest = id - hk * (a.q_tiles * G);
+  if (hk >= a.Hkv) return;
+  const int tile_all = a.q_tiles - 1 - rest / G, h = hk * G + rest % G;
+  int base, none;
+  const int e = find_entry(a.B + 2, tile_all, [&](int x) { return (entry_of(a.starts, x, a.B, a.T).n + ROWS - 1) / ROWS; },
+                           [](int) { return 0; }, base, none);
+  if (e < 0) return;
+  const Span sq = entry_of(a.starts, e, a.B, a.T);
+  const int row0 = (tile_all - base) * ROWS, row = row0 + wave * 32 + r;
+  if (row0 < 0 || row0 >= sq.n) return;    // starts that do not ascend
+  const bool real = row < sq.n;
+  char* dq = a.dq + ((int64_t)(sq.at + row) * a.H + h) * T::RB;
+  floatx16 acc[T::DB];
+#pragma unroll
+  for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+  if (e == 0 || e > a.B) {
+    if (real) store_rows<DT, T>(dq, acc, 0.f);
+    return;
+  }
+  const Span sk = span_of(a.k_starts, e - 1, a.S);
+  const int off = sk.n - sq.n, p0 = off + row0, pw = p0 + wave * 32;
+  const bool idle = row0 + wave * 32 >= sq.n;
+  const KeyRange keys = keys_of<KT>(a, p0, min(p0 + ROWS, sk.n) - 1);
+  const char* kb = a.k + sk.at * a.k_ts + hk * a.k_hs;
+  const char* vb = a.v + sk.at * a.v_ts + hk * a.v_hs;
+  const Row me = row_at(a, off + row);
+  const float grow = DT == DT_F16 ? ds_scale(a, shared) : 1.f;
+
+  u32x4 q[T::KD], dout[T::KD];
+  load_rows<T>(q, a.q + sq.at * a.q_ts + h * a.q_hs, a.q_ts, row, sq.n);
+  signed_rows<DT>(q, a.flip, a.keep);
+  load_rows<T>(dout, a.dout + sq.at * a.do_ts + h * a.do_hs, a.do_ts, row, sq.n);
+  const int64_t stat = (int64_t)h * a.T + sq.at + min(row, sq.n - 1);
+  const float lse = a.row_lse[stat], delta = a.row_delta[stat];
+  if (keys.n) {
+    stage<T>(lds[0][0], kb, a.k_ts, keys.at(0) * KT, sk.n);
+    stage<T>(lds[0][1], vb, a.v_ts, keys.at(0) * KT, sk.n);
+  }
+  for (int t = 0; t < keys.n; ++t) {
+    next_stage();
+    if (t + 1 < keys.n) {
+      stage<T>(lds[t + 1 & 1][0], kb, a.k_ts, keys.at(t + 1) * KT, sk.n);
+      stage<T>(lds[t + 1 & 1][1], vb, a.v_ts, keys.at(t + 1) * KT, sk.n);
+    }
+    const int k0 = keys.at(t) * KT, k1 = k0 + KT - 1;
+    const u32x4 *kt = lds[t & 1][0], *vt = lds[t & 1][1];
+    const int lo_first = max(pw, 0) - a.window + 1, lo_last = max(pw + 31, 0) - a.window + 1;
+    if (idle || k0 > pw + 31 || (k1 < lo_first && k0 >= a.sinks)) continue;
+    const bool all = k1 <= pw && (k0 >= lo_last || k1 < a.sinks);
+#pragma unroll
+    for (int y = 0; y < SUB; ++y) {
+      floatx16 s = rows_product<DT, T>(kt, y * 32, q);
+      const floatx16 dp = rows_product<DT, T>(vt, y * 32, dout);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = exp2_of(fmaf(s[i], a.c, -lse));
+        s[i] = p * (dp[i] - delta) * grow;
+      }
+      if (!all) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!me.sees(k0 + y * 32 + 8 * (i / 4) + h4 + i % 4)) s[i] = 0.f;
+      }
+      Weights<DT> ds;
+      ds.set(s);
+      transposed_product<DT, T>(kt, y * 32, ds, acc);
+    }
+  }
+  if (real) store_rows<DT, T>(dq, acc, a.scale / grow);
+}
+
+// ------------------------------------------------------------------------------------------
+// dk, dv
+// ------------------------------------------------------------------------------------------
+// A work item is a key tile and up to a.steps of its row steps (the heads of the kv head one after the other).  A tile
+// whose rows take one item is written out; else each item leaves a record and the join adds them up in order: tiles
+// with sinks, which every later row sees, and all tiles where there are too few for the chip.
+struct Cut {
+  int tiles, sink_tiles, near, far;        // key tiles, those with sinks, items of a near tile and of one with sinks
+  __device__ __forceinline__ int items() const { return (tiles - sink_tiles) * near + sink_tiles * far; }
+  __device__ __forceinline__ int records() const {
+    return (near > 1 ? (tiles - sink_tiles) * near : 0) + (far > 1 ? sink_tiles * far : 0);
+  }
+};
+template <int KT>
+__device__ __forceinline__ Cut cut_of(const WindowArgs& a, int e) {
+  const Span sk = entry_of(a.k_starts, e, a.B, a.S);
+  Cut c{(sk.n + ROWS - 1) / ROWS, 0, 1, 1};
+  if (e == 0 || e > a.B) return c;
+  const int steps = (span_of(a.starts, e - 1, a.T).n + KT - 1) / KT, G = a.H / a.Hkv;
+  c.near = max((int)(((int64_t)G * min(steps, a.near_steps) + a.steps - 1) / a.steps), 1);
+  c.far = max((int)(((int64_t)G * steps + a.steps - 1) / a.steps), 1);
+  if (a.window != INT32_MAX) c.sink_tiles = min((a.sinks + ROWS - 1) / ROWS, c.tiles);
+  return c;
+}
+// an item's tile, its place among the tile's items, and the tile's first record (< 0: none)
+struct Item {
+  int entry, tile, part, parts;
+  int64_t record;
+};
+template <int KT>
+__device__ __forceinline__ Item item_of(const WindowArgs& a, int at, bool by_tile, int64_t records) {
+  int base, before;
+  Item it;
+  it.entry = find_entry(a.B + 2, at, [&](int x) { const Cut c = cut_of<KT>(a, x); return by_tile ? c.tiles : c.items(); },
+                        [&](int x) { return cut_of<KT>(a, x).records(); }, base, before);
+  if (it.entry < 0) return it;
+  const Cut c = cut_of<KT>(a, it.entry);
+  int x = at - base;
+  if (by_tile) {
+    it.tile = x;
+    it.part = 0;
+  } else if (x < c.sink_tiles * c.far) {
+    it.tile = x / c.far;
+    it.part = x - it.tile * c.far;
+  } else {
+    x -= c.sink_tiles * c.far;
+    it.tile = c.sink_tiles + x / c.near;
+    it.part = x % c.near;
+  }
+  if (it.tile >= c.tiles || x < 0) it.entry = -1;      // starts that do not ascend
+  const bool sink = it.tile < c.sink_tiles;
+  it.parts = sink ? c.far : c.near;
+  it.record = it.parts == 1 ? -1 : before + (sink ? (int64_t)it.tile * c.far
+                                                  : (int64_t)(c.far > 1 ? c.sink_tiles * c.far : 0) + (int64_t)(it.tile - c.sink_tiles) * c.near);
+  if (it.record + it.parts > records || it.record < -1) it.entry = -1;
+  return it;
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dkv_kernel(WindowArgs a, int64_t records) {
+  using T = Tile<DT, D>;
+  constexpr int KT = T::KT, SUB = T::SUB;
+  __shared__ u32x4 lds[2][2][KT * T::CH];
+  __shared__ floatx4 stats[2][2][KT / 4];
+  __shared__ float shared[8];
+  const int G = a.H / a.Hkv, lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
+  const int id = xcd_order(), hk = id / a.items;
+  if (hk >= a.Hkv) return;
+  const Item it = item_of<KT>(a, id - hk * a.items, false, records);
+  if (it.entry < 0) return;
+  const Span sk = entry_of(a.k_starts, it.entry, a.B, a.S);
+  const int key0 = it.tile * ROWS, kw = key0 + wave * 32, key = kw + r;
+  const bool real = key < sk.n;
+  const int64_t at = (int64_t)(sk.at + key) * a.Hkv + hk;
+  floatx16 dk[T::DB], dv[T::DB];
+#pragma unroll
+  for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dk[b][i] = dv[b][i] = 0.f;
+  if (it.entry == 0 || it.entry > a.B) {
+    if (real) {
+      store_rows<DT, T>(a.dk + at * T::RB, dk, 0.f);
+      store_rows<DT, T>(a.dv + at * T::RB, dv, 0.f);
+    }
+    return;
+  }
+  const Span sq = span_of(a.starts, it.entry - 1, a.T);
+  const int off = sk.n - sq.n;
+  // the rows that see any of the tile's keys, in steps of KT
+  const int key1 = min(key0 + ROWS, sk.n) - 1;
+  const bool sink = key0 < a.sinks || a.window == INT32_MAX;
+  const int last = sink ? sq.n : (int)min((int64_t)sq.n, max((int64_t)key1 + a.window - off, (int64_t)0));
+  const int first = max(key0 - off, 0) / KT;
+  const int each = max((last + KT - 1) / KT - first, 0);
+  const int s0 = (int)min((int64_t)it.part * a.steps, (int64_t)each * G), s1 = (int)min((int64_t)s0 + a.steps, (int64_t)each * G);
+  const float grow = DT == DT_F16 ? ds_scale(a, shared) : 1.f;
+  constexpr float SHIFT = DT == DT_F16 ? 15.f : 0.f;   // p times 2^15: fp16 keeps small ones
+
+  u32x4 k[T::KD], v[T::KD];
+  load_rows<T>(k, a.k + sk.at * a.k_ts + hk * a.k_hs, a.k_ts, key, sk.n);
+  signed_rows<DT>(k, a.flip, a.keep);
+  load_rows<T>(v, a.v + sk.at * a.v_ts + hk * a.v_hs, a.v_ts, key, sk.n);
+  auto fetch = [&](int s, int buf) {
+    const int g = s / each, row0 = (first + s - g * each) * KT, head = hk * G + g;
+    stage<T>(lds[buf][0], a.q + sq.at * a.q_ts + head * a.q_hs, a.q_ts, row0, sq.n);
+    stage<T>(lds[buf][1], a.dout + sq.at * a.do_ts + head * a.do_hs, a.do_ts, row0, sq.n);
+    if (wave < 2 && lane < KT / 4) {       // four rows a lane; past the last row its own again
+      const float* from = (wave ? a.row_delta : a.row_lse) + (int64_t)head * a.T + sq.at;
+      floatx4 x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = from[min(row0 + lane * 4 + i, sq.n - 1)];
+      stats[buf][wave][lane] = x;
+    }
+  };
+  if (s0 < s1) fetch(s0, 0);
+  for (int s = s0; s < s1; ++s) {
+    next_stage();
+    const int buf = (s - s0) & 1;
+    if (s + 1 < s1) fetch(s + 1, buf ^ 1);
+    const int row0 = (first + s % each) * KT;
+    const u32x4 *qt = lds[buf][0], *dt = lds[buf][1];
+#pragma unroll
+    for (int y = 0; y < SUB; ++y) {
+      const int rw = row0 + y * 32, p0 = rw + off, p1 = p0 + 31;
+      const int lo0 = max(p0, 0) - a.window + 1, lo1 = max(p1, 0) - a.window + 1;
+      if (p1 < kw || (lo0 > kw + 31 && kw >= a.sinks)) continue;
+      const bool all = p0 >= kw + 31 && (lo1 <= kw || kw + 31 < a.sinks) && rw + 31 < sq.n;
+      floatx16 x = rows_product<DT, T>(qt, y * 32, k);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = exp2_of(fmaf(x[i], a.c, SHIFT - stats[buf][0][y * 8 + 2 * (i / 4) + h][i % 4]));
+      if (!all) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int row = rw + 8 * (i / 4) + 4 * h + i % 4;
+          if (!row_at(a, row + off).sees(key) || row >= sq.n) x[i] = 0.f;
+        }
+      }
+      Weights<DT> p;
+      p.set(x);
+      transposed_product<DT, T>(dt, y * 32, p, dv);
+      const floatx16 dp = rows_product<DT, T>(dt, y * 32, v);
+      const float down = DT == DT_F16 ? grow * (1.f / 32768.f) : 1.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= (dp[i] - stats[buf][1][y * 8 + 2 * (i / 4) + h][i % 4]) * down;
+      p.set(x);
+      transposed_product<DT, T>(qt, y * 32, p, dk);
+    }
+  }
+  const float dv_scale = DT == DT_F16 ? 1.f / 32768.f : 1.f, dk_scale = a.scale / grow;
+  if (it.record >= 0) {
+    float* to = a.record + (hk * records + it.record + it.part) * (2 * ROWS * D) + (wave * 32 + r) * D;
+    using F = Tile<DT_F32, D>;
+    store_rows<DT_F32, F>((char*)to, dk, dk_scale);
+    store_rows<DT_F32, F>((char*)(to + ROWS * D), dv, dv_scale);
+  } else if (real) {
+    store_rows<DT, T>(a.dk + at * T::RB, dk, dk_scale);
+    store_rows<DT, T>(a.dv + at * T::RB, dv, dv_scale);
+  }
+}
+
+// the records of a tile, added in order; four dims a thread, dk and dv
+template <int DT, int D>
+__global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a, int64_t records) {
+  using T = Tile<DT, D>;
+  const int hk = blockIdx.y, tile_all = blockIdx.x / (ROWS * D / 1024), chunk = blockIdx.x % (ROWS * D / 1024);
+  const Item it = item_of<T::KT>(a, tile_all, true, records);
+  if (it.entry < 0 || it.parts == 1) return;
+  const Span sk = entry_of(a.k_starts, it.entry, a.B, a.S);
+  const int word = chunk * 1024 + (int)threadIdx.x * 4, row = word / D, dim = word % D, key = it.tile * ROWS + row;
+  if (key >= sk.n) return;
+  const float* from = a.record + (hk * records + it.record) * (2 * ROWS * D) + word;
+  const int64_t to = (((int64_t)(sk.at + key) * a.Hkv + hk) * D + dim) * T::E;
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    floatx4 sum = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < it.parts; ++p) sum += *(const floatx4*)(from + ((int64_t)p * 2 + y) * (ROWS * D));
+    char* out = (y ? a.dv : a.dk) + to;
+    if constexpr (DT == DT_F32) *(floatx4*)out = sum;
+    else *(u32x2*)out = u32x2{pack2_dt<DT>(sum[0], sum[1]), pack2_dt<DT>(sum[2], sum[3])};
+  }
+}
+
+template <int DT, int D>
+hipError_t launch_dt(const WindowArgs& a, int64_t records, hipStream_t st) {
+  hipError_t e;
+  window_delta_kernel<DT, D><<<a.norm_blocks, 256, 0, st>>>(a);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  if (a.q_tiles) {
+    window_dq_kernel<DT, D><<<((unsigned)a.q_tiles * a.H + 7) / 8 * 8, 256, 0, st>>>(a);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  if (!a.items) return hipSuccess;
+  window_dkv_kernel<DT, D><<<((unsigned)a.items * a.Hkv + 7) / 8 * 8, 256, 0, st>>>(a, records);
+  if ((e = hipGetLastError()) != hipSuccess || !records) return e;
+  window_join_kernel<DT, D><<<dim3((unsigned)a.k_tiles * (ROWS * D / 1024), a.Hkv), 256, 0, st>>>(a, records);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+WindowCut window_cut(int dtype, int D, int T, int S, int H, int Hkv, int B, bool starts, bool k_starts, int window,
+                     int sinks) {
+  WindowCut c{};
+  const int64_t G = H / Hkv, kt = dtype == DT_F32 ? 32 : 64;
+  // an entry's last tile may be partly filled: those of B sequences and of the rows in front of and behind them
+  c.q_tiles = (int)((T + (int64_t)ROWS - 1) / ROWS + (starts ? B + 1 : 0));
+  c.k_tiles = (int)((S + (int64_t)ROWS - 1) / ROWS + (k_starts ? B + 1 : 0));
+  const int64_t all = (T + kt - 1) / kt;                     // row steps of one sequence
+  // rows that see a key of a tile: of 128 + window - 1, from any place of a step on
+  const int64_t near = ((int64_t)window + ROWS - 1 + 2 * (kt - 1)) / kt;
+  const int64_t steps = near < all ? near : all;
+  c.near_steps = (int)(steps < 1 ? 1 : steps);
+  // an item of all steps of a near tile, or where those are fewer than 512, so many that there are 512
+  const int64_t tiles = (S + (int64_t)ROWS - 1) / ROWS * Hkv;
+  int64_t each = G * c.near_steps;
+  const int64_t even = (tiles * each + 511) / 512;
+  if (even < each) each = even < 8 ? 8 : even;
+  c.steps = (int)(each < INT32_MAX ? each : INT32_MAX);
+  const int64_t near_parts = (G * c.near_steps + c.steps - 1) / c.steps;
+  int64_t items = c.k_tiles * near_parts, records = near_parts > 1 ? items : 0;
+  if (window != INT32_MAX && sinks > 0) {
+    // of each tile with sinks: sum over the sequences of ceil(G ceil(rows / kt) / steps)
+    const int64_t far = (G * (T / kt + (B < T ? B : T) + 1) + c.steps - 1) / c.steps + B;
+    const int64_t most = (S + (int64_t)ROWS - 1) / ROWS, of = ((int64_t)sinks + ROWS - 1) / ROWS;
+    items += far * (of < most ? of : most);
+    records += far * (of < most ? of : most);
+  }
+  c.items = (int)(items < INT32_MAX ? items : INT32_MAX);
+  c.records = records;
+  // of 16 rows a block and turn; enough blocks to fill the chip, few enough for their norms to be read again
+  const int64_t rows = (int64_t)T * H, blocks = (rows + 15) / 16;
+  c.norm_blocks = (int)(blocks < 1 ? 1 : blocks < 2048 ? blocks : 2048);
+  return c;
+}
+
+hipError_t launch_window_grad(int dtype, int D, const WindowArgs& a, int64_t records, hipStream_t st) {
+  if (dtype == DT_F32) return D == 64 ? launch_dt<DT_F32, 64>(a, records, st) : launch_dt<DT_F32, 128>(a, records, st);
+  if (dtype == DT_BF16) return D == 64 ? launch_dt<DT_BF16, 64>(a, records, st) : launch_dt<DT_BF16, 128>(a, records, st);
+  return D == 64 ? launch_dt<DT_F16, 64>(a, records, st) : launch_dt<DT_F16, 128>(a, records, st);
+}
+
+}  // namespace sta

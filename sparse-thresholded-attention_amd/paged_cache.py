@@ -5,8 +5,12 @@ of sequences whose keys lie in pages, and a cache held at a budget of keys:
 
     rotary            rotary positions with one or several axes (time, height, width), differentiable
     rotary_grad       the rotation's gradient on its own
+    norm_rotary       each head's row divided by its root mean square, then rotated, in one pass; differentiable
+    norm_rotary_grad  its gradients on their own
     cache_append      new keys and values into the pages
-    paged_attention   a few new tokens of every sequence over its cached keys (dense: no threshold)
+    paged_attention   a few new tokens of every sequence over its cached keys (dense: no threshold), all of
+                      them or the latest of a window and the first few (sinks)
+    prefix_attention  the same for sequences that begin with the same keys, which are read once for all
     cache_evict       drop the keys of least accumulated attention weight
 
 A decoding step of a batch, held at `budget` keys a head:
@@ -19,12 +23,13 @@ A decoding step of a batch, held at `budget` keys a head:
 
 All of them launch on the current stream of the tensors' device, allocate their results and their
 workspace from torch's allocator, and neither synchronise nor keep anything between calls, so a HIP
-graph can capture them (a captured training step calls rotary_grad itself).  rotary alone takes part
-in automatic differentiation, in both modes; the others keep neither gradients nor tangents.  There is
-no fallback: a CPU tensor, an unsupported shape or a missing library raises.
+graph can capture them (a captured training step calls rotary_grad and norm_rotary_grad itself).  rotary
+takes part in automatic differentiation, in both modes, and norm_rotary in reverse mode, once; the others keep
+neither gradients nor tangents.  There is no fallback: a CPU tensor, an unsupported shape or a missing library raises.
 """
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 import _sta_native as native
 from _sta_native import PagedCache  # noqa: F401
@@ -78,6 +83,52 @@ def rotary_grad(dq, dk, positions, inv_freq, sections=None, pos_scale=1.0, rope_
     return native.rotary(dq, dk, positions, inv_freq, sections, pos_scale, rope_scale, inverse=True)
 
 
+class _NormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, pos_scale, rope_scale):
+        return native.norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, pos_scale, rope_scale)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        *tensors, ctx.sections, ctx.eps, ctx.pos_scale, ctx.rope_scale = inputs
+        ctx.save_for_backward(*tensors)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        want = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
+        return (*native.norm_rotary_grad(dq, dk, *ctx.saved_tensors, ctx.sections, ctx.eps, ctx.pos_scale,
+                                         ctx.rope_scale, want), None, None, None, None, None, None)
+
+
+def norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, sections=None, eps=1e-6, pos_scale=1.0, rope_scale=1.0):
+    """Norm each head's row of q (T, H, D) and k (T, Hkv, D), or of q alone (k and k_weight None), and rotate it as
+    rotary does; returns both, in their dtype.
+
+    y = R(x / sqrt(mean(x^2) + eps) * weight), the mean over all D elements of a head's row.  q_weight and k_weight:
+    (D,), shared by the heads, of one dtype of their own (bf16, fp16, fp32), or None for ones.  In fp32, rounded once
+    at the end; positions, inv_freq, sections and scales as in rotary.  eps is at least 0.  Differentiable once, in q, k
+    and the weights; forward-mode tangents are refused."""
+    tensors = [x for x in (q, k, q_weight, k_weight) if x is not None]
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise RuntimeError("norm_rotary has no forward-mode derivative")
+    if torch.is_grad_enabled() and any(x.requires_grad for x in tensors):
+        return _NormRotary.apply(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, pos_scale, rope_scale)
+    return native.norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, sections, eps, pos_scale, rope_scale)
+
+
+def norm_rotary_grad(dq, dk, q, k, q_weight, k_weight, positions, inv_freq, sections=None, eps=1e-6, pos_scale=1.0,
+                     rope_scale=1.0):
+    """The gradients (dq, dk, dq_weight, dk_weight) of norm_rotary's inputs from those of its outputs, without an
+    autograd graph; None where the input is None.  The weights' are summed over tokens and heads in one order: a
+    call repeated gives the same bits.  Inputs with forward-mode tangents are refused."""
+    if forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None
+                                              for x in (dq, dk, q, k, q_weight, k_weight)):
+        raise RuntimeError("norm_rotary_grad keeps no graph and no forward-mode tangents")
+    return native.norm_rotary_grad(dq, dk, q, k, q_weight, k_weight, positions, inv_freq, sections, eps, pos_scale,
+                                   rope_scale)
+
+
 def cache_append(cache, k, v, table, lens, starts=None, seen=None):
     """Write new keys and values k, v (T, Hkv, D) behind the sequences' cached ones; returns the new
     lengths (B,) int32 (lens itself is not changed).
@@ -91,18 +142,32 @@ def cache_append(cache, k, v, table, lens, starts=None, seen=None):
     return native.cache_append(cache, k, v, table, lens, starts, seen)
 
 
-def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want_lse=False, max_len=None):
+def paged_attention(q, cache, table, lens, sm_scale=None, accumulate=False, want_lse=False, max_len=None, window=None,
+                    sinks=0):
     """Attention of the last token, or the last Q tokens, of every sequence over its cached keys (their
     own among them): q (B, H, D) or (B, H, Q, D), query i of Q sees the first len - (Q - 1 - i) keys.
     Returns out like q; with want_lse also the log-sum-exp of the scaled scores, (B, H[, Q]) fp32.
     A query that sees no key gets zeros and -inf.
 
+    window: of those keys a query, at position p, sees j > p - window and j < sinks only (default: all).
+    Pages that no query of a sequence sees may be gone from its table (-1).  Slots count as positions, so
+    not after an eviction, and accumulate does not go with it.
+
     accumulate: add every key's probability, summed over the queries and the heads of its kv head, to
     cache.weight; a page of such a call stands in one place of one sequence's table.  max_len: a bound
     on lens known to the host, at least 1 (default: the table's); lengths past it count as max_len.  It sizes the
     workspace of accumulate, 4 bytes a query row and key for fp32 and below 64 rows (queries times heads
-    of a kv head).  Meant for a few new tokens: the last Q - 1 keys are taken row by row."""
-    return native.paged_attention(q, cache, table, lens, sm_scale, accumulate, want_lse, max_len)
+    of a kv head).  Meant for a few new tokens: the last Q - 1 keys (with a window as many in front of it)
+    are taken row by row."""
+    return native.paged_attention(q, cache, table, lens, sm_scale, accumulate, want_lse, max_len, window, sinks)
+
+
+def prefix_attention(q, cache, prefix, prefix_len, table, lens, sm_scale=None, want_lse=False, max_len=None):
+    """paged_attention for sequences that begin with the same keys: every query sees the prefix_len keys
+    (a number, at least 1) in the pages of prefix (pages,) int32, which all sequences share, and then its
+    sequence's own: the keys of table and lens, which count these alone, as in paged_attention; lens may be 0.
+    The prefix's keys are read once for all sequences.  B * H * Q up to 2^22."""
+    return native.prefix_attention(q, cache, prefix, prefix_len, table, lens, sm_scale, want_lse, max_len)
 
 
 def cache_evict(cache, table, lens, budget, n_global=32, n_local=32, dst_table=None, max_len=None):
