@@ -606,7 +606,7 @@ int sta_rotary(const sta_rotary_args* args, void* stream);
  * 64), rounded once.  Outputs may be the inputs. */
 typedef struct sta_norm_rotary_args {
   sta_rotary_args rot;     /* tensors, positions and frequencies; inverse must be 0 */
-  const void* q_weight;    /* (D,) of weight_dtype; NULL: ones */
+  const void* q_weight;    /* (D,) of weight_dtype, 16-byte aligned; NULL: ones */
   const void* k_weight;
   int32_t weight_dtype;    /* STA_DTYPE_* */
   float eps;               /* finite, not negative */

@@ -1689,6 +1689,12 @@ def rotary(q, k, positions, inv_freq, sections=None, pos_scale=1.0, rope_scale=1
     return q_out, k_out
 
 
+def _packed(x, dev):
+    """x on dev, contiguous and 16-byte aligned."""
+    x = x if x.device == dev else x.to(dev)
+    return x if x.is_contiguous() and not x.data_ptr() & 15 else x.clone(memory_format=torch.contiguous_format)
+
+
 def _norm_weight(w, x, name):
     """A norm weight of x's heads, (D,), on its device; None stays None."""
     if w is None:
@@ -1697,8 +1703,7 @@ def _norm_weight(w, x, name):
     if w.dtype not in DTYPES:
         raise TypeError(f"unsupported dtype {w.dtype} of {name}")
     _require(tuple(w.shape) == (x.shape[-1],), f"{name} must be ({x.shape[-1]},), not {tuple(w.shape)}")
-    w = w if w.device == x.device else w.to(x.device)
-    return w if w.is_contiguous() else w.contiguous()
+    return _packed(w, x.device)
 
 
 def _fill_norm_rotary(a, q, k, q_weight, k_weight, positions, inv_freq, sections, eps, pos_scale, rope_scale):
@@ -1887,12 +1892,6 @@ def cache_evict(cache, table, lens, budget, n_global=32, n_local=32, dst_table=N
 # ---------------------------------------------------------------------------------------------
 # attention over packed sequences with a sliding window and sinks (window_attention.py)
 # ---------------------------------------------------------------------------------------------
-def _packed(x, dev):
-    """x on dev, contiguous and 16-byte aligned."""
-    x = x if x.device == dev else x.to(dev)
-    return x if x.is_contiguous() and not x.data_ptr() & 15 else x.clone(memory_format=torch.contiguous_format)
-
-
 def _fill_window(a, q, k, v, window, sinks, starts, k_starts, sm_scale):
     """a for the attention of q over k, v; the tensors that it points to."""
     _device_input(q, "q")

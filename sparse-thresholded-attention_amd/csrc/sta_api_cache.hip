@@ -144,9 +144,8 @@ int check_norm_rotary(const sta_norm_rotary_args* a) {
   if (a->rot.inverse) return fail(STA_ERR_INVALID_ARG, "the normed rotation has no inverse form");
   if (!dtype_ok(a->weight_dtype))
     return fail(STA_ERR_INVALID_ARG, "weight_dtype %d is not one of STA_DTYPE_F32/BF16/F16", a->weight_dtype);
-  const uintptr_t low = (uintptr_t)esize(a->weight_dtype) - 1;
-  if (((uintptr_t)a->q_weight | (uintptr_t)a->k_weight) & low)
-    return fail(STA_ERR_UNSUPPORTED, "a weight is not aligned to its elements");
+  if (!aligned16(a->q_weight) || !aligned16(a->k_weight))
+    return fail(STA_ERR_UNSUPPORTED, "a weight is not 16-byte aligned");
   if (!(a->eps >= 0.f) || !isfinite(a->eps)) return fail(STA_ERR_INVALID_ARG, "eps must be finite and not negative");
   return STA_OK;
 }
@@ -343,7 +342,7 @@ size_t sta_norm_rotary_grad_workspace_size(const sta_norm_rotary_grad_args* a) {
   // the shapes alone
   if (!a || check_rotary_shape(&a->fwd.rot) != STA_OK) return 0;
   if (!a->dq_weight && !a->dk_weight) return 1;
-  const size_t n = (size_t)norm_grad_blocks(a->fwd.rot) * 2 * a->fwd.rot.D * sizeof(float);
+  const size_t n = (size_t)norm_grad_blocks(a->fwd.rot) * a->fwd.rot.D * sizeof(float);
   return n ? n : 1;
 }
 

@@ -97,7 +97,7 @@ struct EvictArgs {
 
 hipError_t launch_rotary(const sta_rotary_args& a, hipStream_t st);
 hipError_t launch_norm_rotary(const sta_norm_rotary_args& a, hipStream_t st);
-// the weights' gradients only with a workspace, of 2 D floats a block
+// the weights' gradients only with a workspace, of D floats a block
 hipError_t launch_norm_rotary_grad(const sta_norm_rotary_grad_args& a, hipStream_t st);
 int norm_grad_blocks(const sta_rotary_args& a);
 hipError_t launch_append(const AppendArgs& a, hipStream_t st);
