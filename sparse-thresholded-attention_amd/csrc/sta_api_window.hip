@@ -114,6 +114,8 @@ WindowArgs args_of(const sta_window_args* a) {
   d.q_tiles = cut.q_tiles;
   d.k_tiles = cut.k_tiles;
   d.items = cut.items;
+  d.q_waves = cut.q_waves;
+  d.k_waves = cut.k_waves;
   d.steps = cut.steps;
   d.near_steps = cut.near_steps;
   d.norm_blocks = cut.norm_blocks;
@@ -135,7 +137,7 @@ GradLayout layout_of(const sta_window_args* a) {
   l.norms_off = off;
   off = align256(off + (a->dtype == STA_DTYPE_F16 ? (size_t)cut.norm_blocks * 8 : 0));
   l.record_off = off;
-  off = align256(off + (size_t)a->Hkv * cut.records * 2 * 128 * a->D * 4);
+  off = align256(off + (size_t)a->Hkv * cut.records * 2 * (32 * cut.k_waves) * a->D * 4);
   l.total = off ? off : 1;
   return l;
 }

@@ -32,15 +32,16 @@ struct WindowArgs {
   float *row_lse, *row_delta;              // (H, T): log2 of the sum of exp, +inf for rows that see nothing; sum_d out dout
   float* norms;                            // fp16: (blocks, 2) largest |dout row|^2 and |v row|^2
   int norm_blocks;
-  float* record;                           // (records, 2, 128, D) unfinished dk and dv
+  float* record;                           // (records, 2, rows of a key tile, D) unfinished dk and dv
   int steps;                               // row steps of a work item of the key pass
   int near_steps;                          // row steps that a key tile has at most, a query head
   int q_tiles, k_tiles, items;             // bounds of the grids, a head / kv head
+  int q_waves, k_waves;                    // waves of a workgroup: 4, or 1 where there are few rows
 };
 
 // how the key pass is cut (host)
 struct WindowCut {
-  int q_tiles, k_tiles, items, steps, near_steps, norm_blocks;
+  int q_waves, k_waves, q_tiles, k_tiles, items, steps, near_steps, norm_blocks;
   int64_t records;
 };
 WindowCut window_cut(int dtype, int D, int T, int S, int H, int Hkv, int B, bool starts, bool k_starts, int window,
@@ -50,18 +51,20 @@ hipError_t launch_window(int dtype, int D, const WindowArgs& a, hipStream_t st);
 hipError_t launch_window_grad(int dtype, int D, const WindowArgs& a, int64_t records, hipStream_t st);
 
 #ifdef __HIPCC__
+// a lambda that the compiler called instead would have its captured registers in memory
+#define STA_INLINE __attribute__((always_inline))
+
 namespace window {
 
-constexpr int ROWS = 128;                  // rows (keys in the key pass) a workgroup
-
-// COLS_: tiles of 32 rows a wave, so that 4 / COLS_ waves make a workgroup
-template <int DT, int D_, int COLS_ = 1>
+// a workgroup's WAVES_ waves take 32 rows (keys in the key pass) each
+template <int DT, int D_, int WAVES_>
 struct Tile {
-  static constexpr int COLS = COLS_, WAVES = ROWS / 32 / COLS, THREADS = 64 * WAVES;
+  static constexpr int WAVES = WAVES_, THREADS = 64 * WAVES, ROWS = 32 * WAVES;
   static constexpr int D = D_, E = DT == DT_F32 ? 4 : 2, RB = D * E, CH = RB / 16;
   static constexpr int KD = RB / 32;       // products over a row: 32 bytes of it each, 16 a half wave
   static constexpr int DB = D / 32;        // blocks of 32 dims
-  static constexpr int KT = DT == DT_F32 ? 32 : 64;   // rows of a stage
+  static constexpr int LEAST = DT == DT_F32 || WAVES == 1 ? 1 : 2;    // waves of a SIMD that the registers have to allow
+  static constexpr int KT = DT == DT_F32 || WAVES == 1 ? 32 : 64;   // rows of a stage; one wave: room for four workgroups a CU
   static constexpr int SUB = KT / 32;
   static constexpr int COPIES = KT * CH / THREADS;    // a wave's 1 KB copies of a stage's rows
 };
@@ -91,9 +94,18 @@ __device__ __forceinline__ floatx16 mma(u32x4 a, u32x4 b, floatx16 c) {
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ const u32x4 zero_row[32] = {};  // 512 bytes: a row of 128 fp32 elements
 
-// 4 bytes a lane into LDS, lane l's at lds_base + 4 l, as copy16_to_lds
-__device__ __forceinline__ void copy4_to_lds(const void* gsrc, uint32_t lds_base) {
-  asm volatile("global_load_lds_dword %0, off" ::"v"(gsrc), "{m0}"(lds_base) : "memory");
+// Copies from global memory into LDS, lane l's bytes at lds_base + 16 l (4 l), as copy16_to_lds of sta_device.h.  Inline
+// assembly is no memory instruction to the compiler, which keeps no distance between it and the instructions that
+// write its scalar operands: an address in scalar registers that a vector instruction (readfirstlane) wrote may be
+// read 5 wait states later at the earliest, M0 one.  So the copies wait for themselves.
+__device__ __forceinline__ void stage16(const void* sbase, uint32_t voff, uint32_t lds_base) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_base) : "memory");
+}
+__device__ __forceinline__ void stage16(const void* gsrc, uint32_t lds_base) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gsrc), "{m0}"(lds_base) : "memory");
+}
+__device__ __forceinline__ void stage4(const void* gsrc, uint32_t lds_base) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(gsrc), "{m0}"(lds_base) : "memory");
 }
 
 // Rows row0 .. row0 + KT - 1 of a sequence into a stage, this wave's share; rows from n on are zeros.  swz is linear over xor, so
@@ -116,7 +128,7 @@ struct Stager {
       const char* from = base + (row0 + first) * stride;
 #pragma unroll
       for (int y = 0; y < T::COPIES; ++y)
-        copy16_to_lds_s(from + (y * PER) * stride, row + (chunk ^ (uint32_t)((swz<T>(first) ^ swz<T>(y * PER)) * 16)), lds + y * 1024);
+        stage16(from + (y * PER) * stride, row + (chunk ^ (uint32_t)((swz<T>(first) ^ swz<T>(y * PER)) * 16)), lds + y * 1024);
     } else {
       asm volatile("" ::: "memory");
       const int lane = threadIdx.x & 63;
@@ -124,7 +136,7 @@ struct Stager {
       for (int y = 0; y < T::COPIES; ++y) {
         const int r = first + y * PER + lane / T::CH;
         const char* p = row0 + r < n ? base + (row0 + r) * stride : (const char*)zero_row;
-        copy16_to_lds(p + ((lane % T::CH) ^ swz<T>(r)) * 16, lds + y * 1024);
+        stage16(p + ((lane % T::CH) ^ swz<T>(r)) * 16, lds + y * 1024);
       }
     }
   }
@@ -152,19 +164,29 @@ __device__ __forceinline__ Places places_of() {
 
 // scores: 32 rows of a stage from row0 (operand A) times the wave's 32 rows in registers (operand B).  Slot i of lane l is
 // stage row row0 + 8 (i / 4) + 4 (l / 32) + i % 4, own row l % 32.
-// own(c, d): 32 bytes d of the own rows of tile c.
+// own(d): 32 bytes d of the own rows.
 template <int DT, typename T, typename Own>
-__device__ __forceinline__ void rows_product(lds_bytes lds, const Places& at, int row0, Own own, floatx16 (&x)[T::COLS]) {
+__device__ __forceinline__ floatx16 rows_product(lds_bytes lds, const Places& at, int row0, Own own) {
+  floatx16 x;
 #pragma unroll
-  for (int c = 0; c < T::COLS; ++c)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[c][i] = 0.f;
+  for (int i = 0; i < 16; ++i) x[i] = 0.f;
 #pragma unroll
   for (int d = 0; d < T::KD; ++d) {
     const u32x4 w = *(const __attribute__((address_space(3))) u32x4*)(lds + (at.row ^ (uint32_t)(d * 32)) + row0 * T::RB);
-#pragma unroll
-    for (int c = 0; c < T::COLS; ++c) x[c] = mma<DT>(w, own(c, d), x[c]);
+    x = mma<DT>(w, own(d), x);
   }
+  return x;
+}
+
+// Waits until x, the last product's result, may be read (8 passes of 16-bit types 11 wait states, 16 of fp32 18).  The
+// compiler keeps that distance itself, but where the way from a product to the first reader forks and joins again it has
+// counted the longer branch and read the last registers too early: so x settles before a branch.
+template <int DT>
+__device__ __forceinline__ void settle(floatx16& x) {
+  float last = x[15];
+  if constexpr (DT == DT_F32) asm volatile("s_nop 15\n\ts_nop 1" : "+v"(last));
+  else asm volatile("s_nop 10" : "+v"(last));
+  x[15] = last;
 }
 
 // what rows_product leaves, as operand B of the product over the stage's 32 rows: for 16 bits rounded to them
@@ -198,8 +220,8 @@ struct Weights<DT_F32> {
 
 // acc (dims x own rows) += (32 rows of a stage from row0)^T x weights
 template <int DT, typename T>
-__device__ __forceinline__ void transposed_product(lds_bytes lds, const Places& at, int row0, const Weights<DT> (&p)[T::COLS],
-                                                   floatx16 (&acc)[T::COLS][T::DB]) {
+__device__ __forceinline__ void transposed_product(lds_bytes lds, const Places& at, int row0, const Weights<DT>& p,
+                                                   floatx16 (&acc)[T::DB]) {
   if constexpr (DT == DT_F32) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -209,8 +231,7 @@ __device__ __forceinline__ void transposed_product(lds_bytes lds, const Places& 
       for (int b = 0; b < T::DB; ++b) {
         const uint32_t x = at.column ^ (uint32_t)(b * 128) ^ (uint32_t)(swz<T>(r) * 16);
         const float w = *(const __attribute__((address_space(3))) float*)(lds + x + (row0 + r) * RB);
-#pragma unroll
-        for (int c = 0; c < T::COLS; ++c) acc[c][b] = __builtin_amdgcn_mfma_f32_32x32x2f32(w, p[c].w[i], acc[c][b], 0, 0, 0);
+        acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(w, p.w[i], acc[b], 0, 0, 0);
       }
     }
   } else {
@@ -227,8 +248,7 @@ __device__ __forceinline__ void transposed_product(lds_bytes lds, const Places& 
           const u32x2 v = __builtin_bit_cast(u32x2, w);
           a[2 * y] = v[0], a[2 * y + 1] = v[1];
         }
-#pragma unroll
-        for (int c = 0; c < T::COLS; ++c) acc[c][b] = mma<DT>(a, p[c].w[s], acc[c][b]);
+        acc[b] = mma<DT>(a, p.w[s], acc[b]);
       }
   }
 }
@@ -291,6 +311,7 @@ __device__ __forceinline__ void store_rows(char* row, const floatx16 (&acc)[T::D
 struct Span {
   int at, n;                               // first row among the packed ones, rows
 };
+__device__ __forceinline__ Span uniform(Span s) { return Span{uniform(s.at), uniform(s.n)}; }
 __device__ __forceinline__ Span span_of(const int32_t* starts, int b, int total) {
   if (!starts) return Span{0, total};
   const int s = min(max(starts[b], 0), total);
@@ -317,9 +338,9 @@ __device__ __forceinline__ int find_entry(int entries, int at, Count count, Othe
     const unsigned long long hit = __ballot(base + incl > at);
     if (hit) {
       const int first = uniform(__ffsll(hit) - 1);
-      base += __builtin_amdgcn_readlane(incl, first) - __builtin_amdgcn_readlane(n, first);
-      before += __builtin_amdgcn_readlane(oincl, first) - __builtin_amdgcn_readlane(o, first);
-      return e0 + first;
+      base = uniform(base + __builtin_amdgcn_readlane(incl, first) - __builtin_amdgcn_readlane(n, first));
+      before = uniform(before + __builtin_amdgcn_readlane(oincl, first) - __builtin_amdgcn_readlane(o, first));
+      return uniform(e0 + first);
     }
     base += __builtin_amdgcn_readlane(incl, 63);
     before += __builtin_amdgcn_readlane(oincl, 63);

@@ -1,7 +1,7 @@
 // sta_window.hip -- the forward pass of attention with a sliding window and sinks (sta_window.h).
 //
-// A workgroup takes 128 rows of one head, a wave 32 of them, and walks the keys that they see in stages of 64 (fp32: 32)
-// through two LDS buffers, the next one copied while this one is worked on.
+// A workgroup takes 128 rows of one head (32 where there are few), a wave 32 of them, and walks the
+// keys that they see in stages of 64 (fp32 and one wave: 32) through two LDS buffers, the next one copied while this one is worked on.
 //
 //   S^T = K Q^T     K rows of the stage as operand A, the wave's Q rows in registers as B; the result holds
 //                   row l % 32, keys 8 (i / 4) + 4 (l / 32) + i % 4 in slot i of lane l
@@ -25,10 +25,10 @@ using namespace window;
 // erred by 1.5 times what rounding it costs, with the two parts by 1.4.  Nothing but short windows pays for it.
 constexpr int FEW = 256;
 
-template <int DT, int D>
-__global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_kernel(WindowArgs a) {
-  using T = Tile<DT, D>;
-  constexpr int KT = T::KT, SUB = T::SUB;
+template <int DT, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void window_kernel(WindowArgs a) {
+  using T = Tile<DT, D, WAVES>;
+  constexpr int KT = T::KT, SUB = T::SUB, ROWS = T::ROWS;
   __shared__ u32x4 lds[2][2][KT * T::CH];
   const int G = a.H / a.Hkv, lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), r = lane & 31, h4 = (lane >> 5) * 4;
   const int id = xcd_order(), hk = id / (a.q_tiles * G), rest = id - hk * (a.q_tiles * G);
@@ -39,26 +39,26 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_kernel(Windo
   const int e = find_entry(a.B + 2, tile_all, [&](int x) { return (entry_of(a.starts, x, a.B, a.T).n + ROWS - 1) / ROWS; },
                            [](int) { return 0; }, base, none);
   if (e < 0) return;
-  const Span sq = entry_of(a.starts, e, a.B, a.T);
+  const Span sq = uniform(entry_of(a.starts, e, a.B, a.T));
   const int row0 = (tile_all - base) * ROWS, row = row0 + wave * 32 + r;
   if (row0 < 0 || row0 >= sq.n) return;    // starts that do not ascend
   const bool real = row < sq.n;
   char* out = a.out + ((int64_t)(sq.at + row) * a.H + h) * T::RB;
   float* lse = a.lse + (int64_t)h * a.T + sq.at + row;
-  floatx16 acc[1][T::DB];
+  floatx16 acc[T::DB];
 #pragma unroll
   for (int b = 0; b < T::DB; ++b)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[0][b][i] = 0.f;
+    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
   if (e == 0 || e > a.B) {                 // rows of no sequence
     if (real) {
-      store_rows<DT, T>(out, acc[0], 0.f);
-      if (a.rest) store_rows<DT, T>(a.rest + (out - a.out), acc[0], 0.f);
+      store_rows<DT, T>(out, acc, 0.f);
+      if (a.rest) store_rows<DT, T>(a.rest + (out - a.out), acc, 0.f);
       if (lane < 32) *lse = -INFINITY;
     }
     return;
   }
-  const Span sk = span_of(a.k_starts, e - 1, a.S);
+  const Span sk = uniform(span_of(a.k_starts, e - 1, a.S));
   const int off = sk.n - sq.n, p0 = off + row0, pw = p0 + wave * 32;
   const bool idle = row0 + wave * 32 >= sq.n;
   const KeyRange keys = keys_of<KT>(a, p0, min(p0 + ROWS, sk.n) - 1);
@@ -66,9 +66,9 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_kernel(Windo
   const char* vb = a.v + sk.at * a.v_ts + hk * a.v_hs;
   const Row me = row_at(a, off + row);
 
-  u32x4 q[1][T::KD];
-  load_rows<T>(q[0], a.q + sq.at * a.q_ts + h * a.q_hs, a.q_ts, row, sq.n);
-  signed_rows<DT>(q[0], a.flip, a.keep);
+  u32x4 q[T::KD];
+  load_rows<T>(q, a.q + sq.at * a.q_ts + h * a.q_hs, a.q_ts, row, sq.n);
+  signed_rows<DT>(q, a.flip, a.keep);
   // P times 2^shift: an fp16 P below 2^-14 of 2^8 would lose bits
   constexpr float SHIFT = DT == DT_F16 ? 7.f : 0.f, RISE = 8.f;
   float m = -INFINITY, l = 0.f;
@@ -76,57 +76,59 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_kernel(Windo
   Stager<T> ks, vs;
   ks.set(a.k_ts);
   vs.set(a.v_ts);
-  auto fetch = [&](int t, int buf) {
+  auto fetch = [&](int t, int buf) STA_INLINE {
     ks.copy(lds[buf][0], kb, keys.at(t) * KT, sk.n);
     vs.copy(lds[buf][1], vb, keys.at(t) * KT, sk.n);
   };
   const bool few = keys.n * KT <= FEW;
   const int lo_first = max(pw, 0) - a.window + 1, lo_last = max(pw + 31, 0) - a.window + 1;
-  auto turn = [&](int t, auto which) {
+  auto turn = [&](int t, auto which) STA_INLINE {
     constexpr int BUF = decltype(which)::value;
     next_stage();
     if (t + 1 < keys.n) fetch(t + 1, 1 - BUF);
     const int k0 = keys.at(t) * KT, k1 = k0 + KT - 1;
     if (idle || k0 > pw + 31 || (k1 < lo_first && k0 >= a.sinks)) return;
     const lds_bytes kt = (lds_bytes)&lds[BUF][0][0], vt = (lds_bytes)&lds[BUF][1][0];
-    floatx16 s[SUB][1];
+    floatx16 s[SUB];
 #pragma unroll
-    for (int y = 0; y < SUB; ++y) rows_product<DT, T>(kt, at, y * 32, [&](int c, int d) { return q[c][d]; }, s[y]);
+    for (int y = 0; y < SUB; ++y) s[y] = rows_product<DT, T>(kt, at, y * 32, [&](int d) { return q[d]; });
+#pragma unroll
+    for (int y = 0; y < SUB; ++y) settle<DT>(s[y]);
     if (!(k1 <= pw && (k0 >= lo_last || k1 < a.sinks))) {
       const int key = rarely(k0 + h4);
 #pragma unroll
       for (int y = 0; y < SUB; ++y)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (!me.sees(key + y * 32 + 8 * (i / 4) + i % 4)) s[y][0][i] = -INFINITY;
+          if (!me.sees(key + y * 32 + 8 * (i / 4) + i % 4)) s[y][i] = -INFINITY;
     }
-    float top = s[0][0][0];
+    float top = s[0][0];
 #pragma unroll
     for (int y = 0; y < SUB; ++y)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[y][0][i]);
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[y][i]);
     top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
     if (__any(top > m + RISE)) {
       const float m1 = fmaxf(m, top), f = exp2_of(m - at_least(m1));
       m = m1;
       l *= f;
 #pragma unroll
-      for (int b = 0; b < T::DB; ++b) acc[0][b] *= f;
+      for (int b = 0; b < T::DB; ++b) acc[b] *= f;
     }
     const float m0 = at_least(m) - SHIFT;
 #pragma unroll
     for (int y = 0; y < SUB; ++y) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[y][0][i] = exp2_of(fmaf(s[y][0][i], a.c, -m0));
-        l += s[y][0][i];
+        s[y][i] = exp2_of(fmaf(s[y][i], a.c, -m0));
+        l += s[y][i];
       }
-      Weights<DT> p[1];
-      p[0].set(s[y][0]);
+      Weights<DT> p;
+      p.set(s[y]);
       transposed_product<DT, T>(vt, at, y * 32, p, acc);
       if constexpr (DT != DT_F32) {
         if (few) {
-          p[0].rest(s[y][0]);
+          p.rest(s[y]);
           transposed_product<DT, T>(vt, at, y * 32, p, acc);
         }
       }
@@ -140,9 +142,9 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_kernel(Windo
   l += __shfl_xor(l, 32, 64);
   if (!real) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  store_rows<DT, T>(out, acc[0], inv);
+  store_rows<DT, T>(out, acc, inv);
   if constexpr (DT != DT_F32) {
-    if (a.rest) store_rests<DT, T>(a.rest + (out - a.out), acc[0], inv);
+    if (a.rest) store_rests<DT, T>(a.rest + (out - a.out), acc, inv);
   }
   if (lane < 32) *lse = l == 0.f ? -INFINITY : (at_least(m) - SHIFT + log2f(l)) * 0.693147180559945309f;
 }
@@ -150,7 +152,8 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_kernel(Windo
 template <int DT, int D>
 hipError_t launch_dt(const WindowArgs& a, hipStream_t st) {
   const unsigned grid = ((unsigned)a.q_tiles * a.H + 7) / 8 * 8;
-  window_kernel<DT, D><<<grid, 256, 0, st>>>(a);
+  if (a.q_waves == 1) window_kernel<DT, D, 1><<<grid, 64, 0, st>>>(a);
+  else window_kernel<DT, D, 4><<<grid, 256, 0, st>>>(a);
   return hipGetLastError();
 }
 

@@ -40,12 +40,15 @@ __device__ __forceinline__ float ds_scale(const WindowArgs& a, float* shared) {
   return __uint_as_float((uint32_t)uniform((127 + min(max(13 - ilogbf(most), -100), 100)) << 23));
 }
 
+// every row of a sequence of n keys sees one key
+__device__ __forceinline__ bool only_own(const WindowArgs& a, int n) { return n == 1 || (a.window == 1 && a.sinks == 0); }
+
 // delta and the base-2 log of the sum, +inf for rows that see nothing (their p is 0 then); CH lanes a row.  delta of the rounded
 // out would be off by about what rounding a ds costs: with what that rounding left (rest) dq and dk err 1.41 times what
 // rounding them costs, without it 1.5 (bf16) to 1.6 times (fp16).
 template <int DT, int D>
 __global__ __launch_bounds__(256) void window_delta_kernel(WindowArgs a) {
-  using T = Tile<DT, D>;
+  using T = Tile<DT, D, 4>;
   constexpr int V = 16 / T::E, PER = 256 / T::CH;
   __shared__ float most[2][4];
   const int c = threadIdx.x % T::CH, mine = threadIdx.x / T::CH;
@@ -117,10 +120,10 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WindowArgs a) {
 // ------------------------------------------------------------------------------------------
 // dq: the forward pass' walk
 // ------------------------------------------------------------------------------------------
-template <int DT, int D>
-__global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dq_kernel(WindowArgs a) {
-  using T = Tile<DT, D>;
-  constexpr int KT = T::KT, SUB = T::SUB;
+template <int DT, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void window_dq_kernel(WindowArgs a) {
+  using T = Tile<DT, D, WAVES>;
+  constexpr int KT = T::KT, SUB = T::SUB, ROWS = T::ROWS;
   __shared__ u32x4 lds[2][2][KT * T::CH];
   __shared__ float shared[8];
   const int G = a.H / a.Hkv, lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), r = lane & 31, h4 = (lane >> 5) * 4;
@@ -131,21 +134,21 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dq_kernel(Wi
   const int e = find_entry(a.B + 2, tile_all, [&](int x) { return (entry_of(a.starts, x, a.B, a.T).n + ROWS - 1) / ROWS; },
                            [](int) { return 0; }, base, none);
   if (e < 0) return;
-  const Span sq = entry_of(a.starts, e, a.B, a.T);
+  const Span sq = uniform(entry_of(a.starts, e, a.B, a.T));
   const int row0 = (tile_all - base) * ROWS, row = row0 + wave * 32 + r;
   if (row0 < 0 || row0 >= sq.n) return;    // starts that do not ascend
   const bool real = row < sq.n;
   char* dq = a.dq + ((int64_t)(sq.at + row) * a.H + h) * T::RB;
-  floatx16 acc[1][T::DB];
+  floatx16 acc[T::DB];
 #pragma unroll
   for (int b = 0; b < T::DB; ++b)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[0][b][i] = 0.f;
+    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
   if (e == 0 || e > a.B) {
-    if (real) store_rows<DT, T>(dq, acc[0], 0.f);
+    if (real) store_rows<DT, T>(dq, acc, 0.f);
     return;
   }
-  const Span sk = span_of(a.k_starts, e - 1, a.S);
+  const Span sk = uniform(span_of(a.k_starts, e - 1, a.S));
   const int off = sk.n - sq.n, p0 = off + row0, pw = p0 + wave * 32;
   const bool idle = row0 + wave * 32 >= sq.n;
   const KeyRange keys = keys_of<KT>(a, p0, min(p0 + ROWS, sk.n) - 1);
@@ -154,22 +157,22 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dq_kernel(Wi
   const Row me = row_at(a, off + row);
   const float grow = DT == DT_F16 ? ds_scale(a, shared) : 1.f;
 
-  u32x4 q[1][T::KD], dout[1][T::KD];
-  load_rows<T>(q[0], a.q + sq.at * a.q_ts + h * a.q_hs, a.q_ts, row, sq.n);
-  signed_rows<DT>(q[0], a.flip, a.keep);
-  load_rows<T>(dout[0], a.dout + sq.at * a.do_ts + h * a.do_hs, a.do_ts, row, sq.n);
+  u32x4 q[T::KD], dout[T::KD];
+  load_rows<T>(q, a.q + sq.at * a.q_ts + h * a.q_hs, a.q_ts, row, sq.n);
+  signed_rows<DT>(q, a.flip, a.keep);
+  load_rows<T>(dout, a.dout + sq.at * a.do_ts + h * a.do_hs, a.do_ts, row, sq.n);
   const int64_t stat = (int64_t)h * a.T + sq.at + min(row, sq.n - 1);
   const float lse = a.row_lse[stat], delta = a.row_delta[stat];
   const Places at = places_of<DT, T>();
   Stager<T> ks, vs;
   ks.set(a.k_ts);
   vs.set(a.v_ts);
-  auto fetch = [&](int t, int buf) {
+  auto fetch = [&](int t, int buf) STA_INLINE {
     ks.copy(lds[buf][0], kb, keys.at(t) * KT, sk.n);
     vs.copy(lds[buf][1], vb, keys.at(t) * KT, sk.n);
   };
   const int lo_first = max(pw, 0) - a.window + 1, lo_last = max(pw + 31, 0) - a.window + 1;
-  auto turn = [&](int t, auto which) {
+  auto turn = [&](int t, auto which) STA_INLINE {
     constexpr int BUF = decltype(which)::value;
     next_stage();
     if (t + 1 < keys.n) fetch(t + 1, 1 - BUF);
@@ -179,10 +182,8 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dq_kernel(Wi
     const lds_bytes kt = (lds_bytes)&lds[BUF][0][0], vt = (lds_bytes)&lds[BUF][1][0];
 #pragma unroll
     for (int y = 0; y < SUB; ++y) {
-      floatx16 s1[1], dp1[1];
-      rows_product<DT, T>(kt, at, y * 32, [&](int c, int d) { return q[c][d]; }, s1);
-      rows_product<DT, T>(vt, at, y * 32, [&](int c, int d) { return dout[c][d]; }, dp1);
-      floatx16 &s = s1[0], &dp = dp1[0];
+      floatx16 s = rows_product<DT, T>(kt, at, y * 32, [&](int d) { return q[d]; });
+      const floatx16 dp = rows_product<DT, T>(vt, at, y * 32, [&](int d) { return dout[d]; });
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float p = exp2_of(fmaf(s[i], a.c, -lse));
@@ -194,8 +195,8 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dq_kernel(Wi
         for (int i = 0; i < 16; ++i)
           if (!me.sees(key + 8 * (i / 4) + i % 4)) s[i] = 0.f;
       }
-      Weights<DT> ds[1];
-      ds[0].set(s);
+      Weights<DT> ds;
+      ds.set(s);
       transposed_product<DT, T>(kt, at, y * 32, ds, acc);
     }
   };
@@ -204,7 +205,8 @@ __global__ __launch_bounds__(256, DT == DT_F32 ? 1 : 2) void window_dq_kernel(Wi
     turn(t, std::integral_constant<int, 0>());
     if (t + 1 < keys.n) turn(t + 1, std::integral_constant<int, 1>());
   }
-  if (real) store_rows<DT, T>(dq, acc[0], a.scale / grow);
+  // a row that sees its own key alone has p 1 whatever q is: dp - delta, the same number summed in two ways, is 0
+  if (real) store_rows<DT, T>(dq, acc, me.p == 0 || only_own(a, sk.n) ? 0.f : a.scale / grow);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -220,8 +222,9 @@ struct Cut {
     return (near > 1 ? (tiles - sink_tiles) * near : 0) + (far > 1 ? sink_tiles * far : 0);
   }
 };
-template <int KT>
+template <typename T>
 __device__ __forceinline__ Cut cut_of(const WindowArgs& a, int e) {
+  constexpr int KT = T::KT, ROWS = T::ROWS;
   const Span sk = entry_of(a.k_starts, e, a.B, a.S);
   Cut c{(sk.n + ROWS - 1) / ROWS, 0, 1, 1};
   if (e == 0 || e > a.B) return c;
@@ -236,14 +239,14 @@ struct Item {
   int entry, tile, part, parts;
   int64_t record;
 };
-template <int KT>
+template <typename T>
 __device__ __forceinline__ Item item_of(const WindowArgs& a, int at, bool by_tile, int64_t records) {
   int base, before;
   Item it;
-  it.entry = find_entry(a.B + 2, at, [&](int x) { const Cut c = cut_of<KT>(a, x); return by_tile ? c.tiles : c.items(); },
-                        [&](int x) { return cut_of<KT>(a, x).records(); }, base, before);
+  it.entry = find_entry(a.B + 2, at, [&](int x) { const Cut c = cut_of<T>(a, x); return by_tile ? c.tiles : c.items(); },
+                        [&](int x) { return cut_of<T>(a, x).records(); }, base, before);
   if (it.entry < 0) return it;
-  const Cut c = cut_of<KT>(a, it.entry);
+  const Cut c = cut_of<T>(a, it.entry);
   int x = at - base;
   if (by_tile) {
     it.tile = x;
@@ -262,44 +265,43 @@ __device__ __forceinline__ Item item_of(const WindowArgs& a, int at, bool by_til
   it.record = it.parts == 1 ? -1 : before + (sink ? (int64_t)it.tile * c.far
                                                   : (int64_t)(c.far > 1 ? c.sink_tiles * c.far : 0) + (int64_t)(it.tile - c.sink_tiles) * c.near);
   if (it.record + it.parts > records || it.record < -1) it.entry = -1;
+  it.entry = uniform(it.entry);
+  it.tile = uniform(it.tile);
+  it.part = uniform(it.part);
+  it.parts = uniform(it.parts);
   return it;
 }
 
-template <int DT, int D, int COLS>
-__global__ __launch_bounds__((Tile<DT, D, COLS>::THREADS), (COLS == 2 || DT == DT_F32 ? 1 : 2)) void window_dkv_kernel(WindowArgs a, int64_t records) {
-  using T = Tile<DT, D, COLS>;
-  constexpr int KT = T::KT, SUB = T::SUB;
+template <int DT, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void window_dkv_kernel(WindowArgs a, int64_t records) {
+  using T = Tile<DT, D, WAVES>;
+  constexpr int KT = T::KT, SUB = T::SUB, ROWS = T::ROWS;
   __shared__ u32x4 lds[2][2][KT * T::CH];
   __shared__ floatx4 stats[2][2][KT / 4];
   __shared__ float shared[8];
   // parts of v that the registers do not hold beside two sums of 128 dims
   constexpr int PARK = DT != DT_F32 && D == 128 ? 3 : 0;
-  __shared__ u32x4 parked[PARK ? T::WAVES * COLS * PARK : 1][64];
+  __shared__ u32x4 parked[PARK ? WAVES * PARK : 1][64];
   const int G = a.H / a.Hkv, lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
   const int id = xcd_order(), hk = id / a.items;
   if (hk >= a.Hkv) return;
-  const Item it = item_of<KT>(a, id - hk * a.items, false, records);
+  const Item it = item_of<T>(a, id - hk * a.items, false, records);
   if (it.entry < 0) return;
-  const Span sk = entry_of(a.k_starts, it.entry, a.B, a.S);
-  const int key0 = it.tile * ROWS, kw = key0 + wave * (32 * COLS), key = kw + r;
+  const Span sk = uniform(entry_of(a.k_starts, it.entry, a.B, a.S));
+  const int key0 = it.tile * ROWS, kw = key0 + wave * 32, key = kw + r;
   const int64_t at = (int64_t)(sk.at + key) * a.Hkv + hk;
-  floatx16 dk[COLS][T::DB], dv[COLS][T::DB];
+  floatx16 dk[T::DB], dv[T::DB];
 #pragma unroll
-  for (int c = 0; c < COLS; ++c)
+  for (int b = 0; b < T::DB; ++b)
 #pragma unroll
-    for (int b = 0; b < T::DB; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) dk[c][b][i] = dv[c][b][i] = 0.f;
-  auto store = [&](float dk_scale, float dv_scale) {
-#pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-      if (key + c * 32 >= sk.n) continue;
-      store_rows<DT, T>(a.dk + (at + c * 32 * a.Hkv) * T::RB, dk[c], dk_scale);
-      store_rows<DT, T>(a.dv + (at + c * 32 * a.Hkv) * T::RB, dv[c], dv_scale);
-    }
+    for (int i = 0; i < 16; ++i) dk[b][i] = dv[b][i] = 0.f;
+  auto store = [&](float dk_scale, float dv_scale) STA_INLINE {
+    if (key >= sk.n) return;
+    store_rows<DT, T>(a.dk + at * T::RB, dk, dk_scale);
+    store_rows<DT, T>(a.dv + at * T::RB, dv, dv_scale);
   };
   if (it.entry == 0 || it.entry > a.B) return store(0.f, 0.f);
-  const Span sq = span_of(a.starts, it.entry - 1, a.T);
+  const Span sq = uniform(span_of(a.starts, it.entry - 1, a.T));
   const int off = sk.n - sq.n;
   // the rows that see any of the tile's keys, in steps of KT
   const int key1 = min(key0 + ROWS, sk.n) - 1;
@@ -311,32 +313,30 @@ __global__ __launch_bounds__((Tile<DT, D, COLS>::THREADS), (COLS == 2 || DT == D
   const float grow = DT == DT_F16 ? ds_scale(a, shared) : 1.f;
   constexpr float SHIFT = DT == DT_F16 ? 15.f : 0.f;   // p times 2^15: fp16 keeps small ones
 
-  u32x4 k[COLS][T::KD], v[COLS][T::KD];
+  u32x4 k[T::KD], v[T::KD];
+  load_rows<T>(k, a.k + sk.at * a.k_ts + hk * a.k_hs, a.k_ts, key, sk.n);
+  signed_rows<DT>(k, a.flip, a.keep);
+  load_rows<T>(v, a.v + sk.at * a.v_ts + hk * a.v_hs, a.v_ts, key, sk.n);
 #pragma unroll
-  for (int c = 0; c < COLS; ++c) {
-    load_rows<T>(k[c], a.k + sk.at * a.k_ts + hk * a.k_hs, a.k_ts, key + c * 32, sk.n);
-    signed_rows<DT>(k[c], a.flip, a.keep);
-    load_rows<T>(v[c], a.v + sk.at * a.v_ts + hk * a.v_hs, a.v_ts, key + c * 32, sk.n);
-#pragma unroll
-    for (int d = 0; d < PARK; ++d) parked[(wave * COLS + c) * PARK + d][lane] = v[c][d];
-  }
+  for (int d = 0; d < PARK; ++d) parked[wave * PARK + d][lane] = v[d];
   Places place = places_of<DT, T>();
   Stager<T> qs, ds;
   qs.set(a.q_ts);
   ds.set(a.do_ts);
-  auto fetch = [&](int s, int buf) {
+  auto fetch = [&](int s, int buf) STA_INLINE {
     const int g = s / each, row0 = (first + s - g * each) * KT, head = hk * G + g;
     // the places' xors are formed anew every turn: kept over the loop they and parts of k or v would be spilled
     asm volatile("" : "+v"(place.row), "+v"(place.column), "+v"(qs.chunk));
     ds.chunk = qs.chunk;
     qs.copy(lds[buf][0], a.q + sq.at * a.q_ts + head * a.q_hs, row0, sq.n);
     ds.copy(lds[buf][1], a.dout + sq.at * a.do_ts + head * a.do_hs, row0, sq.n);
-    if (wave < 2 && lane < KT) {           // past the last row its own again
-      const float* from = (wave ? a.row_delta : a.row_lse) + (int64_t)head * a.T + sq.at + min(row0 + lane, sq.n - 1);
-      copy4_to_lds(from, uniform((int)lds_addr(&stats[buf][wave][0])));
+    if (lane < KT) {                       // past the last row its own again
+      const int64_t row = (int64_t)head * a.T + sq.at + min(row0 + lane, sq.n - 1);
+      if (wave == 0) stage4(a.row_lse + row, uniform((int)lds_addr(&stats[buf][0][0])));
+      if (wave == WAVES / 2) stage4(a.row_delta + row, uniform((int)lds_addr(&stats[buf][1][0])));
     }
   };
-  auto turn = [&](int s, auto which) {
+  auto turn = [&](int s, auto which) STA_INLINE {
     constexpr int BUF = decltype(which)::value;
     next_stage();
     if (s + 1 < s1) fetch(s + 1, 1 - BUF);
@@ -346,41 +346,33 @@ __global__ __launch_bounds__((Tile<DT, D, COLS>::THREADS), (COLS == 2 || DT == D
     for (int y = 0; y < SUB; ++y) {
       const int rw = row0 + y * 32, p0 = rw + off, p1 = p0 + 31;
       const int lo0 = max(p0, 0) - a.window + 1, lo1 = max(p1, 0) - a.window + 1;
-      constexpr int LAST = 32 * COLS - 1;
-      if (p1 < kw || (lo0 > kw + LAST && kw >= a.sinks)) continue;
-      floatx16 x[COLS], dp[COLS];
-      rows_product<DT, T>(qt, place, y * 32, [&](int c, int d) { return k[c][d]; }, x);
+      if (p1 < kw || (lo0 > kw + 31 && kw >= a.sinks)) continue;
+      floatx16 x = rows_product<DT, T>(qt, place, y * 32, [&](int d) { return k[d]; });
+      settle<DT>(x);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float lse = SHIFT - stats[BUF][0][y * 8 + 2 * (i / 4) + h][i % 4];
-#pragma unroll
-        for (int c = 0; c < COLS; ++c) x[c][i] = exp2_of(fmaf(x[c][i], a.c, lse));
+        x[i] = exp2_of(fmaf(x[i], a.c, lse));
       }
-      if (!(p0 >= kw + LAST && (lo1 <= kw || kw + LAST < a.sinks) && rw + 31 < sq.n)) {
+      if (!(p0 >= kw + 31 && (lo1 <= kw || kw + 31 < a.sinks) && rw + 31 < sq.n)) {
         const int row_h = rarely(rw + 4 * h);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int row = row_h + 8 * (i / 4) + i % 4;
-          const Row at_row = row_at(a, row + off);
-#pragma unroll
-          for (int c = 0; c < COLS; ++c)
-            if (!at_row.sees(key + c * 32) || row >= sq.n) x[c][i] = 0.f;
+          if (!row_at(a, row + off).sees(key) || row >= sq.n) x[i] = 0.f;
         }
       }
-      Weights<DT> p[COLS];
-#pragma unroll
-      for (int c = 0; c < COLS; ++c) p[c].set(x[c]);
+      Weights<DT> p;
+      p.set(x);
       transposed_product<DT, T>(dt, place, y * 32, p, dv);
-      rows_product<DT, T>(dt, place, y * 32, [&](int c, int d) { return d < PARK ? parked[(wave * COLS + c) * PARK + d][lane] : v[c][d]; }, dp);
+      const floatx16 dp = rows_product<DT, T>(dt, place, y * 32, [&](int d) { return d < PARK ? parked[wave * PARK + d][lane] : v[d]; });
       const float down = grow * (1.f / 32768.f);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float delta = stats[BUF][1][y * 8 + 2 * (i / 4) + h][i % 4];
-#pragma unroll
-        for (int c = 0; c < COLS; ++c) x[c][i] *= DT == DT_F16 ? (dp[c][i] - delta) * down : dp[c][i] - delta;
+        x[i] *= DT == DT_F16 ? (dp[i] - delta) * down : dp[i] - delta;
       }
-#pragma unroll
-      for (int c = 0; c < COLS; ++c) p[c].set(x[c]);
+      p.set(x);
       transposed_product<DT, T>(qt, place, y * 32, p, dk);
     }
   };
@@ -389,26 +381,24 @@ __global__ __launch_bounds__((Tile<DT, D, COLS>::THREADS), (COLS == 2 || DT == D
     turn(s, std::integral_constant<int, 0>());
     if (s + 1 < s1) turn(s + 1, std::integral_constant<int, 1>());
   }
-  const float dv_scale = DT == DT_F16 ? 1.f / 32768.f : 1.f, dk_scale = a.scale / grow;
+  const float dv_scale = DT == DT_F16 ? 1.f / 32768.f : 1.f, dk_scale = only_own(a, sk.n) ? 0.f : a.scale / grow;
   if (it.record >= 0) {
-    float* to = a.record + (hk * records + it.record + it.part) * (2 * ROWS * D) + (wave * 32 * COLS + r) * D;
-    using F = Tile<DT_F32, D>;
-#pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-      store_rows<DT_F32, F>((char*)(to + c * 32 * D), dk[c], dk_scale);
-      store_rows<DT_F32, F>((char*)(to + c * 32 * D + ROWS * D), dv[c], dv_scale);
-    }
+    float* to = a.record + (hk * records + it.record + it.part) * (2 * ROWS * D) + (wave * 32 + r) * D;
+    using F = Tile<DT_F32, D, WAVES>;
+    store_rows<DT_F32, F>((char*)to, dk, dk_scale);
+    store_rows<DT_F32, F>((char*)(to + ROWS * D), dv, dv_scale);
   } else {
     store(dk_scale, dv_scale);
   }
 }
 
 // the records of a tile, added in order; four dims a thread, dk and dv
-template <int DT, int D>
+template <int DT, int D, int WAVES>
 __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a, int64_t records) {
-  using T = Tile<DT, D>;
+  using T = Tile<DT, D, WAVES>;
+  constexpr int ROWS = T::ROWS;
   const int hk = blockIdx.y, tile_all = blockIdx.x / (ROWS * D / 1024), chunk = blockIdx.x % (ROWS * D / 1024);
-  const Item it = item_of<T::KT>(a, tile_all, true, records);
+  const Item it = item_of<T>(a, tile_all, true, records);
   if (it.entry < 0 || it.parts == 1) return;
   const Span sk = entry_of(a.k_starts, it.entry, a.B, a.S);
   const int word = chunk * 1024 + (int)threadIdx.x * 4, row = word / D, dim = word % D, key = it.tile * ROWS + row;
@@ -426,49 +416,66 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a, int64_t 
   }
 }
 
+template <int DT, int D, int WAVES>
+hipError_t launch_keys(const WindowArgs& a, int64_t records, hipStream_t st) {
+  window_dkv_kernel<DT, D, WAVES><<<((unsigned)a.items * a.Hkv + 7) / 8 * 8, 64 * WAVES, 0, st>>>(a, records);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !records) return e;
+  window_join_kernel<DT, D, WAVES><<<dim3((unsigned)a.k_tiles * (32 * WAVES * D / 1024), a.Hkv), 256, 0, st>>>(a, records);
+  return hipGetLastError();
+}
+
 template <int DT, int D>
 hipError_t launch_dt(const WindowArgs& a, int64_t records, hipStream_t st) {
   hipError_t e;
   window_delta_kernel<DT, D><<<a.norm_blocks, 256, 0, st>>>(a);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   if (a.q_tiles) {
-    window_dq_kernel<DT, D><<<((unsigned)a.q_tiles * a.H + 7) / 8 * 8, 256, 0, st>>>(a);
+    const unsigned grid = ((unsigned)a.q_tiles * a.H + 7) / 8 * 8;
+    if (a.q_waves == 1) window_dq_kernel<DT, D, 1><<<grid, 64, 0, st>>>(a);
+    else window_dq_kernel<DT, D, 4><<<grid, 256, 0, st>>>(a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (!a.items) return hipSuccess;
-  constexpr int COLS = 1;
-  window_dkv_kernel<DT, D, COLS><<<((unsigned)a.items * a.Hkv + 7) / 8 * 8, Tile<DT, D, COLS>::THREADS, 0, st>>>(a, records);
-  if ((e = hipGetLastError()) != hipSuccess || !records) return e;
-  window_join_kernel<DT, D><<<dim3((unsigned)a.k_tiles * (ROWS * D / 1024), a.Hkv), 256, 0, st>>>(a, records);
-  return hipGetLastError();
+  return a.k_waves == 1 ? launch_keys<DT, D, 1>(a, records, st) : launch_keys<DT, D, 4>(a, records, st);
 }
 
 }  // namespace
 
+// Up to so many workgroups of 128 rows (keys) a pass takes 32 each instead, one wave: 1000 tokens, 8 / 8 heads x 64, fp32, window
+// 100, 64 of them: forward 30 -> 23 us, dq 35 -> 27.
+constexpr int64_t FEW_TILES = 256;
+
 WindowCut window_cut(int dtype, int D, int T, int S, int H, int Hkv, int B, bool starts, bool k_starts, int window,
                      int sinks) {
   WindowCut c{};
-  const int64_t G = H / Hkv, kt = dtype == DT_F32 ? 32 : 64;
+  const int64_t G = H / Hkv;
+  // one wave a workgroup where four would leave CUs without work
+  c.q_waves = (T + (int64_t)127) / 128 * H < FEW_TILES ? 1 : 4;
+  c.k_waves = (S + (int64_t)127) / 128 * Hkv < FEW_TILES ? 1 : 4;
+  const int64_t q_rows = 32 * c.q_waves, ROWS = 32 * c.k_waves, kt = dtype == DT_F32 || c.k_waves == 1 ? 32 : 64;
   // an entry's last tile may be partly filled: those of B sequences and of the rows in front of and behind them
-  c.q_tiles = (int)((T + (int64_t)ROWS - 1) / ROWS + (starts ? B + 1 : 0));
-  c.k_tiles = (int)((S + (int64_t)ROWS - 1) / ROWS + (k_starts ? B + 1 : 0));
+  c.q_tiles = (int)((T + q_rows - 1) / q_rows + (starts ? B + 1 : 0));
+  c.k_tiles = (int)((S + ROWS - 1) / ROWS + (k_starts ? B + 1 : 0));
   const int64_t all = (T + kt - 1) / kt;                     // row steps of one sequence
-  // rows that see a key of a tile: of 128 + window - 1, from any place of a step on
+  // rows that see a key of a tile: of its keys + window - 1, from any place of a step on
   const int64_t near = ((int64_t)window + ROWS - 1 + 2 * (kt - 1)) / kt;
   const int64_t steps = near < all ? near : all;
   c.near_steps = (int)(steps < 1 ? 1 : steps);
-  // an item of all steps of a near tile, or where those are fewer than 512, so many that there are 512
-  const int64_t tiles = (S + (int64_t)ROWS - 1) / ROWS * Hkv;
+  // an item of all steps of a near tile, or where those are fewer than the chip holds workgroups, so few that there are
+  // as many items, down to what a record costs to be written and read
+  const int64_t tiles = (S + ROWS - 1) / ROWS * Hkv, items_wanted = c.k_waves == 1 ? 1024 : 512;
+  const int64_t fewest = dtype == DT_F32 ? 2 : 4;
   int64_t each = G * c.near_steps;
-  const int64_t even = (tiles * each + 511) / 512;
-  if (even < each) each = even < 8 ? 8 : even;
+  const int64_t even = (tiles * each + items_wanted - 1) / items_wanted;
+  if (even < each) each = even < fewest ? fewest : even;
   c.steps = (int)(each < INT32_MAX ? each : INT32_MAX);
   const int64_t near_parts = (G * c.near_steps + c.steps - 1) / c.steps;
   int64_t items = c.k_tiles * near_parts, records = near_parts > 1 ? items : 0;
   if (window != INT32_MAX && sinks > 0) {
     // of each tile with sinks: sum over the sequences of ceil(G ceil(rows / kt) / steps)
     const int64_t far = (G * (T / kt + (B < T ? B : T) + 1) + c.steps - 1) / c.steps + B;
-    const int64_t most = (S + (int64_t)ROWS - 1) / ROWS, of = ((int64_t)sinks + ROWS - 1) / ROWS;
+    const int64_t most = (S + ROWS - 1) / ROWS, of = (sinks + ROWS - 1) / ROWS;
     items += far * (of < most ? of : most);
     records += far * (of < most ? of : most);
   }

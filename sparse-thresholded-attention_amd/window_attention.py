@@ -17,6 +17,8 @@ allocator, and neither synchronise nor keep anything between calls, so a HIP gra
 training step calls window_attention_grad itself).  Gradients have one order of sums: a call repeated gives the same
 bits.  There is no fallback: a CPU tensor, an unsupported shape or a missing library raises.
 """
+import inspect
+
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
@@ -42,6 +44,10 @@ class _WindowAttention(torch.autograd.Function):
         *tensors, starts, k_starts = ctx.saved_tensors
         return (*native.window_attention_grad(dout, *tensors, *ctx.how, starts, k_starts, ctx.sm_scale),
                 None, None, None, None, None)
+
+
+# apply() asks for it in every call: formed anew it would take 20 us of them
+_WindowAttention.forward.__signature__ = inspect.signature(_WindowAttention.forward)
 
 
 def window_attention(q, k, v, window=None, sinks=0, starts=None, k_starts=None, sm_scale=None, want_lse=False,
