@@ -306,6 +306,80 @@ __device__ __forceinline__ void store_rows(char* row, const floatx16 (&acc)[T::D
 }
 
 // ------------------------------------------------------------------------------------------
+// Sums that are no finite numbers.  A product over a stage multiplies what a row does not see by a p of 0, and 0 times an
+// infinity or a NaN would reach it; sums of large values may also have passed the type's largest on the way.  A wave whose
+// sums end so forms them again, row by row, of what each of its rows sees.
+// ------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ bool not_finite(const floatx16 (&acc)[T::DB]) {
+  float zero = 0.f;                        // an infinity or a NaN times 0 is NaN
+#pragma unroll
+  for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) zero = fmaf(acc[b][i], 0.f, zero);
+  return __any(zero != 0.f);
+}
+
+// a row in memory, the same for the whole wave, times the lane's own (own(d): 32 bytes d of it)
+template <int DT, typename T, typename Own>
+__device__ __forceinline__ float row_dot(const char* row, Own own) {
+  const int h = (threadIdx.x & 63) >> 5;
+  float sum = 0.f;
+#pragma unroll
+  for (int d = 0; d < T::KD; ++d) {
+    const u32x4 x = *(const u32x4*)(row + (2 * d + h) * 16), y = own(d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (DT == DT_F32) {
+        sum = fmaf(__uint_as_float(x[e]), __uint_as_float(y[e]), sum);
+      } else if constexpr (DT == DT_BF16) {
+        sum = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16), sum);
+        sum = fmaf(__uint_as_float(x[e] & 0xffff0000u), __uint_as_float(y[e] & 0xffff0000u), sum);
+      } else {
+        sum = fmaf(f16_bits_to_f32(x[e] & 0xffffu), f16_bits_to_f32(y[e] & 0xffffu), sum);
+        sum = fmaf(f16_bits_to_f32(x[e] >> 16), f16_bits_to_f32(y[e] >> 16), sum);
+      }
+    }
+  }
+  return sum + __shfl_xor(sum, 32, 64);
+}
+
+// acc (dims x own rows) += weight x a row in memory, for lanes that see it
+template <int DT, typename T>
+__device__ __forceinline__ void add_row(floatx16 (&acc)[T::DB], const char* row, float weight, bool sees) {
+  const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int dim = b * 32 + s * 8 + h * 4;
+      float x[4];
+      if constexpr (DT == DT_F32) {
+        const float4 w = *(const float4*)(row + dim * 4);
+        x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+      } else {
+        const u32x2 w = *(const u32x2*)(row + dim * 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t bits = i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu;
+          x[i] = DT == DT_F16 ? f16_bits_to_f32(bits) : bf16_bits_to_f32(bits);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (sees) acc[b][4 * s + i] = fmaf(weight, x[i], acc[b][4 * s + i]);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void clear(floatx16 (&acc)[T::DB]) {
+#pragma unroll
+  for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+}
+
+// ------------------------------------------------------------------------------------------
 // sequences
 // ------------------------------------------------------------------------------------------
 struct Span {
@@ -316,6 +390,12 @@ __device__ __forceinline__ Span span_of(const int32_t* starts, int b, int total)
   if (!starts) return Span{0, total};
   const int s = min(max(starts[b], 0), total);
   return Span{s, max(min(starts[b + 1], total) - s, 0)};
+}
+// those of all sequences
+__device__ __forceinline__ Span all_of(const int32_t* starts, int B, int total) {
+  if (!starts) return Span{0, total};
+  const int s = min(max(starts[0], 0), total);
+  return Span{s, max(min(starts[B], total) - s, 0)};
 }
 // entry 0: the rows in front of the first sequence, 1 .. B: the sequences, B + 1: the rows behind the last
 __device__ __forceinline__ Span entry_of(const int32_t* starts, int e, int B, int total) {

@@ -46,10 +46,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   char* out = a.out + ((int64_t)(sq.at + row) * a.H + h) * T::RB;
   float* lse = a.lse + (int64_t)h * a.T + sq.at + row;
   floatx16 acc[T::DB];
-#pragma unroll
-  for (int b = 0; b < T::DB; ++b)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+  clear<T>(acc);
   if (e == 0 || e > a.B) {                 // rows of no sequence
     if (real) {
       store_rows<DT, T>(out, acc, 0.f);
@@ -139,9 +136,34 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
     turn(t, std::integral_constant<int, 0>());
     if (t + 1 < keys.n) turn(t + 1, std::integral_constant<int, 1>());
   }
+  float unit = 1.f;                        // of the sums
+  if (__builtin_expect(not_finite<T>(acc), 0)) {
+    // p so small that no sum of up to 2^28 values exceeds the largest of them
+    unit = 0x1p28f;
+    clear<T>(acc);
+    m = -INFINITY;
+    l = 0.f;
+    auto each_key = [&](auto f) STA_INLINE {
+      for (int t = 0; t < keys.n; ++t) {
+        const int k0 = keys.at(t) * KT, k1 = min(k0 + KT, sk.n);
+        for (int j = k0; j < k1; ++j) {
+          const float s = row_dot<DT, T>(kb + j * a.k_ts, [&](int d) { return q[d]; });
+          f(j, me.sees(j) ? s : -INFINITY);
+        }
+      }
+    };
+    each_key([&](int, float s) { m = fmaxf(m, s * a.c); });
+    const float m0 = at_least(m) - SHIFT;
+    each_key([&](int j, float s) {
+      const float p = exp2_of(fmaf(s, a.c, -m0));
+      l += p;
+      add_row<DT, T>(acc, vb + j * a.v_ts, p * 0x1p-28f, s != -INFINITY);
+    });
+    if (h4) l = 0.f;                       // both lanes of a row have all of it
+  }
   l += __shfl_xor(l, 32, 64);
   if (!real) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : unit / l;
   store_rows<DT, T>(out, acc, inv);
   if constexpr (DT != DT_F32) {
     if (a.rest) store_rests<DT, T>(a.rest + (out - a.out), acc, inv);

@@ -70,6 +70,13 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WindowArgs a) {
   };
   float do2 = 0.f, v2 = 0.f;
   const int64_t rows = (int64_t)a.T * a.H;
+  // the scale's: rows and keys of sequences, without those that hold an infinity or a NaN
+  auto square = [](float sq, int64_t t, const Span& s) { return t >= s.at && t < s.at + s.n && sq < INFINITY ? sq : 0.f; };
+  Span of_rows{0, 0}, of_keys{0, 0};
+  if constexpr (DT == DT_F16) {
+    of_rows = all_of(a.starts, a.B, a.T);
+    of_keys = all_of(a.k_starts, a.B, a.S);
+  }
   for (int64_t i = (int64_t)blockIdx.x * PER + mine; i < rows; i += (int64_t)gridDim.x * PER) {
     const int64_t t = i / a.H;
     const int h = (int)(i - t * a.H);
@@ -89,7 +96,7 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WindowArgs a) {
       sq = fmaf(y[e], y[e], sq);
     }
     dot = row_sum(dot);
-    if constexpr (DT == DT_F16) do2 = fmaxf(do2, row_sum(sq));
+    if constexpr (DT == DT_F16) do2 = fmaxf(do2, square(row_sum(sq), t, of_rows));
     if (c == 0) {
       const float lse = a.lse_in[h * (int64_t)a.T + t];
       a.row_lse[h * (int64_t)a.T + t] = lse == -INFINITY ? INFINITY : lse * 1.44269504088896340736f;
@@ -104,7 +111,7 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WindowArgs a) {
       elements(a.v + t * a.v_ts + (i - t * a.Hkv) * a.v_hs + c * 16, x);
 #pragma unroll
       for (int e = 0; e < V; ++e) sq = fmaf(x[e], x[e], sq);
-      v2 = fmaxf(v2, row_sum(sq));
+      v2 = fmaxf(v2, square(row_sum(sq), t, of_keys));
     }
     do2 = wave_max_f32(do2);
     v2 = wave_max_f32(v2);
@@ -140,10 +147,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   const bool real = row < sq.n;
   char* dq = a.dq + ((int64_t)(sq.at + row) * a.H + h) * T::RB;
   floatx16 acc[T::DB];
-#pragma unroll
-  for (int b = 0; b < T::DB; ++b)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+  clear<T>(acc);
   if (e == 0 || e > a.B) {
     if (real) store_rows<DT, T>(dq, acc, 0.f);
     return;
@@ -204,6 +208,17 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   for (int t = 0; t < keys.n; t += 2) {
     turn(t, std::integral_constant<int, 0>());
     if (t + 1 < keys.n) turn(t + 1, std::integral_constant<int, 1>());
+  }
+  if (__builtin_expect(not_finite<T>(acc), 0)) {
+    clear<T>(acc);
+    for (int t = 0; t < keys.n; ++t) {
+      const int k0 = keys.at(t) * KT, k1 = min(k0 + KT, sk.n);
+      for (int j = k0; j < k1; ++j) {
+        const float s = row_dot<DT, T>(kb + j * a.k_ts, [&](int d) { return q[d]; });
+        const float dp = row_dot<DT, T>(vb + j * a.v_ts, [&](int d) { return dout[d]; });
+        add_row<DT, T>(acc, kb + j * a.k_ts, exp2_of(fmaf(s, a.c, -lse)) * (dp - delta) * grow, me.sees(j));
+      }
+    }
   }
   // a row that sees its own key alone has p 1 whatever q is: dp - delta, the same number summed in two ways, is 0
   if (real) store_rows<DT, T>(dq, acc, me.p == 0 || only_own(a, sk.n) ? 0.f : a.scale / grow);
@@ -291,17 +306,18 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   const int key0 = it.tile * ROWS, kw = key0 + wave * 32, key = kw + r;
   const int64_t at = (int64_t)(sk.at + key) * a.Hkv + hk;
   floatx16 dk[T::DB], dv[T::DB];
-#pragma unroll
-  for (int b = 0; b < T::DB; ++b)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) dk[b][i] = dv[b][i] = 0.f;
+  clear<T>(dk);
+  clear<T>(dv);
   auto store = [&](float dk_scale, float dv_scale) STA_INLINE {
     if (key >= sk.n) return;
     store_rows<DT, T>(a.dk + at * T::RB, dk, dk_scale);
     store_rows<DT, T>(a.dv + at * T::RB, dv, dv_scale);
   };
   if (it.entry == 0 || it.entry > a.B) return store(0.f, 0.f);
-  const Span sq = uniform(span_of(a.starts, it.entry - 1, a.T));
+  // rows in front of the first key see nothing and are left out
+  Span sq = uniform(span_of(a.starts, it.entry - 1, a.T));
+  const int blind = max(sq.n - sk.n, 0);
+  sq = Span{sq.at + blind, sq.n - blind};
   const int off = sk.n - sq.n;
   // the rows that see any of the tile's keys, in steps of KT
   const int key1 = min(key0 + ROWS, sk.n) - 1;
@@ -380,6 +396,11 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   for (int s = s0; s < s1; s += 2) {
     turn(s, std::integral_constant<int, 0>());
     if (s + 1 < s1) turn(s + 1, std::integral_constant<int, 1>());
+  }
+  // a key in front of every window: its own k and v may hold anything
+  if (__builtin_expect(key <= off - a.window && key >= a.sinks, 0)) {
+    clear<T>(dk);
+    clear<T>(dv);
   }
   const float dv_scale = DT == DT_F16 ? 1.f / 32768.f : 1.f, dk_scale = only_own(a, sk.n) ? 0.f : a.scale / grow;
   if (it.record >= 0) {
