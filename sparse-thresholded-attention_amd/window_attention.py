@@ -54,7 +54,7 @@ def window_attention(q, k, v, window=None, sinks=0, starts=None, k_starts=None, 
                      want_rest=False):
     """Attention of q (T, H, D) over k, v (S, Hkv, D), H a multiple of Hkv, D 64 or 128, in one dtype of bf16, fp16
     and fp32; returns out like q, with want_lse also the log-sum-exp of the scaled scores (T, H) fp32, with want_rest
-also what rounding out to a 16-bit type left (None for fp32), both for window_attention_grad.
+    also what rounding out to a 16-bit type left (None for fp32), both for window_attention_grad and without gradients.
 
     starts (B + 1,) int32 or int64, ascending: sequence b has the rows starts[b] .. starts[b + 1] - 1 of q, and of k
     and v the rows k_starts[b] .. k_starts[b + 1] - 1 (default: starts, with S = T).  Without starts all rows are one
@@ -63,6 +63,8 @@ also what rounding out to a 16-bit type left (None for fp32), both for window_at
     with a score above -inf, gets zeros and -inf, and so do rows outside all sequences, which are not read.
     sm_scale: default D ** -0.5.  Scores, softmax and sums are fp32; 16-bit types round the probabilities (and
     the gradients of the scores) once to the type for the second product.
+    What a row does not see reaches neither its out nor its dq, infinities and NaN included; a row of q or of the
+    gradient that holds such makes dk and dv of its sequence's keys so, whether it sees them or not.
 
     Differentiable once, in q, k and v; forward-mode tangents are refused.  T and S up to 2^28."""
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in (q, k, v)):
