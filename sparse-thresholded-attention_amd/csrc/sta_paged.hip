@@ -606,15 +606,16 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, MergeLds<D, NT, 
   }
 }
 
+// block: the workgroup's number among those of these rows
 template <int DT, int D, int NT, bool ACC, bool MULTI, Form F>
-__global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_kernel(PagedArgs a, int tiles) {
+__device__ __forceinline__ void attend_runs(const PagedArgs& a, int tiles, unsigned block,
+                                            MergeLds<D, NT, Tile<DT, D, NT>::VE>& lds) {
   using T = Tile<DT, D, NT>;
-  __shared__ MergeLds<D, NT, T::VE> lds;
   const CacheView& c = a.c;
   // workgroups go to the XCDs in turn: the row tiles of a run are 8 apart, on one XCD, and find each other's keys in
   // its L2 (16 queries of 32 heads over 8 kv heads x 128, bf16, 8 sequences up to 8192 keys: 58 -> 50 us)
-  const int x = blockIdx.x / 8, tile = tiles == 1 ? 0 : x % tiles;
-  const int run = tiles == 1 ? blockIdx.x : x / tiles * 8 + blockIdx.x % 8;
+  const int x = block / 8, tile = tiles == 1 ? 0 : x % tiles;
+  const int run = tiles == 1 ? block : x / tiles * 8 + block % 8;
   const int64_t each = units_each<F>(a, T::UNIT);
   const int64_t run0 = run * each, run1 = run0 + each;
   int64_t base = 0;
@@ -640,24 +641,35 @@ __global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_ke
   }
 }
 
+template <int DT, int D, int NT, bool ACC, bool MULTI, Form F>
+__global__ __launch_bounds__(256, (Tile<DT, D, NT>::WAVES)) void paged_attend_kernel(PagedArgs a, int tiles) {
+  __shared__ MergeLds<D, NT, Tile<DT, D, NT>::VE> lds;
+  attend_runs<DT, D, NT, ACC, MULTI, F>(a, tiles, blockIdx.x, lds);
+}
+
 // Many rows a kv head (PagedCut::many): 128 of them a workgroup, 32 a wave, over the same keys.  A turn's 32 keys and
 // values go to LDS by asynchronous copies, two turns ahead in three buffers, each wave fetching 8 keys whose page is
 // uniform; a row's 16-byte chunks lie permuted by its number, so that the reads of 16 rows' equal chunks and of one row's
 // chunks both spread over the banks.  Against 32 rows a workgroup, whose waves read the keys for themselves (32 queries of
 // 32 heads over 8 kv heads x 128, 4 sequences up to 12288 keys): 51 -> 42 us.
+template <int D>
+struct ManyLds {
+  u32x4 staged[2][3][32 * (D / 8)];
+  int again;
+};
 template <int DT, int D, Form F>
-__global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int tiles) {
+__device__ __forceinline__ void many_runs(const PagedArgs& a, int tiles, unsigned block, ManyLds<D>& lds) {
   using T = Tile<DT, D, 2>;
   constexpr int NT = 2, KS = T::KS, VE = T::VE, VW = T::VW, ROWS = Tile<DT, D, 8>::ROWS;
   constexpr int CH = T::RB / 16, PER = 64 / CH, COPIES = 8 / PER;    // chunks of a row, rows of a copy, copies of 8 rows
-  __shared__ u32x4 staged[2][3][32 * CH];
-  __shared__ int again;
+  auto& staged = lds.staged;
+  int& again = lds.again;
   u32x4 (&keys)[3][32 * CH] = staged[0], (&values)[3][32 * CH] = staged[1];
   const CacheView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, g4 = lane >> 4;
   const int G = a.H / c.Hkv, R = G * a.Q;
-  const int x = blockIdx.x / 8, tile = tiles == 1 ? 0 : x % tiles;
-  const int run = tiles == 1 ? blockIdx.x : x / tiles * 8 + blockIdx.x % 8;
+  const int x = block / 8, tile = tiles == 1 ? 0 : x % tiles;
+  const int run = tiles == 1 ? block : x / tiles * 8 + block % 8;
   const int64_t each = units_each<F>(a, T::UNIT);
   const int64_t run0 = run * each, run1 = run0 + each;
   int64_t base = 0;
@@ -833,6 +845,42 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int til
     at = first + u1;
     ++hk;
   }
+}
+
+template <int DT, int D, Form F>
+__global__ __launch_bounds__(256, 2) void paged_many_kernel(PagedArgs a, int tiles) {
+  __shared__ ManyLds<D> lds;
+  many_runs<DT, D, F>(a, tiles, blockIdx.x, lds);
+}
+
+// Both passes of a call behind a prefix: the prefix's keys for the rows of all sequences (p), and behind those workgroups
+// each sequence's own (a), which fill what the first leave free.  NT 8: 128 rows a workgroup.  In launches of their own:
+// 64 sequences of 32 heads over 8 kv heads x 128, bf16, a prefix of 16384 keys, up to 1024 own: 49 + 17 -> 62 us; 12
+// sequences of 4 queries, 40 heads over 8 x 64, 2000 and up to 500 keys: 14 + 7 -> 15 us; 8 sequences, 16 heads over 8 x
+// 128, fp16, 131072 and up to 300 keys: 96 + 7 -> 98 us (541 MB, 5.5 TB/s).  Eights of either pass in turn instead: 88 us
+// in the first case, whose prefix fills the chip once.
+template <int DT, int D, int NT>
+struct RunLds {
+  using Type = MergeLds<D, NT, Tile<DT, D, NT>::VE>;
+};
+template <int DT, int D>
+struct RunLds<DT, D, 8> {
+  using Type = ManyLds<D>;
+};
+template <int DT, int D, int NT, Form F>
+__device__ __forceinline__ void runs(const PagedArgs& a, int tiles, unsigned block, typename RunLds<DT, D, NT>::Type& lds) {
+  if constexpr (NT == 8) many_runs<DT, D, F>(a, tiles, block, lds);
+  else attend_runs<DT, D, NT, false, true, F>(a, tiles, block, lds);
+}
+template <int DT, int D, int P_NT, int NT>
+__global__ __launch_bounds__(256, (P_NT == 8 ? 2 : Tile<DT, D, P_NT == 8 ? 2 : P_NT>::WAVES)) void
+prefix_attend_kernel(PagedArgs a, int tiles, PagedArgs p, int p_tiles, unsigned p_blocks) {
+  __shared__ union {
+    typename RunLds<DT, D, P_NT>::Type shared;
+    typename RunLds<DT, D, NT>::Type own;
+  } lds;
+  if (blockIdx.x < p_blocks) runs<DT, D, P_NT, SHARED>(p, p_tiles, blockIdx.x, lds.shared);
+  else runs<DT, D, NT, PLAIN>(a, tiles, blockIdx.x - p_blocks, lds.own);
 }
 
 // Calls whose sequences are all short: one launch.  A workgroup of 8 waves (16 where the registers allow) takes a kv
@@ -1036,12 +1084,29 @@ __device__ __forceinline__ void join_row(const PagedArgs& a, int tiles, const Pa
     for (int e = 0; e < W; ++e) y[e] += f * part[at * D + e];
   }
   if constexpr (BEHIND) {
-#pragma unroll 4
-    for (int x = 0; x < shared.n; ++x) {
-      const int64_t at = shared_record(x);
-      const float f = exp_of(p.part_ml[at].x - m0) * (p_scale / shared_scale);
+    // a record and its factor a lane, then 16 records' sums in flight: 64 records of 128 rows x 128 in 13.8 -> 12.4 us, 4.8 of
+    // them the launch; 32 of 2048 rows in 12, the sums' 33 MB at the copy rate
+    for (int x0 = 0; x0 < shared.n; x0 += 64) {
+      const int n = min(shared.n - x0, 64);
+      const int mine = (int)shared_record(x0 + min(lane, n - 1));
+      const float factor = exp_of(p.part_ml[mine].x - m0) * (p_scale / shared_scale);
+      for (int t = 0; t < n; t += 16) {
+        float w[16][W];
 #pragma unroll
-      for (int e = 0; e < W; ++e) y[e] += f * p.part_o[at * D + lane * W + e];
+        for (int u = 0; u < 16; ++u) {
+          const float* from = p.part_o + (int64_t)__builtin_amdgcn_readlane(mine, min(t + u, n - 1)) * D + lane * W;
+#pragma unroll
+          for (int e = 0; e < W; ++e) w[u][e] = from[e];
+        }
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(factor), min(t + u, n - 1)));
+          if (t + u < n) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) y[e] += f * w[u][e];
+          }
+        }
+      }
     }
   }
   l *= p_scale;
@@ -1363,26 +1428,28 @@ hipError_t launch_rows(const PagedArgs& a, const PagedCut& cut, hipStream_t st) 
   return a.Q == 1 ? launch_attend<DT, D, 1, false, F>(a, cut, st) : launch_attend<DT, D, 1, true, F>(a, cut, st);
 }
 
-// records of every row tile, for a join that adds others
-template <int DT, int D, Form F>
-hipError_t launch_records(const PagedArgs& a, const PagedCut& cut, hipStream_t st) {
-  if constexpr (DT != DT_F32) {
-    if (cut.many) {
-      paged_many_kernel<DT, D, F><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
-      return hipGetLastError();
-    }
-  }
-  if (cut.rows > 16) paged_attend_kernel<DT, D, 2, false, true, F><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
-  else paged_attend_kernel<DT, D, 1, false, true, F><<<cut.grid, 256, 0, st>>>(a, cut.tiles);
+// Behind a prefix that all sequences share: its keys once for the rows of all sequences, 128 or fewer of them a workgroup,
+// each sequence's own keys as in a call without one, and a join of both.
+template <int DT, int D, int P_NT, int NT>
+hipError_t launch_both(const PagedArgs& a, const PagedCut& cut, const PagedArgs& p, const PagedCut& p_cut, hipStream_t st) {
+  const unsigned p_blocks = (p_cut.grid + 7) / 8 * 8;       // a multiple of 8, so that the numbers behind it keep their XCDs
+  prefix_attend_kernel<DT, D, P_NT, NT><<<p_blocks + cut.grid, 256, 0, st>>>(a, cut.tiles, p, p_cut.tiles, p_blocks);
   return hipGetLastError();
 }
 
-// Behind a prefix that all sequences share: its keys once for the rows of all sequences, 128 or fewer of them a workgroup,
-// each sequence's own keys as in a call without one, and a join of both.
 template <int DT, int D>
 hipError_t launch_prefix_dt(const PagedArgs& a, const PagedCut& cut, const PagedArgs& p, const PagedCut& p_cut, hipStream_t st) {
-  hipError_t e = launch_records<DT, D, SHARED>(p, p_cut, st);
-  if (e == hipSuccess) e = launch_records<DT, D, PLAIN>(a, cut, st);
+  // the prefix's rows are those of all sequences, never fewer than a sequence's
+  hipError_t e;
+  if (p_cut.rows == 128 && DT != DT_F32) {
+    if (cut.rows == 128) e = launch_both<DT, D, DT == DT_F32 ? 2 : 8, DT == DT_F32 ? 2 : 8>(a, cut, p, p_cut, st);
+    else if (cut.rows > 16) e = launch_both<DT, D, DT == DT_F32 ? 2 : 8, 2>(a, cut, p, p_cut, st);
+    else e = launch_both<DT, D, DT == DT_F32 ? 2 : 8, 1>(a, cut, p, p_cut, st);
+  } else if (p_cut.rows > 16) {
+    e = cut.rows > 16 ? launch_both<DT, D, 2, 2>(a, cut, p, p_cut, st) : launch_both<DT, D, 2, 1>(a, cut, p, p_cut, st);
+  } else {
+    e = launch_both<DT, D, 1, 1>(a, cut, p, p_cut, st);
+  }
   if (e != hipSuccess) return e;
   const dim3 grid((a.H * a.Q + 3) / 4, a.c.B);
   if (cut.rows == 128) prefix_join_kernel<DT, D, 8><<<grid, 256, 0, st>>>(a, cut.tiles, p, p_cut.tiles, p_cut.rows);
