@@ -268,14 +268,16 @@ __device__ __forceinline__ float min_arg_for(float thr, float c) {
 // assembly so that the compiler does not track it as an LDS write: its own wait insertion would
 // otherwise drain every copy in flight (s_waitcnt vmcnt(0)) in front of the next LDS read and
 // serialise a multi-buffered copy pipeline.  Callers order the copies themselves with explicit
-// s_waitcnt vmcnt and barriers.
+// s_waitcnt vmcnt and barriers.  To the compiler inline assembly is no memory instruction either: it keeps no distance
+// between it and the scalar instruction that writes M0, which may be read one wait state later at the earliest, so
+// the copies wait for themselves.
 __device__ __forceinline__ void copy16_to_lds(const void* gsrc, uint32_t lds_base) {
-  asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(gsrc), "{m0}"(lds_base) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gsrc), "{m0}"(lds_base) : "memory");
 }
 // the same copy with a wave-uniform 64-bit base in SGPRs and a per-lane 32-bit byte offset (lane
 // l's 16 bytes from sbase + voff): one offset register serves every copy of a wave
 __device__ __forceinline__ void copy16_to_lds_s(const void* sbase, uint32_t voff, uint32_t lds_base) {
-  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_base) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_base) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
   return (uint32_t)(size_t)(const __attribute__((address_space(3))) void*)p;
