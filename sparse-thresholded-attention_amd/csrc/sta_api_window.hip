@@ -13,7 +13,8 @@ using namespace sta_api;
 
 namespace {
 
-int check_rows(const char* name, const void* p, int dtype, int64_t s0, int64_t s1) {
+// a copy's rows are 32-bit offsets from its first one, up to 7 token strides
+int check_rows(const char* name, const void* p, int dtype, int rows, int64_t s0, int64_t s1) {
   if (!p) return fail(STA_ERR_INVALID_ARG, "%s is NULL", name);
   if (!aligned16(p)) return fail(STA_ERR_UNSUPPORTED, "%s is not 16-byte aligned", name);
   const int64_t s[2] = {s0, s1};
@@ -21,6 +22,8 @@ int check_rows(const char* name, const void* p, int dtype, int64_t s0, int64_t s
     if (s[i] < 0 || s[i] > (INT64_MAX >> 36) || (s[i] * esize(dtype)) % 16 != 0)
       return fail(STA_ERR_UNSUPPORTED, "%s stride %lld is negative, too large or not 16-byte aligned", name,
                   (long long)s[i]);
+  if (rows > 1 && s0 * esize(dtype) > (1 << 29))
+    return fail(STA_ERR_UNSUPPORTED, "%s token stride %lld is above 2^29 bytes", name, (long long)s0);
   return STA_OK;
 }
 
@@ -67,14 +70,14 @@ int check_call(const sta_window_args* a) {
   int rc = check_shape(a);
   if (rc != STA_OK) return rc;
   if (a->T) {
-    if ((rc = check_rows("q", a->q, a->dtype, a->q_tok_stride, a->q_head_stride)) != STA_OK) return rc;
+    if ((rc = check_rows("q", a->q, a->dtype, a->T, a->q_tok_stride, a->q_head_stride)) != STA_OK) return rc;
     if ((rc = check_out("out", a->out)) != STA_OK) return rc;
     if (a->rest && !aligned16(a->rest)) return fail(STA_ERR_UNSUPPORTED, "rest is not 16-byte aligned");
     if (!a->lse) return fail(STA_ERR_INVALID_ARG, "lse must be non-NULL");
   }
   if (a->S) {
-    if ((rc = check_rows("k", a->k, a->dtype, a->k_tok_stride, a->k_head_stride)) != STA_OK) return rc;
-    if ((rc = check_rows("v", a->v, a->dtype, a->v_tok_stride, a->v_head_stride)) != STA_OK) return rc;
+    if ((rc = check_rows("k", a->k, a->dtype, a->S, a->k_tok_stride, a->k_head_stride)) != STA_OK) return rc;
+    if ((rc = check_rows("v", a->v, a->dtype, a->S, a->v_tok_stride, a->v_head_stride)) != STA_OK) return rc;
   }
   return STA_OK;
 }
@@ -164,7 +167,7 @@ int sta_window_attention_grad(const sta_window_grad_args* a, void* stream) {
   if (rc != STA_OK) return rc;
   const sta_window_args& f = a->fwd;
   if (f.T) {
-    if ((rc = check_rows("dout", a->dout, f.dtype, a->dout_tok_stride, a->dout_head_stride)) != STA_OK) return rc;
+    if ((rc = check_rows("dout", a->dout, f.dtype, f.T, a->dout_tok_stride, a->dout_head_stride)) != STA_OK) return rc;
     if ((rc = check_out("dq", a->dq)) != STA_OK) return rc;
   }
   if (f.S && ((rc = check_out("dk", a->dk)) != STA_OK || (rc = check_out("dv", a->dv)) != STA_OK)) return rc;

@@ -149,6 +149,17 @@ def test_window_attention_refuses_places_off_16_bytes():
         assert L.sta_window_attention_grad(ctypes.byref(a), None) == code, field
 
 
+def test_window_attention_refuses_token_strides_whose_copies_pass_32_bits():
+    import _sta_native as native
+    buf, p = _host()
+    for x in ("q", "k", "v", "dout"):
+        g = _window(native, p, True)
+        _set(g, x + "_tok_stride" if x == "dout" else f"fwd.{x}_tok_stride", (1 << 28) + 8)      # bf16: above 2^29 bytes
+        assert native.lib().sta_window_attention_grad(ctypes.byref(g), None) == -2, x
+        if x != "dout":
+            assert native.lib().sta_window_attention(ctypes.byref(g.fwd), None) == -2, x
+
+
 @pytest.mark.parametrize("field,value,code", [("dout", None, -1), ("dq", None, -1), ("dk", None, -1), ("dv", None, -1),
                                               ("dout_head_stride", 4, -2), ("workspace", None, -4),
                                               ("workspace_bytes", 1000, -4)])
