@@ -4,7 +4,8 @@
 //   out_i = sum_j p_ij v_j,  p_ij = exp(s_ij - m_i) / sum_j exp(s_ij - m_i),  s_ij = sm_scale q_i . k_j
 //
 // over the keys j < len - (Q - 1 - i) of the sequence whose page exists; weight_j += sum_i p_ij over
-// the rows i of the kv head.
+// the rows i of the kv head.  With a window, of those the keys j > len - Q + i - window and j < sinks; behind a prefix,
+// the prefix's keys and then those.
 #include "sta_cache.h"
 #include "sta_device.h"
 
