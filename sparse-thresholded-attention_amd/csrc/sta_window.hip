@@ -15,8 +15,8 @@
 //
 // Measured, products of the visible pairs alone: a prompt of 8192 tokens, 32 heads over 8 x 128, bf16, window 4096, 128 sinks:
 // 421 GFLOP in 436 us, 965 TFLOP/s, 79% of what a product of two 8192^2 matrices reaches; the same heads, 5 packed
-// sequences of together 8192, window 1024: 192 us, 540 TFLOP/s (short sequences and the two masked ends of each window weigh
-// more); 24 heads x 64, fp16, 6001 tokens in 3 sequences, causal: 119 us, 400 TFLOP/s (twice the exponentials a
+// sequences of together 8192, window 1024, for a backward pass: 206 us, 500 TFLOP/s (short sequences and the two masked ends of each window weigh
+// more); 24 heads x 64, fp16, 6001 tokens in 3 sequences, causal, likewise: 122 us, 390 TFLOP/s (twice the exponentials a
 // product).  Bound by the matrix cores beside LDS reads of as many cycles and
 // the exponentials: the cores are busy half of the time, LDS has no bank conflicts.  128 rows a workgroup: 64 rows a wave
 // would halve those reads, but not fit the registers at D 128.
@@ -28,10 +28,11 @@ namespace {
 
 using namespace window;
 
-// Up to so many keys of a workgroup the second product takes P in two parts.  The backward pass' delta inherits the error of
-// P, and beside ds' own rounding it weighs by the sum of p^2: 3 sequences of 2000 tokens, 24 heads x 64, fp16, causal, dq
-// erred by 1.5 times what rounding it costs, with the two parts by 1.4.  Nothing but short windows pays for it.
-constexpr int FEW = 256;
+// Up to so many keys of a workgroup the second product takes P in two parts; with a backward pass to come up to the second
+// number.  Its delta inherits the error of P, and beside ds' own rounding that weighs by the sum of p^2: 3 sequences of
+// 2000 tokens, 24 heads x 64, fp16, causal, dq erred by 1.48 to 1.51 times what rounding it costs with two parts up to 256 keys,
+// by 1.46 to 1.47 up to 1024 (114 -> 122 us; 5 of together 8192, 32 heads over 8 x 128, bf16, window 1024: 192 -> 206).
+constexpr int FEW = 256, FEW_TRAIN = 1024;
 
 template <int DT, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void window_kernel(WindowArgs a) {
@@ -85,7 +86,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
     ks.copy(lds[buf][0], kb, keys.at(t) * KT, sk.n);
     vs.copy(lds[buf][1], vb, keys.at(t) * KT, sk.n);
   };
-  const bool few = keys.n * KT <= FEW;
+  const bool few = keys.n * KT <= (a.rest ? FEW_TRAIN : FEW);
   const int lo_first = max(pw, 0) - a.window + 1, lo_last = max(pw + 31, 0) - a.window + 1;
   auto turn = [&](int t, auto which) STA_INLINE {
     constexpr int BUF = decltype(which)::value;
