@@ -172,6 +172,15 @@ __device__ __forceinline__ floatx16 mfma32_f16(const u32x4& a, const u32x4& b, f
                                                 __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// Waits until x, the result of one of these products (8 passes: 12 wait states), may be read or its registers written
+// again.  The compiler keeps that distance itself, but where the way from a product to the first reader forks and joins
+// again it has counted the longer branch: so x settles before such a branch.
+__device__ __forceinline__ void settle_mfma32(floatx16& x) {
+  float last = x[15];
+  asm volatile("s_nop 11" : "+v"(last));
+  x[15] = last;
+}
+
 __device__ __forceinline__ floatx4 mfma16(const u32x4& a, const u32x4& b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);

@@ -1359,6 +1359,11 @@ void score_kernel(ScoreArgs a) {
       }
       chunk_end(c);
     }
+    // a single chunk comes here past branches alone
+    if constexpr (FUSED) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) settle_mfma32(accB[rb]);
+    }
     if (active && pendingB) flush(passc, accB, keyB);
   };
   if constexpr (MODE == 1) {

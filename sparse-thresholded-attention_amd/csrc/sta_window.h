@@ -178,15 +178,16 @@ __device__ __forceinline__ floatx16 rows_product(lds_bytes lds, const Places& at
   return x;
 }
 
-// Waits until x, the last product's result, may be read (8 passes of 16-bit types 11 wait states, 16 of fp32 18).  The
-// compiler keeps that distance itself, but where the way from a product to the first reader forks and joins again it has
-// counted the longer branch and read the last registers too early: so x settles before a branch.
+// settle_mfma32 of sta_device.h; the fp32 products take 16 passes, 18 wait states
 template <int DT>
 __device__ __forceinline__ void settle(floatx16& x) {
-  float last = x[15];
-  if constexpr (DT == DT_F32) asm volatile("s_nop 15\n\ts_nop 1" : "+v"(last));
-  else asm volatile("s_nop 10" : "+v"(last));
-  x[15] = last;
+  if constexpr (DT == DT_F32) {
+    float last = x[15];
+    asm volatile("s_nop 15\n\ts_nop 1" : "+v"(last));
+    x[15] = last;
+  } else {
+    settle_mfma32(x);
+  }
 }
 
 // what rows_product leaves, as operand B of the product over the stage's 32 rows: for 16 bits rounded to them
