@@ -453,6 +453,10 @@ struct Row {
 };
 __device__ __forceinline__ Row row_at(const WindowArgs& a, int p) { return Row{p, max(p, 0) - a.window + 1, a.sinks}; }
 
+// x y, and 0 where either is 0, whatever the other holds (v_mul_legacy_f32)
+extern "C" __device__ __attribute__((const)) float sta_mul_zero(float, float) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ float mul_zero(float x, float y) { return sta_mul_zero(x, y); }
+
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float at_least(float m) { return m == -INFINITY ? 0.f : m; }
 

@@ -311,12 +311,12 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   if (it.entry < 0) return;
   const Span sk = uniform(entry_of(a.k_starts, it.entry, a.B, a.S));
   const int key0 = it.tile * ROWS, kw = key0 + wave * 32, key = kw + r;
-  const int64_t at = (int64_t)(sk.at + key) * a.Hkv + hk;
   floatx16 dk[T::DB], dv[T::DB];
   clear<T>(dk);
   clear<T>(dv);
   auto store = [&](float dk_scale, float dv_scale) STA_INLINE {
     if (key >= sk.n) return;
+    const int64_t at = (int64_t)(sk.at + key) * a.Hkv + hk;
     store_rows<DT, T>(a.dk + at * T::RB, dk, dk_scale);
     store_rows<DT, T>(a.dv + at * T::RB, dv, dv_scale);
   };
@@ -393,7 +393,9 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float delta = stats[BUF][1][y * 8 + 2 * (i / 4) + h][i % 4];
-        x[i] *= DT == DT_F16 ? (dp[i] - delta) * down : dp[i] - delta;
+        // a product in which 0 times anything is 0: a row that sees a bad key has a delta that is no number, and
+        // the keys that it does not see would get it
+        x[i] = mul_zero(x[i], DT == DT_F16 ? (dp[i] - delta) * down : dp[i] - delta);
       }
       p.set(x);
       transposed_product<DT, T>(qt, place, y * 32, p, dk);
