@@ -121,12 +121,12 @@ WindowArgs args_of(const sta_window_args* a) {
   d.k_waves = cut.k_waves;
   d.steps = cut.steps;
   d.near_steps = cut.near_steps;
-  d.norm_blocks = cut.norm_blocks;
+  d.delta_blocks = cut.delta_blocks;
   return d;
 }
 
 struct GradLayout {
-  size_t lse_off, delta_off, norms_off, record_off, total;
+  size_t lse_off, delta_off, row_norm_off, key_norm_off, record_off, total;
 };
 GradLayout layout_of(const sta_window_args* a) {
   const WindowCut cut = cut_of(a);
@@ -137,8 +137,10 @@ GradLayout layout_of(const sta_window_args* a) {
   off = align256(off + rows * 4);
   l.delta_off = off;
   off = align256(off + rows * 4);
-  l.norms_off = off;
-  off = align256(off + (a->dtype == STA_DTYPE_F16 ? (size_t)cut.norm_blocks * 8 : 0));
+  l.row_norm_off = off;
+  off = align256(off + (a->dtype == STA_DTYPE_F16 ? rows * 4 : 0));
+  l.key_norm_off = off;
+  off = align256(off + (a->dtype == STA_DTYPE_F16 ? (size_t)a->S * a->Hkv * 4 : 0));
   l.record_off = off;
   off = align256(off + (size_t)a->Hkv * cut.records * 2 * (32 * cut.k_waves) * a->D * 4);
   l.total = off ? off : 1;
@@ -187,7 +189,8 @@ int sta_window_attention_grad(const sta_window_grad_args* a, void* stream) {
   d.dv = (char*)a->dv;
   d.row_lse = (float*)(ws + l.lse_off);
   d.row_delta = (float*)(ws + l.delta_off);
-  d.norms = (float*)(ws + l.norms_off);
+  d.row_norm = (float*)(ws + l.row_norm_off);
+  d.key_norm = (float*)(ws + l.key_norm_off);
   d.record = (float*)(ws + l.record_off);
   hipError_t e = launch_window_grad(f.dtype, f.D, d, cut_of(&f).records, (hipStream_t)stream);
   return e == hipSuccess ? STA_OK : hip_fail(e, "window attention gradient");

@@ -30,8 +30,8 @@ struct WindowArgs {
   // backward
   char *dq, *dk, *dv;
   float *row_lse, *row_delta;              // (H, T): log2 of the sum of exp, +inf for rows that see nothing; sum_d out dout
-  float* norms;                            // fp16: (blocks, 2) largest |dout row|^2 and |v row|^2
-  int norm_blocks;
+  float *row_norm, *key_norm;              // fp16: (H, T) |dout|^2 and (Hkv, S) |v|^2 of rows without infinities and NaN, 0 of others
+  int delta_blocks;                        // workgroups of the pass over out and dout
   float* record;                           // (records, 2, rows of a key tile, D) unfinished dk and dv
   int steps;                               // row steps of a work item of the key pass
   int near_steps;                          // row steps that a key tile has at most, a query head
@@ -41,7 +41,7 @@ struct WindowArgs {
 
 // how the key pass is cut (host)
 struct WindowCut {
-  int q_waves, k_waves, q_tiles, k_tiles, items, steps, near_steps, norm_blocks;
+  int q_waves, k_waves, q_tiles, k_tiles, items, steps, near_steps, delta_blocks;
   int64_t records;
 };
 WindowCut window_cut(int dtype, int D, int T, int S, int H, int Hkv, int B, bool starts, bool k_starts, int window,
@@ -391,12 +391,6 @@ __device__ __forceinline__ Span span_of(const int32_t* starts, int b, int total)
   if (!starts) return Span{0, total};
   const int s = min(max(starts[b], 0), total);
   return Span{s, max(min(starts[b + 1], total) - s, 0)};
-}
-// those of all sequences
-__device__ __forceinline__ Span all_of(const int32_t* starts, int B, int total) {
-  if (!starts) return Span{0, total};
-  const int s = min(max(starts[0], 0), total);
-  return Span{s, max(min(starts[B], total) - s, 0)};
 }
 // entry 0: the rows in front of the first sequence, 1 .. B: the sequences, B + 1: the rows behind the last
 __device__ __forceinline__ Span entry_of(const int32_t* starts, int e, int B, int total) {

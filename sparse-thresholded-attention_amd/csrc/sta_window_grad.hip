@@ -23,28 +23,26 @@ namespace {
 
 using namespace window;
 
-// An fp16 ds would pass the type's range: it is scaled by a power of two that keeps |ds| <= p 2 |dout| |v| below 2^14, from
-// the largest row of each.
-__device__ __forceinline__ float ds_scale(const WindowArgs& a, float* shared) {
-  const int tid = threadIdx.x;
-  float x = 0.f, y = 0.f;
-  const int waves = blockDim.x / 64;
-  for (int i = tid; i < a.norm_blocks; i += blockDim.x) {
-    x = fmaxf(x, a.norms[2 * i]);
-    y = fmaxf(y, a.norms[2 * i + 1]);
-  }
-  x = wave_max_f32(x);
-  y = wave_max_f32(y);
-  if ((tid & 63) == 0) shared[tid >> 6] = x, shared[4 + (tid >> 6)] = y;
-  __syncthreads();
-  for (int w = 0; w < waves; ++w) {
-    x = fmaxf(x, shared[w]);
-    y = fmaxf(y, shared[4 + w]);
-  }
-  __syncthreads();
-  const float most = 2.f * sqrtf(x) * sqrtf(y);
+// An fp16 ds would pass the type's range: it is scaled by a power of two that keeps |ds| <= p (|dout| |v| + |delta|) below
+// 2^14.  dq's are a row's own, from the largest v that its workgroup's rows see; the key pass takes one for the rows and
+// keys of a work item.  So large values of other sequences, heads and far places cost a row or a key no bits.
+__device__ __forceinline__ float grow_of(float most) {
   if (!(most > 0.f && most < INFINITY)) return 1.f;
-  return __uint_as_float((uint32_t)uniform((127 + min(max(13 - ilogbf(most), -100), 100)) << 23));
+  return __uint_as_float((uint32_t)(127 + min(max(13 - ilogbf(most), -100), 100)) << 23);
+}
+
+// the largest x of a workgroup's threads, in all of them
+template <int WAVES>
+__device__ __forceinline__ float group_max(float x, float* shared) {
+  x = wave_max_f32(x);
+  if constexpr (WAVES > 1) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) x = fmaxf(x, shared[w]);
+  }
+  return x;
 }
 
 // every row of a sequence of n keys sees one key
@@ -57,7 +55,6 @@ template <int DT, int D>
 __global__ __launch_bounds__(256) void window_delta_kernel(WindowArgs a) {
   using T = Tile<DT, D, 4>;
   constexpr int V = 16 / T::E, PER = 256 / T::CH;
-  __shared__ float most[2][4];
   const int c = threadIdx.x % T::CH, mine = threadIdx.x / T::CH;
   auto elements = [](const char* p, float* x) {
     const u32x4 w = *(const u32x4*)p;
@@ -75,15 +72,9 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WindowArgs a) {
     for (int s = 1; s < T::CH; s *= 2) x += __shfl_xor(x, s, 64);
     return x;
   };
-  float do2 = 0.f, v2 = 0.f;
   const int64_t rows = (int64_t)a.T * a.H;
-  // the scale's: rows and keys of sequences, without those that hold an infinity or a NaN
-  auto square = [](float sq, int64_t t, const Span& s) { return t >= s.at && t < s.at + s.n && sq < INFINITY ? sq : 0.f; };
-  Span of_rows{0, 0}, of_keys{0, 0};
-  if constexpr (DT == DT_F16) {
-    of_rows = all_of(a.starts, a.B, a.T);
-    of_keys = all_of(a.k_starts, a.B, a.S);
-  }
+  // the scale's: without rows that hold an infinity or a NaN
+  auto square = [](float sq) { return sq < INFINITY ? sq : 0.f; };
   for (int64_t i = (int64_t)blockIdx.x * PER + mine; i < rows; i += (int64_t)gridDim.x * PER) {
     const int64_t t = i / a.H;
     const int h = (int)(i - t * a.H);
@@ -103,30 +94,24 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WindowArgs a) {
       sq = fmaf(y[e], y[e], sq);
     }
     dot = row_sum(dot);
-    if constexpr (DT == DT_F16) do2 = fmaxf(do2, square(row_sum(sq), t, of_rows));
+    if constexpr (DT == DT_F16) sq = square(row_sum(sq));
     if (c == 0) {
       const float lse = a.lse_in[h * (int64_t)a.T + t];
       a.row_lse[h * (int64_t)a.T + t] = lse == -INFINITY ? INFINITY : lse * 1.44269504088896340736f;
       a.row_delta[h * (int64_t)a.T + t] = dot;
+      if constexpr (DT == DT_F16) a.row_norm[h * (int64_t)a.T + t] = sq;
     }
   }
   if constexpr (DT == DT_F16) {
     const int64_t keys = (int64_t)a.S * a.Hkv;
     for (int64_t i = (int64_t)blockIdx.x * PER + mine; i < keys; i += (int64_t)gridDim.x * PER) {
-      const int64_t t = i / a.Hkv;
+      const int64_t t = i / a.Hkv, hk = i - t * a.Hkv;
       float x[V], sq = 0.f;
-      elements(a.v + t * a.v_ts + (i - t * a.Hkv) * a.v_hs + c * 16, x);
+      elements(a.v + t * a.v_ts + hk * a.v_hs + c * 16, x);
 #pragma unroll
       for (int e = 0; e < V; ++e) sq = fmaf(x[e], x[e], sq);
-      v2 = fmaxf(v2, square(row_sum(sq), t, of_keys));
-    }
-    do2 = wave_max_f32(do2);
-    v2 = wave_max_f32(v2);
-    if ((threadIdx.x & 63) == 0) most[0][threadIdx.x >> 6] = do2, most[1][threadIdx.x >> 6] = v2;
-    __syncthreads();
-    if (threadIdx.x < 2) {
-      const float* x = most[threadIdx.x];
-      a.norms[2 * blockIdx.x + threadIdx.x] = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      sq = square(row_sum(sq));
+      if (c == 0) a.key_norm[hk * a.S + t] = sq;
     }
   }
 }
@@ -139,7 +124,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   using T = Tile<DT, D, WAVES>;
   constexpr int KT = T::KT, SUB = T::SUB, ROWS = T::ROWS;
   __shared__ u32x4 lds[2][2][KT * T::CH];
-  __shared__ float shared[8];
+  __shared__ float shared[4];
   const int G = a.H / a.Hkv, lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), r = lane & 31, h4 = (lane >> 5) * 4;
   const int id = xcd_order(), hk = id / (a.q_tiles * G), rest = id - hk * (a.q_tiles * G);
   if (hk >= a.Hkv) return;
@@ -166,7 +151,6 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   const char* kb = a.k + sk.at * a.k_ts + hk * a.k_hs;
   const char* vb = a.v + sk.at * a.v_ts + hk * a.v_hs;
   const Row me = row_at(a, off + row);
-  const float grow = DT == DT_F16 ? ds_scale(a, shared) : 1.f;
 
   u32x4 q[T::KD], dout[T::KD];
   load_rows<T>(q, a.q + sq.at * a.q_ts + h * a.q_hs, a.q_ts, row, sq.n);
@@ -174,6 +158,17 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   load_rows<T>(dout, a.dout + sq.at * a.do_ts + h * a.do_hs, a.do_ts, row, sq.n);
   const int64_t stat = (int64_t)h * a.T + sq.at + min(row, sq.n - 1);
   const float lse = a.row_lse[stat], delta = a.row_delta[stat];
+  float grow = 1.f;
+  if constexpr (DT == DT_F16) {
+    float v2 = 0.f;
+    const float* norms = a.key_norm + (int64_t)hk * a.S + sk.at;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < keys.n * KT; i += T::THREADS) {
+      const int key = keys.at(i / KT) * KT + i % KT;
+      if (key < sk.n) v2 = fmaxf(v2, norms[key]);
+    }
+    grow = grow_of(sqrtf(a.row_norm[stat]) * sqrtf(group_max<WAVES>(v2, shared)) + fabsf(delta));
+  }
   const Places at = places_of<DT, T>();
   Stager<T> ks, vs;
   ks.set(a.k_ts);
@@ -300,7 +295,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   constexpr int KT = T::KT, SUB = T::SUB, ROWS = T::ROWS;
   __shared__ u32x4 lds[2][2][KT * T::CH];
   __shared__ floatx4 stats[2][2][KT / 4];
-  __shared__ float shared[8];
+  __shared__ float shared[4];
   // parts of v that the registers do not hold beside two sums of 128 dims
   constexpr int PARK = DT != DT_F32 && D == 128 ? 3 : 0;
   __shared__ u32x4 parked[PARK ? WAVES * PARK : 1][64];
@@ -333,7 +328,27 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   const int first = max(key0 - off, 0) / KT;
   const int each = max((last + KT - 1) / KT - first, 0);
   const int s0 = (int)min((int64_t)it.part * a.steps, (int64_t)each * G), s1 = (int)min((int64_t)s0 + a.steps, (int64_t)each * G);
-  const float grow = DT == DT_F16 ? ds_scale(a, shared) : 1.f;
+  float grow = 1.f;
+  if constexpr (DT == DT_F16) {
+    float do2 = 0.f, delta = 0.f;
+    for (int s = s0; s < s1;) {            // the item's rows, a head after the other
+      const int g = s / each, in = s - g * each, end = min(each, in + s1 - s);
+      const int64_t head = (int64_t)(hk * G + g) * a.T + sq.at;
+      const int row1 = min((first + end) * KT, sq.n);
+#pragma unroll 4
+      for (int row = (first + in) * KT + (int)threadIdx.x; row < row1; row += T::THREADS) {
+        do2 = fmaxf(do2, a.row_norm[head + row]);
+        const float x = fabsf(a.row_delta[head + row]);
+        if (x < INFINITY) delta = fmaxf(delta, x);
+      }
+      s += end - in;
+    }
+    const float v2 = key < sk.n ? a.key_norm[(int64_t)hk * a.S + sk.at + key] : 0.f;
+    do2 = group_max<WAVES>(do2, shared);
+    delta = group_max<WAVES>(delta, shared);
+    grow = grow_of(sqrtf(do2) * sqrtf(group_max<WAVES>(v2, shared)) + delta);
+    grow = __uint_as_float((uint32_t)uniform((int)__float_as_uint(grow)));
+  }
   constexpr float SHIFT = DT == DT_F16 ? 15.f : 0.f;   // p times 2^15: fp16 keeps small ones
 
   u32x4 k[T::KD], v[T::KD];
@@ -458,7 +473,7 @@ hipError_t launch_keys(const WindowArgs& a, int64_t records, hipStream_t st) {
 template <int DT, int D>
 hipError_t launch_dt(const WindowArgs& a, int64_t records, hipStream_t st) {
   hipError_t e;
-  window_delta_kernel<DT, D><<<a.norm_blocks, 256, 0, st>>>(a);
+  window_delta_kernel<DT, D><<<a.delta_blocks, 256, 0, st>>>(a);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   if (a.q_tiles) {
     const unsigned grid = ((unsigned)a.q_tiles * a.H + 7) / 8 * 8;
@@ -511,9 +526,9 @@ WindowCut window_cut(int dtype, int D, int T, int S, int H, int Hkv, int B, bool
   }
   c.items = (int)(items < INT32_MAX ? items : INT32_MAX);
   c.records = records;
-  // of 16 rows a block and turn; enough blocks to fill the chip, few enough for their norms to be read again
+  // of 16 rows a block and turn
   const int64_t rows = (int64_t)T * H, blocks = (rows + 15) / 16;
-  c.norm_blocks = (int)(blocks < 1 ? 1 : blocks < 2048 ? blocks : 2048);
+  c.delta_blocks = (int)(blocks < 1 ? 1 : blocks < 2048 ? blocks : 2048);
   return c;
 }
 
