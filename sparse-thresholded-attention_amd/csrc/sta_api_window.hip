@@ -32,8 +32,10 @@ int check_out(const char* name, const void* p) {
   return STA_OK;
 }
 
-// keys of a window and sinks as the kernels take them: a window that reaches every key is none
-int window_of(const sta_window_args* a) { return a->window == 0 || a->window >= a->S ? INT_MAX : a->window; }
+// keys of a window and sinks as the kernels take them: a window that with the sinks reaches every key is none
+int window_of(const sta_window_args* a) {
+  return a->window == 0 || (int64_t)a->window + a->sinks >= a->S ? INT_MAX : a->window;
+}
 int sinks_of(const sta_window_args* a) { return a->sinks < a->S ? a->sinks : a->S; }
 
 WindowCut cut_of(const sta_window_args* a) {
@@ -120,6 +122,7 @@ WindowArgs args_of(const sta_window_args* a) {
   d.q_waves = cut.q_waves;
   d.k_waves = cut.k_waves;
   d.steps = cut.steps;
+  d.far_steps = cut.far_steps;
   d.near_steps = cut.near_steps;
   d.delta_blocks = cut.delta_blocks;
   return d;

@@ -34,6 +34,7 @@ struct WindowArgs {
   int delta_blocks;                        // workgroups of the pass over out and dout
   float* record;                           // (records, 2, rows of a key tile, D) unfinished dk and dv
   int steps;                               // row steps of a work item of the key pass
+  int far_steps;                           // of one of a key tile with sinks
   int near_steps;                          // row steps that a key tile has at most, a query head
   int q_tiles, k_tiles, items;             // bounds of the grids, a head / kv head
   int q_waves, k_waves;                    // waves of a workgroup: 4, or 1 where there are few rows
@@ -41,7 +42,7 @@ struct WindowArgs {
 
 // how the key pass is cut (host)
 struct WindowCut {
-  int q_waves, k_waves, q_tiles, k_tiles, items, steps, near_steps, delta_blocks;
+  int q_waves, k_waves, q_tiles, k_tiles, items, steps, far_steps, near_steps, delta_blocks;
   int64_t records;
 };
 WindowCut window_cut(int dtype, int D, int T, int S, int H, int Hkv, int B, bool starts, bool k_starts, int window,

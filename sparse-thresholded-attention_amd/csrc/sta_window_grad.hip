@@ -229,9 +229,10 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
 // ------------------------------------------------------------------------------------------
 // dk, dv
 // ------------------------------------------------------------------------------------------
-// A work item is a key tile and up to a.steps of its row steps (the heads of the kv head one after the other).  A tile
-// whose rows take one item is written out; else each item leaves a record and the join adds them up in order: tiles
-// with sinks, which every later row sees, and all tiles where there are too few for the chip.
+// A work item is a key tile and up to a.steps of its row steps (the heads of the kv head one after the other), of a tile
+// with sinks, which every later row sees, up to a.far_steps.  A tile whose rows take one item is written out; else each
+// item leaves a record and the join adds them up in order: tiles with sinks, and all tiles where there are too few for
+// the chip.
 struct Cut {
   int tiles, sink_tiles, near, far;        // key tiles, those with sinks, items of a near tile and of one with sinks
   __device__ __forceinline__ int items() const { return (tiles - sink_tiles) * near + sink_tiles * far; }
@@ -247,13 +248,13 @@ __device__ __forceinline__ Cut cut_of(const WindowArgs& a, int e) {
   if (e == 0 || e > a.B) return c;
   const int steps = (span_of(a.starts, e - 1, a.T).n + KT - 1) / KT, G = a.H / a.Hkv;
   c.near = max((int)(((int64_t)G * min(steps, a.near_steps) + a.steps - 1) / a.steps), 1);
-  c.far = max((int)(((int64_t)G * steps + a.steps - 1) / a.steps), 1);
+  c.far = max((int)(((int64_t)G * steps + a.far_steps - 1) / a.far_steps), 1);
   if (a.window != INT32_MAX) c.sink_tiles = min((a.sinks + ROWS - 1) / ROWS, c.tiles);
   return c;
 }
 // an item's tile, its place among the tile's items, and the tile's first record (< 0: none)
 struct Item {
-  int entry, tile, part, parts;
+  int entry, tile, part, parts, steps;     // steps: of an item of the tile, at most
   int64_t record;
 };
 template <typename T>
@@ -279,6 +280,7 @@ __device__ __forceinline__ Item item_of(const WindowArgs& a, int at, bool by_til
   if (it.tile >= c.tiles || x < 0) it.entry = -1;      // starts that do not ascend
   const bool sink = it.tile < c.sink_tiles;
   it.parts = sink ? c.far : c.near;
+  it.steps = sink ? a.far_steps : a.steps;
   it.record = it.parts == 1 ? -1 : before + (sink ? (int64_t)it.tile * c.far
                                                   : (int64_t)(c.far > 1 ? c.sink_tiles * c.far : 0) + (int64_t)(it.tile - c.sink_tiles) * c.near);
   if (it.record + it.parts > records || it.record < -1) it.entry = -1;
@@ -286,6 +288,7 @@ __device__ __forceinline__ Item item_of(const WindowArgs& a, int at, bool by_til
   it.tile = uniform(it.tile);
   it.part = uniform(it.part);
   it.parts = uniform(it.parts);
+  it.steps = uniform(it.steps);
   return it;
 }
 
@@ -327,7 +330,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
   const int last = sink ? sq.n : (int)min((int64_t)sq.n, max((int64_t)key1 + a.window - off, (int64_t)0));
   const int first = max(key0 - off, 0) / KT;
   const int each = max((last + KT - 1) / KT - first, 0);
-  const int s0 = (int)min((int64_t)it.part * a.steps, (int64_t)each * G), s1 = (int)min((int64_t)s0 + a.steps, (int64_t)each * G);
+  const int s0 = (int)min((int64_t)it.part * it.steps, (int64_t)each * G), s1 = (int)min((int64_t)s0 + it.steps, (int64_t)each * G);
   float grow = 1.f;
   if constexpr (DT == DT_F16) {
     float do2 = 0.f, delta = 0.f;
@@ -515,14 +518,24 @@ WindowCut window_cut(int dtype, int D, int T, int S, int H, int Hkv, int B, bool
   const int64_t even = (tiles * each + items_wanted - 1) / items_wanted;
   if (even < each) each = even < fewest ? fewest : even;
   c.steps = (int)(each < INT32_MAX ? each : INT32_MAX);
-  const int64_t near_parts = (G * c.near_steps + c.steps - 1) / c.steps;
-  int64_t items = c.k_tiles * near_parts, records = near_parts > 1 ? items : 0;
+  const int64_t near_parts = (G * c.near_steps + c.steps - 1) / c.steps, key_tiles = (S + ROWS - 1) / ROWS;
+  // sequences of which a tile takes several items of n steps: their rows have more than n / G steps
+  auto shared = [&](int64_t n) { const int64_t most = T / (kt * (n / G) + 1); return B < most ? B : most; };
+  int64_t records = near_parts > 1 ? (key_tiles + shared(c.steps)) * near_parts : 0, items = c.k_tiles + records;
+  c.far_steps = c.steps;
   if (window != INT32_MAX && sinks > 0) {
-    // of each tile with sinks: sum over the sequences of ceil(G ceil(rows / kt) / steps)
-    const int64_t far = (G * (T / kt + (B < T ? B : T) + 1) + c.steps - 1) / c.steps + B;
-    const int64_t most = (S + ROWS - 1) / ROWS, of = (sinks + ROWS - 1) / ROWS;
-    items += far * (of < most ? of : most);
-    records += far * (of < most ? of : most);
+    // As many steps that the tiles with sinks make two items for each place on the chip, if their steps are more than
+    // that: where many keys are sinks, items of c.steps would leave records of more bytes than all gradients, quadratic in
+    // the tokens (8192 tokens, 32 / 8 heads x 128, bf16, window 128, 4096 sinks: 0.91 GB, so 0.17; 1.87 -> 1.71 ms).
+    const int64_t of = (sinks + ROWS - 1) / ROWS, sink_tiles = of < key_tiles ? of : key_tiles;
+    const int64_t all_far = sink_tiles * G * (T / kt + (B < T ? B : T)) * Hkv, far = (all_far + 1023) / 1024;
+    if (far > c.far_steps) c.far_steps = (int)(far < INT32_MAX ? far : INT32_MAX);
+    // of each tile with sinks the sum over the sequences of ceil(G ceil(rows / kt) / steps)
+    const int64_t n = shared(c.far_steps), parts = G * (T / kt + n) / c.far_steps + n;
+    const int64_t most = (key_tiles + n) * ((G * all + c.far_steps - 1) / c.far_steps);
+    const int64_t far_records = sink_tiles * parts < most ? sink_tiles * parts : most;
+    items += far_records;
+    records += far_records;
   }
   c.items = (int)(items < INT32_MAX ? items : INT32_MAX);
   c.records = records;
