@@ -28,11 +28,13 @@ namespace {
 
 using namespace window;
 
-// Up to so many keys of a workgroup the second product takes P in two parts; with a backward pass to come up to the second
-// number.  Its delta inherits the error of P, and beside ds' own rounding that weighs by the sum of p^2: 3 sequences of
-// 2000 tokens, 24 heads x 64, fp16, causal, dq erred by 1.48 to 1.51 times what rounding it costs with two parts up to 256 keys,
-// by 1.46 to 1.47 up to 1024 (114 -> 122 us; 5 of together 8192, 32 heads over 8 x 128, bf16, window 1024: 192 -> 206).
-constexpr int FEW = 256, FEW_TRAIN = 1024;
+// Up to so many keys of a workgroup the second product takes P in two parts.  A backward pass' delta inherits the error of
+// P, and beside ds' own rounding that weighs by the sum of p^2: 3 sequences of 2000 tokens, 24 heads x 64, fp16, causal, dq
+// erred by 1.48 to 1.51 times what rounding it costs with two parts up to 256 keys, by 1.46 to 1.47 up to 1024 (114 -> 122 us; 5
+// of together 8192, 32 heads over 8 x 128, bf16, window 1024: 192 -> 206).  One number with and without a backward pass
+// to come, so that both give the same bits; with 256 a call without would take 125 us in place of 149 (8192 tokens, 32 heads
+// over 8 x 128, bf16, window 512; window 1024: 187 and 191; a prompt of 1024: 30 and 36).
+constexpr int FEW = 1024;
 
 template <int DT, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void window_kernel(WindowArgs a) {
@@ -86,7 +88,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<DT, D, WAVES>::LEAST)) void windo
     ks.copy(lds[buf][0], kb, keys.at(t) * KT, sk.n);
     vs.copy(lds[buf][1], vb, keys.at(t) * KT, sk.n);
   };
-  const bool few = keys.n * KT <= (a.rest ? FEW_TRAIN : FEW);
+  const bool few = keys.n * KT <= FEW;
   const int lo_first = max(pw, 0) - a.window + 1, lo_last = max(pw + 31, 0) - a.window + 1;
   auto turn = [&](int t, auto which) STA_INLINE {
     constexpr int BUF = decltype(which)::value;
