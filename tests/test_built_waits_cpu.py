@@ -159,3 +159,16 @@ def test_no_copy_into_lds_reads_its_scalar_operands_too_early(kernels):
     assert sum("_lds_" in text for _, code in kernels for text, _ in code) > 1000
     early = [f"{name}: {x}" for name, code in kernels for x in _early_addresses(code)]
     assert not early, f"{len(early)} in all, the first {early[:4]}"
+
+
+def test_copies_into_lds_wait_for_their_scalar_operands_themselves():
+    """Whatever is built around them: a copy with a scalar base waits 5 states, any other one for M0."""
+    found = 0
+    for name in sorted(os.listdir(os.path.join(PKG, "csrc"))):
+        text = open(os.path.join(PKG, "csrc", name)).read()
+        for wait, operands in re.findall(r'asm volatile\("(?:s_nop (\d+)\\n\\t)?global_load_lds_\w+ [^"]*"\s*:[^:]*:([^;]*);', text):
+            found += 1
+            assert wait and int(wait) >= (4 if '"s"(' in operands else 0), (name, operands)
+        assert text.count("global_load_lds_dword") - len(re.findall(r"//.*global_load_lds_dword|\(global_load_lds_dword", text)) \
+            == len(re.findall(r'asm volatile\("s_nop \d\\n\\tglobal_load_lds_dword', text)), name
+    assert found >= 5
