@@ -19,7 +19,7 @@ int check_rows(const char* name, const void* p, int dtype, int rows, int64_t s0,
   if (!aligned16(p)) return fail(STA_ERR_UNSUPPORTED, "%s is not 16-byte aligned", name);
   const int64_t s[2] = {s0, s1};
   for (int i = 0; i < 2; ++i)
-    if (s[i] < 0 || s[i] > (INT64_MAX >> 36) || (s[i] * esize(dtype)) % 16 != 0)
+    if (s[i] < 0 || s[i] > (INT64_MAX >> 20) || (s[i] * esize(dtype)) % 16 != 0)
       return fail(STA_ERR_UNSUPPORTED, "%s stride %lld is negative, too large or not 16-byte aligned", name,
                   (long long)s[i]);
   if (rows > 1 && s0 * esize(dtype) > (1 << 29))
