@@ -637,7 +637,7 @@ int sta_norm_rotary_grad(const sta_norm_rotary_grad_args* args, void* stream);
  * of k and v; row i of its nq is at position p = nk - nq + i among its nk keys and sees the keys j <= p with
  * j > p - window or j < sinks.  out = sum_j p_j v_j with p the softmax of sm_scale * q . k_j over them; a row
  * that sees no key, or whose scores are all -inf, gets zeros and lse -inf, and so do rows of no sequence.
- * Offsets below 0 or past T (S) count as 0 or T (S).  Token strides up to 2^29 bytes. */
+ * Offsets below 0 or past T (S) count as 0 or T (S).  Token strides up to 2^29 bytes, head strides up to 2^43 elements. */
 typedef struct sta_window_args {
   const void* q;           /* (T, H, D), 16-byte rows, element strides */
   const void* k;           /* (S, Hkv, D) */

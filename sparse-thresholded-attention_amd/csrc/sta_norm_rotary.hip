@@ -428,7 +428,7 @@ NormCut cut_of(const sta_rotary_args& a) {
   if (a.Hkv) c.k_blocks = ((int64_t)a.T + (c.k_per = tokens_of(a, a.Hkv)) - 1) / c.k_per;
   return c;
 }
-// The gradient's workgroups are at most MOST, q's and k's in the ratio of their rows, since each leaves a sum of its weight's.
+// The gradient's workgroups are at most MOST and one, q's and k's in the ratio of their rows, since each leaves a sum of its weight's.
 // 16384 tokens of 32 + 8 heads x 128, bf16, with 768 / 1536 / 2048 / 3000 / 8192: 155 / 126 / 119 / 116 / 117 us with the
 // second kernel (few stay until the last is done, many leave it more to add).
 constexpr int64_t MOST = 2560;

@@ -65,7 +65,8 @@ struct Tile {
   static constexpr int KD = RB / 32;       // products over a row: 32 bytes of it each, 16 a half wave
   static constexpr int DB = D / 32;        // blocks of 32 dims
   static constexpr int LEAST = DT == DT_F32 || WAVES == 1 ? 1 : 2;    // waves of a SIMD that the registers have to allow
-  static constexpr int KT = DT == DT_F32 || WAVES == 1 ? 32 : 64;   // rows of a stage; one wave: room for four workgroups a CU
+  // rows of a stage; one wave: room for four workgroups a CU, but for fp32 at D 128, whose 65 KB leave room for two
+  static constexpr int KT = DT == DT_F32 || WAVES == 1 ? 32 : 64;
   static constexpr int SUB = KT / 32;
   static constexpr int COPIES = KT * CH / THREADS;    // a wave's 1 KB copies of a stage's rows
 };

@@ -11,15 +11,19 @@
 // so P never moves between lanes.  The running maximum and sum of a row are fp32, a lane pair's own; a maximum that rises
 // by less than 2^8 leaves the sums as they are.  P is rounded once to 16 bits for the second product (its sum is of the
 // unrounded one): an error of 2^-9 (fp16 2^-12) of each probability, which adds up at random over the keys to about
-// what rounding the output itself costs.  Workgroups whose rows see few keys add the product with what the rounding left.
+// what rounding the output itself costs.  Workgroups whose rows see up to FEW keys add the product with what the rounding left.
 //
 // Measured, products of the visible pairs alone: a prompt of 8192 tokens, 32 heads over 8 x 128, bf16, window 4096, 128 sinks:
 // 421 GFLOP in 436 us, 965 TFLOP/s, 79% of what a product of two 8192^2 matrices reaches; the same heads, 5 packed
-// sequences of together 8192, window 1024, for a backward pass: 206 us, 500 TFLOP/s (short sequences and the two masked ends of each window weigh
-// more); 24 heads x 64, fp16, 6001 tokens in 3 sequences, causal, likewise: 122 us, 390 TFLOP/s (twice the exponentials a
+// sequences of together 8192, window 1024: 205 us, 500 TFLOP/s (short sequences and the two masked ends of each window weigh
+// more); 24 heads x 64, fp16, 6001 tokens in 3 sequences, causal: 125 us, 380 TFLOP/s (twice the exponentials a
 // product).  Bound by the matrix cores beside LDS reads of as many cycles and
 // the exponentials: the cores are busy half of the time, LDS has no bank conflicts.  128 rows a workgroup: 64 rows a wave
-// would halve those reads, but not fit the registers at D 128.
+// would halve those reads; they do not fit the registers at D 128, and are untried at D 64.  fp32, 2370 tokens, 16 heads over 2 x 128,
+// causal: 23 GFLOP in 453 us, a third of its product rate: one wave a SIMD, whose products and exponentials take turns.
+//
+// A wave whose sums end as no finite numbers goes over its rows' keys one by one: 8192 tokens, 32 heads over 8 x 128, bf16, causal, a
+// NaN in key 10 of every head: 0.69 -> 30 ms (the gradient 2.6 -> 53; window 1024: 0.22 -> 1.7 and 0.59 -> 3.6).
 #include "sta_window.h"
 
 namespace sta {

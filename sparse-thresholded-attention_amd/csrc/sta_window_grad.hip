@@ -10,8 +10,8 @@
 // transposed for the sums.  p and ds are rounded once to 16 bits for those, as p is in the forward pass.
 //
 // Measured: 5 packed sequences of together 8192, 32 heads over 8 x 128, bf16, window 1024, 4 sinks: delta 39 us (201 MB,
-// 5.1 TB/s), dq 218 (155 GFLOP, 710 TFLOP/s), dk and dv 388 (207 GFLOP, 530 TFLOP/s, 44% of a large product), the join 21;
-// 24 heads x 64, fp16, 3 sequences of together 6001, causal: 17 / 141 / 196 us.  The key pass is bound by its registers: two
+// 5.1 TB/s), dq 216 (155 GFLOP, 710 TFLOP/s), dk and dv 387 (207 GFLOP, 530 TFLOP/s, 44% of a large product), the join 22;
+// 24 heads x 64, fp16, 3 sequences of together 6001, causal: 16 / 141 / 193 us.  The key pass is bound by its registers: two
 // sums of 128 dims and the keys' own k and v leave two waves a SIMD, and every stage is read four times from LDS.  Its
 // 70 or so items a kv head run on 64 places, one of them nearly twice: shares of one length would save at most a fifth
 // and leave records of nearly every tile, whose 134 MB cost about as much to write and read.
@@ -490,8 +490,17 @@ hipError_t launch_dt(const WindowArgs& a, int64_t records, hipStream_t st) {
 
 }  // namespace
 
-// Up to so many workgroups of 128 rows (keys) a pass takes 32 each instead, one wave: 1000 tokens, 8 / 8 heads x 64, fp32, window
-// 100, 64 of them: forward 30 -> 23 us, dq 35 -> 27.
+// Up to so many workgroups of 128 rows (keys) a pass takes 32 each instead, one wave.  It gains where the rows see few keys, and
+// in the key pass it costs where they see many: there four waves would fill the chip too, since the items cut a tile's steps, and a
+// wave alone copies every stage for itself.  Calls from Python with one wave and with four, forward / gradient in us:
+//   8 / 8 heads x 64, fp32, 4 x 250 tokens, window 100     20 / 54     29 / 68
+//   8 / 2 x 128, bf16, 300                                 20 / 43     19 / 48
+//   32 / 8 x 128, bf16, 512                                28 / 65     24 / 63
+//   28 / 4 x 128, bf16, 4000, window 1000                  97 / 514    98 / 374
+//   24 / 1 x 128, bf16, 2000                               64 / 368    63 / 270
+//   16 / 2 x 128, fp16, 3062                               97 / 619    99 / 390
+//   16 / 2 x 128, fp32, 2370                              453 / 2639  444 / 1770
+// A rule that takes the key pass' items into account would have both; not built.
 constexpr int64_t FEW_TILES = 256;
 
 WindowCut window_cut(int dtype, int D, int T, int S, int H, int Hkv, int B, bool starts, bool k_starts, int window,
